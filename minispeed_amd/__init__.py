@@ -9,7 +9,7 @@ master->model cast) runs as hand-written gfx950 HIP kernels from
 ``libminispeed_boundary.so``.
 """
 
-from . import comm
+from . import comm, ops
 from .config import ConfigError, DeepSpeedConfig
 from .engine import DeepSpeedEngine, initialize
 from .optim import WarmupDecayLR, WarmupLR
@@ -31,5 +31,6 @@ __all__ = [
     "Timers",
     "set_seed",
     "comm",
+    "ops",
     "__version__",
 ]

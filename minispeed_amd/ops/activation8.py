@@ -1,0 +1,231 @@
+"""Activations held in 8 bits between forward and backward.
+
+Blocks of 32 consecutive values share a power-of-two scale of one byte; a value
+is a signed byte times that scale, 1.03 bytes in all.  The error of a value is
+at most half a step, less than 1/127 of its block's largest magnitude.  A block
+that holds an inf or a NaN comes back as NaN throughout, so that an overflow in
+a held activation still reaches the gradients and the loss scaler skips the
+step.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple
+
+import torch
+import torch.nn.functional as F
+
+from . import _native
+
+KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2, "swiglu": 3}
+
+
+class Checkpoint8:
+    """A tensor in its 8-bit form: ``codes`` (int8, one per value), ``exponents``
+    (uint8, one per 32 values), and the ``shape`` and ``dtype`` it comes back
+    with."""
+
+    __slots__ = ("codes", "exponents", "shape", "dtype")
+
+    def __init__(self, codes: torch.Tensor, exponents: torch.Tensor, shape, dtype: torch.dtype):
+        self.codes, self.exponents = codes, exponents
+        self.shape, self.dtype = tuple(shape), dtype
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.exponents.numel()
+
+
+def pack8(x: torch.Tensor) -> Checkpoint8:
+    """The 8-bit form of ``x`` (float32 / float16 / bfloat16)."""
+    codes, exponents = _native.pack8(x)
+    return Checkpoint8(codes, exponents, x.shape, x.dtype)
+
+
+def unpack8(held: Checkpoint8) -> torch.Tensor:
+    """The values that an 8-bit form stands for."""
+    return _native.unpack8(held.codes, held.exponents, held.shape, held.dtype)
+
+
+def _kind(kind: str) -> int:
+    try:
+        return KINDS[kind]
+    except KeyError:
+        raise ValueError(f"unknown activation {kind!r}; expected one of {sorted(KINDS)}") from None
+
+
+def activation8(h: torch.Tensor, kind: str = "gelu", up: Optional[torch.Tensor] = None
+                ) -> Tuple[torch.Tensor, Tuple[Checkpoint8, ...]]:
+    """``(a, saved)``: the activation of ``h`` and its input in 8 bits, in one pass.
+
+    ``kind`` is ``"gelu"`` (with the error function), ``"gelu_tanh"``, ``"silu"`` or
+    ``"swiglu"`` (``silu(h) * up``).  ``a`` is computed from ``h`` itself; ``saved``
+    (one checkpoint, two for ``"swiglu"``) is what :func:`activation8_grad` takes.
+    """
+    a, codes, exponents, up_codes, up_exponents = _native.act8(h, up, _kind(kind))
+    saved = (Checkpoint8(codes, exponents, h.shape, h.dtype),)
+    if up is not None:
+        saved += (Checkpoint8(up_codes, up_exponents, h.shape, h.dtype),)
+    return a, saved
+
+
+def activation8_grad(saved: Sequence[Checkpoint8], grad: torch.Tensor, kind: str = "gelu",
+                     again: bool = True
+                     ) -> Tuple[Tuple[torch.Tensor, ...], Optional[torch.Tensor]]:
+    """``(grads, a)``: the backward pass of :func:`activation8`, in one pass.
+
+    ``grads`` holds the gradient of ``h`` (and of ``up``); ``a`` is the activation
+    again, from the held values, for the weight gradient of the product behind it
+    (``None`` with ``again=False``).
+    """
+    if not 1 <= len(saved) <= 2:
+        raise ValueError(f"{len(saved)} checkpoints, expected one or two")
+    if saved[0].dtype != grad.dtype or saved[0].shape != tuple(grad.shape):
+        raise ValueError(f"grad is {grad.dtype} {tuple(grad.shape)}, the checkpoint "
+                         f"{saved[0].dtype} {saved[0].shape}")
+    up = saved[1] if len(saved) == 2 else None
+    dh, dup, a = _native.act8_grad(saved[0].codes, saved[0].exponents, up and up.codes,
+                                   up and up.exponents, grad, _kind(kind), again)
+    return ((dh,) if dup is None else (dh, dup)), a
+
+
+class _ActivationLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, up, weight, bias, kind):
+        a, saved = activation8(h, kind, up)
+        ctx.kind, ctx.meta = kind, [(s.shape, s.dtype) for s in saved]
+        ctx.save_for_backward(weight, *(t for s in saved for t in (s.codes, s.exponents)))
+        ctx.has_bias = bias is not None
+        return F.linear(a, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        weight, *held = ctx.saved_tensors
+        saved = [Checkpoint8(held[2 * k], held[2 * k + 1], *m) for k, m in enumerate(ctx.meta)]
+        need = ctx.needs_input_grad
+        dh = dup = dw = db = None
+        flat = grad.reshape(-1, grad.shape[-1])
+        if need[0] or need[1] or need[2]:
+            grads, a = activation8_grad(saved, grad.matmul(weight), ctx.kind, again=need[2])
+            dh, dup = grads if len(grads) == 2 else (grads[0], None)
+            if need[2]:
+                dw = flat.t().mm(a.reshape(-1, a.shape[-1]))
+        if ctx.has_bias and need[3]:
+            db = flat.sum(0)
+        return dh, dup, dw, db, None
+
+
+def activation8_linear(h: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                       kind: str = "gelu", up: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``linear(act(h), weight, bias)`` that keeps only ``h`` (and ``up``) in 8 bits.
+
+    The second half of a transformer's MLP.  torch would keep ``h`` for the
+    activation and ``act(h)`` for the weight's gradient, 4 bytes per value in half
+    precision; this keeps 1.03 (2.06 gated).  The backward pass reads the held
+    values once, for the gradient of ``h`` and for the activation that the weight's
+    gradient needs.  The products are the library's.
+    """
+    return _ActivationLinear.apply(h, up, weight, bias, kind)
+
+
+class _Checkpoint(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, fn, preserve_rng, *args):
+        ctx.fn, ctx.preserve_rng = fn, preserve_rng
+        ctx.autocast = dict(device_type="cuda", enabled=torch.is_autocast_enabled("cuda"),
+                            dtype=torch.get_autocast_dtype("cuda"))
+        if preserve_rng:
+            ctx.rng = _rng_state(args)
+        ctx.slots, held = [], []
+        for arg in args:
+            if not isinstance(arg, torch.Tensor):
+                ctx.slots.append(("value", arg, False))
+            elif arg.is_floating_point() and arg.dim() > 0 and arg.dtype in _HELD:
+                packed = pack8(arg)
+                ctx.slots.append(("held", (packed.shape, packed.dtype), arg.requires_grad))
+                held += [packed.codes, packed.exponents]
+            else:
+                ctx.slots.append(("tensor", None, arg.requires_grad))
+                held.append(arg)
+        ctx.save_for_backward(*held)
+        with torch.no_grad():
+            return fn(*args)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        held, args = list(ctx.saved_tensors), []
+        for what, meta, needs in ctx.slots:
+            if what == "value":
+                arg = meta
+            elif what == "held":
+                codes, exponents = held.pop(0), held.pop(0)
+                arg = unpack8(Checkpoint8(codes, exponents, *meta))
+            else:
+                arg = held.pop(0).detach()
+            if needs:
+                arg.requires_grad_()
+            args.append(arg)
+        with torch.enable_grad(), torch.autocast(**ctx.autocast), \
+                _RngOf(ctx.rng if ctx.preserve_rng else None):
+            out = ctx.fn(*args)
+        outs = out if isinstance(out, tuple) else (out,)
+        pairs = [(o, g) for o, g in zip(outs, grads)
+                 if isinstance(o, torch.Tensor) and o.requires_grad and g is not None]
+        if pairs:
+            torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
+        return None, None, *(a.grad if needs else None
+                             for a, (_, _, needs) in zip(args, ctx.slots))
+
+
+_HELD = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _rng_state(args):
+    device = next((a.device for a in args if isinstance(a, torch.Tensor) and a.is_cuda), None)
+    return (torch.get_rng_state(), device,
+            None if device is None else torch.cuda.get_rng_state(device))
+
+
+class _RngOf:
+    """Inside, the random generators are where ``state`` was taken; afterwards they
+    are where they were."""
+
+    def __init__(self, state):
+        self.state = state
+
+    def __enter__(self):
+        if self.state is not None:
+            device = self.state[1]
+            self.now = (torch.get_rng_state(), device,
+                        None if device is None else torch.cuda.get_rng_state(device))
+            self._set(self.state)
+
+    def __exit__(self, *exc):
+        if self.state is not None:
+            self._set(self.now)
+
+    @staticmethod
+    def _set(state):
+        cpu, device, cuda = state
+        torch.set_rng_state(cpu)
+        if device is not None:
+            torch.cuda.set_rng_state(cuda, device)
+
+
+def checkpoint8(fn, *args, preserve_rng_state: bool = True):
+    """``fn(*args)`` whose activations are computed again in the backward pass, from
+    arguments held in 8 bits.
+
+    The floating tensors among ``args`` are kept in their 8-bit form (other
+    tensors as they are), and ``fn`` runs again on the values they stand for when
+    the gradients come: the use of minispeed's ``checkpoint``
+    (minispeed/activation_checkpointing.py:17-20) with a quarter to a half of its
+    memory.  The first run sees the arguments themselves.  Parameters that ``fn``
+    reaches by itself get their gradients; with ``preserve_rng_state`` random
+    operations (dropout) draw the same numbers in both runs.  Gradients reach
+    ``args`` only if one of them requires a gradient, as with any reentrant
+    checkpoint.
+    """
+    return _Checkpoint.apply(fn, preserve_rng_state, *args)
