@@ -20,6 +20,8 @@
  *     row r starts at (r / inner) * outer_stride + (r % inner) * inner_stride
  *     elements; elements of a row are consecutive.  Token lists are the same
  *     with one element per row.  A plain list has inner = its length.
+ *     Lists, rows and vocabularies hold fewer than 2^31 entries; offsets are
+ *     64-bit.
  */
 #ifndef MINISPEED_OPS_H
 #define MINISPEED_OPS_H
@@ -92,7 +94,7 @@ int ms_embedding(const ms_tokens_t* ids, const ms_rows_t* table, float scale,
  * gradient's type and written whole (rows without tokens are zeros).  Sums
  * are fp32 in an order that depends on the ids alone, multiplied by scale
  * and rounded once.  Ids outside [0, vocab) and `padding_idx` (-1: none) add
- * nothing.
+ * nothing.  dtable is 16-byte aligned.
  */
 int64_t ms_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t width);
 int ms_embedding_grad(const ms_tokens_t* ids, const ms_rows_t* grad, int64_t vocab,

@@ -30,29 +30,73 @@ __device__ __forceinline__ T narrow(float x) {
 
 __device__ __forceinline__ float quiet_nan() { return __builtin_nanf(""); }
 
-// Token t of a list, as a 64-bit number.
+// Token t of a list, as a 64-bit number.  Lists hold fewer than 2^31 tokens.
 __device__ __forceinline__ int64_t token(const ms_tokens_t& ids, int64_t t) {
-  const int64_t at = t < ids.inner ? t * ids.inner_stride
-                                   : (t / ids.inner) * ids.outer_stride +
-                                         (t % ids.inner) * ids.inner_stride;
+  int64_t at;
+  if (t < ids.inner) {
+    at = t * ids.inner_stride;
+  } else {
+    const uint32_t inner = static_cast<uint32_t>(ids.inner), q = static_cast<uint32_t>(t) / inner;
+    at = q * ids.outer_stride + (static_cast<uint32_t>(t) - q * inner) * ids.inner_stride;
+  }
   return ids.wide ? static_cast<const int64_t*>(ids.data)[at]
                   : static_cast<int64_t>(static_cast<const int32_t*>(ids.data)[at]);
 }
 
-// First element of row r.
+// First element of row r; fewer than 2^31 rows.
 __device__ __forceinline__ int64_t row_start(const ms_rows_t& m, int64_t r) {
-  return r < m.inner ? r * m.inner_stride
-                     : (r / m.inner) * m.outer_stride + (r % m.inner) * m.inner_stride;
+  if (r < m.inner) return r * m.inner_stride;
+  const uint32_t inner = static_cast<uint32_t>(m.inner), q = static_cast<uint32_t>(r) / inner;
+  return q * m.outer_stride + (static_cast<uint32_t>(r) - q * inner) * m.inner_stride;
+}
+
+// N values at any element alignment, as one load or store of up to 16 bytes:
+// gfx950's global memory takes vectors at 2- and 4-byte addresses.
+template <int B> struct raw_of;
+template <> struct raw_of<2> { typedef uint16_t type; };
+template <> struct raw_of<4> { typedef uint32_t type __attribute__((aligned(2))); };
+template <> struct raw_of<8> { typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct raw_of<16> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
+
+template <typename T, int N>
+struct Pack {
+  T v[N];
+};
+
+template <int N, typename T>
+__device__ __forceinline__ Pack<T, N> load(const T* p) {
+  typedef typename raw_of<N * sizeof(T)>::type raw;
+  const raw r = *reinterpret_cast<const raw*>(p);
+  Pack<T, N> x;
+  static_assert(sizeof(x) == sizeof(r), "");
+  __builtin_memcpy(&x, &r, sizeof(r));
+  return x;
+}
+template <int N, typename T>
+__device__ __forceinline__ void store(T* p, const Pack<T, N>& x) {
+  typedef typename raw_of<N * sizeof(T)>::type raw;
+  raw r;
+  __builtin_memcpy(&r, &x, sizeof(r));
+  *reinterpret_cast<raw*>(p) = r;
+}
+
+__device__ __forceinline__ int read_lane(int x, int lane) {
+  return __builtin_amdgcn_readlane(x, lane);
+}
+__device__ __forceinline__ int64_t read_lane(int64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), lane);
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 inline bool good_dtype(int32_t d) { return d >= MS_OPS_F32 && d <= MS_OPS_BF16; }
 inline int64_t dtype_bytes(int32_t d) { return d == MS_OPS_F32 ? 4 : 2; }
 
 inline bool good_tokens(const ms_tokens_t* t) {
-  return t && t->n >= 0 && t->inner >= 1 && (t->n == 0 || t->data);
+  return t && t->n >= 0 && t->n <= INT32_MAX && t->inner >= 1 && (t->n == 0 || t->data);
 }
 inline bool good_rows(const ms_rows_t* m) {
-  return m && m->n >= 0 && m->width >= 0 && m->inner >= 1 && good_dtype(m->dtype) &&
+  return m && m->n >= 0 && m->n <= INT32_MAX && m->width >= 0 && m->inner >= 1 && good_dtype(m->dtype) &&
          (m->n == 0 || m->width == 0 || m->data);
 }
 
