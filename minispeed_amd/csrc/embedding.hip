@@ -25,30 +25,60 @@ __global__ void __launch_bounds__(256) k_lookup(ms_tokens_t ids, ms_rows_t table
   }
 }
 
-// The gradient's table, in three launches:
+// The gradient's table.  Tokens are sorted by (id, t) on the device, then each
+// id's rows are added in that order; no atomics touch a sum.
 //
-//   k_sort_tokens  kSortRows rows of the table or fewer to a block: it counts
-//                  its rows' tokens in LDS, wave w over the w-th part of the
-//                  list, and places their positions stably, so `position` ends
-//                  up sorted by (id, t).  The other blocks of the same launch
-//                  clear the table, which takes longer.
-//   k_sum_spans    `span` sorted positions to a wave and a slice of the width:
-//                  fp32 sums of each id's rows, written to the table where the
-//                  id's tokens lie within the span, left as a partial sum where
-//                  they go on before (slot 0) or behind (slot 1) it.  An id
-//                  with half of the tokens costs what others cost.
-//   k_join_spans   adds up the partial sums of ids that cross spans.
+// Few tokens and a small table, one launch (k_grad_small): every block sorts
+// all tokens for a few rows of the table in LDS, adds and clears them.
 //
-// Every order is that of (id, t) and of the spans: no atomics on sums.
+// Otherwise three:
+//   k_sort_tokens  a bucket of ids to a block, which goes through all tokens:
+//                  its ids' positions end up grouped by id and rising.  Other
+//                  blocks of the launch clear the first rows of the table.
+//                  Buckets take every 2^k-th id: the frequent tokens of a
+//                  vocabulary often have neighbouring numbers, and one block
+//                  with most of the tokens took 75 us where 13 are usual.
+//   k_sum_spans    kSpan sorted positions to a wave and a slice of the width.
+//                  Ids of up to kLight tokens belong to the span they begin in;
+//                  of longer ones every span adds its piece, left as a partial
+//                  sum, so that an id with half of the tokens costs what others
+//                  cost.  Other blocks clear the remaining rows without tokens.
+//   k_join_spans   adds up the partial sums.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kSortRows = 1024;
-constexpr int kSortSteps = 8;             // groups of 64 tokens in flight per wave
+constexpr int kSortSteps = 16;            // groups of 64 tokens in flight per wave
 
 struct Sorted {
-  int32_t* start;       // [vocab + 1]: where each id's tokens begin
+  int32_t* start;       // [buckets * rows + 1]: where each id's tokens begin, by slot
   int32_t* id;          // [n]
   int32_t* position;    // [n]
   float* partial;       // [spans, 2, width]
+  int32_t rows;         // ids to a bucket
+  int32_t shift;        // 2^shift buckets
+  int64_t slots;        // buckets * rows
+
+  // ids in their sorted order
+  __device__ __forceinline__ int64_t slot(int64_t id) const {
+    return (id & ((1ll << shift) - 1)) * rows + (id >> shift);
+  }
+};
+
+// Consecutive rows [lo, lo + rows) of the table, and every 2^shift-th row: the
+// rows that come before a bucket's, and a row's number in it (at least `rows`:
+// it has none).
+struct Consecutive {
+  uint32_t lo;
+  __device__ __forceinline__ bool before(uint32_t id) const { return id < lo; }
+  __device__ __forceinline__ uint32_t row(uint32_t id) const { return id - lo; }
+};
+struct Strided {
+  uint32_t bucket, mask, shift, vocab;
+  __device__ __forceinline__ bool before(uint32_t id) const {
+    return (id & mask) < bucket && id < vocab;
+  }
+  __device__ __forceinline__ uint32_t row(uint32_t id) const {
+    return (id & mask) == bucket && id < vocab ? id >> shift : ~0u;
+  }
 };
 
 __device__ __forceinline__ int wave_scan(int x) {
@@ -60,43 +90,69 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-__global__ void __launch_bounds__(kSortThreads)
-    k_sort_tokens(ms_tokens_t ids, int64_t vocab, int64_t skip, int buckets, int rows_each,
-                  Sorted out, uint4* table, int64_t table_bytes) {
-  __shared__ int count[kSortWaves][kSortRows];
-  __shared__ int wave_sum[kSortWaves];
-  if (blockIdx.x >= static_cast<unsigned>(buckets)) {
-    const int64_t step = static_cast<int64_t>(gridDim.x - buckets) * kSortThreads;
-    int64_t i = static_cast<int64_t>(blockIdx.x - buckets) * kSortThreads + threadIdx.x;
-    const int64_t vectors = table_bytes / 16, rest = (table_bytes & 15) / 2;
-    if (i < rest) reinterpret_cast<uint16_t*>(table + vectors)[i] = 0;
-    for (; i < vectors; i += step) table[i] = uint4{0, 0, 0, 0};
-    return;
-  }
+// The tokens of a bucket of `rows` rows, stably sorted by a block of
+// kSortThreads: wave w counts and then places the w-th part of the list.
+// begin(r, p): row r's tokens begin at p of the whole sorted list (r = rows:
+// they end there); place(p, r, t): token t of row r belongs at p.
+// kWide: 8-byte ids.  kPlain: consecutive ids (`token` without its branches, so
+// that a group's loads stay in flight together).  A block goes through all
+// tokens, on one CU: what this costs is its instructions per token, so ids are
+// compared as 32-bit words.
+template <int kRows, int kSteps, bool kWide, bool kPlain, typename Rows, typename Begin,
+          typename Place>
+__device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Rows bucket, int rows,
+                                            int64_t skip, int (&count)[kSortWaves][kRows],
+                                            int (&wave_sum)[kSortWaves], Begin begin,
+                                            Place place) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * rows_each;
-  const int rows = static_cast<int>(vocab - lo < rows_each ? vocab - lo : rows_each);
-  for (int i = threadIdx.x; i < kSortWaves * kSortRows; i += kSortThreads) (&count[0][0])[i] = 0;
-  const int64_t part = ((ids.n + kSortThreads - 1) / kSortThreads) * kWave;
-  const int64_t first = wave * part, last = first + part < ids.n ? first + part : ids.n;
+  const int n = static_cast<int>(ids.n);
+  const int part = ((n + kSortThreads - 1) / kSortThreads) * kWave;
+  const int first = wave * part < n ? wave * part : n;
+  const int last = n - first < part ? n : first + part;
+  const uint32_t none = static_cast<uint32_t>(skip);
+
+  // as an unsigned word, 2^32 - 1 for what is no row of any table
+  auto one = [&](int t) -> uint32_t {
+    if (kPlain && kWide) {
+      const uint2 word = static_cast<const uint2*>(ids.data)[t];
+      return word.y ? ~0u : word.x;
+    }
+    if (kPlain) return static_cast<const uint32_t*>(ids.data)[t];
+    const int64_t x = token(ids, t);
+    return static_cast<uint64_t>(x) >> 31 ? ~0u : static_cast<uint32_t>(x);
+  };
+  auto load_ids = [&](int t0, uint32_t (&id)[kSteps]) {
+    if (last - t0 >= kSteps * kWave) {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) id[k] = one(t0 + lane + k * kWave);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int t = t0 + lane + k * kWave;
+        id[k] = one(t < last ? t : last - 1);
+        if (t >= last) id[k] = ~0u;
+      }
+    }
+    if (none != ~0u) {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+        if (id[k] == none) id[k] = ~0u;
+    }
+  };
+  uint32_t id[kSteps];
+  if (first < last) load_ids(first, id);
+  for (int i = threadIdx.x; i < kSortWaves * rows; i += kSortThreads)
+    count[i / rows][i % rows] = 0;
   __syncthreads();
 
-  // row of my bucket, -1: below it, -2: no row of mine or above
-  auto row_of = [&](int64_t t) {
-    if (t >= last) return -2;
-    const int64_t id = token(ids, t);
-    if (id < 0 || id >= lo + rows || id == skip) return -2;
-    return id < lo ? -1 : static_cast<int>(id - lo);
-  };
   int below = 0;
-  for (int64_t t0 = first; t0 < last; t0 += kWave * kSortSteps) {
-    int row[kSortSteps];
+  for (int t0 = first; t0 < last; t0 += kWave * kSteps) {
+    if (t0 != first) load_ids(t0, id);
 #pragma unroll
-    for (int k = 0; k < kSortSteps; ++k) row[k] = row_of(t0 + k * kWave + lane);
-#pragma unroll
-    for (int k = 0; k < kSortSteps; ++k) {
-      below += row[k] == -1;
-      if (row[k] >= 0) atomicAdd(&count[wave][row[k]], 1);
+    for (int k = 0; k < kSteps; ++k) {
+      below += bucket.before(id[k]);
+      const uint32_t r = bucket.row(id[k]);
+      if (r < static_cast<uint32_t>(rows)) atomicAdd(&count[wave][r], 1);
     }
   }
   for (int k = 32; k; k >>= 1) below += __shfl_xor(below, k);
@@ -117,38 +173,64 @@ __global__ void __launch_bounds__(kSortThreads)
   int at = base + upto - mine;
   for (int w = 0; w < wave; ++w) at += wave_sum[w];
   if (r < rows) {
-    out.start[lo + r] = at;
+    begin(r, at);
     for (int w = 0; w < kSortWaves; ++w) {
       const int c = count[w][r];
       count[w][r] = at;
       at += c;
     }
-    if (lo + r == vocab - 1) out.start[vocab] = at;
+    if (r == rows - 1) begin(rows, at);
   }
   __syncthreads();
 
-  for (int64_t t0 = first; t0 < last; t0 += kWave * kSortSteps) {
-    int row[kSortSteps];
+  for (int t0 = first; t0 < last; t0 += kWave * kSteps) {
+    if (part > kWave * kSteps) load_ids(t0, id);      // else they are still here
 #pragma unroll
-    for (int k = 0; k < kSortSteps; ++k) row[k] = row_of(t0 + k * kWave + lane);
-#pragma unroll
-    for (int k = 0; k < kSortSteps; ++k) {
-      uint64_t left = __ballot(row[k] >= 0);
+    for (int k = 0; k < kSteps; ++k) {
+      const uint32_t row = bucket.row(id[k]);
+      uint64_t left = __ballot(row < static_cast<uint32_t>(rows));
       while (left) {                               // once per different id
         const int lead = __ffsll(static_cast<unsigned long long>(left)) - 1;
-        const int which = read_lane(row[k], lead);
-        const uint64_t same = __ballot(row[k] == which);
+        const uint32_t which = read_lane(static_cast<int>(row), lead);
+        const uint64_t same = __ballot(row == which);
         const int to = count[wave][which];
-        if (row[k] == which) {
-          const int p = to + __popcll(same & ((1ull << lane) - 1));
-          out.id[p] = static_cast<int32_t>(lo + which);
-          out.position[p] = static_cast<int32_t>(t0 + k * kWave + lane);
-        }
+        if (row == which)
+          place(to + __popcll(same & ((1ull << lane) - 1)), static_cast<int>(which),
+                t0 + k * kWave + lane);
         if (lane == lead) count[wave][which] = to + __popcll(same);
         left &= ~same;
       }
     }
   }
+}
+
+template <bool kWide, bool kPlain>
+__global__ void __launch_bounds__(kSortThreads)
+    k_sort_tokens(ms_tokens_t ids, int64_t vocab, int64_t skip, int buckets, Sorted out,
+                  uint4* table, int64_t clear_bytes) {
+  __shared__ int count[kSortWaves][kSortRows];
+  __shared__ int wave_sum[kSortWaves];
+  if (blockIdx.x >= static_cast<unsigned>(buckets)) {
+    const int64_t step = static_cast<int64_t>(gridDim.x - buckets) * kSortThreads;
+    int64_t i = static_cast<int64_t>(blockIdx.x - buckets) * kSortThreads + threadIdx.x;
+    const int64_t vectors = clear_bytes / 16, rest = (clear_bytes & 15) / 2;
+    if (i < rest) reinterpret_cast<uint16_t*>(table + vectors)[i] = 0;
+    for (; i < vectors; i += step) table[i] = uint4{0, 0, 0, 0};
+    return;
+  }
+  const uint32_t b = blockIdx.x;
+  const Strided bucket = {b, static_cast<uint32_t>(buckets - 1),
+                          static_cast<uint32_t>(out.shift), static_cast<uint32_t>(vocab)};
+  const int64_t slot = static_cast<int64_t>(b) * out.rows;
+  sort_bucket<kSortRows, kSortSteps, kWide, kPlain>(
+      ids, bucket, out.rows, skip, count, wave_sum,
+      [&](int r, int p) {
+        if (r < out.rows || b == static_cast<uint32_t>(buckets) - 1) out.start[slot + r] = p;
+      },
+      [&](int p, int r, int t) {
+        out.id[p] = static_cast<int32_t>(static_cast<uint32_t>(r) << out.shift | b);
+        out.position[p] = t;
+      });
 }
 
 // My N values of a row; `whole`: none of the wave's reach past the width.
@@ -174,90 +256,327 @@ __device__ __forceinline__ void store_slice(T* row, int64_t c, int64_t width, bo
 }
 
 constexpr int kSumThreads = 256, kSumWaves = kSumThreads / kWave;
+constexpr int kSpan = 16;                 // sorted positions to a block
 constexpr int kSumDepth = 8;              // rows in flight per wave
+// An id of up to kLight tokens is added by one wave.  A wave looks at 64
+// positions from kLead before its span on, which is enough to tell for every
+// id in the span whether it has more.
+constexpr int kLight = 20, kLead = 24;
+static_assert(kLead >= kLight && kLead + kSpan + kLight <= 63, "");
+constexpr int kClearRows = 32, kClearBytes = 16384;     // of the table per clearing block
 
-template <typename T, int N>
-__global__ void __launch_bounds__(kSumThreads)
-    k_sum_spans(ms_rows_t grad, int64_t vocab, float scale, int span, int slices, Sorted in,
-                T* __restrict__ table) {
-  const int lane = threadIdx.x & 63;
-  const int64_t job = blockIdx.x * static_cast<int64_t>(kSumWaves) + (threadIdx.x >> 6);
-  const int64_t s = job / slices, width = grad.width;
-  const int64_t c = ((job - s * slices) * kWave + lane) * N;
-  const int total = in.start[vocab];
-  const int64_t first = s * span;
-  if (first >= total) return;
-  const int n = static_cast<int>(total - first < span ? total - first : span);
-  const int mine = lane < n ? lane : n - 1;
-  const int id = in.id[first + mine];
-  const int64_t offset = row_start(grad, in.position[first + mine]);
-  const int before = first > 0 ? in.id[first - 1] : -1;
-  const int behind = first + n < total ? in.id[first + n] : -1;
-  const int next = __shfl_down(id, 1);
-  const uint64_t ends = __ballot(lane < n && (lane == n - 1 || next != id));
-  const T* g = static_cast<const T*>(grad.data);
+// fp32 sums of N columns in each of G chunks of kWave * N, from column c on.
+template <typename T, int N, int G>
+struct Tile {
+  float sum[G][N];
 
-  const bool whole = __all(c + N <= width);
-  float sum[N];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int k = 0; k < N; ++k) sum[k] = 0.f;
-  bool open = read_lane(id, 0) == before;
-  for (int i0 = 0; i0 < n; i0 += kSumDepth) {
-    Pack<T, N> x[kSumDepth];                        // past the last: the last again, not added
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int k = 0; k < N; ++k) sum[j][k] = 0.f;
+  }
+  // rows q0 .. q1 - 1, at most kSumDepth of them; row(q): its first element
+  template <typename Row>
+  __device__ __forceinline__ void add(int q0, int q1, int64_t c, int64_t width, Row row) {
+    Pack<T, N> x[kSumDepth][G];
 #pragma unroll
     for (int u = 0; u < kSumDepth; ++u)
-      x[u] = load_slice<N>(g + read_lane(offset, i0 + u < n ? i0 + u : n - 1), c, width, whole);
+      if (q0 + u < q1) {
+        const T* src = row(q0 + u);
 #pragma unroll
-    for (int u = 0; u < kSumDepth; ++u) {
-      const int i = i0 + u;
-      if (i >= n) break;
-#pragma unroll
-      for (int k = 0; k < N; ++k) sum[k] += widen(x[u].v[k]);
-      if (!(ends >> i & 1)) continue;
-      const int row = read_lane(id, i);
-      if (open || (i == n - 1 && row == behind)) {
-        Pack<float, N> y;
-#pragma unroll
-        for (int k = 0; k < N; ++k) y.v[k] = sum[k];
-        store_slice<N>(in.partial + (s * 2 + (open ? 0 : 1)) * width, c, width, whole, y);
-      } else {
-        Pack<T, N> y;
-#pragma unroll
-        for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[k] * scale);
-        store_slice<N>(table + row * width, c, width, whole, y);
+        for (int j = 0; j < G; ++j) {
+          const int64_t at = c + j * kWave * N;
+          x[u][j] = load_slice<N>(src, at, width, at + N <= width);
+        }
       }
-      open = false;
 #pragma unroll
-      for (int k = 0; k < N; ++k) sum[k] = 0.f;
+    for (int u = 0; u < kSumDepth; ++u)
+      if (q0 + u < q1)
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+#pragma unroll
+          for (int k = 0; k < N; ++k) sum[j][k] += widen(x[u][j].v[k]);
+  }
+  __device__ __forceinline__ void write(T* row, int64_t c, int64_t width, float scale) const {
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int64_t at = c + j * kWave * N;
+      Pack<T, N> y;
+#pragma unroll
+      for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[j][k] * scale);
+      store_slice<N>(row, at, width, at + N <= width, y);
+    }
+  }
+  __device__ __forceinline__ void leave(float* row, int64_t c, int64_t width) const {
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int k0 = 0; k0 < N; k0 += 4) {
+        const int64_t at = c + j * kWave * N + k0;
+        Pack<float, 4> y;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y.v[k] = sum[j][k0 + k];
+        store_slice<4>(row, at, width, at + 4 <= width, y);
+      }
+  }
+};
+
+// Blocks below sum_blocks: a span and kWave * N * G columns; wave w adds the
+// span's w-th, (w + kSumWaves)-th .. run of equal ids.  The other blocks: rows
+// from clear_from on that have no tokens.  16384 x 768 bf16 into 12000 rows,
+// uniform ids or falling off as 1 / rank: 15.5 and 16.1 us (39 and 32 MB moved).
+// A wave to a span that keeps its 16 rows in registers, the loop over them
+// unrolled: 16.5 and more; the rows set down in LDS for a short loop: 17.3
+// and 23.
+template <typename T, int N, int G>
+__global__ void __launch_bounds__(kSumThreads)
+    k_sum_spans(ms_rows_t grad, int64_t vocab, float scale, int slices, unsigned sum_blocks,
+                int64_t clear_from, int clear_rows, Sorted in, T* __restrict__ table) {
+  const int lane = threadIdx.x & 63;
+  const int64_t width = grad.width;
+  if (blockIdx.x >= sum_blocks) {
+    // consecutive vectors of `clear_rows` rows to the block's threads
+    const int64_t r0 = clear_from + static_cast<int64_t>(blockIdx.x - sum_blocks) * clear_rows;
+    const int rows = static_cast<int>(vocab - r0 < clear_rows ? vocab - r0 : clear_rows);
+    const int64_t slot = in.slot(r0 + (lane < rows ? lane : rows - 1));
+    const uint64_t empty = __ballot(lane < rows && in.start[slot] == in.start[slot + 1]);
+    constexpr int kVec = 16 / sizeof(T);
+    Pack<T, kVec> zero;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) zero.v[k] = static_cast<T>(0.f);
+    const uint32_t vectors = static_cast<uint32_t>((width + kVec - 1) / kVec);
+    for (uint32_t v = threadIdx.x; v < vectors * rows; v += kSumThreads) {
+      const uint32_t k = rows == 1 ? 0 : v / vectors;
+      const int64_t c = static_cast<int64_t>(v - k * vectors) * kVec;
+      if (empty >> k & 1) store_slice<kVec>(table + (r0 + k) * width, c, width, c + kVec <= width, zero);
+    }
+    return;
+  }
+  const int64_t s = blockIdx.x / slices, first = s * kSpan;
+  const int64_t c =
+      static_cast<int64_t>(blockIdx.x - s * slices) * (kWave * N * G) + lane * N;
+  // lane q has position first - kLead + q of the sorted list.  The lists beyond
+  // `total` hold nothing; they are read with it, not after it.
+  const int64_t at = first + lane - kLead;
+  const int64_t in_list = at < 0 ? 0 : at < grad.n ? at : grad.n - 1;
+  const int total = in.start[in.slots];
+  int id = in.id[in_list];
+  int position = in.position[in_list];
+  if (first >= total) return;
+  if (at < 0 || at >= total) id = -1, position = 0;
+  const int64_t offset = row_start(grad, position);
+  const int next = __shfl_down(id, 1);
+  // bit q: lane q's id ends there (lane 63: not known, and not needed)
+  const uint64_t ends = __ballot(lane < 63 && next != id);
+  const int n = static_cast<int>(total - first < kSpan ? total - first : kSpan);
+  const int last = kLead + n - 1;
+  const T* g = static_cast<const T*>(grad.data);
+  int run = 0;
+  for (int from = kLead; from <= last; ++run) {
+    // the run of equal ids that position `from` is in: all of it is
+    // [begin, end], begin -1: before lane 0, end 64: behind lane 62
+    const uint64_t before = ends & ((1ull << from) - 1), behind = ends >> from;
+    const int begin = before ? 64 - __clzll(before) : -1;
+    const int end = behind ? from + __ffsll(static_cast<unsigned long long>(behind)) - 1 : 64;
+    const bool light = begin >= 0 && end < 64 && end - begin < kLight;
+    const int to = light || end <= last ? end : last;
+    const bool mine = (run & (kSumWaves - 1)) == static_cast<int>(threadIdx.x >> 6) &&
+                      !(light && begin < kLead);          // else an earlier span's
+    if (mine) {
+      Tile<T, N, G> tile;
+      tile.clear();
+      for (int q = from; q <= to; q += kSumDepth)
+        tile.add(q, to + 1, c, width, [&](int i) { return g + read_lane(offset, i); });
+      if (light)
+        tile.write(table + read_lane(id, from) * width, c, width, scale);
+      else
+        tile.leave(in.partial + (s * 2 + (begin >= kLead)) * width, c, width);
+    }
+    from = to + 1;
+  }
+}
+
+constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / kWave;
+constexpr int kJoinFew = 16;              // partial sums that one wave adds by itself
+constexpr int kJoinDepth = 8;             // partial sums in flight per wave
+
+// Every block looks at all spans, kJoinThreads at a time, for those that an id
+// of many tokens begins in.  Such a span and a slice of the width make a job:
+// a wave's (4 columns to a lane) where there are few partial sums, the block's
+// (1 column to a lane) where there are many; then its waves take a part of them
+// each and are added in their order.  Jobs go round the waves and blocks.
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads)
+    k_join_spans(int64_t n, int64_t width, float scale, Sorted in, T* __restrict__ table) {
+  struct Found {
+    int span, id, parts;
+  };
+  __shared__ Found found[2][kJoinThreads];
+  __shared__ int found_by[2][kJoinWaves];
+  __shared__ float part[kJoinWaves][kWave];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int total = in.start[in.slots];
+  // partial sums [from, to) of the id that begins in span s
+  auto add_parts = [&](auto& sum, int64_t s, int from, int to, int64_t c, bool whole) {
+    constexpr int N = sizeof(sum) / sizeof(float);
+    for (int k0 = from; k0 < to; k0 += kJoinDepth) {
+      Pack<float, N> x[kJoinDepth];
+#pragma unroll
+      for (int u = 0; u < kJoinDepth; ++u) {
+        const int k = k0 + u < to ? k0 + u : to - 1;
+        x[u] = load_slice<N>(in.partial + ((s + k) * 2 + (k == 0)) * width, c, width, whole);
+      }
+#pragma unroll
+      for (int u = 0; u < kJoinDepth; ++u)
+        if (k0 + u < to)
+#pragma unroll
+          for (int k = 0; k < N; ++k) sum[k] += x[u].v[k];
+    }
+  };
+  for (int64_t s0 = 0; (s0 + 1) * kSpan < n; s0 += kJoinThreads) {
+    const int64_t end = (s0 + threadIdx.x + 1) * kSpan, at = end < n ? end : n - 1;
+    const int a = in.id[at - 1], b = in.id[at];               // n > kSpan here
+    int kind = -1, parts = 0;
+    if (end < total && a == b) {
+      const int64_t slot = in.slot(a);
+      const int from = in.start[slot], to = in.start[slot + 1];
+      parts = (to - 1) / kSpan - static_cast<int>(end / kSpan - 1) + 1;
+      if (from >= end - kSpan && to - from > kLight) kind = parts > kJoinFew;
+    }
+    __syncthreads();
+    for (int u = 0; u < 2; ++u) {
+      const uint64_t hits = __ballot(kind == u);
+      if (lane == 0) found_by[u][wave] = __popcll(hits);
+    }
+    __syncthreads();
+    int all[2] = {0, 0};
+    for (int u = 0; u < 2; ++u) {
+      const uint64_t hits = __ballot(kind == u);
+      int to = __popcll(hits & ((1ull << lane) - 1));
+      for (int w = 0; w < kJoinWaves; ++w) {
+        if (w < wave) to += found_by[u][w];
+        all[u] += found_by[u][w];
+      }
+      if (kind == u) found[u][to] = Found{static_cast<int>(s0 + threadIdx.x), a, parts};
+    }
+    __syncthreads();
+
+    const int64_t lots = (width + kWave - 1) / kWave;
+    for (int64_t j = blockIdx.x; j < all[1] * lots; j += gridDim.x) {
+      const Found f = found[1][j / lots];
+      const int64_t s = f.span, id = f.id, c = (j % lots) * kWave + lane;
+      const int each = (f.parts + kJoinWaves - 1) / kJoinWaves;
+      const int from = wave * each, to = from + each < f.parts ? from + each : f.parts;
+      float sum[1] = {0.f};
+      add_parts(sum, s, from, to, c, __all(c < width));
+      part[wave][lane] = sum[0];
+      __syncthreads();
+      if (wave == 0 && c < width) {
+        for (int w = 1; w < kJoinWaves; ++w) sum[0] += part[w][lane];
+        table[id * width + c] = narrow<T>(sum[0] * scale);
+      }
+      __syncthreads();
+    }
+    // from the last block on, which has the fewest of the others
+    const int64_t few = (width + 4 * kWave - 1) / (4 * kWave);
+    const int64_t waves = static_cast<int64_t>(gridDim.x) * kJoinWaves;
+    for (int64_t j = static_cast<int64_t>(wave) * gridDim.x + gridDim.x - 1 - blockIdx.x;
+         j < all[0] * few; j += waves) {
+      const Found f = found[0][j / few];
+      const int64_t s = f.span, id = f.id, c = (j % few) * (4 * kWave) + lane * 4;
+      const bool whole = __all(c + 4 <= width);
+      float sum[4] = {};
+      add_parts(sum, s, 0, f.parts, c, whole);
+      Pack<T, 4> y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y.v[k] = narrow<T>(sum[k] * scale);
+      store_slice<4>(table + id * width, c, width, whole, y);
     }
   }
 }
 
-// One block per span that an id's tokens leave to the right, having begun in
-// it, and per kWave values of the width: its waves take a part of the partial
-// sums each.
-template <typename T>
-__global__ void __launch_bounds__(kSumThreads)
-    k_join_spans(int64_t width, int64_t vocab, float scale, int span, Sorted in,
-                 T* __restrict__ table) {
-  __shared__ float part[kSumWaves][kWave];
-  const int64_t s = blockIdx.x, end = (s + 1) * span;
-  if (end >= in.start[vocab]) return;
-  const int id = in.id[end - 1];
-  if (in.id[end] != id || in.start[id] < s * span) return;
+// Few tokens: every block sorts all of them for its rows of the table, in LDS.
+// A wave takes a row and a slice of the width at a time; rows of more than
+// kLight tokens are split over the waves, whose sums are added in their order.
+constexpr int kSmallTokens = 2048, kSmallRows = 64;
+
+template <typename T, int N, bool kWide, bool kPlain>
+__global__ void __launch_bounds__(kSortThreads)
+    k_grad_small(ms_tokens_t ids, ms_rows_t grad, int64_t vocab, int64_t skip, float scale,
+                 int rows_each, T* __restrict__ table) {
+  __shared__ int count[kSortWaves][kSmallRows];
+  __shared__ int wave_sum[kSortWaves];
+  __shared__ int start[kSmallRows + 1];
+  __shared__ uint16_t position[kSmallTokens];
+  __shared__ float part[kSortWaves][kWave * N];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = blockIdx.y * static_cast<int64_t>(kWave) + lane;
-  const int64_t parts = (in.start[id + 1] - 1) / span - s + 1;
-  const int64_t each = (parts + kSumWaves - 1) / kSumWaves;
-  float sum = 0.f;
-  if (c < width)
-    for (int64_t k = wave * each; k < (wave + 1) * each && k < parts; ++k)
-      sum += in.partial[((s + k) * 2 + (k == 0)) * width + c];
-  part[wave][lane] = sum;
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * rows_each, width = grad.width;
+  const int rows = static_cast<int>(vocab - lo < rows_each ? vocab - lo : rows_each);
+  sort_bucket<kSmallRows, kSmallTokens / kSortThreads, kWide, kPlain>(
+      ids, Consecutive{static_cast<uint32_t>(lo)}, rows, skip, count, wave_sum, [&](int r, int p) { start[r] = p; },
+      [&](int p, int, int t) { position[p] = static_cast<uint16_t>(t); });
   __syncthreads();
-  if (wave == 0 && c < width) {
-    for (int w = 1; w < kSumWaves; ++w) sum += part[w][lane];
-    table[id * width + c] = narrow<T>(sum * scale);
+
+  const T* g = static_cast<const T*>(grad.data);
+  constexpr int kDepth = 8;
+  auto add_rows = [&](int from, int to, int64_t c, bool whole, float (&sum)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) sum[k] = 0.f;
+    for (int p0 = from; p0 < to; p0 += kDepth) {
+      Pack<T, N> x[kDepth];
+#pragma unroll
+      for (int u = 0; u < kDepth; ++u) {
+        const int t = __builtin_amdgcn_readfirstlane(position[p0 + u < to ? p0 + u : to - 1]);
+        x[u] = load_slice<N>(g + row_start(grad, t), c, width, whole);
+      }
+#pragma unroll
+      for (int u = 0; u < kDepth; ++u)
+        if (p0 + u < to)
+#pragma unroll
+          for (int k = 0; k < N; ++k) sum[k] += widen(x[u].v[k]);
+    }
+  };
+  const int slices = static_cast<int>((width + kWave * N - 1) / (kWave * N));
+  bool heavy = false;
+  for (int item = wave; item < rows * slices; item += kSortWaves) {
+    const int r = item / slices;
+    const int64_t c = (static_cast<int64_t>(item - r * slices) * kWave + lane) * N;
+    const int from = start[r], to = start[r + 1];
+    if (to - from > kLight) {
+      heavy = true;
+      continue;
+    }
+    const bool whole = __all(c + N <= width);
+    float sum[N];
+    add_rows(from, to, c, whole, sum);
+    Pack<T, N> y;
+#pragma unroll
+    for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[k] * scale);
+    if (from == to)                                 // +0, whatever the scale
+      for (int k = 0; k < N; ++k) y.v[k] = static_cast<T>(0.f);
+    store_slice<N>(table + (lo + r) * width, c, width, whole, y);
+  }
+  if (!__syncthreads_or(heavy)) return;
+  for (int r = 0; r < rows; ++r) {
+    const int from = start[r], each = (start[r + 1] - from + kSortWaves - 1) / kSortWaves;
+    if (start[r + 1] - from <= kLight) continue;
+    for (int slice = 0; slice < slices; ++slice) {
+      const int64_t c0 = static_cast<int64_t>(slice) * kWave * N;
+      const int64_t c = c0 + lane * N;
+      const int a = from + wave * each, b = a + each < start[r + 1] ? a + each : start[r + 1];
+      float sum[N];
+      add_rows(a, b, c, __all(c + N <= width), sum);
+#pragma unroll
+      for (int k = 0; k < N; ++k) part[wave][lane * N + k] = sum[k];
+      __syncthreads();
+      for (int k = threadIdx.x; k < kWave * N; k += kSortThreads) {
+        float y = part[0][k];
+        for (int w = 1; w < kSortWaves; ++w) y += part[w][k];
+        if (c0 + k < width) table[(lo + r) * width + c0 + k] = narrow<T>(y * scale);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -266,64 +585,119 @@ int64_t align16(int64_t bytes) { return (bytes + 15) & ~15ll; }
 // How the work is cut; a function of the sizes alone, as the order of the sums
 // follows from it.
 struct GradShape {
-  int buckets, rows_each, vector, slices, span;
+  int shift, rows;
   int64_t spans, start_bytes, list_bytes, partial_bytes;
 };
 
 GradShape shape_of(int64_t n, int64_t vocab, int64_t width) {
   GradShape g;
-  const int64_t wanted = std::max((vocab + kSortRows - 1) / kSortRows,
-                                  std::min<int64_t>((vocab + 7) / 8, 64));
-  g.rows_each = static_cast<int>((vocab + wanted - 1) / wanted);
-  g.buckets = static_cast<int>((vocab + g.rows_each - 1) / g.rows_each);
-  g.vector = width >= 2 * kWave ? 4 : width >= kWave ? 2 : 1;
-  g.slices = static_cast<int>((width + g.vector * kWave - 1) / (g.vector * kWave));
-  g.span = n * g.slices >= (1 << 18) ? 32 : 16;
-  g.spans = (n + g.span - 1) / g.span;
-  g.start_bytes = align16((vocab + 1) * 4);
+  // 256 buckets, a CU each: as many as go round beside each other, few ids to
+  // each.  Small vocabularies: 8 ids; large ones: what fits the LDS.
+  g.shift = 0;
+  while (g.shift < 8 ? vocab >> g.shift > 8 : vocab > static_cast<int64_t>(kSortRows) << g.shift)
+    ++g.shift;
+  g.rows = static_cast<int>(((vocab - 1) >> g.shift) + 1);
+  g.spans = (n + kSpan - 1) / kSpan;
+  g.start_bytes = align16(((static_cast<int64_t>(g.rows) << g.shift) + 1) * 4);
   g.list_bytes = align16(n * 4);
   g.partial_bytes = align16(g.spans * 2 * width * 4);
   return g;
 }
 
+// What the sort's launch clears while it sorts; the sort takes some 8 us.
+constexpr int64_t kClearBesideSort = 48 << 20;
+
+template <typename T, int N, int G>
+int sum_as(const ms_rows_t& grad, int64_t vocab, float scale, int64_t clear_from,
+           const GradShape& g, const Sorted& sorted, T* table, hipStream_t s) {
+  const int slices = static_cast<int>((grad.width + kWave * N * G - 1) / (kWave * N * G));
+  const int64_t sums = g.spans * slices;
+  const int64_t row_bytes = grad.width * static_cast<int64_t>(sizeof(T));
+  const int clear_rows = static_cast<int>(
+      std::min<int64_t>(kClearRows, std::max<int64_t>(kClearBytes / row_bytes, 1)));
+  const int64_t clears = (vocab - clear_from + clear_rows - 1) / clear_rows;
+  if (sums + clears > INT32_MAX) return MS_OPS_EINVAL;
+  if (sums + clears == 0) return MS_OPS_OK;
+  k_sum_spans<T, N, G><<<static_cast<unsigned>(sums + clears), kSumThreads, 0, s>>>(
+      grad, vocab, scale, slices, static_cast<unsigned>(sums), clear_from, clear_rows, sorted,
+      table);
+  return launched();
+}
+
+// One launch where three would mostly wait for each other: up to kSmallTokens
+// tokens and kSmallTable bytes of table.
+constexpr int64_t kSmallTable = 32 << 20;
+
+bool is_small(int64_t n, int64_t table_bytes) {
+  return n <= kSmallTokens && table_bytes <= kSmallTable;
+}
+
+template <typename T, int N>
+int small_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float scale,
+             int64_t skip, T* table, hipStream_t s) {
+  // some 64 KB of the table to a block, but a block for each CU if it has the rows
+  const int64_t row_bytes = grad.width * static_cast<int64_t>(sizeof(T));
+  const int64_t most = std::min<int64_t>(kSmallRows, std::max<int64_t>(65536 / row_bytes, 1));
+  const int rows_each = static_cast<int>(std::min(most, (vocab + 255) / 256));
+  const unsigned blocks = static_cast<unsigned>((vocab + rows_each - 1) / rows_each);
+  const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
+#define SMALL(W, P)                                                                          \
+  k_grad_small<T, N, W, P><<<blocks, kSortThreads, 0, s>>>(ids, grad, vocab, skip, scale, \
+                                                           rows_each, table)
+  if (wide && plain) SMALL(true, true);
+  else if (wide) SMALL(true, false);
+  else if (plain) SMALL(false, true);
+  else SMALL(false, false);
+#undef SMALL
+  return launched();
+}
+
 template <typename T>
 int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float scale,
             int64_t skip, void* dtable, void* workspace, hipStream_t s) {
-  const GradShape g = shape_of(ids.n, vocab, grad.width);
+  const int64_t width = grad.width;
+  const int64_t row_bytes = width * static_cast<int64_t>(sizeof(T));
+  T* table = static_cast<T*>(dtable);
+  if (is_small(ids.n, vocab * row_bytes))
+    return width >= 2 * kWave ? small_as<T, 4>(ids, grad, vocab, scale, skip, table, s)
+                              : small_as<T, 1>(ids, grad, vocab, scale, skip, table, s);
+  const GradShape g = shape_of(ids.n, vocab, width);
   char* w = static_cast<char*>(workspace);
   Sorted sorted;
   sorted.start = reinterpret_cast<int32_t*>(w);
   sorted.id = reinterpret_cast<int32_t*>(w + g.start_bytes);
   sorted.position = reinterpret_cast<int32_t*>(w + g.start_bytes + g.list_bytes);
   sorted.partial = reinterpret_cast<float*>(w + g.start_bytes + 2 * g.list_bytes);
-  T* table = static_cast<T*>(dtable);
-  const int64_t bytes = vocab * grad.width * static_cast<int64_t>(sizeof(T));
-  const int64_t clear =
-      std::min<int64_t>((bytes / 16 + kSortThreads) / kSortThreads, 2048);
-  k_sort_tokens<<<static_cast<unsigned>(g.buckets + clear), kSortThreads, 0, s>>>(
-      ids, vocab, skip, g.buckets, g.rows_each, sorted, static_cast<uint4*>(dtable), bytes);
+  sorted.rows = g.rows;
+  sorted.shift = g.shift;
+  sorted.slots = static_cast<int64_t>(g.rows) << g.shift;
+  const int buckets = 1 << g.shift;
+  const int64_t clear_rows = std::min<int64_t>(vocab, kClearBesideSort / row_bytes);
+  const int64_t clear_bytes = clear_rows * row_bytes;
+  const int64_t clear = (clear_bytes / 16 + kSortThreads) / kSortThreads;
+  const unsigned blocks = static_cast<unsigned>(buckets + std::min<int64_t>(clear, 1024));
+  const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
+#define SORT(W, P)                                                                     \
+  k_sort_tokens<W, P><<<blocks, kSortThreads, 0, s>>>(ids, vocab, skip, buckets, sorted, \
+                                                      static_cast<uint4*>(dtable), clear_bytes)
+  if (wide && plain) SORT(true, true);
+  else if (wide) SORT(true, false);
+  else if (plain) SORT(false, true);
+  else SORT(false, false);
+#undef SORT
   if (int rc = launched()) return rc;
-  if (ids.n == 0) return MS_OPS_OK;
-  const unsigned blocks =
-      static_cast<unsigned>((g.spans * g.slices + kSumWaves - 1) / kSumWaves);
-  switch (g.vector) {
-    case 4:
-      k_sum_spans<T, 4><<<blocks, kSumThreads, 0, s>>>(grad, vocab, scale, g.span, g.slices,
-                                                       sorted, table);
-      break;
-    case 2:
-      k_sum_spans<T, 2><<<blocks, kSumThreads, 0, s>>>(grad, vocab, scale, g.span, g.slices,
-                                                       sorted, table);
-      break;
-    default:
-      k_sum_spans<T, 1><<<blocks, kSumThreads, 0, s>>>(grad, vocab, scale, g.span, g.slices,
-                                                       sorted, table);
-  }
-  if (int rc = launched()) return rc;
-  if (g.spans > 1) {
-    const dim3 grid(static_cast<unsigned>(g.spans),
-                    static_cast<unsigned>((grad.width + kWave - 1) / kWave));
-    k_join_spans<T><<<grid, kSumThreads, 0, s>>>(grad.width, vocab, scale, g.span, sorted, table);
+  // 512 columns to a wave (256 of a narrow fp32 table), 16 bytes to a lane
+  constexpr int kVec = 16 / sizeof(T);
+  const int rc =
+      sizeof(T) == 4 && width > kVec * kWave
+          ? sum_as<T, kVec, (sizeof(T) == 4 ? 2 : 1)>(grad, vocab, scale, clear_rows, g, sorted,
+                                                      table, s)
+          : sum_as<T, kVec, 1>(grad, vocab, scale, clear_rows, g, sorted, table, s);
+  if (rc) return rc;
+  if (ids.n > kLight) {
+    const int64_t lots = (width + kWave - 1) / kWave;
+    k_join_spans<T><<<static_cast<unsigned>(std::min<int64_t>(g.spans * lots, 512)), kJoinThreads,
+                      0, s>>>(ids.n, width, scale, sorted, table);
   }
   return launched();
 }

@@ -107,6 +107,23 @@ def test_grad_of_many_tokens(kind):
     check_grad(_rand((70_000, 72), "bf16", 9, 0.1), _ids(70_000, 5000, 10, kind), 5000)
 
 
+@pytest.mark.parametrize("rows,width,n", [(50257, 768, 100), (128256, 1024, 3000), (9001, 515, 2500),
+                                          (400, 64, 30), (3, 40000, 2100), (70000, 1, 5000)])
+def test_grad_writes_every_row(rows, width, n):
+    for dtype in ("bf16", "fp32"):
+        g, ids = _rand((n, width), dtype, 27), _ids(n, rows, 28)
+        dirty = torch.full((rows, width), float("nan"), dtype=g.dtype, device=DEV)
+        at = dirty.data_ptr()
+        del dirty                                 # the allocator hands it out again
+        got = ms.ops.embedding_grad(g, ids, rows)
+        assert got.data_ptr() == at
+        seen = torch.zeros(rows, dtype=torch.bool, device=DEV)
+        seen[ids] = True
+        assert not bool(got[~seen].any())
+        want = torch.zeros(rows, width, device=DEV).index_add_(0, ids, g.float())
+        assert torch.allclose(got.float(), want, rtol=0.01, atol=0.1)
+
+
 def test_grad_of_no_tokens_is_zeros():
     got = ms.ops.embedding_grad(torch.empty(0, 48, device=DEV),
                                 torch.empty(0, dtype=torch.int64, device=DEV), 100)
