@@ -1,5 +1,14 @@
 // logprobs.hip — log probabilities of given tokens, entropy, the most likely
 // alternatives, and the gradient of the logits (gfx950).
+//
+//   lse = log sum exp x,  logprob = x_target - lse,  entropy = lse - sum p x
+//   dx  = g (1[j = target] - p) - h p (log p + entropy)
+//
+// One read of the logits forward, one read and one write backward: both are
+// bound by memory, the forward with 4 to 6 instructions and one exponential per
+// value not far from its arithmetic.
+
+#include <algorithm>
 
 #include "ops_common.h"
 
@@ -7,15 +16,10 @@ namespace {
 
 using namespace ops;
 
-// exp x = 2^(x L); the same rounded L everywhere, and its own inverse, so
-// that what L is off by only rescales the logits by 1 + 1.3e-8.
+// exp x = 2^(x L), with the same rounded L everywhere: what it is off by only
+// rescales the logits by 1 + 1.3e-8.
 constexpr float kLog2e = 1.44269504f;
 constexpr float kLn2 = 0.69314718f;
-
-// Rows whose maximum (or lse) is beyond this are computed from x - max, and
-// their gradient finds max and sum again: an fp32 lse no longer tells them
-// apart from their maximum (a row masked with the type's lowest value).
-constexpr float kFar = 1024.f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
@@ -31,206 +35,615 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
-// Over the block, the result in every thread; `slot`: one float per wave.
-template <int W, typename F>
-__device__ __forceinline__ float block_join(float x, float* slot, F join) {
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
-  __syncthreads();
-  float r = slot[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) r = join(r, slot[w]);
-  return r;
-}
-
 // Falling value, then rising index: a 64-bit key that is larger for what
-// comes first.  NaN is above +inf; -0 equals +0.
-constexpr uint32_t kNanKey = 0xFFFFFFF0u;      // with any index below all ones
-__device__ __forceinline__ uint32_t order_key(float x) {
-  if (x != x) return kNanKey;
+// comes first, never 0.  NaN is above +inf; -0 equals +0.
+typedef uint64_t Key;
+constexpr uint32_t kNanKey = 0xFFFFFFF0u;
+__device__ __forceinline__ Key key_of(float x, int index) {
   const uint32_t b = __float_as_uint(x + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const uint32_t order = x != x ? kNanKey : b & 0x80000000u ? ~b : b | 0x80000000u;
+  return static_cast<Key>(order) << 32 | ~static_cast<uint32_t>(index);
 }
-__device__ __forceinline__ float key_value(uint32_t k) {
+__device__ __forceinline__ float value_of(Key key) {
+  const uint32_t k = static_cast<uint32_t>(key >> 32);
   if (k == kNanKey) return quiet_nan();
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
+__device__ __forceinline__ int index_of(Key key) {
+  return static_cast<int>(~static_cast<uint32_t>(key));
+}
 
-struct RowStats {
-  float lse, logprob, entropy;
+// Over the values with y = x L - m2: s = sum 2^y, t = sum 2^y y.  m2 is a whole
+// number near L max x (0 for no values or only -inf: then s is 0), so that
+// lse = (m2 + log2 s) / L keeps what x L - m2 rounds.
+struct Sums {
+  float m2, s, t;
 };
 
-// Sums of the row over y = x L - m2 (m2 a whole number near max L, or far
-// rows: y = (x - max) L): s = sum 2^y, t = sum 2^y y.
-__device__ __forceinline__ RowStats finish(float most, float s, float t, float given, bool good) {
-  RowStats r;
-  const bool far = !(fabsf(most) <= kFar);
-  const float ls = log2_fast(s);
-  const bool empty = most == -INFINITY && s == 0.f;
-  if (empty) {
-    r.lse = -INFINITY;
-    r.logprob = -INFINITY;
-    r.entropy = 0.f;
-  } else if (far && most != -INFINITY) {
-    r.lse = most + ls * kLn2;
-    r.logprob = (given - most) - ls * kLn2;
-    r.entropy = (ls - t / s) * kLn2;
-  } else {
-    const float m2 = most == -INFINITY ? 0.f : rintf(most * kLog2e);
-    r.lse = (m2 + ls) * kLn2;
-    // given - max is (nearly) exact; what m2 rounded off comes back with log s
-    const float base = most == -INFINITY ? 0.f : most;
-    r.logprob = (given - base) + (fmaf(base, kLog2e, -m2) - ls) * kLn2;
-    r.entropy = (ls - t / s) * kLn2;
-  }
-  if (!good) r.logprob = quiet_nan();
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+  const float m2 = a.s == 0.f ? b.m2 : b.s == 0.f ? a.m2 : fmaxf(a.m2, b.m2);
+  const float da = a.m2 - m2, db = b.m2 - m2;
+  const float ka = a.s == 0.f ? 0.f : exp2_fast(da), kb = b.s == 0.f ? 0.f : exp2_fast(db);
+  Sums r;
+  r.m2 = m2;
+  r.s = a.s * ka + b.s * kb;
+  r.t = (ka == 0.f ? 0.f : fmaf(da, a.s, a.t) * ka) + (kb == 0.f ? 0.f : fmaf(db, b.s, b.t) * kb);
   return r;
 }
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
+// What a row's sums say.
+struct Row {
+  float m2, ls, lse, entropy;
 
+  __device__ __forceinline__ explicit Row(Sums a) {
+    m2 = a.m2;
+    ls = log2_fast(a.s);
+    lse = (m2 + ls) * kLn2;
+    entropy = (ls - a.t / a.s) * kLn2;
+    if (a.s == 0.f) lse = -INFINITY, entropy = 0.f;      // nothing left by a mask
+  }
+  __device__ __forceinline__ float logprob(float x) const {
+    if (lse == -INFINITY) return -INFINITY;
+    if (fabsf(x) > 1e30f) return x - lse;                // x L may overflow
+    return (fmaf(x, kLog2e, -m2) - ls) * kLn2;
+  }
+};
+
+struct Outputs {
+  float *logprob, *entropy, *lse, *top_logprob;
+  int64_t* top_id;
+  int top;
+};
+
+__device__ __forceinline__ void write_row(const Outputs& out, int64_t r, const Row& row,
+                                          int64_t target, int64_t ignore, int64_t vocab,
+                                          float given) {
+  out.lse[r] = row.lse;
+  if (out.entropy) out.entropy[r] = row.entropy;
+  const bool good = target >= 0 && target < vocab;
+  out.logprob[r] = target == ignore ? 0.f : good ? row.logprob(given) : quiet_nan();
+}
+
+constexpr int kThreads = 512, kWaves = kThreads / kWave;
+constexpr int kGroup = 4;                 // 16-byte loads in flight per lane
+constexpr int kMost = MS_OPS_MAX_TOP;
+constexpr int kCandidates = 4096;
+constexpr int kSorts = 128;               // sets of which the thresholds are maxima
+static_assert(kSorts >= kMost && kSorts <= kThreads, "");
+
+struct Shared {
+  Key list[kCandidates];
+  Key sets[kSorts];
+  Key threshold;
+  int count;
+  Sums sums[kWaves];
+  float value[kWaves];
+};
+
+// A key of which at least k of the n in `list` are as large: the k-th largest of
+// the maxima of kSorts sets (0 where fewer sets hold anything).
+__device__ void find_threshold(Shared& sh, int n, int k) {
+  if (threadIdx.x < kSorts) {
+    Key most = 0;
+    for (int i = threadIdx.x; i < n; i += kSorts) most = sh.list[i] > most ? sh.list[i] : most;
+    sh.sets[threadIdx.x] = most;
+  }
+  if (threadIdx.x == 0) sh.threshold = 0;
+  __syncthreads();
+  if (threadIdx.x < kSorts) {
+    const Key mine = sh.sets[threadIdx.x];
+    int above = 0;
+    for (int i = 0; i < kSorts; ++i) above += sh.sets[i] > mine;
+    if (mine && above == k - 1) sh.threshold = mine;
+  }
+  __syncthreads();
+}
+
+// The k largest of the n keys in `list`, in order: put(rank, key).
+template <typename Put>
+__device__ void select_top(Shared& sh, int n, int k, Put put) {
+  find_threshold(sh, n, k);
+  const Key least = sh.threshold;
+  constexpr int kEach = kCandidates / kThreads;
+  Key mine[kEach];
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int i = threadIdx.x + u * kThreads;
+    mine[u] = i < n ? sh.list[i] : 0;
+  }
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kEach; ++u)
+    if (mine[u] && mine[u] >= least) sh.list[atomicAdd(&sh.count, 1)] = mine[u];
+  __syncthreads();
+  const int left = sh.count;
+  for (int i = threadIdx.x; i < left; i += kThreads) {
+    const Key key = sh.list[i];
+    int above = 0;
+    for (int j = 0; j < left; ++j) above += sh.list[j] > key;
+    if (above < k) put(above, key);
+  }
+  __syncthreads();
+}
+
+// A row by itself whatever it holds: the maximum first, then the sums, then one
+// pass for each alternative.  For rows that the fast way gives up: NaN, +inf,
+// logits beyond 2^20 or 88 above all that the first look saw.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    k_logprobs(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, int top, float* logprob,
-               float* entropy, float* lse, float* top_logprob, int64_t* top_id) {
-  __shared__ float slot[kWaves];
-  __shared__ uint64_t best[kWaves];
-  for (int64_t r = blockIdx.x; r < logits.n; r += gridDim.x) {
-    const T* x = static_cast<const T*>(logits.data) + row_start(logits, r);
-    const int64_t v = logits.width;
-    float most = -INFINITY;
-    for (int64_t j = threadIdx.x; j < v; j += kThreads) most = fmaxf(most, widen(x[j]));
-    most = block_join<kWaves>(wave_max(most), slot, [](float a, float b) { return fmaxf(a, b); });
-    const bool far = !(fabsf(most) <= kFar) && most != -INFINITY;
-    const float base = most == -INFINITY ? 0.f : most;
-    const float m2 = rintf(base * kLog2e);
-    float s = 0.f, t = 0.f;
-    for (int64_t j = threadIdx.x; j < v; j += kThreads) {
-      const float xj = widen(x[j]);
-      const float y = far ? (xj - base) * kLog2e : fmaf(xj, kLog2e, -m2);
-      const float e = exp2_fast(y);
-      s += e;
-      t += e * fmaxf(y, -1e30f);
+__device__ __noinline__ void slow_row(Shared& sh, const T* x, int64_t vocab, int64_t r,
+                                      const Outputs& out, int64_t target, int64_t ignore) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto block = [&](float v, auto op) {
+    __syncthreads();
+    if (lane == 0) sh.value[wave] = v;
+    __syncthreads();
+    float y = sh.value[0];
+    for (int w = 1; w < kWaves; ++w) y = op(y, sh.value[w]);
+    return y;
+  };
+  float most = -INFINITY;
+  for (int64_t j = threadIdx.x; j < vocab; j += kThreads) most = fmaxf(most, widen(x[j]));
+  most = block(wave_max(most), [](float a, float b) { return fmaxf(a, b); });
+  const float base = most == -INFINITY ? 0.f : most;
+  float s = 0.f, t = 0.f;
+  for (int64_t j = threadIdx.x; j < vocab; j += kThreads) {
+    const float y = (widen(x[j]) - base) * kLog2e, e = exp2_fast(y);
+    s += e;
+    t = fmaf(e, fmaxf(y, -1e30f), t);
+  }
+  auto add = [](float a, float b) { return a + b; };
+  s = block(wave_sum(s), add);
+  t = block(wave_sum(t), add);
+  const bool empty = s == 0.f;
+  const float ls = log2_fast(s);
+  auto logprob = [&](float v) { return empty ? -INFINITY : (v - base) - ls * kLn2; };
+  if (threadIdx.x == 0) {
+    out.lse[r] = empty ? -INFINITY : base + ls * kLn2;
+    if (out.entropy) out.entropy[r] = empty ? 0.f : (ls - t / s) * kLn2;
+    const bool good = target >= 0 && target < vocab;
+    out.logprob[r] = target == ignore ? 0.f : good ? logprob(widen(x[target])) : quiet_nan();
+  }
+  Key last = ~0ull;
+  for (int k = 0; k < out.top; ++k) {
+    Key mine = 0;
+    for (int64_t j = threadIdx.x; j < vocab; j += kThreads) {
+      const Key key = key_of(widen(x[j]), static_cast<int>(j));
+      if (key > mine && key < last) mine = key;
     }
-    auto add = [](float a, float b) { return a + b; };
-    s = block_join<kWaves>(wave_sum(s), slot, add);
-    t = block_join<kWaves>(wave_sum(t), slot, add);
-    const int64_t y = token(targets, r);
-    const bool good = y >= 0 && y < v;
-    const RowStats st = finish(most, s, t, good ? widen(x[y]) : 0.f, good);
+    for (int b = 32; b; b >>= 1) {
+      const Key other = __shfl_xor(static_cast<unsigned long long>(mine), b);
+      if (other > mine) mine = other;
+    }
+    __syncthreads();
+    if (lane == 0) sh.list[wave] = mine;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) mine = sh.list[w] > mine ? sh.list[w] : mine;
+    last = mine;
     if (threadIdx.x == 0) {
-      lse[r] = st.lse;
-      logprob[r] = y == ignore ? 0.f : st.logprob;
-      if (entropy) entropy[r] = st.entropy;
-    }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < top; ++k) {
-      uint64_t mine = 0;
-      for (int64_t j = threadIdx.x; j < v; j += kThreads) {
-        const uint64_t key = static_cast<uint64_t>(order_key(widen(x[j]))) << 32 |
-                             static_cast<uint32_t>(~static_cast<uint32_t>(j));
-        if (key > mine && key < last) mine = key;
-      }
-      for (int b = 32; b; b >>= 1) {
-        const uint64_t other = __shfl_xor(static_cast<unsigned long long>(mine), b);
-        if (other > mine) mine = other;
-      }
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = mine;
-      __syncthreads();
-      mine = best[0];
-      for (int w = 1; w < kWaves; ++w) mine = best[w] > mine ? best[w] : mine;
-      last = mine;
-      if (threadIdx.x == 0) {
-        const uint32_t j = ~static_cast<uint32_t>(mine);
-        const float value = key_value(static_cast<uint32_t>(mine >> 32));
-        top_id[r * top + k] = j;
-        top_logprob[r * top + k] = finish(most, s, t, value, true).logprob;
-      }
+      out.top_id[r * out.top + k] = index_of(mine);
+      out.top_logprob[r * out.top + k] = logprob(value_of(mine));
     }
   }
 }
 
+// What a part of a split row leaves for k_join_parts, its keys behind it.
+struct Part {
+  Sums sums;
+  int given_up;
+};
+
+struct Split {
+  int parts;            // of a row
+  int64_t length;       // of a part
+  char* work;           // [n, parts] of `stride` bytes: a Part and `top` keys
+  int64_t stride;
+};
+
+// A block takes a row, or a part of one where there are few rows.
+//
+// It looks at its first kGroup * 8192 bytes for a reference, one per wave, so
+// that no running maximum is kept: s only overflows where later logits are 88
+// above all the wave saw, and the row is then done again by slow_row.  The
+// same look gives a threshold that at least `top` values reach; what reaches it,
+// a few times `top` values, is put on a list in LDS, of which the largest are
+// taken at the end.
+template <typename T, bool kTop, bool kEntropy>
+__global__ void __launch_bounds__(kThreads)
+    k_logprobs(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out, Split split) {
+  constexpr int kVec = 16 / sizeof(T);
+  __shared__ Shared sh;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = blockIdx.x / split.parts, vocab = logits.width;
+  const int64_t begin = (blockIdx.x - r * split.parts) * split.length;
+  const T* row = static_cast<const T*>(logits.data) + row_start(logits, r);
+  const T* x = row + begin;
+  const int n = static_cast<int>(vocab - begin < split.length ? vocab - begin : split.length);
+  const int units = n / kVec, rest = n - units * kVec;
+  const int64_t target = token(targets, r);
+  const float given = target >= 0 && target < vocab ? widen(row[target]) : 0.f;
+
+  // unit tid + k kThreads, and the last values one to a thread
+  Pack<T, kVec> look[kGroup];
+#pragma unroll
+  for (int k = 0; k < kGroup; ++k) {
+    const int u = threadIdx.x + k * kThreads;
+    if (u < units) {
+      look[k] = load<kVec>(x + u * kVec);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) look[k].v[i] = static_cast<T>(-INFINITY);
+    }
+  }
+  const float single =
+      threadIdx.x < rest ? widen(x[units * kVec + threadIdx.x]) : -INFINITY;
+  float most = single;
+#pragma unroll
+  for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) most = fmaxf(most, widen(look[k].v[i]));
+
+  Key least = 0;
+  float least_value = -INFINITY;
+  if (threadIdx.x == 0) sh.count = 0;
+  auto offer = [&](float v, int j) {
+    const Key key = key_of(v, static_cast<int>(begin) + j);
+    if (key >= least) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCandidates) sh.list[at] = key;
+    }
+  };
+  if (kTop) {
+    // the thread's largest, with the lowest index that has it
+    int at = -1;
+    if (single == most && threadIdx.x < rest) at = units * kVec + threadIdx.x;
+#pragma unroll
+    for (int k = kGroup - 1; k >= 0; --k) {
+      const int u = threadIdx.x + k * kThreads;
+      if (u < units)
+#pragma unroll
+        for (int i = kVec - 1; i >= 0; --i)
+          if (widen(look[k].v[i]) == most) at = u * kVec + i;
+    }
+    sh.list[threadIdx.x] = at < 0 ? 0 : key_of(most, static_cast<int>(begin) + at);
+    __syncthreads();
+    find_threshold(sh, kThreads, out.top);
+    least = sh.threshold;
+    least_value = least ? value_of(least) : -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) {
+      const int u = threadIdx.x + k * kThreads;
+      if (u < units && most >= least_value)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          if (widen(look[k].v[i]) >= least_value) offer(widen(look[k].v[i]), u * kVec + i);
+    }
+    if (threadIdx.x < rest && single >= least_value) offer(single, units * kVec + threadIdx.x);
+  }
+
+  // a wave that has seen nothing but -inf looks again at every group
+  float seen = wave_max(most);
+  float m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
+  float s = 0.f, t = 0.f;
+  auto add = [&](float v) {
+    const float y = fmaf(v, kLog2e, -m2), e = exp2_fast(y);
+    s += e;
+    if (kEntropy) t = fmaf(e, fmaxf(y, -1e30f), t);
+  };
+#pragma unroll
+  for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) add(widen(look[k].v[i]));
+  add(single);
+
+  auto take = [&](const Pack<T, kVec>& p, int u) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) add(widen(p.v[i]));
+    if (kTop) {
+      float high = widen(p.v[0]);
+#pragma unroll
+      for (int i = 1; i < kVec; ++i) high = fmaxf(high, widen(p.v[i]));
+      if (high >= least_value)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          if (widen(p.v[i]) >= least_value) offer(widen(p.v[i]), u * kVec + i);
+    }
+  };
+  auto look_again = [&](const Pack<T, kVec>& p) {
+    float high = widen(p.v[0]);
+#pragma unroll
+    for (int i = 1; i < kVec; ++i) high = fmaxf(high, widen(p.v[i]));
+    seen = wave_max(high);
+    m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
+  };
+  int u = kGroup * kThreads + threadIdx.x;
+  for (; u + (kGroup - 1) * kThreads < units; u += kGroup * kThreads) {
+    Pack<T, kVec> p[kGroup];
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) p[k] = load<kVec>(x + (u + k * kThreads) * kVec);
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) {
+      if (seen == -INFINITY) look_again(p[k]);
+      take(p[k], u + k * kThreads);
+    }
+  }
+  for (; u < units; u += kThreads) {
+    const Pack<T, kVec> p = load<kVec>(x + u * kVec);
+    if (seen == -INFINITY) look_again(p);
+    take(p, u);
+  }
+
+  s = wave_sum(s);
+  if (kEntropy) t = wave_sum(t);
+  if (lane == 0) sh.sums[wave] = Sums{m2, s, t};
+  __syncthreads();
+  Sums all = sh.sums[0];
+  for (int w = 1; w < kWaves; ++w) all = join(all, sh.sums[w]);
+  bool give_up = !(all.s < INFINITY);
+  for (int w = 0; w < kWaves; ++w)
+    give_up |= !(sh.sums[w].s < INFINITY) || !(fabsf(sh.sums[w].m2) <= 1 << 20);
+  const int count = kTop ? sh.count : 0;
+  if (kTop) give_up |= count > kCandidates;
+
+  if (split.parts == 1) {
+    if (give_up) {
+      slow_row(sh, row, vocab, r, out, target, ignore);
+      return;
+    }
+    const Row done(all);
+    if (threadIdx.x == 0) write_row(out, r, done, target, ignore, vocab, given);
+    if (kTop)
+      select_top(sh, count, out.top, [&](int rank, Key key) {
+        out.top_id[r * out.top + rank] = index_of(key);
+        out.top_logprob[r * out.top + rank] = done.logprob(value_of(key));
+      });
+    return;
+  }
+  char* left = split.work + blockIdx.x * split.stride;
+  if (threadIdx.x == 0) *reinterpret_cast<Part*>(left) = Part{all, give_up};
+  if (kTop && !give_up) {
+    Key* keys = reinterpret_cast<Key*>(left + sizeof(Part));
+    if (threadIdx.x < out.top) keys[threadIdx.x] = 0;
+    __syncthreads();
+    select_top(sh, count, out.top, [&](int rank, Key key) { keys[rank] = key; });
+  }
+}
+
+// A row's parts.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
+    k_join_parts(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out,
+                 Split split) {
+  __shared__ Shared sh;
+  const int64_t r = blockIdx.x, vocab = logits.width;
+  const T* row = static_cast<const T*>(logits.data) + row_start(logits, r);
+  const int64_t target = token(targets, r);
+  const float given = target >= 0 && target < vocab ? widen(row[target]) : 0.f;
+  const char* work = split.work + r * split.parts * split.stride;
+  const int keys = split.parts * out.top;          // at most kCandidates
+  for (int i = threadIdx.x; i < keys; i += kThreads) {
+    const int p = i / out.top;
+    sh.list[i] =
+        reinterpret_cast<const Key*>(work + p * split.stride + sizeof(Part))[i - p * out.top];
+  }
+  // as many parts as lanes, in every wave
+  const int lane = threadIdx.x & 63;
+  Part mine{{0.f, 0.f, 0.f}, 0};
+  if (lane < split.parts) mine = *reinterpret_cast<const Part*>(work + lane * split.stride);
+  const bool give_up = __any(mine.given_up);
+  Sums all = mine.sums;
+  for (int k = 1; k < kWave; k <<= 1) {
+    Sums other;
+    other.m2 = __shfl_xor(all.m2, k);
+    other.s = __shfl_xor(all.s, k);
+    other.t = __shfl_xor(all.t, k);
+    all = lane & k ? join(other, all) : join(all, other);
+  }
+  __syncthreads();
+  if (give_up) {
+    slow_row(sh, row, vocab, r, out, target, ignore);
+    return;
+  }
+  const Row done(all);
+  if (threadIdx.x == 0) write_row(out, r, done, target, ignore, vocab, given);
+  if (out.top)
+    select_top(sh, keys, out.top, [&](int rank, Key key) {
+      out.top_id[r * out.top + rank] = index_of(key);
+      out.top_logprob[r * out.top + rank] = done.logprob(value_of(key));
+    });
+}
+
+// -- gradient -----------------------------------------------------------------
+
+// Beyond this an fp32 lse no longer tells logits from each other (a row masked
+// with the type's lowest value: lse - max is lost), and the row's maximum and
+// sum are found again.
+constexpr float kFarLse = 256.f;
+
+constexpr int kGradThreads = 256, kGradWaves = kGradThreads / kWave;
+constexpr int kGradGroup = 4;
+
+// A block takes kGradGroup * kGradThreads units of a row.  With c a whole
+// number near lse L and p' = 2^(x L - c): dx = p' (a + b x), where a and b hold
+// what c rounded off; the target's g is added to the one value.
+template <typename T, bool kEntropy>
+__global__ void __launch_bounds__(kGradThreads)
     k_logprobs_grad(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, const float* lse,
                     const float* entropy, const float* grad_logprob, const float* grad_entropy,
-                    T* __restrict__ out) {
-  __shared__ float slot[kWaves];
-  for (int64_t r = blockIdx.x; r < logits.n; r += gridDim.x) {
-    const T* x = static_cast<const T*>(logits.data) + row_start(logits, r);
-    const int64_t v = logits.width;
-    T* d = out + r * v;
-    const int64_t y = token(targets, r);
-    float g = grad_logprob && y != ignore ? grad_logprob[r] : 0.f;
-    if (grad_logprob && y != ignore && (y < 0 || y >= v)) g = quiet_nan();
-    const float h = grad_entropy ? grad_entropy[r] : 0.f;
-    const float big_h = grad_entropy ? entropy[r] : 0.f;
-    const float l = lse[r];
-    if (l == -INFINITY) {
-      for (int64_t j = threadIdx.x; j < v; j += kThreads) d[j] = narrow<T>(0.f);
-      continue;
-    }
-    float base = l, ls = 0.f;
-    if (fabsf(l) > kFar) {
-      float most = -INFINITY;
-      for (int64_t j = threadIdx.x; j < v; j += kThreads) most = fmaxf(most, widen(x[j]));
-      most =
-          block_join<kWaves>(wave_max(most), slot, [](float a, float b) { return fmaxf(a, b); });
-      float s = 0.f;
-      for (int64_t j = threadIdx.x; j < v; j += kThreads)
+                    int blocks_per_row, T* __restrict__ out) {
+  constexpr int kVec = 16 / sizeof(T);
+  __shared__ float slot[kGradWaves];
+  const int64_t r = blockIdx.x / blocks_per_row, vocab = logits.width;
+  const int part = static_cast<int>(blockIdx.x - r * blocks_per_row);
+  const T* x = static_cast<const T*>(logits.data) + row_start(logits, r);
+  T* d = out + r * vocab;
+  const int64_t target = token(targets, r);
+  float g = grad_logprob && target != ignore ? grad_logprob[r] : 0.f;
+  const bool outside = target < 0 || target >= vocab;
+  if (grad_logprob && target != ignore && outside) g = quiet_nan();
+  const float h = kEntropy ? grad_entropy[r] : 0.f, big_h = kEntropy ? entropy[r] : 0.f;
+  const float l = lse[r];
+
+  const int units = static_cast<int>(vocab / kVec), rest = static_cast<int>(vocab) - units * kVec;
+  const int first = part * kGradGroup * kGradThreads + threadIdx.x;
+  if (l == -INFINITY || fabsf(l) > kFarLse) {
+    // every block of the row finds the maximum and the sum for itself
+    auto block = [&](float v, auto op) {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+      __syncthreads();
+      float y = slot[0];
+      for (int w = 1; w < kGradWaves; ++w) y = op(y, slot[w]);
+      return y;
+    };
+    float most = 0.f, s = 1.f;
+    if (l != -INFINITY) {
+      most = -INFINITY;
+      for (int64_t j = threadIdx.x; j < vocab; j += kGradThreads) most = fmaxf(most, widen(x[j]));
+      most = block(wave_max(most), [](float a, float b) { return fmaxf(a, b); });
+      s = 0.f;
+      for (int64_t j = threadIdx.x; j < vocab; j += kGradThreads)
         s += exp2_fast((widen(x[j]) - most) * kLog2e);
-      s = block_join<kWaves>(wave_sum(s), slot, [](float a, float b) { return a + b; });
-      base = most;
-      ls = log2_fast(s) * kLn2;
+      s = block(wave_sum(s), [](float a, float b) { return a + b; });
     }
-    for (int64_t j = threadIdx.x; j < v; j += kThreads) {
-      const float logp = (widen(x[j]) - base) - ls;
-      const float p = exp2_fast(logp * kLog2e);
-      float dj = j == y ? g - g * p : -g * p;
-      if (p != 0.f) dj -= h * p * (logp + big_h);
+    const float ls = log2_fast(s) * kLn2;
+    const int64_t end = part == blocks_per_row - 1
+                            ? vocab
+                            : static_cast<int64_t>(part + 1) * kGradGroup * kGradThreads * kVec;
+    for (int64_t j = static_cast<int64_t>(part) * kGradGroup * kGradThreads * kVec + threadIdx.x;
+         j < end; j += kGradThreads) {
+      float dj = 0.f;
+      if (l != -INFINITY) {
+        const float logp = (widen(x[j]) - most) - ls, p = exp2_fast(logp * kLog2e);
+        dj = j == target ? g - g * p : -g * p;
+        if (kEntropy && p != 0.f) dj -= h * p * (logp + big_h);
+      }
       d[j] = narrow<T>(dj);
     }
+    return;
+  }
+
+  const float c = rintf(l * kLog2e), k = exp2_fast(-fmaf(l, kLog2e, -c));
+  const float b = -h * k, a = -(g + h * (big_h - l)) * k;
+  auto one = [&](float v) {
+    const float p = exp2_fast(fmaf(v, kLog2e, -c));
+    if (!kEntropy) return p * a;
+    return p * fmaf(b, fmaxf(v, -1e6f), a);        // -inf: p is 0, and 0 * inf must not be
+  };
+  Pack<T, kVec> in[kGradGroup];
+#pragma unroll
+  for (int i = 0; i < kGradGroup; ++i) {
+    const int u = first + i * kGradThreads;
+    if (u < units) in[i] = load<kVec>(x + static_cast<int64_t>(u) * kVec);
+  }
+#pragma unroll
+  for (int i = 0; i < kGradGroup; ++i) {
+    const int u = first + i * kGradThreads;
+    if (u < units) {
+      float y[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) y[j] = one(widen(in[i].v[j]));
+      const int64_t at = target - static_cast<int64_t>(u) * kVec;
+      if (at >= 0 && at < kVec)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) y[j] += at == j ? g : 0.f;
+      Pack<T, kVec> z;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) z.v[j] = narrow<T>(y[j]);
+      store<kVec>(d + static_cast<int64_t>(u) * kVec, z);
+    }
+  }
+  if (part == blocks_per_row - 1 && threadIdx.x < rest) {
+    const int64_t j = static_cast<int64_t>(units) * kVec + threadIdx.x;
+    d[j] = narrow<T>(one(widen(x[j])) + (j == target ? g : 0.f));
   }
 }
 
-unsigned blocks_for(int64_t n) {
-  const int64_t most = 1 << 20;
-  return static_cast<unsigned>(n < most ? n : most);
+// How a row is split: not at all from 512 rows on, two blocks to a CU; else so
+// that there are as many blocks, each with a unit to every thread at least.
+Split split_of(int64_t n, int64_t vocab, int32_t dtype, int32_t top) {
+  const int64_t least = kThreads * (16 / dtype_bytes(dtype));
+  Split s;
+  const int64_t wanted = std::min<int64_t>(kWave, 512 / std::max<int64_t>(n, 1));
+  s.length = vocab;
+  if (wanted > 1 && vocab > least) {
+    s.length = (vocab + wanted - 1) / wanted;
+    s.length = std::max(least, (s.length + 63) / 64 * 64);
+  }
+  s.parts = static_cast<int>((vocab + s.length - 1) / s.length);
+  s.stride = (static_cast<int64_t>(sizeof(Part)) + 8 * top + 15) & ~15ll;
+  s.work = nullptr;
+  return s;
+}
+
+template <typename T>
+int logprobs_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
+                const Outputs& out, const Split& split, hipStream_t s) {
+  const unsigned blocks = static_cast<unsigned>(logits.n * split.parts);
+  if (out.top && out.entropy)
+    k_logprobs<T, true, true><<<blocks, kThreads, 0, s>>>(logits, targets, ignore, out, split);
+  else if (out.top)
+    k_logprobs<T, true, false><<<blocks, kThreads, 0, s>>>(logits, targets, ignore, out, split);
+  else if (out.entropy)
+    k_logprobs<T, false, true><<<blocks, kThreads, 0, s>>>(logits, targets, ignore, out, split);
+  else
+    k_logprobs<T, false, false><<<blocks, kThreads, 0, s>>>(logits, targets, ignore, out, split);
+  if (int rc = launched()) return rc;
+  if (split.parts > 1)
+    k_join_parts<T><<<static_cast<unsigned>(logits.n), kThreads, 0, s>>>(logits, targets, ignore,
+                                                                         out, split);
+  return launched();
+}
+
+template <typename T>
+int grad_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore, const float* lse,
+            const float* entropy, const float* grad_logprob, const float* grad_entropy,
+            void* dlogits, hipStream_t s) {
+  constexpr int64_t kEach = kGradGroup * kGradThreads * (16 / sizeof(T));
+  const int64_t per_row = std::max<int64_t>((logits.width + kEach - 1) / kEach, 1);
+  if (logits.n * per_row > INT32_MAX) return MS_OPS_EINVAL;
+  const unsigned blocks = static_cast<unsigned>(logits.n * per_row);
+  if (grad_entropy)
+    k_logprobs_grad<T, true><<<blocks, kGradThreads, 0, s>>>(
+        logits, targets, ignore, lse, entropy, grad_logprob, grad_entropy,
+        static_cast<int>(per_row), static_cast<T*>(dlogits));
+  else
+    k_logprobs_grad<T, false><<<blocks, kGradThreads, 0, s>>>(
+        logits, targets, ignore, lse, entropy, grad_logprob, grad_entropy,
+        static_cast<int>(per_row), static_cast<T*>(dlogits));
+  return launched();
 }
 
 }  // namespace
 
-extern "C" int64_t ms_logprobs_workspace(int64_t, int64_t, int32_t, int32_t) { return 0; }
+extern "C" int64_t ms_logprobs_workspace(int64_t n, int64_t vocab, int32_t dtype, int32_t top) {
+  if (n < 0 || n > INT32_MAX || vocab < 1 || !good_dtype(dtype) || top < 0) return -1;
+  const Split s = split_of(n, vocab, dtype, top);
+  return s.parts > 1 ? n * s.parts * s.stride : 0;
+}
 
 extern "C" int ms_logprobs(const ms_rows_t* logits, const ms_tokens_t* targets,
                            int64_t ignore_index, int32_t top, float* logprob, float* entropy,
                            float* lse, float* top_logprob, int64_t* top_id, void* workspace,
                            int64_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   if (!good_rows(logits) || !good_tokens(targets) || targets->n != logits->n) return MS_OPS_EINVAL;
-  if (logits->width < 1 || logits->width > INT32_MAX) return MS_OPS_EINVAL;
+  if (logits->width < 1 || logits->width > INT32_MAX - 65536) return MS_OPS_EINVAL;
   if (top < 0 || top > MS_OPS_MAX_TOP || top > logits->width) return MS_OPS_EINVAL;
   if (logits->n == 0) return MS_OPS_OK;
   if (!logprob || !lse || (top && (!top_logprob || !top_id))) return MS_OPS_EINVAL;
+  Split split = split_of(logits->n, logits->width, logits->dtype, top);
+  if (split.parts > 1 &&
+      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+       workspace_bytes < ms_logprobs_workspace(logits->n, logits->width, logits->dtype, top)))
+    return MS_OPS_EWORKSPACE;
+  split.work = static_cast<char*>(workspace);
+  const Outputs out = {logprob, entropy, lse, top_logprob, top_id, top};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned blocks = blocks_for(logits->n);
   switch (logits->dtype) {
-    case MS_OPS_F32:
-      k_logprobs<float><<<blocks, kThreads, 0, s>>>(*logits, *targets, ignore_index, top, logprob,
-                                                    entropy, lse, top_logprob, top_id);
-      break;
-    case MS_OPS_F16:
-      k_logprobs<f16><<<blocks, kThreads, 0, s>>>(*logits, *targets, ignore_index, top, logprob,
-                                                  entropy, lse, top_logprob, top_id);
-      break;
-    default:
-      k_logprobs<bf16><<<blocks, kThreads, 0, s>>>(*logits, *targets, ignore_index, top, logprob,
-                                                   entropy, lse, top_logprob, top_id);
+    case MS_OPS_F32: return logprobs_as<float>(*logits, *targets, ignore_index, out, split, s);
+    case MS_OPS_F16: return logprobs_as<f16>(*logits, *targets, ignore_index, out, split, s);
+    default: return logprobs_as<bf16>(*logits, *targets, ignore_index, out, split, s);
   }
-  return launched();
 }
 
 extern "C" int ms_logprobs_grad(const ms_rows_t* logits, const ms_tokens_t* targets,
@@ -238,26 +651,19 @@ extern "C" int ms_logprobs_grad(const ms_rows_t* logits, const ms_tokens_t* targ
                                 const float* grad_logprob, const float* grad_entropy,
                                 void* dlogits, void* stream) {
   if (!good_rows(logits) || !good_tokens(targets) || targets->n != logits->n) return MS_OPS_EINVAL;
-  if (logits->width < 1 || logits->width > INT32_MAX) return MS_OPS_EINVAL;
+  if (logits->width < 1 || logits->width > INT32_MAX - 65536) return MS_OPS_EINVAL;
   if (logits->n == 0) return MS_OPS_OK;
   if (!lse || !dlogits || (grad_entropy && !entropy)) return MS_OPS_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned blocks = blocks_for(logits->n);
   switch (logits->dtype) {
     case MS_OPS_F32:
-      k_logprobs_grad<float><<<blocks, kThreads, 0, s>>>(*logits, *targets, ignore_index, lse,
-                                                         entropy, grad_logprob, grad_entropy,
-                                                         static_cast<float*>(dlogits));
-      break;
+      return grad_as<float>(*logits, *targets, ignore_index, lse, entropy, grad_logprob,
+                            grad_entropy, dlogits, s);
     case MS_OPS_F16:
-      k_logprobs_grad<f16><<<blocks, kThreads, 0, s>>>(*logits, *targets, ignore_index, lse,
-                                                       entropy, grad_logprob, grad_entropy,
-                                                       static_cast<f16*>(dlogits));
-      break;
+      return grad_as<f16>(*logits, *targets, ignore_index, lse, entropy, grad_logprob,
+                          grad_entropy, dlogits, s);
     default:
-      k_logprobs_grad<bf16><<<blocks, kThreads, 0, s>>>(*logits, *targets, ignore_index, lse,
-                                                        entropy, grad_logprob, grad_entropy,
-                                                        static_cast<bf16*>(dlogits));
+      return grad_as<bf16>(*logits, *targets, ignore_index, lse, entropy, grad_logprob,
+                           grad_entropy, dlogits, s);
   }
-  return launched();
 }
