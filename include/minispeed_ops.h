@@ -14,8 +14,9 @@
  *   - Return value: 0, a negative MS_OPS_E* code for an argument error found
  *     on the host (nothing was launched), or a positive hipError_t from the
  *     launch.  ms_ops_error_string() names both kinds.
- *   - Results do not depend on addresses, alignment, stream or launch shape
- *     timing: no floating-point atomics, every sum in a fixed order.
+ *   - The same call gives the same bits: no floating-point atomics, every sum
+ *     in a fixed order.  (That of a row of logits follows from the row's
+ *     address modulo 16; nothing else depends on addresses.)
  *   - Row-strided operands are given as (inner, outer_stride, inner_stride):
  *     row r starts at (r / inner) * outer_stride + (r % inner) * inner_stride
  *     elements; elements of a row are consecutive.  Token lists are the same

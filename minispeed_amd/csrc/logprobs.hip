@@ -24,30 +24,46 @@ constexpr float kLn2 = 0.69314718f;
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
+// Over the wave, the result in every lane; a fixed order.  DPP moves instead of
+// shuffles, which go through the LDS.
+template <typename Op>
+__device__ __forceinline__ float wave_reduce(float x, float none, Op op) {
+#define STEP(ctrl, rows)                                                               \
+  x = op(x, __uint_as_float(__builtin_amdgcn_update_dpp(                               \
+                __float_as_uint(none), __float_as_uint(x), ctrl, rows, 0xf, false)))
+  STEP(0x111, 0xf);      // row_shr 1, 2, 4, 8: lane 15 of each 16 has them all
+  STEP(0x112, 0xf);
+  STEP(0x114, 0xf);
+  STEP(0x118, 0xf);
+  STEP(0x142, 0xa);      // row_bcast 15, 31: lane 63 has all
+  STEP(0x143, 0xc);
+#undef STEP
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int k = 32; k; k >>= 1) x = fmaxf(x, __shfl_xor(x, k));
-  return x;
+  return wave_reduce(x, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k);
-  return x;
+  return wave_reduce(x, 0.f, [](float a, float b) { return a + b; });
 }
 
 // Falling value, then rising index: a 64-bit key that is larger for what
 // comes first, never 0.  NaN is above +inf; -0 equals +0.
 typedef uint64_t Key;
 constexpr uint32_t kNanKey = 0xFFFFFFF0u;
-__device__ __forceinline__ Key key_of(float x, int index) {
+__device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
-  const uint32_t order = x != x ? kNanKey : b & 0x80000000u ? ~b : b | 0x80000000u;
-  return static_cast<Key>(order) << 32 | ~static_cast<uint32_t>(index);
+  return x != x ? kNanKey : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float value_of(Key key) {
-  const uint32_t k = static_cast<uint32_t>(key >> 32);
+__device__ __forceinline__ Key key_of(float x, int index) {
+  return static_cast<Key>(order_of(x)) << 32 | ~static_cast<uint32_t>(index);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
   if (k == kNanKey) return quiet_nan();
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+__device__ __forceinline__ float value_of(Key key) {
+  return value_of(static_cast<uint32_t>(key >> 32));
 }
 __device__ __forceinline__ int index_of(Key key) {
   return static_cast<int>(~static_cast<uint32_t>(key));
@@ -104,82 +120,89 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t r, const R
   out.logprob[r] = target == ignore ? 0.f : good ? row.logprob(given) : quiet_nan();
 }
 
-constexpr int kThreads = 512, kWaves = kThreads / kWave;
-constexpr int kGroup = 4;                 // 16-byte loads in flight per lane
 constexpr int kMost = MS_OPS_MAX_TOP;
-constexpr int kCandidates = 4096;
-constexpr int kSorts = 128;               // sets of which the thresholds are maxima
-static_assert(kSorts >= kMost && kSorts <= kThreads, "");
+static_assert(kMost <= kWave, "");
 
-struct Shared {
-  Key list[kCandidates];
-  Key sets[kSorts];
-  Key threshold;
+// NT threads: 512, or 128 for vocabularies of at most kFewUnits units.
+template <int NT>
+struct Lists {
+  static constexpr int kCandidates = 8 * NT;
+  alignas(16) Key list[kCandidates];
+  alignas(16) uint32_t high[NT];
+  int at[NT];
   int count;
-  Sums sums[kWaves];
-  float value[kWaves];
 };
 
-// A key of which at least k of the n in `list` are as large: the k-th largest of
-// the maxima of kSorts sets (0 where fewer sets hold anything).
-__device__ void find_threshold(Shared& sh, int n, int k) {
-  if (threadIdx.x < kSorts) {
-    Key most = 0;
-    for (int i = threadIdx.x; i < n; i += kSorts) most = sh.list[i] > most ? sh.list[i] : most;
-    sh.sets[threadIdx.x] = most;
+// The largest word (its last kSkip bits 0) that at least k of the wave's 128 are
+// as large as; 0 if there are fewer, none of them 0.
+template <int kSkip>
+__device__ __forceinline__ uint32_t kth_largest(uint32_t a, uint32_t b, int k) {
+  uint32_t least = 0;
+#pragma unroll
+  for (int bit = 31; bit >= kSkip; --bit) {
+    const uint32_t more = least | 1u << bit;
+    if (__popcll(__ballot(a >= more)) + __popcll(__ballot(b >= more)) >= k) least = more;
   }
-  if (threadIdx.x == 0) sh.threshold = 0;
-  __syncthreads();
-  if (threadIdx.x < kSorts) {
-    const Key mine = sh.sets[threadIdx.x];
-    int above = 0;
-    for (int i = 0; i < kSorts; ++i) above += sh.sets[i] > mine;
-    if (mine && above == k - 1) sh.threshold = mine;
-  }
-  __syncthreads();
+  return least;
+}
+__device__ __forceinline__ int count_above(uint32_t a, uint32_t b, uint32_t than) {
+  return __popcll(__ballot(a > than)) + __popcll(__ballot(b > than));
 }
 
 // The k largest of the n keys in `list`, in order: put(rank, key).
-template <typename Put>
-__device__ void select_top(Shared& sh, int n, int k, Put put) {
-  find_threshold(sh, n, k);
-  const Key least = sh.threshold;
-  constexpr int kEach = kCandidates / kThreads;
-  Key mine[kEach];
+template <int NT, typename Put>
+__device__ __forceinline__ void select_top(Lists<NT>& sh, int n, int k, Put put) {
+  constexpr int kFew = 192;                 // that are counted against each other at once
+  if (n > kFew) {
+    uint32_t high[2] = {0, 0};              // of 128 sets, in every wave
+    for (int i = threadIdx.x & 63; i < n; i += 2 * kWave)
 #pragma unroll
-  for (int u = 0; u < kEach; ++u) {
-    const int i = threadIdx.x + u * kThreads;
-    mine[u] = i < n ? sh.list[i] : 0;
+      for (int u = 0; u < 2; ++u) {
+        const int j = i + u * kWave;
+        const uint32_t h = j < n ? static_cast<uint32_t>(sh.list[j] >> 32) : 0;
+        high[u] = h > high[u] ? h : high[u];
+      }
+    const uint32_t least = kth_largest<0>(high[0], high[1], k);
+    constexpr int kEach = Lists<NT>::kCandidates / NT;
+    Key mine[kEach];
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int i = threadIdx.x + u * NT;
+      mine[u] = i < n ? sh.list[i] : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kEach; ++u)
+      if (mine[u] && mine[u] >> 32 >= least) sh.list[atomicAdd(&sh.count, 1)] = mine[u];
+    __syncthreads();
+    n = sh.count;
   }
-  if (threadIdx.x == 0) sh.count = 0;
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < kEach; ++u)
-    if (mine[u] && mine[u] >= least) sh.list[atomicAdd(&sh.count, 1)] = mine[u];
-  __syncthreads();
-  const int left = sh.count;
-  for (int i = threadIdx.x; i < left; i += kThreads) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const Key key = sh.list[i];
     int above = 0;
-    for (int j = 0; j < left; ++j) above += sh.list[j] > key;
-    if (above < k) put(above, key);
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) above += sh.list[j] > key;
+    if (key && above < k) put(above, key);
   }
-  __syncthreads();
 }
 
 // A row by itself whatever it holds: the maximum first, then the sums, then one
-// pass for each alternative.  For rows that the fast way gives up: NaN, +inf,
+// pass for each alternative.  (Inlined: a call's stack alone took the whole
+// kernel from 126 to 190 us for 8192 x 50257.)  For rows that the fast way gives up: NaN, +inf,
 // logits beyond 2^20 or 88 above all that the first look saw.
-template <typename T>
-__device__ __noinline__ void slow_row(Shared& sh, const T* x, int64_t vocab, int64_t r,
+template <int NT, typename T>
+__device__ __forceinline__ void slow_row(float* value, Key* keys, const T* x, int64_t vocab, int64_t r,
                                       const Outputs& out, int64_t target, int64_t ignore) {
+  constexpr int kThreads = NT, kWaves = NT / kWave;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   auto block = [&](float v, auto op) {
     __syncthreads();
-    if (lane == 0) sh.value[wave] = v;
+    if (lane == 0) value[wave] = v;
     __syncthreads();
-    float y = sh.value[0];
-    for (int w = 1; w < kWaves; ++w) y = op(y, sh.value[w]);
+    float y = value[0];
+    for (int w = 1; w < kWaves; ++w) y = op(y, value[w]);
     return y;
   };
   float most = -INFINITY;
@@ -216,9 +239,9 @@ __device__ __noinline__ void slow_row(Shared& sh, const T* x, int64_t vocab, int
       if (other > mine) mine = other;
     }
     __syncthreads();
-    if (lane == 0) sh.list[wave] = mine;
+    if (lane == 0) keys[wave] = mine;
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) mine = sh.list[w] > mine ? sh.list[w] : mine;
+    for (int w = 0; w < kWaves; ++w) mine = keys[w] > mine ? keys[w] : mine;
     last = mine;
     if (threadIdx.x == 0) {
       out.top_id[r * out.top + k] = index_of(mine);
@@ -240,159 +263,216 @@ struct Split {
   int64_t stride;
 };
 
-// A block takes a row, or a part of one where there are few rows.
+// A block takes a row, or a part of one where there are few rows, in groups of
+// some rounds of an aligned 16-byte unit to every thread; the next group is
+// loaded while one is worked on.  (At the rows' own alignment, 50257 values of 2
+// bytes, units of which 7 of 8 lie across 16 bytes, the loads alone ran at 4.5
+// TB/s instead of 6.8.)
 //
-// It looks at its first kGroup * 8192 bytes for a reference, one per wave, so
-// that no running maximum is kept: s only overflows where later logits are 88
-// above all the wave saw, and the row is then done again by slow_row.  The
-// same look gives a threshold that at least `top` values reach; what reaches it,
-// a few times `top` values, is put on a list in LDS, of which the largest are
-// taken at the end.
-template <typename T, bool kTop, bool kEntropy>
-__global__ void __launch_bounds__(kThreads)
+// The first group gives a reference, one per wave, so that no running maximum
+// is kept: s only overflows where later logits are 88 above all the wave saw,
+// and the row is then done again by slow_row.  It also gives a threshold that at
+// least `top` values reach; what reaches it, a few times `top` values, is put on
+// a list in LDS, of which the largest are taken at the end.
+template <typename T, int NT, bool kTop, bool kEntropy>
+__global__ void __launch_bounds__(NT, 8)
     k_logprobs(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out, Split split) {
-  constexpr int kVec = 16 / sizeof(T);
-  __shared__ Shared sh;
+  constexpr int kVec = 16 / sizeof(T), kWaves = NT / kWave;
+  // rounds to a group; with the lists' registers 2, so that four blocks fit a CU
+  constexpr int kGroup = kTop ? 2 : 4;
+  typedef Pack<T, kVec> Unit;
+  __shared__ Sums sums[kWaves];
+  __shared__ float value[kWaves];
+  __shared__ Lists<(kTop ? NT : 1)> sh;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r = blockIdx.x / split.parts, vocab = logits.width;
   const int64_t begin = (blockIdx.x - r * split.parts) * split.length;
+  const int64_t target = token(targets, r);
   const T* row = static_cast<const T*>(logits.data) + row_start(logits, r);
   const T* x = row + begin;
   const int n = static_cast<int>(vocab - begin < split.length ? vocab - begin : split.length);
-  const int units = n / kVec, rest = n - units * kVec;
-  const int64_t target = token(targets, r);
-  const float given = target >= 0 && target < vocab ? widen(row[target]) : 0.f;
+  const int off = static_cast<int>(-(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (kVec - 1));
+  const int head = off < n ? off : n;               // values before the first whole unit
+  const int units = (n - head) / kVec, rest = n - head - units * kVec;
+  const int rounds = (units + NT - 1) / NT;
+  const T* first = x + head;
 
-  // unit tid + k kThreads, and the last values one to a thread
-  Pack<T, kVec> look[kGroup];
+  // the last round's threads without a unit load the last one
+  auto load_group = [&](int k0, Unit (&p)[kGroup]) {
 #pragma unroll
-  for (int k = 0; k < kGroup; ++k) {
-    const int u = threadIdx.x + k * kThreads;
-    if (u < units) {
-      look[k] = load<kVec>(x + u * kVec);
-    } else {
+    for (int k = 0; k < kGroup; ++k)
+      if (k0 + k < rounds) {
+        const int u = (k0 + k) * NT + threadIdx.x;
+        p[k] = load_stream<kVec>(first + static_cast<int64_t>(u < units ? u : units - 1) * kVec);
+      }
+  };
+  // ... and drop it
+  auto mask_group = [&](int k0, Unit (&p)[kGroup]) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) look[k].v[i] = static_cast<T>(-INFINITY);
-    }
-  }
-  const float single =
-      threadIdx.x < rest ? widen(x[units * kVec + threadIdx.x]) : -INFINITY;
+    for (int k = 0; k < kGroup; ++k)
+      if (k0 + k >= rounds - 1 && (k0 + k) * NT + static_cast<int>(threadIdx.x) >= units)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) p[k].v[i] = static_cast<T>(-INFINITY);
+  };
+  Unit now[kGroup], next[kGroup];
+  load_group(0, now);
+  // the values before and behind the units, one to a thread
+  const int tid = threadIdx.x;
+  const int alone = tid < head                          ? tid
+                    : tid >= kVec && tid - kVec < rest ? head + units * kVec + tid - kVec
+                                                       : -1;
+  // loads come back in order: what waits for one waits for those before it
+  const T single_raw = x[alone >= 0 ? alone : 0];
+  load_group(kGroup, next);
+  const bool good = target >= 0 && target < vocab;
+  const T given_raw = row[good ? target : 0];
+  mask_group(0, now);
+  const float single = alone >= 0 ? widen(single_raw) : -INFINITY;
   float most = single;
 #pragma unroll
   for (int k = 0; k < kGroup; ++k)
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) most = fmaxf(most, widen(look[k].v[i]));
+    for (int i = 0; i < kVec; ++i) most = fmaxf(most, widen(now[k].v[i]));
 
-  Key least = 0;
+  uint32_t least = 0;
+  int last = INT32_MAX;              // of those equal to `least`, indices up to here
   float least_value = -INFINITY;
-  if (threadIdx.x == 0) sh.count = 0;
   auto offer = [&](float v, int j) {
-    const Key key = key_of(v, static_cast<int>(begin) + j);
-    if (key >= least) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kCandidates) sh.list[at] = key;
-    }
+    if (!(v >= least_value) || (order_of(v) == least && j > last)) return;
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < sh.kCandidates) sh.list[at] = key_of(v, static_cast<int>(begin) + j);
   };
-  if (kTop) {
-    // the thread's largest, with the lowest index that has it
-    int at = -1;
-    if (single == most && threadIdx.x < rest) at = units * kVec + threadIdx.x;
-#pragma unroll
-    for (int k = kGroup - 1; k >= 0; --k) {
-      const int u = threadIdx.x + k * kThreads;
-      if (u < units)
-#pragma unroll
-        for (int i = kVec - 1; i >= 0; --i)
-          if (widen(look[k].v[i]) == most) at = u * kVec + i;
-    }
-    sh.list[threadIdx.x] = at < 0 ? 0 : key_of(most, static_cast<int>(begin) + at);
+  if constexpr (kTop) {
+    const bool has = tid < units || alone >= 0;
+    sh.high[tid] = has ? order_of(most) : 0;
+    if (tid == 0) sh.count = 0;
     __syncthreads();
-    find_threshold(sh, kThreads, out.top);
-    least = sh.threshold;
-    least_value = least ? value_of(least) : -INFINITY;
+    // 128 sets of neighbouring threads, two to a lane, the same in every wave
+    constexpr int kSet = NT / (2 * kWave);
+    uint32_t high[2] = {0, 0};
 #pragma unroll
-    for (int k = 0; k < kGroup; ++k) {
-      const int u = threadIdx.x + k * kThreads;
-      if (u < units && most >= least_value)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i)
-          if (widen(look[k].v[i]) >= least_value) offer(widen(look[k].v[i]), u * kVec + i);
+    for (int i = 0; i < 2 * kSet; ++i) {
+      const uint32_t h = sh.high[lane * 2 * kSet + i];
+      high[i / kSet] = h > high[i / kSet] ? h : high[i / kSet];
     }
-    if (threadIdx.x < rest && single >= least_value) offer(single, units * kVec + threadIdx.x);
+    // (2-byte types widen to words whose last bits are all the same)
+    constexpr int kSkip = sizeof(T) == 2 ? 13 : 0;
+    constexpr uint32_t kRest = (1u << kSkip) - 1;
+    least = kth_largest<kSkip>(high[0], high[1], out.top);
+    if (least && count_above(high[0], high[1], least - 1) > out.top + 16) {
+      // many equal ones: tell them by their indices
+      uint32_t mine = 0;                              // the whole of that word
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if ((high[u] & ~kRest) == least) mine = high[u];
+      least = read_lane(static_cast<int>(mine),
+                        __ffsll(static_cast<unsigned long long>(__ballot(mine != 0))) - 1);
+      int at = INT32_MAX;                             // the thread's first that equals it
+      if (alone >= 0 && order_of(single) == least) at = alone;
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const int j = head + (k * NT + tid) * kVec + i;
+          if (k * NT + tid < units && order_of(widen(now[k].v[i])) == least && j < at) at = j;
+        }
+      sh.at[tid] = at;
+      __syncthreads();
+      uint32_t early[2] = {0, 0};                     // ~index: larger for what comes first
+#pragma unroll
+      for (int i = 0; i < 2 * kSet; ++i) {
+        const int j = sh.at[lane * 2 * kSet + i];
+        const uint32_t e = j == INT32_MAX ? 0 : ~static_cast<uint32_t>(j);
+        early[i / kSet] = e > early[i / kSet] ? e : early[i / kSet];
+      }
+      // a set with a larger one counts for that
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (high[u] > least) early[u] = 0;
+      last = static_cast<int>(~kth_largest<0>(
+          early[0], early[1], out.top - count_above(high[0], high[1], least)));
+      if (last < 0) last = INT32_MAX;
+    }
+    least_value = least > 0x007FFFFFu ? value_of(least) : -INFINITY;
+    if (most >= least_value) {
+#pragma unroll 1
+      for (int k = 0; k < kGroup; ++k) {
+        const int u = k * NT + tid;
+        const Unit p = k == 0 ? now[0] : now[kGroup - 1];
+        if (u < units)
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) offer(widen(p.v[i]), head + u * kVec + i);
+      }
+      if (alone >= 0) offer(single, alone);
+    }
   }
 
-  // a wave that has seen nothing but -inf looks again at every group
-  float seen = wave_max(most);
+  float seen = wave_max(most), s = 0.f, t = 0.f;
   float m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
-  float s = 0.f, t = 0.f;
   auto add = [&](float v) {
     const float y = fmaf(v, kLog2e, -m2), e = exp2_fast(y);
     s += e;
     if (kEntropy) t = fmaf(e, fmaxf(y, -1e30f), t);
   };
-#pragma unroll
-  for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) add(widen(look[k].v[i]));
   add(single);
-
-  auto take = [&](const Pack<T, kVec>& p, int u) {
+  for (int k0 = 0;;) {
+    if (k0 && seen == -INFINITY) {
+      // a wave that has seen nothing but -inf looks again
+      float high = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) add(widen(p.v[i]));
-    if (kTop) {
-      float high = widen(p.v[0]);
+      for (int k = 0; k < kGroup; ++k)
+        if (k0 + k < rounds)
 #pragma unroll
-      for (int i = 1; i < kVec; ++i) high = fmaxf(high, widen(p.v[i]));
-      if (high >= least_value)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i)
-          if (widen(p.v[i]) >= least_value) offer(widen(p.v[i]), u * kVec + i);
+          for (int i = 0; i < kVec; ++i) high = fmaxf(high, widen(now[k].v[i]));
+      seen = wave_max(high);
+      m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
     }
-  };
-  auto look_again = [&](const Pack<T, kVec>& p) {
-    float high = widen(p.v[0]);
-#pragma unroll
-    for (int i = 1; i < kVec; ++i) high = fmaxf(high, widen(p.v[i]));
-    seen = wave_max(high);
-    m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
-  };
-  int u = kGroup * kThreads + threadIdx.x;
-  for (; u + (kGroup - 1) * kThreads < units; u += kGroup * kThreads) {
-    Pack<T, kVec> p[kGroup];
-#pragma unroll
-    for (int k = 0; k < kGroup; ++k) p[k] = load<kVec>(x + (u + k * kThreads) * kVec);
 #pragma unroll
     for (int k = 0; k < kGroup; ++k) {
-      if (seen == -INFINITY) look_again(p[k]);
-      take(p[k], u + k * kThreads);
+      if (k0 + k >= rounds) break;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) add(widen(now[k].v[i]));
+      if (kTop && k0) {
+        float high = widen(now[k].v[0]);
+#pragma unroll
+        for (int i = 1; i < kVec; ++i) high = fmaxf(high, widen(now[k].v[i]));
+        const int u = (k0 + k) * NT + tid;
+        if (high >= least_value && u < units)
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) offer(widen(now[k].v[i]), head + u * kVec + i);
+      }
     }
-  }
-  for (; u < units; u += kThreads) {
-    const Pack<T, kVec> p = load<kVec>(x + u * kVec);
-    if (seen == -INFINITY) look_again(p);
-    take(p, u);
+    k0 += kGroup;
+    if (k0 >= rounds) break;
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) now[k] = next[k];
+    load_group(k0 + kGroup, next);
+    if (k0 + kGroup >= rounds) mask_group(k0, now);
   }
 
   s = wave_sum(s);
   if (kEntropy) t = wave_sum(t);
-  if (lane == 0) sh.sums[wave] = Sums{m2, s, t};
+  if (lane == 0) sums[wave] = Sums{m2, s, t};
   __syncthreads();
-  Sums all = sh.sums[0];
-  for (int w = 1; w < kWaves; ++w) all = join(all, sh.sums[w]);
-  bool give_up = !(all.s < INFINITY);
+  bool give_up = false;
+#pragma unroll
   for (int w = 0; w < kWaves; ++w)
-    give_up |= !(sh.sums[w].s < INFINITY) || !(fabsf(sh.sums[w].m2) <= 1 << 20);
+    give_up |= !(sums[w].s < INFINITY) || !(fabsf(sums[w].m2) <= 1 << 20);
+  if (!kTop && !give_up && wave) return;
+  Sums all = sums[0];
+  for (int w = 1; w < kWaves; ++w) all = join(all, sums[w]);
+  const float given = widen(given_raw);
   const int count = kTop ? sh.count : 0;
-  if (kTop) give_up |= count > kCandidates;
+  if (kTop) give_up |= count > sh.kCandidates;
 
   if (split.parts == 1) {
     if (give_up) {
-      slow_row(sh, row, vocab, r, out, target, ignore);
+      slow_row<NT>(value, sh.list, row, vocab, r, out, target, ignore);
       return;
     }
     const Row done(all);
-    if (threadIdx.x == 0) write_row(out, r, done, target, ignore, vocab, given);
-    if (kTop)
+    if (tid == 0) write_row(out, r, done, target, ignore, vocab, given);
+    if constexpr (kTop)
       select_top(sh, count, out.top, [&](int rank, Key key) {
         out.top_id[r * out.top + rank] = index_of(key);
         out.top_logprob[r * out.top + rank] = done.logprob(value_of(key));
@@ -400,27 +480,33 @@ __global__ void __launch_bounds__(kThreads)
     return;
   }
   char* left = split.work + blockIdx.x * split.stride;
-  if (threadIdx.x == 0) *reinterpret_cast<Part*>(left) = Part{all, give_up};
-  if (kTop && !give_up) {
+  if (tid == 0) *reinterpret_cast<Part*>(left) = Part{all, give_up};
+  if constexpr (kTop) {
+    if (give_up) return;
     Key* keys = reinterpret_cast<Key*>(left + sizeof(Part));
-    if (threadIdx.x < out.top) keys[threadIdx.x] = 0;
-    __syncthreads();
+    if (n < out.top) {                               // a last part of few values
+      if (tid < out.top) keys[tid] = 0;
+      __syncthreads();
+    }
     select_top(sh, count, out.top, [&](int rank, Key key) { keys[rank] = key; });
   }
 }
+
+constexpr int kThreads = 512, kFewThreads = 128, kFewUnits = 512;
 
 // A row's parts.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_join_parts(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out,
                  Split split) {
-  __shared__ Shared sh;
+  __shared__ Lists<kThreads> sh;
+  __shared__ float value[kThreads / kWave];
   const int64_t r = blockIdx.x, vocab = logits.width;
   const T* row = static_cast<const T*>(logits.data) + row_start(logits, r);
   const int64_t target = token(targets, r);
   const float given = target >= 0 && target < vocab ? widen(row[target]) : 0.f;
   const char* work = split.work + r * split.parts * split.stride;
-  const int keys = split.parts * out.top;          // at most kCandidates
+  const int keys = split.parts * out.top;          // at most kMost * kWave, as long as the list
   for (int i = threadIdx.x; i < keys; i += kThreads) {
     const int p = i / out.top;
     sh.list[i] =
@@ -441,7 +527,7 @@ __global__ void __launch_bounds__(kThreads)
   }
   __syncthreads();
   if (give_up) {
-    slow_row(sh, row, vocab, r, out, target, ignore);
+    slow_row<kThreads>(value, sh.list, row, vocab, r, out, target, ignore);
     return;
   }
   const Row done(all);
@@ -576,18 +662,28 @@ Split split_of(int64_t n, int64_t vocab, int32_t dtype, int32_t top) {
   return s;
 }
 
+template <typename T, int NT>
+void launch_rows(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
+                 const Outputs& out, const Split& split, hipStream_t s) {
+  const unsigned blocks = static_cast<unsigned>(logits.n * split.parts);
+  if (out.top && out.entropy)
+    k_logprobs<T, NT, true, true><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
+  else if (out.top)
+    k_logprobs<T, NT, true, false><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
+  else if (out.entropy)
+    k_logprobs<T, NT, false, true><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
+  else
+    k_logprobs<T, NT, false, false><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
+}
+
 template <typename T>
 int logprobs_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
                 const Outputs& out, const Split& split, hipStream_t s) {
-  const unsigned blocks = static_cast<unsigned>(logits.n * split.parts);
-  if (out.top && out.entropy)
-    k_logprobs<T, true, true><<<blocks, kThreads, 0, s>>>(logits, targets, ignore, out, split);
-  else if (out.top)
-    k_logprobs<T, true, false><<<blocks, kThreads, 0, s>>>(logits, targets, ignore, out, split);
-  else if (out.entropy)
-    k_logprobs<T, false, true><<<blocks, kThreads, 0, s>>>(logits, targets, ignore, out, split);
+  constexpr int kVec = 16 / sizeof(T);
+  if (logits.width <= kFewUnits * kVec)
+    launch_rows<T, kFewThreads>(logits, targets, ignore, out, split, s);
   else
-    k_logprobs<T, false, false><<<blocks, kThreads, 0, s>>>(logits, targets, ignore, out, split);
+    launch_rows<T, kThreads>(logits, targets, ignore, out, split, s);
   if (int rc = launched()) return rc;
   if (split.parts > 1)
     k_join_parts<T><<<static_cast<unsigned>(logits.n), kThreads, 0, s>>>(logits, targets, ignore,

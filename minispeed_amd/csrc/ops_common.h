@@ -80,6 +80,17 @@ __device__ __forceinline__ void store(T* p, const Pack<T, N>& x) {
   *reinterpret_cast<raw*>(p) = r;
 }
 
+// 16 aligned bytes that are read once: not kept in the caches.
+template <int N, typename T>
+__device__ __forceinline__ Pack<T, N> load_stream(const T* p) {
+  typedef uint32_t raw __attribute__((ext_vector_type(4)));
+  static_assert(N * sizeof(T) == 16, "");
+  const raw r = __builtin_nontemporal_load(reinterpret_cast<const raw*>(p));
+  Pack<T, N> x;
+  __builtin_memcpy(&x, &r, 16);
+  return x;
+}
+
 __device__ __forceinline__ int read_lane(int x, int lane) {
   return __builtin_amdgcn_readlane(x, lane);
 }
