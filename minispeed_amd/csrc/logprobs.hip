@@ -123,14 +123,16 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t r, const R
 constexpr int kMost = MS_OPS_MAX_TOP;
 static_assert(kMost <= kWave, "");
 
-// NT threads: 512, or 128 for vocabularies of at most kFewUnits units.
-template <int NT>
+// For blocks of NT threads; `list` takes C keys.
+template <int NT, int C>
 struct Lists {
-  static constexpr int kCandidates = 8 * NT;
+  static constexpr int kCandidates = C;
   alignas(16) Key list[kCandidates];
+  Key few[256];
   alignas(16) uint32_t high[NT];
   int at[NT];
-  int count;
+  int looks[2 * NT];        // thread + NT * group
+  int look_count, count;
 };
 
 // The largest word (its last kSkip bits 0) that at least k of the wave's 128 are
@@ -149,12 +151,13 @@ __device__ __forceinline__ int count_above(uint32_t a, uint32_t b, uint32_t than
   return __popcll(__ballot(a > than)) + __popcll(__ballot(b > than));
 }
 
-// The k largest of the n keys in `list`, in order: put(rank, key).
-template <int NT, typename Put>
-__device__ __forceinline__ void select_top(Lists<NT>& sh, int n, int k, Put put) {
-  constexpr int kFew = 192;                 // that are counted against each other at once
-  if (n > kFew) {
-    uint32_t high[2] = {0, 0};              // of 128 sets, in every wave
+// The k largest of the n keys in `list`, in order: put(rank, key).  Of more than
+// a wave's, those that 128 sets' maxima leave are counted against each other.
+template <int NT, int C, typename Put>
+__device__ __forceinline__ void select_top(Lists<NT, C>& sh, int n, int k, Put put) {
+  const Key* keys = sh.list;
+  if (n > kWave) {
+    uint32_t high[2] = {0, 0};              // the same in every wave
     for (int i = threadIdx.x & 63; i < n; i += 2 * kWave)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -163,27 +166,27 @@ __device__ __forceinline__ void select_top(Lists<NT>& sh, int n, int k, Put put)
         high[u] = h > high[u] ? h : high[u];
       }
     const uint32_t least = kth_largest<0>(high[0], high[1], k);
-    constexpr int kEach = Lists<NT>::kCandidates / NT;
-    Key mine[kEach];
-#pragma unroll
-    for (int u = 0; u < kEach; ++u) {
-      const int i = threadIdx.x + u * NT;
-      mine[u] = i < n ? sh.list[i] : 0;
-    }
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kEach; ++u)
-      if (mine[u] && mine[u] >> 32 >= least) sh.list[atomicAdd(&sh.count, 1)] = mine[u];
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const Key key = sh.list[i];
+      if (key && key >> 32 >= least) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < 256) sh.few[at] = key;
+      }
+    }
     __syncthreads();
-    n = sh.count;
+    if (sh.count <= 256) {
+      keys = sh.few;
+      n = sh.count;
+    }
   }
   for (int i = threadIdx.x; i < n; i += NT) {
-    const Key key = sh.list[i];
+    const Key key = keys[i];
     int above = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) above += sh.list[j] > key;
+    for (int j = 0; j < n; ++j) above += keys[j] > key;
     if (key && above < k) put(above, key);
   }
 }
@@ -263,27 +266,52 @@ struct Split {
   int64_t stride;
 };
 
+// The largest of the values seen, in as few instructions as the type has.
+template <typename T>
+struct Largest {
+  float value = -INFINITY;
+  template <int N>
+  __device__ __forceinline__ void see(const Pack<T, N>& p) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) value = fmaxf(value, widen(p.v[i]));
+  }
+  __device__ __forceinline__ float get() const { return value; }
+};
+template <>
+struct Largest<f16> {
+  typedef f16 two __attribute__((ext_vector_type(2)));
+  two value = {static_cast<f16>(-INFINITY), static_cast<f16>(-INFINITY)};
+  template <int N>
+  __device__ __forceinline__ void see(const Pack<f16, N>& p) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      value = __builtin_elementwise_max(value, two{p.v[i], p.v[i + 1]});
+  }
+  __device__ __forceinline__ float get() const { return fmaxf(widen(value.x), widen(value.y)); }
+};
+
 // A block takes a row, or a part of one where there are few rows, in groups of
-// some rounds of an aligned 16-byte unit to every thread; the next group is
+// kGroup rounds of an aligned 16-byte unit to every thread; the next group is
 // loaded while one is worked on.  (At the rows' own alignment, 50257 values of 2
 // bytes, units of which 7 of 8 lie across 16 bytes, the loads alone ran at 4.5
 // TB/s instead of 6.8.)
 //
 // The first group gives a reference, one per wave, so that no running maximum
 // is kept: s only overflows where later logits are 88 above all the wave saw,
-// and the row is then done again by slow_row.  It also gives a threshold that at
-// least `top` values reach; what reaches it, a few times `top` values, is put on
-// a list in LDS, of which the largest are taken at the end.
+// and the row is then done again by slow_row.
+//
+// For the alternatives each thread keeps the largest value of its best group and
+// that of its others.  The k-th largest of the threads' values bounds the k-th
+// largest of all from below; the few groups that may reach it are read again,
+// their values that do listed in LDS and counted against each other.
 template <typename T, int NT, bool kTop, bool kEntropy>
-__global__ void __launch_bounds__(NT, 8)
+__global__ void __launch_bounds__(NT, kTop ? 6 : 8)
     k_logprobs(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out, Split split) {
-  constexpr int kVec = 16 / sizeof(T), kWaves = NT / kWave;
-  // rounds to a group; with the lists' registers 2, so that four blocks fit a CU
-  constexpr int kGroup = kTop ? 2 : 4;
+  constexpr int kVec = 16 / sizeof(T), kWaves = NT / kWave, kGroup = 4;
   typedef Pack<T, kVec> Unit;
   __shared__ Sums sums[kWaves];
   __shared__ float value[kWaves];
-  __shared__ Lists<(kTop ? NT : 1)> sh;
+  __shared__ Lists<(kTop ? NT : 1), (kTop ? 1024 : kMost)> sh;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r = blockIdx.x / split.parts, vocab = logits.width;
   const int64_t begin = (blockIdx.x - r * split.parts) * split.length;
@@ -328,86 +356,11 @@ __global__ void __launch_bounds__(NT, 8)
   const T given_raw = row[good ? target : 0];
   mask_group(0, now);
   const float single = alone >= 0 ? widen(single_raw) : -INFINITY;
-  float most = single;
-#pragma unroll
-  for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) most = fmaxf(most, widen(now[k].v[i]));
 
-  uint32_t least = 0;
-  int last = INT32_MAX;              // of those equal to `least`, indices up to here
-  float least_value = -INFINITY;
-  auto offer = [&](float v, int j) {
-    if (!(v >= least_value) || (order_of(v) == least && j > last)) return;
-    const int at = atomicAdd(&sh.count, 1);
-    if (at < sh.kCandidates) sh.list[at] = key_of(v, static_cast<int>(begin) + j);
-  };
-  if constexpr (kTop) {
-    const bool has = tid < units || alone >= 0;
-    sh.high[tid] = has ? order_of(most) : 0;
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    // 128 sets of neighbouring threads, two to a lane, the same in every wave
-    constexpr int kSet = NT / (2 * kWave);
-    uint32_t high[2] = {0, 0};
+  Largest<T> largest;
 #pragma unroll
-    for (int i = 0; i < 2 * kSet; ++i) {
-      const uint32_t h = sh.high[lane * 2 * kSet + i];
-      high[i / kSet] = h > high[i / kSet] ? h : high[i / kSet];
-    }
-    // (2-byte types widen to words whose last bits are all the same)
-    constexpr int kSkip = sizeof(T) == 2 ? 13 : 0;
-    constexpr uint32_t kRest = (1u << kSkip) - 1;
-    least = kth_largest<kSkip>(high[0], high[1], out.top);
-    if (least && count_above(high[0], high[1], least - 1) > out.top + 16) {
-      // many equal ones: tell them by their indices
-      uint32_t mine = 0;                              // the whole of that word
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if ((high[u] & ~kRest) == least) mine = high[u];
-      least = read_lane(static_cast<int>(mine),
-                        __ffsll(static_cast<unsigned long long>(__ballot(mine != 0))) - 1);
-      int at = INT32_MAX;                             // the thread's first that equals it
-      if (alone >= 0 && order_of(single) == least) at = alone;
-#pragma unroll
-      for (int k = 0; k < kGroup; ++k)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const int j = head + (k * NT + tid) * kVec + i;
-          if (k * NT + tid < units && order_of(widen(now[k].v[i])) == least && j < at) at = j;
-        }
-      sh.at[tid] = at;
-      __syncthreads();
-      uint32_t early[2] = {0, 0};                     // ~index: larger for what comes first
-#pragma unroll
-      for (int i = 0; i < 2 * kSet; ++i) {
-        const int j = sh.at[lane * 2 * kSet + i];
-        const uint32_t e = j == INT32_MAX ? 0 : ~static_cast<uint32_t>(j);
-        early[i / kSet] = e > early[i / kSet] ? e : early[i / kSet];
-      }
-      // a set with a larger one counts for that
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (high[u] > least) early[u] = 0;
-      last = static_cast<int>(~kth_largest<0>(
-          early[0], early[1], out.top - count_above(high[0], high[1], least)));
-      if (last < 0) last = INT32_MAX;
-    }
-    least_value = least > 0x007FFFFFu ? value_of(least) : -INFINITY;
-    if (most >= least_value) {
-#pragma unroll 1
-      for (int k = 0; k < kGroup; ++k) {
-        const int u = k * NT + tid;
-        const Unit p = k == 0 ? now[0] : now[kGroup - 1];
-        if (u < units)
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) offer(widen(p.v[i]), head + u * kVec + i);
-      }
-      if (alone >= 0) offer(single, alone);
-    }
-  }
-
-  float seen = wave_max(most), s = 0.f, t = 0.f;
+  for (int k = 0; k < kGroup; ++k) largest.see(now[k]);
+  float seen = wave_max(fmaxf(single, largest.get())), s = 0.f, t = 0.f;
   float m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
   auto add = [&](float v) {
     const float y = fmaf(v, kLog2e, -m2), e = exp2_fast(y);
@@ -415,32 +368,32 @@ __global__ void __launch_bounds__(NT, 8)
     if (kEntropy) t = fmaf(e, fmaxf(y, -1e30f), t);
   };
   add(single);
+  float best = largest.get(), others = -INFINITY;
+  int best_group = 0;
   for (int k0 = 0;;) {
     if (k0 && seen == -INFINITY) {
       // a wave that has seen nothing but -inf looks again
-      float high = -INFINITY;
+      Largest<T> here;
 #pragma unroll
       for (int k = 0; k < kGroup; ++k)
-        if (k0 + k < rounds)
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) high = fmaxf(high, widen(now[k].v[i]));
-      seen = wave_max(high);
+        if (k0 + k < rounds) here.see(now[k]);
+      seen = wave_max(here.get());
       m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
     }
+    Largest<T> here;
 #pragma unroll
     for (int k = 0; k < kGroup; ++k) {
       if (k0 + k >= rounds) break;
 #pragma unroll
       for (int i = 0; i < kVec; ++i) add(widen(now[k].v[i]));
-      if (kTop && k0) {
-        float high = widen(now[k].v[0]);
-#pragma unroll
-        for (int i = 1; i < kVec; ++i) high = fmaxf(high, widen(now[k].v[i]));
-        const int u = (k0 + k) * NT + tid;
-        if (high >= least_value && u < units)
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) offer(widen(now[k].v[i]), head + u * kVec + i);
-      }
+      if (kTop) here.see(now[k]);
+    }
+    if (kTop && k0) {
+      const float high = here.get();
+      const bool better = high > best;
+      others = fmaxf(others, better ? best : high);
+      best_group = better ? k0 / kGroup : best_group;
+      best = better ? high : best;
     }
     k0 += kGroup;
     if (k0 >= rounds) break;
@@ -453,6 +406,11 @@ __global__ void __launch_bounds__(NT, 8)
   s = wave_sum(s);
   if (kEntropy) t = wave_sum(t);
   if (lane == 0) sums[wave] = Sums{m2, s, t};
+  const float most = fmaxf(single, best);
+  if constexpr (kTop) {
+    sh.high[tid] = tid < units || alone >= 0 ? order_of(most) : 0;
+    if (tid == 0) sh.count = sh.look_count = 0;
+  }
   __syncthreads();
   bool give_up = false;
 #pragma unroll
@@ -462,8 +420,106 @@ __global__ void __launch_bounds__(NT, 8)
   Sums all = sums[0];
   for (int w = 1; w < kWaves; ++w) all = join(all, sums[w]);
   const float given = widen(given_raw);
-  const int count = kTop ? sh.count : 0;
-  if (kTop) give_up |= count > sh.kCandidates;
+
+  if constexpr (kTop) {
+    if (!give_up) {
+      // 128 sets of neighbouring threads, two to a lane, the same in every wave
+      constexpr int kSet = NT / (2 * kWave);
+      uint32_t high[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 2 * kSet; ++i) {
+        const uint32_t h = sh.high[lane * 2 * kSet + i];
+        high[i / kSet] = h > high[i / kSet] ? h : high[i / kSet];
+      }
+      // (2-byte types widen to words whose last bits are all the same)
+      constexpr int kSkip = sizeof(T) == 2 ? 13 : 0;
+      constexpr uint32_t kRest = (1u << kSkip) - 1;
+      uint32_t least = kth_largest<kSkip>(high[0], high[1], out.top);
+      int last = INT32_MAX;              // of those equal to `least`, indices up to here
+      constexpr int kAgain = 2;
+      auto unit_of = [&](int k, int thread) {
+        return load<kVec>(first + static_cast<int64_t>(k * NT + thread) * kVec);
+      };
+      if (least && count_above(high[0], high[1], least - 1) > out.top + 16) {
+        // many equal ones: tell them by their indices
+        uint32_t mine = 0;                              // the whole of that word
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if ((high[u] & ~kRest) == least) mine = high[u];
+        least = read_lane(static_cast<int>(mine),
+                          __ffsll(static_cast<unsigned long long>(__ballot(mine != 0))) - 1);
+        int at = INT32_MAX;                             // the thread's first that equals it
+        if (alone >= 0 && order_of(single) == least) at = alone;
+        if (order_of(most) >= least)
+          for (int k = 0; k * NT + tid < units; ++k) {
+            const Unit p = unit_of(k, tid);
+#pragma unroll
+            for (int i = kVec - 1; i >= 0; --i) {
+              const int j = head + (k * NT + tid) * kVec + i;
+              if (order_of(widen(p.v[i])) == least && j < at) at = j;
+            }
+            if (at != INT32_MAX && at != alone) break;
+          }
+        sh.at[tid] = at;
+        __syncthreads();
+        uint32_t early[2] = {0, 0};                     // ~index: larger for what comes first
+#pragma unroll
+        for (int i = 0; i < 2 * kSet; ++i) {
+          const int j = sh.at[lane * 2 * kSet + i];
+          const uint32_t e = j == INT32_MAX ? 0 : ~static_cast<uint32_t>(j);
+          early[i / kSet] = e > early[i / kSet] ? e : early[i / kSet];
+        }
+        // a set with a larger one counts for that
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (high[u] > least) early[u] = 0;
+        last = static_cast<int>(~kth_largest<0>(
+            early[0], early[1], out.top - count_above(high[0], high[1], least)));
+        if (last < 0) last = INT32_MAX;
+      }
+      auto offer = [&](float v, int j) {
+        const uint32_t o = order_of(v);
+        if (o < least || (o == least && j > last)) return;
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < sh.kCandidates) sh.list[at] = key_of(v, static_cast<int>(begin) + j);
+      };
+      const float least_value = least > 0x007FFFFFu ? value_of(least) : -INFINITY;
+      if (alone >= 0) offer(single, alone);
+      if (tid < units && order_of(best) >= least)
+        for (int g = 0; g * kGroup * NT + tid < units; ++g) {
+          // (of a thread whose best only equals `least`, groups behind `last` are out)
+          const bool out_of_reach =
+              order_of(best) == least && (g * kGroup * NT + tid) * kVec + head > last;
+          if ((g == best_group || order_of(others) >= least) && !out_of_reach) {
+            const int at = atomicAdd(&sh.look_count, 1);
+            if (at < 2 * NT) sh.looks[at] = tid + NT * g;
+          }
+        }
+      __syncthreads();
+      const int again = sh.look_count < 2 * NT ? sh.look_count * kGroup : 0;
+      for (int i0 = tid; i0 < again; i0 += kAgain * NT) {
+        Unit p[kAgain];
+        int u[kAgain];
+#pragma unroll
+        for (int j = 0; j < kAgain; ++j) {
+          const int i = i0 + j * NT < again ? i0 + j * NT : i0;
+          const int look = sh.looks[i / kGroup];
+          u[j] = ((look / NT) * kGroup + i % kGroup) * NT + look % NT;
+          p[j] = load<kVec>(first + static_cast<int64_t>(u[j] < units ? u[j] : 0) * kVec);
+          if (i0 + j * NT >= again) u[j] = units;
+        }
+#pragma unroll
+        for (int j = 0; j < kAgain; ++j)
+          if (u[j] < units)
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+              if (widen(p[j].v[i]) >= least_value)
+                offer(widen(p[j].v[i]), head + u[j] * kVec + i);
+      }
+      __syncthreads();
+      give_up = sh.count > sh.kCandidates || sh.look_count >= 2 * NT;
+    }
+  }
 
   if (split.parts == 1) {
     if (give_up) {
@@ -473,7 +529,7 @@ __global__ void __launch_bounds__(NT, 8)
     const Row done(all);
     if (tid == 0) write_row(out, r, done, target, ignore, vocab, given);
     if constexpr (kTop)
-      select_top(sh, count, out.top, [&](int rank, Key key) {
+      select_top(sh, sh.count, out.top, [&](int rank, Key key) {
         out.top_id[r * out.top + rank] = index_of(key);
         out.top_logprob[r * out.top + rank] = done.logprob(value_of(key));
       });
@@ -488,25 +544,29 @@ __global__ void __launch_bounds__(NT, 8)
       if (tid < out.top) keys[tid] = 0;
       __syncthreads();
     }
-    select_top(sh, count, out.top, [&](int rank, Key key) { keys[rank] = key; });
+    select_top(sh, sh.count, out.top, [&](int rank, Key key) { keys[rank] = key; });
   }
 }
 
-constexpr int kThreads = 512, kFewThreads = 128, kFewUnits = 512;
+// Threads to a block.  With alternatives 256, of which more fit a CU beside their
+// LDS and end together: 8192 x 50257 bf16 with entropy, 8 and 50 alternatives
+// 143 and 187 us, 198 and 226 with 512 (and 1024 or 4096 keys to the list: 143
+// and 170).  Without, 512: 126 us, 130 with 256.  Small vocabularies: 128.
+constexpr int kThreads = 512, kTopThreads = 256, kFewThreads = 128, kFewUnits = 512;
 
 // A row's parts.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_join_parts(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out,
                  Split split) {
-  __shared__ Lists<kThreads> sh;
+  __shared__ Lists<kThreads, kMost * kWave> sh;
   __shared__ float value[kThreads / kWave];
   const int64_t r = blockIdx.x, vocab = logits.width;
   const T* row = static_cast<const T*>(logits.data) + row_start(logits, r);
   const int64_t target = token(targets, r);
   const float given = target >= 0 && target < vocab ? widen(row[target]) : 0.f;
   const char* work = split.work + r * split.parts * split.stride;
-  const int keys = split.parts * out.top;          // at most kMost * kWave, as long as the list
+  const int keys = split.parts * out.top;          // no more than the list takes
   for (int i = threadIdx.x; i < keys; i += kThreads) {
     const int p = i / out.top;
     sh.list[i] =
@@ -648,7 +708,7 @@ __global__ void __launch_bounds__(kGradThreads)
 // How a row is split: not at all from 512 rows on, two blocks to a CU; else so
 // that there are as many blocks, each with a unit to every thread at least.
 Split split_of(int64_t n, int64_t vocab, int32_t dtype, int32_t top) {
-  const int64_t least = kThreads * (16 / dtype_bytes(dtype));
+  const int64_t least = (top ? kTopThreads : kThreads) * (16 / dtype_bytes(dtype));
   Split s;
   const int64_t wanted = std::min<int64_t>(kWave, 512 / std::max<int64_t>(n, 1));
   s.length = vocab;
@@ -662,28 +722,29 @@ Split split_of(int64_t n, int64_t vocab, int32_t dtype, int32_t top) {
   return s;
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool kTop>
 void launch_rows(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
                  const Outputs& out, const Split& split, hipStream_t s) {
   const unsigned blocks = static_cast<unsigned>(logits.n * split.parts);
-  if (out.top && out.entropy)
-    k_logprobs<T, NT, true, true><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
-  else if (out.top)
-    k_logprobs<T, NT, true, false><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
-  else if (out.entropy)
-    k_logprobs<T, NT, false, true><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
+  if (out.entropy)
+    k_logprobs<T, NT, kTop, true><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
   else
-    k_logprobs<T, NT, false, false><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
+    k_logprobs<T, NT, kTop, false><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
 }
 
 template <typename T>
 int logprobs_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
                 const Outputs& out, const Split& split, hipStream_t s) {
   constexpr int kVec = 16 / sizeof(T);
-  if (logits.width <= kFewUnits * kVec)
-    launch_rows<T, kFewThreads>(logits, targets, ignore, out, split, s);
+  const bool few = logits.width <= kFewUnits * kVec;
+  if (few && out.top)
+    launch_rows<T, kFewThreads, true>(logits, targets, ignore, out, split, s);
+  else if (few)
+    launch_rows<T, kFewThreads, false>(logits, targets, ignore, out, split, s);
+  else if (out.top)
+    launch_rows<T, kTopThreads, true>(logits, targets, ignore, out, split, s);
   else
-    launch_rows<T, kThreads>(logits, targets, ignore, out, split, s);
+    launch_rows<T, kThreads, false>(logits, targets, ignore, out, split, s);
   if (int rc = launched()) return rc;
   if (split.parts > 1)
     k_join_parts<T><<<static_cast<unsigned>(logits.n), kThreads, 0, s>>>(logits, targets, ignore,
