@@ -2,6 +2,11 @@
 //
 // Blocks of 32 values share a power-of-two scale, so that dividing by it is
 // exact and a code is one rounding of the value.
+//
+// All kernels stream: a lane takes units of 16 bytes of the unheld type, 8 or 4
+// values, so that 4 or 8 neighbouring lanes have a block.  They are bound by
+// memory, the error-function GELU of 2-byte types (29 instructions and two
+// quarter-rate ones a value, forward) about as much by arithmetic.
 
 #include "ops_common.h"
 
@@ -25,9 +30,6 @@ __device__ __forceinline__ float inverse_step(uint32_t e) {
 }
 __device__ __forceinline__ float step_of(uint32_t e) {
   return e == 255u ? quiet_nan() : __uint_as_float(e << 23);
-}
-__device__ __forceinline__ int8_t code_of(float x, uint32_t e) {
-  return e == 255u ? 0 : static_cast<int8_t>(static_cast<int>(rintf(x * inverse_step(e))));
 }
 
 struct Act {
@@ -65,7 +67,7 @@ __device__ __forceinline__ Act act(float x) {
     // Phi(-a) = exp(-a^2 / 2) Q(a), Q = erfcx(a / sqrt 2) / 2 as t P(t) with
     // t = 1 / (1 + 0.37 a): P by a weighted least squares fit of the relative
     // error (2e-7; 5e-7 as evaluated), so the tail needs no difference.
-    const float m = fabsf(x), a = m > 15.f ? 15.f : m;      // NaN stays
+    const float a = __builtin_elementwise_minimum(fabsf(x), 15.f);      // NaN stays
     const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.37f, 1.f));
     float q = -0.0313271917f;
     q = fmaf(q, t, 0.135133371f);
@@ -92,102 +94,397 @@ __device__ __forceinline__ Act act(float x) {
   return logistic_act(x, x, 1.f);
 }
 
-// One thread per block of 32.
-template <typename T, bool kRows>
-__device__ __forceinline__ uint32_t hold(const T* x, const ms_rows_t& m, int64_t i0, int64_t n,
-                                         int8_t* codes, uint8_t* exponents) {
-  uint32_t most = 0;
-  for (int64_t i = i0; i < n && i < i0 + kBlock; ++i) {
-    const float v = widen(kRows ? x[row_start(m, i / m.width) + i % m.width] : x[i]);
-    const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-    most = b > most ? b : most;
+template <typename T>
+struct Units {
+  static constexpr int kVec = 16 / sizeof(T), kLanes = kBlock / kVec;
+  typedef Pack<T, kVec> Unit;
+  typedef typename raw_of<kVec>::type Codes;         // kVec codes, 4 or 8 bytes
+};
+// Any byte alignment: a checkpoint may begin anywhere.
+typedef uint32_t any4 __attribute__((aligned(1)));
+typedef uint32_t any8 __attribute__((ext_vector_type(2), aligned(1)));
+
+// The block's largest magnitude as fp32 bits, in each of its lanes.
+__device__ __forceinline__ uint32_t lanes_max(uint32_t m, int lanes) {
+#define STEP(ctrl)                                                                             \
+  {                                                                                            \
+    const uint32_t o = __builtin_amdgcn_update_dpp(0, m, ctrl, 0xf, 0xf, true);                \
+    m = o > m ? o : m;                                                                         \
   }
-  const uint32_t e = exponent_of(most);
-  exponents[i0 / kBlock] = static_cast<uint8_t>(e);
-  for (int64_t i = i0; i < n && i < i0 + kBlock; ++i)
-    codes[i] = code_of(widen(kRows ? x[row_start(m, i / m.width) + i % m.width] : x[i]), e);
-  return e;
+  STEP(0xB1);                       // quad_perm 1 0 3 2
+  STEP(0x4E);                       // quad_perm 2 3 0 1
+  if (lanes == 8) STEP(0x141);      // row_half_mirror: the other four
+#undef STEP
+  return m;
+}
+// Magnitudes compare as whole numbers, 2-byte types' two at a time.
+__device__ __forceinline__ uint32_t block_max(const Pack<float, 4>& x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = __float_as_uint(x.v[i]) & 0x7FFFFFFFu;
+    m = b > m ? b : m;
+  }
+  return lanes_max(m, 8);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t block_max(const Pack<T, 8>& x) {
+  typedef uint16_t two __attribute__((ext_vector_type(2)));
+  uint32_t w[4];
+  __builtin_memcpy(w, &x, 16);
+  two m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    two b;
+    const uint32_t magnitude = w[i] & 0x7FFF7FFFu;
+    __builtin_memcpy(&b, &magnitude, 4);
+    m = __builtin_elementwise_max(m, b);
+  }
+  const uint16_t most = static_cast<uint16_t>(lanes_max(m.x > m.y ? m.x : m.y, 4));
+  T as;
+  __builtin_memcpy(&as, &most, 2);
+  return __float_as_uint(widen(as));
 }
 
+// Codes of N values: adding 1.5 * 2^23 rounds x / step to nearest even and
+// leaves it in the low byte; an infinity or NaN (inverse step 0) leaves 0.
+template <int N>
+__device__ __forceinline__ void encode(const float (&x)[N], float inverse, uint32_t (&codes)[N / 4]) {
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    uint32_t k[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      k[j] = __float_as_uint(fmaf(x[4 * i + j], inverse, 12582912.f));
+    const uint32_t lo = __builtin_amdgcn_perm(k[1], k[0], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(k[3], k[2], 0x0c0c0400u);
+    codes[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+  }
+}
+template <int N>
+__device__ __forceinline__ void decode(const uint32_t (&codes)[N / 4], float step, float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    x[i] = static_cast<float>(static_cast<int8_t>(codes[i / 4] >> (8 * (i % 4)))) * step;
+}
+
+__device__ __forceinline__ void put_codes(int8_t* p, const uint32_t (&c)[1]) {
+  __builtin_nontemporal_store(c[0], reinterpret_cast<any4*>(p));
+}
+__device__ __forceinline__ void put_codes(int8_t* p, const uint32_t (&c)[2]) {
+  __builtin_nontemporal_store(any8{c[0], c[1]}, reinterpret_cast<any8*>(p));
+}
+__device__ __forceinline__ void get_codes(const int8_t* p, uint32_t (&c)[1]) {
+  c[0] = __builtin_nontemporal_load(reinterpret_cast<const any4*>(p));
+}
+__device__ __forceinline__ void get_codes(const int8_t* p, uint32_t (&c)[2]) {
+  const any8 v = __builtin_nontemporal_load(reinterpret_cast<const any8*>(p));
+  c[0] = v.x;
+  c[1] = v.y;
+}
+
+// kWhole in what follows: all of the block's units lie within n.  It is asked
+// once for the block; a branch at every load would wait for each.
+
+// Writes the 8-bit form of the unit at `i` of n values; all lanes of its block
+// take part.  Values from n on are zeros.
+template <bool kWhole, typename T>
+__device__ __forceinline__ void hold(const typename Units<T>::Unit& x,
+                                     const float (&v)[Units<T>::kVec], int64_t i, int64_t n,
+                                     int8_t* codes, uint8_t* exponents) {
+  constexpr int N = Units<T>::kVec;
+  const uint32_t e = exponent_of(block_max(x));
+  uint32_t c[N / 4];
+  encode(v, inverse_step(e), c);
+  if (kWhole || i + N <= n) {
+    put_codes(codes + i, c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j < n) codes[i + j] = static_cast<int8_t>(c[j / 4] >> (8 * (j % 4)));
+  }
+  if (i % kBlock == 0 && (kWhole || i < n)) exponents[i / kBlock] = static_cast<uint8_t>(e);
+}
+// The values of the unit at `i`, those from n on zeros.
+template <bool kWhole, typename T>
+__device__ __forceinline__ void fetch(const int8_t* codes, const uint8_t* exponents, int64_t i,
+                                      int64_t n, uint32_t (&c)[Units<T>::kVec / 4], uint32_t& e) {
+  constexpr int N = Units<T>::kVec;
+  if (kWhole) {
+    e = exponents[i / kBlock];
+    get_codes(codes + i, c);
+    return;
+  }
+  e = 1;
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) c[j] = 0;
+  if (i < n) e = exponents[i / kBlock];
+  if (i + N <= n) {
+    get_codes(codes + i, c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j < n)
+        c[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(codes[i + j])) << (8 * (j % 4));
+  }
+}
+template <bool kWhole, typename T>
+__device__ __forceinline__ typename Units<T>::Unit fetch(const T* x, int64_t i, int64_t n) {
+  constexpr int N = Units<T>::kVec;
+  if (kWhole || i + N <= n) return load_stream_any<N>(x + i);
+  typename Units<T>::Unit u;
+#pragma unroll
+  for (int j = 0; j < N; ++j) u.v[j] = i + j < n ? x[i + j] : static_cast<T>(0.f);
+  return u;
+}
+template <bool kWhole, typename T>
+__device__ __forceinline__ void put(T* x, int64_t i, int64_t n, const float (&v)[Units<T>::kVec]) {
+  constexpr int N = Units<T>::kVec;
+  typename Units<T>::Unit u;
+#pragma unroll
+  for (int j = 0; j < N; ++j) u.v[j] = narrow<T>(v[j]);
+  if (kWhole || i + N <= n) {
+    store_stream_any<N>(x + i, u);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j < n) x[i + j] = u.v[j];
+  }
+}
+
+constexpr int kThreads = 256;
+constexpr int kEach = 2;                  // units to a lane, in flight together
+
+// Where unit k of this lane begins.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__device__ __forceinline__ bool block_within(int64_t n) {
+  return (static_cast<int64_t>(blockIdx.x) + 1) * (kEach * kThreads * Units<T>::kVec) <= n;
+}
+template <typename T>
+__device__ __forceinline__ int64_t unit_at(int k) {
+  return ((static_cast<int64_t>(blockIdx.x) * kEach + k) * kThreads + threadIdx.x) *
+         Units<T>::kVec;
+}
+
+template <bool kWhole, typename T>
+__device__ __forceinline__ void pack_block(const T* x, int64_t n, int8_t* codes, uint8_t* exponents) {
+  constexpr int N = Units<T>::kVec;
+  typename Units<T>::Unit u[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) u[k] = fetch<kWhole>(x, unit_at<T>(k), n);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    float v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = widen(u[k].v[j]);
+    hold<kWhole, T>(u[k], v, unit_at<T>(k), n, codes, exponents);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
     k_pack(const T* x, int64_t n, int8_t* codes, uint8_t* exponents) {
-  const ms_rows_t none = {};
-  for (int64_t b = blockIdx.x * 256ll + threadIdx.x; b * kBlock < n; b += gridDim.x * 256ll)
-    hold<T, false>(x, none, b * kBlock, n, codes, exponents);
+  if (block_within<T>(n))
+    pack_block<true, T>(x, n, codes, exponents);
+  else
+    pack_block<false, T>(x, n, codes, exponents);
 }
 
+template <bool kWhole, typename T>
+__device__ __forceinline__ void unpack_block(const int8_t* codes, const uint8_t* exponents, int64_t n, T* out) {
+  constexpr int N = Units<T>::kVec;
+  uint32_t c[kEach][N / 4], e[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) fetch<kWhole, T>(codes, exponents, unit_at<T>(k), n, c[k], e[k]);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    float v[N];
+    decode(c[k], step_of(e[k]), v);
+    put<kWhole>(out, unit_at<T>(k), n, v);
+  }
+}
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
     k_unpack(const int8_t* codes, const uint8_t* exponents, int64_t n, T* out) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll)
-    out[i] = narrow<T>(static_cast<float>(codes[i]) * step_of(exponents[i / kBlock]));
+  if (block_within<T>(n))
+    unpack_block<true, T>(codes, exponents, n, out);
+  else
+    unpack_block<false, T>(codes, exponents, n, out);
 }
 
-template <typename T, int K>
-__global__ void __launch_bounds__(256)
+// Rows that are not one after the other: units within a row (kRows 1), or value
+// by value (2).
+template <bool kWhole, typename T, int kRows>
+__device__ __forceinline__ typename Units<T>::Unit fetch_rows(const ms_rows_t& m, int64_t i,
+                                                              int64_t n) {
+  constexpr int N = Units<T>::kVec;
+  const T* x = static_cast<const T*>(m.data);
+  if (kRows == 0) return fetch<kWhole>(x, i, n);
+  typename Units<T>::Unit u;
+  if (kRows == 1) {
+    const int64_t at = kWhole || i < n ? i : 0, r = at / m.width;
+    u = load_stream_any<N>(x + row_start(m, r) + (at - r * m.width));
+    if (!kWhole && i >= n)
+#pragma unroll
+      for (int j = 0; j < N; ++j) u.v[j] = static_cast<T>(0.f);
+    return u;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int64_t at = i + j < n ? i + j : 0, r = at / m.width;
+    u.v[j] = i + j < n ? x[row_start(m, r) + (at - r * m.width)] : static_cast<T>(0.f);
+  }
+  return u;
+}
+
+template <bool kWhole, typename T, int K, int kRows>
+__device__ __forceinline__ void act8_block(ms_rows_t h, ms_rows_t up, T* a, int8_t* codes, uint8_t* exponents, int8_t* up_codes,
+         uint8_t* up_exponents) {
+  constexpr int N = Units<T>::kVec;
+  constexpr bool kGated = K == MS_ACT_SWIGLU;
+  const int64_t n = h.n * h.width;
+  typename Units<T>::Unit x[kEach], u[kGated ? kEach : 1];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    x[k] = fetch_rows<kWhole, T, kRows>(h, unit_at<T>(k), n);
+    if constexpr (kGated) u[k] = fetch_rows<kWhole, T, kRows>(up, unit_at<T>(k), n);
+  }
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int64_t i = unit_at<T>(k);
+    float v[N], f[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = widen(x[k].v[j]);
+    hold<kWhole, T>(x[k], v, i, n, codes, exponents);
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = act<K>(v[j]).f;
+    if constexpr (kGated) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = widen(u[k].v[j]);
+      hold<kWhole, T>(u[k], v, i, n, up_codes, up_exponents);
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] *= v[j];
+    }
+    put<kWhole>(a, i, n, f);
+  }
+}
+template <typename T, int K, int kRows>
+__global__ void __launch_bounds__(kThreads)
     k_act8(ms_rows_t h, ms_rows_t up, T* a, int8_t* codes, uint8_t* exponents, int8_t* up_codes,
            uint8_t* up_exponents) {
-  const T* x = static_cast<const T*>(h.data);
-  const T* u = static_cast<const T*>(up.data);
   const int64_t n = h.n * h.width;
-  for (int64_t b = blockIdx.x * 256ll + threadIdx.x; b * kBlock < n; b += gridDim.x * 256ll) {
-    hold<T, true>(x, h, b * kBlock, n, codes, exponents);
-    if (K == MS_ACT_SWIGLU) hold<T, true>(u, up, b * kBlock, n, up_codes, up_exponents);
-    for (int64_t i = b * kBlock; i < n && i < (b + 1) * kBlock; ++i) {
-      float f = act<K>(widen(x[row_start(h, i / h.width) + i % h.width])).f;
-      if (K == MS_ACT_SWIGLU) f *= widen(u[row_start(up, i / up.width) + i % up.width]);
-      a[i] = narrow<T>(f);
-    }
+  if (block_within<T>(n))
+    act8_block<true, T, K, kRows>(h, up, a, codes, exponents, up_codes, up_exponents);
+  else
+    act8_block<false, T, K, kRows>(h, up, a, codes, exponents, up_codes, up_exponents);
+}
+
+template <bool kWhole, typename T, int K, bool kAgain>
+__device__ __forceinline__ void act8_grad_block(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
+              const uint8_t* up_exponents, const T* grad, int64_t n, T* dh, T* dup, T* a) {
+  constexpr int N = Units<T>::kVec;
+  constexpr bool kGated = K == MS_ACT_SWIGLU;
+  uint32_t c[kEach][N / 4], e[kEach], uc[kGated ? kEach : 1][N / 4], ue[kGated ? kEach : 1];
+  typename Units<T>::Unit g[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int64_t i = unit_at<T>(k);
+    fetch<kWhole, T>(codes, exponents, i, n, c[k], e[k]);
+    if constexpr (kGated) fetch<kWhole, T>(up_codes, up_exponents, i, n, uc[k], ue[k]);
+    g[k] = fetch<kWhole>(grad, i, n);
   }
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int64_t i = unit_at<T>(k);
+    float x[N], u[N], d[N], du[N], f[N];
+    decode(c[k], step_of(e[k]), x);
+    if constexpr (kGated) decode(uc[k], step_of(ue[k]), u);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const Act y = act<K>(x[j]);
+      const float gj = widen(g[k].v[j]);
+      if constexpr (kGated) {
+        d[j] = gj * u[j] * y.df;
+        du[j] = gj * y.f;
+        f[j] = y.f * u[j];
+      } else {
+        d[j] = gj * y.df;
+        f[j] = y.f;
+      }
+    }
+    put<kWhole>(dh, i, n, d);
+    if constexpr (kGated) put<kWhole>(dup, i, n, du);
+    if constexpr (kAgain) put<kWhole>(a, i, n, f);
+  }
+}
+template <typename T, int K, bool kAgain>
+__global__ void __launch_bounds__(kThreads)
+    k_act8_grad(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
+                const uint8_t* up_exponents, const T* grad, int64_t n, T* dh, T* dup, T* a) {
+  if (block_within<T>(n))
+    act8_grad_block<true, T, K, kAgain>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup, a);
+  else
+    act8_grad_block<false, T, K, kAgain>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup, a);
+}
+
+// Blocks for n values; 0: too many.
+template <typename T>
+unsigned blocks_for(int64_t n) {
+  constexpr int64_t kValues = kThreads * kEach * Units<T>::kVec;
+  const int64_t blocks = (n + kValues - 1) / kValues;
+  return blocks > INT32_MAX ? 0 : static_cast<unsigned>(blocks);
 }
 
 template <typename T, int K>
-__global__ void __launch_bounds__(256)
-    k_act8_grad(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
-                const uint8_t* up_exponents, const T* grad, int64_t n, T* dh, T* dup, T* a) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const Act r = act<K>(static_cast<float>(codes[i]) * step_of(exponents[i / kBlock]));
-    const float g = widen(grad[i]);
-    if (K == MS_ACT_SWIGLU) {
-      const float u = static_cast<float>(up_codes[i]) * step_of(up_exponents[i / kBlock]);
-      dh[i] = narrow<T>(g * u * r.df);
-      dup[i] = narrow<T>(g * r.f);
-      if (a) a[i] = narrow<T>(r.f * u);
-    } else {
-      dh[i] = narrow<T>(g * r.df);
-      if (a) a[i] = narrow<T>(r.f);
-    }
-  }
-}
-
-unsigned blocks_for(int64_t items) {
-  const int64_t n = (items + 255) / 256, most = 1 << 20;
-  return static_cast<unsigned>(n < most ? n : most);
+int act8_kind(const ms_rows_t& h, const ms_rows_t& up, void* a, int8_t* codes, uint8_t* exponents,
+              int8_t* up_codes, uint8_t* up_exponents, hipStream_t s) {
+  const unsigned blocks = blocks_for<T>(h.n * h.width);
+  if (!blocks) return MS_OPS_EINVAL;
+  T* out = static_cast<T*>(a);
+  auto dense = [](const ms_rows_t& m) {
+    return m.n <= 1 || (m.inner >= m.n && m.inner_stride == m.width);
+  };
+  const bool gated = K == MS_ACT_SWIGLU;
+  if (dense(h) && (!gated || dense(up)))
+    k_act8<T, K, 0><<<blocks, kThreads, 0, s>>>(h, up, out, codes, exponents, up_codes,
+                                                up_exponents);
+  else if (h.width % Units<T>::kVec == 0)
+    k_act8<T, K, 1><<<blocks, kThreads, 0, s>>>(h, up, out, codes, exponents, up_codes,
+                                                up_exponents);
+  else
+    k_act8<T, K, 2><<<blocks, kThreads, 0, s>>>(h, up, out, codes, exponents, up_codes,
+                                                up_exponents);
+  return launched();
 }
 
 template <typename T>
 int act8_as(const ms_rows_t& h, const ms_rows_t& up, int kind, void* a, int8_t* codes,
             uint8_t* exponents, int8_t* up_codes, uint8_t* up_exponents, hipStream_t s) {
-  const unsigned blocks = blocks_for((h.n * h.width + kBlock - 1) / kBlock);
-  T* out = static_cast<T*>(a);
   switch (kind) {
     case MS_ACT_GELU:
-      k_act8<T, MS_ACT_GELU><<<blocks, 256, 0, s>>>(h, up, out, codes, exponents, up_codes,
-                                                    up_exponents);
-      break;
+      return act8_kind<T, MS_ACT_GELU>(h, up, a, codes, exponents, up_codes, up_exponents, s);
     case MS_ACT_GELU_TANH:
-      k_act8<T, MS_ACT_GELU_TANH><<<blocks, 256, 0, s>>>(h, up, out, codes, exponents, up_codes,
-                                                         up_exponents);
-      break;
+      return act8_kind<T, MS_ACT_GELU_TANH>(h, up, a, codes, exponents, up_codes, up_exponents, s);
     case MS_ACT_SILU:
-      k_act8<T, MS_ACT_SILU><<<blocks, 256, 0, s>>>(h, up, out, codes, exponents, up_codes,
-                                                    up_exponents);
-      break;
+      return act8_kind<T, MS_ACT_SILU>(h, up, a, codes, exponents, up_codes, up_exponents, s);
     default:
-      k_act8<T, MS_ACT_SWIGLU><<<blocks, 256, 0, s>>>(h, up, out, codes, exponents, up_codes,
-                                                      up_exponents);
+      return act8_kind<T, MS_ACT_SWIGLU>(h, up, a, codes, exponents, up_codes, up_exponents, s);
   }
+}
+
+template <typename T, int K>
+int grad_kind(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
+              const uint8_t* up_exponents, const void* grad, int64_t n, void* dh, void* dup,
+              void* a, hipStream_t s) {
+  const unsigned blocks = blocks_for<T>(n);
+  if (!blocks) return MS_OPS_EINVAL;
+  const T* g = static_cast<const T*>(grad);
+  T *d = static_cast<T*>(dh), *du = static_cast<T*>(dup), *out = static_cast<T*>(a);
+  if (out)
+    k_act8_grad<T, K, true><<<blocks, kThreads, 0, s>>>(codes, exponents, up_codes, up_exponents,
+                                                        g, n, d, du, out);
+  else
+    k_act8_grad<T, K, false><<<blocks, kThreads, 0, s>>>(codes, exponents, up_codes, up_exponents,
+                                                         g, n, d, du, out);
   return launched();
 }
 
@@ -195,30 +492,39 @@ template <typename T>
 int act8_grad_as(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
                  const uint8_t* up_exponents, const void* grad, int kind, int64_t n, void* dh,
                  void* dup, void* a, hipStream_t s) {
-  const unsigned blocks = blocks_for(n);
-  const T* g = static_cast<const T*>(grad);
-  T *d = static_cast<T*>(dh), *du = static_cast<T*>(dup), *out = static_cast<T*>(a);
   switch (kind) {
     case MS_ACT_GELU:
-      k_act8_grad<T, MS_ACT_GELU><<<blocks, 256, 0, s>>>(codes, exponents, up_codes, up_exponents,
-                                                         g, n, d, du, out);
-      break;
+      return grad_kind<T, MS_ACT_GELU>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup,
+                                       a, s);
     case MS_ACT_GELU_TANH:
-      k_act8_grad<T, MS_ACT_GELU_TANH><<<blocks, 256, 0, s>>>(codes, exponents, up_codes,
-                                                              up_exponents, g, n, d, du, out);
-      break;
+      return grad_kind<T, MS_ACT_GELU_TANH>(codes, exponents, up_codes, up_exponents, grad, n, dh,
+                                            dup, a, s);
     case MS_ACT_SILU:
-      k_act8_grad<T, MS_ACT_SILU><<<blocks, 256, 0, s>>>(codes, exponents, up_codes, up_exponents,
-                                                         g, n, d, du, out);
-      break;
+      return grad_kind<T, MS_ACT_SILU>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup,
+                                       a, s);
     default:
-      k_act8_grad<T, MS_ACT_SWIGLU><<<blocks, 256, 0, s>>>(codes, exponents, up_codes,
-                                                           up_exponents, g, n, d, du, out);
+      return grad_kind<T, MS_ACT_SWIGLU>(codes, exponents, up_codes, up_exponents, grad, n, dh,
+                                         dup, a, s);
   }
-  return launched();
 }
 
 bool good_kind(int32_t k) { return k >= MS_ACT_GELU && k <= MS_ACT_SWIGLU; }
+
+template <typename T>
+int pack_as(const void* x, int64_t n, int8_t* codes, uint8_t* exponents, hipStream_t s) {
+  const unsigned blocks = blocks_for<T>(n);
+  if (!blocks) return MS_OPS_EINVAL;
+  k_pack<T><<<blocks, kThreads, 0, s>>>(static_cast<const T*>(x), n, codes, exponents);
+  return launched();
+}
+template <typename T>
+int unpack_as(const int8_t* codes, const uint8_t* exponents, int64_t n, void* out,
+              hipStream_t s) {
+  const unsigned blocks = blocks_for<T>(n);
+  if (!blocks) return MS_OPS_EINVAL;
+  k_unpack<T><<<blocks, kThreads, 0, s>>>(codes, exponents, n, static_cast<T*>(out));
+  return launched();
+}
 
 }  // namespace
 
@@ -228,18 +534,11 @@ extern "C" int ms_pack8(const void* x, int32_t dtype, int64_t n, int8_t* codes, 
   if (n == 0) return MS_OPS_OK;
   if (!x || !codes || !exponents) return MS_OPS_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned blocks = blocks_for((n + kBlock - 1) / kBlock);
   switch (dtype) {
-    case MS_OPS_F32:
-      k_pack<float><<<blocks, 256, 0, s>>>(static_cast<const float*>(x), n, codes, exponents);
-      break;
-    case MS_OPS_F16:
-      k_pack<f16><<<blocks, 256, 0, s>>>(static_cast<const f16*>(x), n, codes, exponents);
-      break;
-    default:
-      k_pack<bf16><<<blocks, 256, 0, s>>>(static_cast<const bf16*>(x), n, codes, exponents);
+    case MS_OPS_F32: return pack_as<float>(x, n, codes, exponents, s);
+    case MS_OPS_F16: return pack_as<f16>(x, n, codes, exponents, s);
+    default: return pack_as<bf16>(x, n, codes, exponents, s);
   }
-  return launched();
 }
 
 extern "C" int ms_unpack8(const int8_t* codes, const uint8_t* exponents, int64_t n, int32_t dtype,
@@ -248,18 +547,11 @@ extern "C" int ms_unpack8(const int8_t* codes, const uint8_t* exponents, int64_t
   if (n == 0) return MS_OPS_OK;
   if (!out || !codes || !exponents) return MS_OPS_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned blocks = blocks_for(n);
   switch (dtype) {
-    case MS_OPS_F32:
-      k_unpack<float><<<blocks, 256, 0, s>>>(codes, exponents, n, static_cast<float*>(out));
-      break;
-    case MS_OPS_F16:
-      k_unpack<f16><<<blocks, 256, 0, s>>>(codes, exponents, n, static_cast<f16*>(out));
-      break;
-    default:
-      k_unpack<bf16><<<blocks, 256, 0, s>>>(codes, exponents, n, static_cast<bf16*>(out));
+    case MS_OPS_F32: return unpack_as<float>(codes, exponents, n, out, s);
+    case MS_OPS_F16: return unpack_as<f16>(codes, exponents, n, out, s);
+    default: return unpack_as<bf16>(codes, exponents, n, out, s);
   }
-  return launched();
 }
 
 extern "C" int ms_act8(const ms_rows_t* h, const ms_rows_t* up, int32_t kind, void* a,

@@ -607,36 +607,47 @@ __global__ void __launch_bounds__(kThreads)
 constexpr float kFarLse = 256.f;
 
 constexpr int kGradThreads = 256, kGradWaves = kGradThreads / kWave;
-constexpr int kGradGroup = 4;
+constexpr int kGradGroup = 2;             // 16-byte units to a thread; 1, 2, 4: 276, 279, 282 us
 
-// A block takes kGradGroup * kGradThreads units of a row.  With c a whole
-// number near lse L and p' = 2^(x L - c): dx = p' (a + b x), where a and b hold
-// what c rounded off; the target's g is added to the one value.
+// A block takes kGradGroup rounds of aligned 16-byte units of the gradient's row
+// (the logits' row may lie otherwise).  With c a whole number near lse L and
+// p' = 2^(x L - c): dx = p' (a + b x), where a and b hold what c rounded off; the
+// target's g is added to the one value.
 template <typename T, bool kEntropy>
 __global__ void __launch_bounds__(kGradThreads)
     k_logprobs_grad(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, const float* lse,
                     const float* entropy, const float* grad_logprob, const float* grad_entropy,
                     int blocks_per_row, T* __restrict__ out) {
-  constexpr int kVec = 16 / sizeof(T);
+  constexpr int kVec = 16 / sizeof(T), kEach = kGradGroup * kGradThreads;
   __shared__ float slot[kGradWaves];
-  const int64_t r = blockIdx.x / blocks_per_row, vocab = logits.width;
+  const int64_t r = blockIdx.x / static_cast<unsigned>(blocks_per_row);
   const int part = static_cast<int>(blockIdx.x - r * blocks_per_row);
+  const int vocab = static_cast<int>(logits.width), tid = threadIdx.x;
   const T* x = static_cast<const T*>(logits.data) + row_start(logits, r);
   T* d = out + r * vocab;
+  const int off = static_cast<int>(-(reinterpret_cast<uintptr_t>(d) / sizeof(T)) & (kVec - 1));
+  const int head = off < vocab ? off : vocab;
+  const int units = (vocab - head) / kVec, rest = vocab - head - units * kVec;
+
+  Pack<T, kVec> in[kGradGroup];
+#pragma unroll
+  for (int i = 0; i < kGradGroup; ++i) {
+    const int u = part * kEach + i * kGradThreads + tid;
+    if (u < units) in[i] = load_stream_any<kVec>(x + head + static_cast<int64_t>(u) * kVec);
+  }
   const int64_t target = token(targets, r);
-  float g = grad_logprob && target != ignore ? grad_logprob[r] : 0.f;
-  const bool outside = target < 0 || target >= vocab;
-  if (grad_logprob && target != ignore && outside) g = quiet_nan();
+  const bool counts = grad_logprob && target != ignore;
+  float g = counts ? grad_logprob[r] : 0.f;
+  if (counts && (target < 0 || target >= vocab)) g = quiet_nan();
+  const int hit = target >= 0 && target < vocab ? static_cast<int>(target) : -1;
   const float h = kEntropy ? grad_entropy[r] : 0.f, big_h = kEntropy ? entropy[r] : 0.f;
   const float l = lse[r];
 
-  const int units = static_cast<int>(vocab / kVec), rest = static_cast<int>(vocab) - units * kVec;
-  const int first = part * kGradGroup * kGradThreads + threadIdx.x;
   if (l == -INFINITY || fabsf(l) > kFarLse) {
     // every block of the row finds the maximum and the sum for itself
     auto block = [&](float v, auto op) {
       __syncthreads();
-      if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+      if ((tid & 63) == 0) slot[tid >> 6] = v;
       __syncthreads();
       float y = slot[0];
       for (int w = 1; w < kGradWaves; ++w) y = op(y, slot[w]);
@@ -645,23 +656,22 @@ __global__ void __launch_bounds__(kGradThreads)
     float most = 0.f, s = 1.f;
     if (l != -INFINITY) {
       most = -INFINITY;
-      for (int64_t j = threadIdx.x; j < vocab; j += kGradThreads) most = fmaxf(most, widen(x[j]));
+      for (int j = tid; j < vocab; j += kGradThreads) most = fmaxf(most, widen(x[j]));
       most = block(wave_max(most), [](float a, float b) { return fmaxf(a, b); });
       s = 0.f;
-      for (int64_t j = threadIdx.x; j < vocab; j += kGradThreads)
+      for (int j = tid; j < vocab; j += kGradThreads)
         s += exp2_fast((widen(x[j]) - most) * kLog2e);
       s = block(wave_sum(s), [](float a, float b) { return a + b; });
     }
     const float ls = log2_fast(s) * kLn2;
-    const int64_t end = part == blocks_per_row - 1
-                            ? vocab
-                            : static_cast<int64_t>(part + 1) * kGradGroup * kGradThreads * kVec;
-    for (int64_t j = static_cast<int64_t>(part) * kGradGroup * kGradThreads * kVec + threadIdx.x;
-         j < end; j += kGradThreads) {
+    // the first block takes the head too, the last one what is behind the units
+    const int begin = part ? head + part * kEach * kVec : 0;
+    const int end = part == blocks_per_row - 1 ? vocab : head + (part + 1) * kEach * kVec;
+    for (int j = begin + tid; j < end; j += kGradThreads) {
       float dj = 0.f;
       if (l != -INFINITY) {
         const float logp = (widen(x[j]) - most) - ls, p = exp2_fast(logp * kLog2e);
-        dj = j == target ? g - g * p : -g * p;
+        dj = j == hit ? g - g * p : -g * p;
         if (kEntropy && p != 0.f) dj -= h * p * (logp + big_h);
       }
       d[j] = narrow<T>(dj);
@@ -676,33 +686,29 @@ __global__ void __launch_bounds__(kGradThreads)
     if (!kEntropy) return p * a;
     return p * fmaf(b, fmaxf(v, -1e6f), a);        // -inf: p is 0, and 0 * inf must not be
   };
-  Pack<T, kVec> in[kGradGroup];
 #pragma unroll
   for (int i = 0; i < kGradGroup; ++i) {
-    const int u = first + i * kGradThreads;
-    if (u < units) in[i] = load<kVec>(x + static_cast<int64_t>(u) * kVec);
-  }
-#pragma unroll
-  for (int i = 0; i < kGradGroup; ++i) {
-    const int u = first + i * kGradThreads;
+    const int u = part * kEach + i * kGradThreads + tid;
     if (u < units) {
       float y[kVec];
 #pragma unroll
       for (int j = 0; j < kVec; ++j) y[j] = one(widen(in[i].v[j]));
-      const int64_t at = target - static_cast<int64_t>(u) * kVec;
-      if (at >= 0 && at < kVec)
+      const unsigned at = static_cast<unsigned>(hit - head - u * kVec);
+      if (at < kVec && hit >= 0)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) y[j] += at == j ? g : 0.f;
       Pack<T, kVec> z;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) z.v[j] = narrow<T>(y[j]);
-      store<kVec>(d + static_cast<int64_t>(u) * kVec, z);
+      store_stream<kVec>(d + head + static_cast<int64_t>(u) * kVec, z);
     }
   }
-  if (part == blocks_per_row - 1 && threadIdx.x < rest) {
-    const int64_t j = static_cast<int64_t>(units) * kVec + threadIdx.x;
-    d[j] = narrow<T>(one(widen(x[j])) + (j == target ? g : 0.f));
-  }
+  // the values before and behind the units
+  const int alone = part == 0 && tid < head ? tid
+                    : part == blocks_per_row - 1 && tid >= kVec && tid - kVec < rest
+                        ? head + units * kVec + tid - kVec
+                        : -1;
+  if (alone >= 0) d[alone] = narrow<T>(one(widen(x[alone])) + (alone == hit ? g : 0.f));
 }
 
 // How a row is split: not at all from 512 rows on, two blocks to a CU; else so

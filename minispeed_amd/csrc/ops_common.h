@@ -91,6 +91,32 @@ __device__ __forceinline__ Pack<T, N> load_stream(const T* p) {
   return x;
 }
 
+// ... at any element alignment.
+template <int N, typename T>
+__device__ __forceinline__ Pack<T, N> load_stream_any(const T* p) {
+  typedef typename raw_of<N * sizeof(T)>::type raw;
+  const raw r = __builtin_nontemporal_load(reinterpret_cast<const raw*>(p));
+  Pack<T, N> x;
+  __builtin_memcpy(&x, &r, sizeof(r));
+  return x;
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_stream_any(T* p, const Pack<T, N>& x) {
+  typedef typename raw_of<N * sizeof(T)>::type raw;
+  raw r;
+  __builtin_memcpy(&r, &x, sizeof(r));
+  __builtin_nontemporal_store(r, reinterpret_cast<raw*>(p));
+}
+// 16 aligned bytes that are not read soon.
+template <int N, typename T>
+__device__ __forceinline__ void store_stream(T* p, const Pack<T, N>& x) {
+  typedef uint32_t raw __attribute__((ext_vector_type(4)));
+  static_assert(N * sizeof(T) == 16, "");
+  raw r;
+  __builtin_memcpy(&r, &x, 16);
+  __builtin_nontemporal_store(r, reinterpret_cast<raw*>(p));
+}
+
 __device__ __forceinline__ int read_lane(int x, int lane) {
   return __builtin_amdgcn_readlane(x, lane);
 }
