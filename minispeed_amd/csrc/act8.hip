@@ -237,14 +237,17 @@ __device__ __forceinline__ typename Units<T>::Unit fetch(const T* x, int64_t i, 
   for (int j = 0; j < N; ++j) u.v[j] = i + j < n ? x[i + j] : static_cast<T>(0.f);
   return u;
 }
-template <bool kWhole, typename T>
+template <bool kWhole, bool kKeep = false, typename T>
 __device__ __forceinline__ void put(T* x, int64_t i, int64_t n, const float (&v)[Units<T>::kVec]) {
   constexpr int N = Units<T>::kVec;
   typename Units<T>::Unit u;
 #pragma unroll
   for (int j = 0; j < N; ++j) u.v[j] = narrow<T>(v[j]);
   if (kWhole || i + N <= n) {
-    store_stream_any<N>(x + i, u);
+    if (kKeep)
+      store<N>(x + i, u);
+    else
+      store_stream_any<N>(x + i, u);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -252,15 +255,21 @@ __device__ __forceinline__ void put(T* x, int64_t i, int64_t n, const float (&v)
   }
 }
 
+// Units to a lane, in flight together: 2 where few streams meet, 1 where many do.
+// Of fp16, 8192 x 8192, with 2 and 1: forward 60 and 63 us, gated 91 and 87,
+// gated backward 114 both (16384 rows more: 336 and 331), pack 35 and 37, unpack
+// 36 and 32 (2048 rows: 13.2 and 8.7).  Outputs are written past the caches but
+// for the ungated backward's, 72 against 78 us.
 constexpr int kThreads = 256;
-constexpr int kEach = 2;                  // units to a lane, in flight together
+template <int K>
+constexpr int kEachOf = K == MS_ACT_SWIGLU ? 1 : 2;
 
-// Where unit k of this lane begins.
-template <typename T>
+template <typename T, int kEach>
 __device__ __forceinline__ bool block_within(int64_t n) {
   return (static_cast<int64_t>(blockIdx.x) + 1) * (kEach * kThreads * Units<T>::kVec) <= n;
 }
-template <typename T>
+// Where unit k of this lane begins.
+template <typename T, int kEach>
 __device__ __forceinline__ int64_t unit_at(int k) {
   return ((static_cast<int64_t>(blockIdx.x) * kEach + k) * kThreads + threadIdx.x) *
          Units<T>::kVec;
@@ -268,22 +277,23 @@ __device__ __forceinline__ int64_t unit_at(int k) {
 
 template <bool kWhole, typename T>
 __device__ __forceinline__ void pack_block(const T* x, int64_t n, int8_t* codes, uint8_t* exponents) {
+  constexpr int kEach = 2;
   constexpr int N = Units<T>::kVec;
   typename Units<T>::Unit u[kEach];
 #pragma unroll
-  for (int k = 0; k < kEach; ++k) u[k] = fetch<kWhole>(x, unit_at<T>(k), n);
+  for (int k = 0; k < kEach; ++k) u[k] = fetch<kWhole>(x, unit_at<T, kEach>(k), n);
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
     float v[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = widen(u[k].v[j]);
-    hold<kWhole, T>(u[k], v, unit_at<T>(k), n, codes, exponents);
+    hold<kWhole, T>(u[k], v, unit_at<T, kEach>(k), n, codes, exponents);
   }
 }
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_pack(const T* x, int64_t n, int8_t* codes, uint8_t* exponents) {
-  if (block_within<T>(n))
+  if (block_within<T, 2>(n))
     pack_block<true, T>(x, n, codes, exponents);
   else
     pack_block<false, T>(x, n, codes, exponents);
@@ -291,21 +301,22 @@ __global__ void __launch_bounds__(kThreads)
 
 template <bool kWhole, typename T>
 __device__ __forceinline__ void unpack_block(const int8_t* codes, const uint8_t* exponents, int64_t n, T* out) {
+  constexpr int kEach = 1;
   constexpr int N = Units<T>::kVec;
   uint32_t c[kEach][N / 4], e[kEach];
 #pragma unroll
-  for (int k = 0; k < kEach; ++k) fetch<kWhole, T>(codes, exponents, unit_at<T>(k), n, c[k], e[k]);
+  for (int k = 0; k < kEach; ++k) fetch<kWhole, T>(codes, exponents, unit_at<T, kEach>(k), n, c[k], e[k]);
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
     float v[N];
     decode(c[k], step_of(e[k]), v);
-    put<kWhole>(out, unit_at<T>(k), n, v);
+    put<kWhole>(out, unit_at<T, kEach>(k), n, v);
   }
 }
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_unpack(const int8_t* codes, const uint8_t* exponents, int64_t n, T* out) {
-  if (block_within<T>(n))
+  if (block_within<T, 1>(n))
     unpack_block<true, T>(codes, exponents, n, out);
   else
     unpack_block<false, T>(codes, exponents, n, out);
@@ -339,18 +350,19 @@ __device__ __forceinline__ typename Units<T>::Unit fetch_rows(const ms_rows_t& m
 template <bool kWhole, typename T, int K, int kRows>
 __device__ __forceinline__ void act8_block(ms_rows_t h, ms_rows_t up, T* a, int8_t* codes, uint8_t* exponents, int8_t* up_codes,
          uint8_t* up_exponents) {
+  constexpr int kEach = kEachOf<K>;
   constexpr int N = Units<T>::kVec;
   constexpr bool kGated = K == MS_ACT_SWIGLU;
   const int64_t n = h.n * h.width;
   typename Units<T>::Unit x[kEach], u[kGated ? kEach : 1];
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    x[k] = fetch_rows<kWhole, T, kRows>(h, unit_at<T>(k), n);
-    if constexpr (kGated) u[k] = fetch_rows<kWhole, T, kRows>(up, unit_at<T>(k), n);
+    x[k] = fetch_rows<kWhole, T, kRows>(h, unit_at<T, kEach>(k), n);
+    if constexpr (kGated) u[k] = fetch_rows<kWhole, T, kRows>(up, unit_at<T, kEach>(k), n);
   }
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int64_t i = unit_at<T>(k);
+    const int64_t i = unit_at<T, kEach>(k);
     float v[N], f[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = widen(x[k].v[j]);
@@ -372,7 +384,7 @@ __global__ void __launch_bounds__(kThreads)
     k_act8(ms_rows_t h, ms_rows_t up, T* a, int8_t* codes, uint8_t* exponents, int8_t* up_codes,
            uint8_t* up_exponents) {
   const int64_t n = h.n * h.width;
-  if (block_within<T>(n))
+  if (block_within<T, kEachOf<K>>(n))
     act8_block<true, T, K, kRows>(h, up, a, codes, exponents, up_codes, up_exponents);
   else
     act8_block<false, T, K, kRows>(h, up, a, codes, exponents, up_codes, up_exponents);
@@ -381,20 +393,21 @@ __global__ void __launch_bounds__(kThreads)
 template <bool kWhole, typename T, int K, bool kAgain>
 __device__ __forceinline__ void act8_grad_block(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
               const uint8_t* up_exponents, const T* grad, int64_t n, T* dh, T* dup, T* a) {
+  constexpr int kEach = kEachOf<K>;
   constexpr int N = Units<T>::kVec;
   constexpr bool kGated = K == MS_ACT_SWIGLU;
   uint32_t c[kEach][N / 4], e[kEach], uc[kGated ? kEach : 1][N / 4], ue[kGated ? kEach : 1];
   typename Units<T>::Unit g[kEach];
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int64_t i = unit_at<T>(k);
+    const int64_t i = unit_at<T, kEach>(k);
     fetch<kWhole, T>(codes, exponents, i, n, c[k], e[k]);
     if constexpr (kGated) fetch<kWhole, T>(up_codes, up_exponents, i, n, uc[k], ue[k]);
     g[k] = fetch<kWhole>(grad, i, n);
   }
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int64_t i = unit_at<T>(k);
+    const int64_t i = unit_at<T, kEach>(k);
     float x[N], u[N], d[N], du[N], f[N];
     decode(c[k], step_of(e[k]), x);
     if constexpr (kGated) decode(uc[k], step_of(ue[k]), u);
@@ -411,23 +424,23 @@ __device__ __forceinline__ void act8_grad_block(const int8_t* codes, const uint8
         f[j] = y.f;
       }
     }
-    put<kWhole>(dh, i, n, d);
+    put<kWhole, !kGated>(dh, i, n, d);
     if constexpr (kGated) put<kWhole>(dup, i, n, du);
-    if constexpr (kAgain) put<kWhole>(a, i, n, f);
+    if constexpr (kAgain) put<kWhole, !kGated>(a, i, n, f);
   }
 }
 template <typename T, int K, bool kAgain>
 __global__ void __launch_bounds__(kThreads)
     k_act8_grad(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
                 const uint8_t* up_exponents, const T* grad, int64_t n, T* dh, T* dup, T* a) {
-  if (block_within<T>(n))
+  if (block_within<T, kEachOf<K>>(n))
     act8_grad_block<true, T, K, kAgain>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup, a);
   else
     act8_grad_block<false, T, K, kAgain>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup, a);
 }
 
 // Blocks for n values; 0: too many.
-template <typename T>
+template <typename T, int kEach>
 unsigned blocks_for(int64_t n) {
   constexpr int64_t kValues = kThreads * kEach * Units<T>::kVec;
   const int64_t blocks = (n + kValues - 1) / kValues;
@@ -437,7 +450,7 @@ unsigned blocks_for(int64_t n) {
 template <typename T, int K>
 int act8_kind(const ms_rows_t& h, const ms_rows_t& up, void* a, int8_t* codes, uint8_t* exponents,
               int8_t* up_codes, uint8_t* up_exponents, hipStream_t s) {
-  const unsigned blocks = blocks_for<T>(h.n * h.width);
+  const unsigned blocks = blocks_for<T, kEachOf<K>>(h.n * h.width);
   if (!blocks) return MS_OPS_EINVAL;
   T* out = static_cast<T*>(a);
   auto dense = [](const ms_rows_t& m) {
@@ -475,7 +488,7 @@ template <typename T, int K>
 int grad_kind(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
               const uint8_t* up_exponents, const void* grad, int64_t n, void* dh, void* dup,
               void* a, hipStream_t s) {
-  const unsigned blocks = blocks_for<T>(n);
+  const unsigned blocks = blocks_for<T, kEachOf<K>>(n);
   if (!blocks) return MS_OPS_EINVAL;
   const T* g = static_cast<const T*>(grad);
   T *d = static_cast<T*>(dh), *du = static_cast<T*>(dup), *out = static_cast<T*>(a);
@@ -512,7 +525,7 @@ bool good_kind(int32_t k) { return k >= MS_ACT_GELU && k <= MS_ACT_SWIGLU; }
 
 template <typename T>
 int pack_as(const void* x, int64_t n, int8_t* codes, uint8_t* exponents, hipStream_t s) {
-  const unsigned blocks = blocks_for<T>(n);
+  const unsigned blocks = blocks_for<T, 2>(n);
   if (!blocks) return MS_OPS_EINVAL;
   k_pack<T><<<blocks, kThreads, 0, s>>>(static_cast<const T*>(x), n, codes, exponents);
   return launched();
@@ -520,7 +533,7 @@ int pack_as(const void* x, int64_t n, int8_t* codes, uint8_t* exponents, hipStre
 template <typename T>
 int unpack_as(const int8_t* codes, const uint8_t* exponents, int64_t n, void* out,
               hipStream_t s) {
-  const unsigned blocks = blocks_for<T>(n);
+  const unsigned blocks = blocks_for<T, 1>(n);
   if (!blocks) return MS_OPS_EINVAL;
   k_unpack<T><<<blocks, kThreads, 0, s>>>(codes, exponents, n, static_cast<T*>(out));
   return launched();
