@@ -83,7 +83,8 @@ const char* ms_ops_error_string(int code);
 
 /*
  * Embedding lookup: out[t, :] = scale * table[id_t, :], computed in fp32 and
- * rounded once to the table's type.  `table->n` rows; out is dense
+ * rounded once to the table's type.  `table->n` rows at one stride (inner >= n);
+ * out is dense
  * [ids->n, width].  An id outside [0, table->n) gives a row of NaN.
  */
 int ms_embedding(const ms_tokens_t* ids, const ms_rows_t* table, float scale,

@@ -11,18 +11,88 @@ namespace {
 
 using namespace ops;
 
-template <typename T>
-__global__ void __launch_bounds__(256) k_lookup(ms_tokens_t ids, ms_rows_t table, float scale,
-                                                T* __restrict__ out) {
+// Token t of a list with one of its layouts: kWide 8-byte ids, kPlain
+// consecutive ones (`token` without its branches, which would wait for one load
+// after the other).
+template <bool kWide, bool kPlain>
+__device__ __forceinline__ int64_t token_of(const ms_tokens_t& ids, int64_t t) {
+  if (!kPlain) return token(ids, t);
+  return kWide ? static_cast<const int64_t*>(ids.data)[t]
+               : static_cast<int64_t>(static_cast<const int32_t*>(ids.data)[t]);
+}
+
+// Where a row's vector of N values from column c on is taken: the last one ends
+// with the row and covers again what the one before it has, which then is
+// computed twice, the same.  (With a branch for a short last vector every load
+// was waited for before the next.)  Columns beyond the row: the last vector.
+template <int N>
+__device__ __forceinline__ int64_t vector_at(int64_t c, int64_t width) {
+  return c + N <= width ? c : width - N;
+}
+
+// The output is cut into vectors of 16 bytes, which go to the lanes one after
+// the other whatever the width, kLookupEach of them in flight.
+constexpr int kLookupThreads = 256, kLookupEach = 4;
+
+// kShort: rows of less than a vector, value by value.
+template <typename T, bool kWide, bool kPlain, bool kShort>
+__global__ void __launch_bounds__(kLookupThreads)
+    k_lookup(ms_tokens_t ids, ms_rows_t table, float scale, uint32_t vectors,
+             T* __restrict__ out) {
+  constexpr int N = kShort ? 1 : 16 / sizeof(T);
   const T* rows = static_cast<const T*>(table.data);
-  for (int64_t t = blockIdx.x; t < ids.n; t += gridDim.x) {
-    const int64_t id = token(ids, t);
-    const bool good = id >= 0 && id < table.n;
-    const T* src = rows + (good ? row_start(table, id) : 0);
-    T* dst = out + t * table.width;
-    for (int64_t c = threadIdx.x; c < table.width; c += blockDim.x)
-      dst[c] = narrow<T>(good ? widen(src[c]) * scale : quiet_nan());
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kLookupThreads * kLookupEach);
+  const int64_t t0 = item / vectors;
+  const uint32_t v0 = static_cast<uint32_t>(item - t0 * vectors) + threadIdx.x;
+  int64_t t[kLookupEach], id[kLookupEach];
+  uint32_t v[kLookupEach];
+#pragma unroll
+  for (int k = 0; k < kLookupEach; ++k) {
+    const uint32_t i = v0 + k * kLookupThreads, down = i / vectors;
+    v[k] = i - down * vectors;
+    t[k] = t0 + down;
+    id[k] = token_of<kWide, kPlain>(ids, t[k] < ids.n ? t[k] : ids.n - 1);
   }
+  Pack<T, N> x[kLookupEach];
+#pragma unroll
+  for (int k = 0; k < kLookupEach; ++k) {
+    const bool good = static_cast<uint64_t>(id[k]) < static_cast<uint64_t>(table.n);
+    const T* row = rows + (good ? id[k] : 0) * table.inner_stride;
+    x[k] = load<N>(row + vector_at<N>(static_cast<int64_t>(v[k]) * N, table.width));
+  }
+#pragma unroll
+  for (int k = 0; k < kLookupEach; ++k) {
+    if (t[k] >= ids.n) continue;
+    const bool good = static_cast<uint64_t>(id[k]) < static_cast<uint64_t>(table.n);
+    Pack<T, N> y;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      y.v[j] = narrow<T>(good ? widen(x[k].v[j]) * scale : quiet_nan());
+    store<N>(out + t[k] * table.width +
+                 vector_at<N>(static_cast<int64_t>(v[k]) * N, table.width), y);
+  }
+}
+
+template <typename T>
+int lookup_as(const ms_tokens_t& ids, const ms_rows_t& table, float scale, void* out,
+              hipStream_t s) {
+  const bool brief = table.width < static_cast<int64_t>(16 / sizeof(T));
+  const int64_t n = brief ? 1 : 16 / sizeof(T);
+  const int64_t vectors = (table.width + n - 1) / n, each = kLookupThreads * kLookupEach;
+  if (vectors > INT32_MAX) return MS_OPS_EINVAL;
+  const int64_t blocks = (ids.n * vectors + each - 1) / each;
+  if (blocks > INT32_MAX) return MS_OPS_EINVAL;
+  const bool plain = ids.inner >= ids.n && ids.inner_stride == 1;
+#define LOOKUP(W, P)                                                                        \
+  (brief ? k_lookup<T, W, P, true> : k_lookup<T, W, P, false>)                             \
+      <<<static_cast<unsigned>(blocks), kLookupThreads, 0, s>>>(                            \
+          ids, table, scale, static_cast<uint32_t>(vectors), static_cast<T*>(out))
+  if (ids.wide && plain) LOOKUP(true, true);
+  else if (ids.wide) LOOKUP(true, false);
+  else if (plain) LOOKUP(false, true);
+  else LOOKUP(false, false);
+#undef LOOKUP
+  return launched();
 }
 
 // The gradient's table.  Tokens are sorted by (id, t) on the device, then each
@@ -63,15 +133,9 @@ struct Sorted {
   }
 };
 
-// Consecutive rows [lo, lo + rows) of the table, and every 2^shift-th row: the
-// rows that come before a bucket's, and a row's number in it (at least `rows`:
-// it has none).
-struct Consecutive {
-  uint32_t lo;
-  __device__ __forceinline__ bool before(uint32_t id) const { return id < lo; }
-  __device__ __forceinline__ uint32_t row(uint32_t id) const { return id - lo; }
-};
-struct Strided {
+// A bucket, every 2^shift-th row of the table: the rows of those before it, and a
+// row's number in it (2^32 - 1: it is none of its).
+struct Bucket {
   uint32_t bucket, mask, shift, vocab;
   __device__ __forceinline__ bool before(uint32_t id) const {
     return (id & mask) < bucket && id < vocab;
@@ -98,9 +162,8 @@ __device__ __forceinline__ int wave_scan(int x) {
 // that a group's loads stay in flight together).  A block goes through all
 // tokens, on one CU: what this costs is its instructions per token, so ids are
 // compared as 32-bit words.
-template <int kRows, int kSteps, bool kWide, bool kPlain, typename Rows, typename Begin,
-          typename Place>
-__device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Rows bucket, int rows,
+template <int kRows, int kSteps, bool kWide, bool kPlain, typename Begin, typename Place>
+__device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Bucket bucket, int rows,
                                             int64_t skip, int (&count)[kSortWaves][kRows],
                                             int (&wave_sum)[kSortWaves], Begin begin,
                                             Place place) {
@@ -219,8 +282,8 @@ __global__ void __launch_bounds__(kSortThreads)
     return;
   }
   const uint32_t b = blockIdx.x;
-  const Strided bucket = {b, static_cast<uint32_t>(buckets - 1),
-                          static_cast<uint32_t>(out.shift), static_cast<uint32_t>(vocab)};
+  const Bucket bucket = {b, static_cast<uint32_t>(buckets - 1),
+                         static_cast<uint32_t>(out.shift), static_cast<uint32_t>(vocab)};
   const int64_t slot = static_cast<int64_t>(b) * out.rows;
   sort_bucket<kSortRows, kSortSteps, kWide, kPlain>(
       ids, bucket, out.rows, skip, count, wave_sum,
@@ -231,28 +294,6 @@ __global__ void __launch_bounds__(kSortThreads)
         out.id[p] = static_cast<int32_t>(static_cast<uint32_t>(r) << out.shift | b);
         out.position[p] = t;
       });
-}
-
-// My N values of a row; `whole`: none of the wave's reach past the width.
-template <int N, typename T>
-__device__ __forceinline__ Pack<T, N> load_slice(const T* row, int64_t c, int64_t width,
-                                                 bool whole) {
-  if (whole) return load<N>(row + c);
-  Pack<T, N> x;
-#pragma unroll
-  for (int k = 0; k < N; ++k) x.v[k] = c + k < width ? row[c + k] : static_cast<T>(0.f);
-  return x;
-}
-template <int N, typename T>
-__device__ __forceinline__ void store_slice(T* row, int64_t c, int64_t width, bool whole,
-                                            const Pack<T, N>& x) {
-  if (whole) {
-    store<N>(row + c, x);
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    if (c + k < width) row[c + k] = x.v[k];
 }
 
 constexpr int kSumThreads = 256, kSumWaves = kSumThreads / kWave;
@@ -279,24 +320,28 @@ struct Tile {
   // rows q0 .. q1 - 1, at most kSumDepth of them; row(q): its first element
   template <typename Row>
   __device__ __forceinline__ void add(int q0, int q1, int64_t c, int64_t width, Row row) {
-    Pack<T, N> x[kSumDepth][G];
+    // as words until all are on their way: taken apart into values beside each
+    // load, every one was waited for before the next
+    typedef typename raw_of<N * sizeof(T)>::type raw;
+    raw x[kSumDepth][G];
 #pragma unroll
     for (int u = 0; u < kSumDepth; ++u)
       if (q0 + u < q1) {
         const T* src = row(q0 + u);
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-          const int64_t at = c + j * kWave * N;
-          x[u][j] = load_slice<N>(src, at, width, at + N <= width);
-        }
+        for (int j = 0; j < G; ++j)
+          x[u][j] = *reinterpret_cast<const raw*>(src + vector_at<N>(c + j * kWave * N, width));
       }
 #pragma unroll
     for (int u = 0; u < kSumDepth; ++u)
       if (q0 + u < q1)
 #pragma unroll
-        for (int j = 0; j < G; ++j)
+        for (int j = 0; j < G; ++j) {
+          Pack<T, N> y;
+          __builtin_memcpy(&y, &x[u][j], sizeof(y));
 #pragma unroll
-          for (int k = 0; k < N; ++k) sum[j][k] += widen(x[u][j].v[k]);
+          for (int k = 0; k < N; ++k) sum[j][k] += widen(y.v[k]);
+        }
   }
   __device__ __forceinline__ void write(T* row, int64_t c, int64_t width, float scale) const {
 #pragma unroll
@@ -305,22 +350,47 @@ struct Tile {
       Pack<T, N> y;
 #pragma unroll
       for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[j][k] * scale);
-      store_slice<N>(row, at, width, at + N <= width, y);
+      if (at < width) store<N>(row + vector_at<N>(at, width), y);
     }
   }
   __device__ __forceinline__ void leave(float* row, int64_t c, int64_t width) const {
+    constexpr int kVec = N < 4 ? N : 4;
 #pragma unroll
-    for (int j = 0; j < G; ++j)
+    for (int j = 0; j < G; ++j) {
+      const int64_t at = c + j * kWave * N;
+      if (at >= width) continue;
 #pragma unroll
-      for (int k0 = 0; k0 < N; k0 += 4) {
-        const int64_t at = c + j * kWave * N + k0;
-        Pack<float, 4> y;
+      for (int k0 = 0; k0 < N; k0 += kVec) {
+        Pack<float, kVec> y;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y.v[k] = sum[j][k0 + k];
-        store_slice<4>(row, at, width, at + 4 <= width, y);
+        for (int k = 0; k < kVec; ++k) y.v[k] = sum[j][k0 + k];
+        store<kVec>(row + vector_at<N>(at, width) + k0, y);
       }
+    }
   }
 };
+
+// Zeros for `rows` rows of which bit r of `empty` is set, row(r) the r-th: the
+// block's threads take consecutive vectors.
+template <typename T, typename Row>
+__device__ __forceinline__ void clear_rows_of(uint64_t empty, int rows, int64_t width, Row row) {
+  constexpr int kVec = 16 / sizeof(T);
+  if (width < kVec) {
+    for (int64_t i = threadIdx.x; i < width * rows; i += blockDim.x)
+      if (empty >> (i / width) & 1) row(static_cast<int>(i / width))[i % width] = static_cast<T>(0.f);
+    return;
+  }
+  Pack<T, kVec> zero;
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) zero.v[k] = static_cast<T>(0.f);
+  const uint32_t vectors = static_cast<uint32_t>((width + kVec - 1) / kVec);
+  for (uint32_t v = threadIdx.x; v < vectors * rows; v += blockDim.x) {
+    const uint32_t r = rows == 1 ? 0 : v / vectors;
+    if (empty >> r & 1)
+      store<kVec>(row(static_cast<int>(r)) +
+                      vector_at<kVec>(static_cast<int64_t>(v - r * vectors) * kVec, width), zero);
+  }
+}
 
 // Blocks below sum_blocks: a span and kWave * N * G columns; wave w adds the
 // span's w-th, (w + kSumWaves)-th .. run of equal ids.  The other blocks: rows
@@ -341,16 +411,7 @@ __global__ void __launch_bounds__(kSumThreads)
     const int rows = static_cast<int>(vocab - r0 < clear_rows ? vocab - r0 : clear_rows);
     const int64_t slot = in.slot(r0 + (lane < rows ? lane : rows - 1));
     const uint64_t empty = __ballot(lane < rows && in.start[slot] == in.start[slot + 1]);
-    constexpr int kVec = 16 / sizeof(T);
-    Pack<T, kVec> zero;
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) zero.v[k] = static_cast<T>(0.f);
-    const uint32_t vectors = static_cast<uint32_t>((width + kVec - 1) / kVec);
-    for (uint32_t v = threadIdx.x; v < vectors * rows; v += kSumThreads) {
-      const uint32_t k = rows == 1 ? 0 : v / vectors;
-      const int64_t c = static_cast<int64_t>(v - k * vectors) * kVec;
-      if (empty >> k & 1) store_slice<kVec>(table + (r0 + k) * width, c, width, c + kVec <= width, zero);
-    }
+    clear_rows_of<T>(empty, rows, width, [&](int k) { return table + (r0 + k) * width; });
     return;
   }
   const int64_t s = blockIdx.x / slices, first = s * kSpan;
@@ -403,10 +464,10 @@ constexpr int kJoinDepth = 8;             // partial sums in flight per wave
 
 // Every block looks at all spans, kJoinThreads at a time, for those that an id
 // of many tokens begins in.  Such a span and a slice of the width make a job:
-// a wave's (4 columns to a lane) where there are few partial sums, the block's
+// a wave's (N columns to a lane) where there are few partial sums, the block's
 // (1 column to a lane) where there are many; then its waves take a part of them
 // each and are added in their order.  Jobs go round the waves and blocks.
-template <typename T>
+template <typename T, int N>
 __global__ void __launch_bounds__(kJoinThreads)
     k_join_spans(int64_t n, int64_t width, float scale, Sorted in, T* __restrict__ table) {
   struct Found {
@@ -418,20 +479,20 @@ __global__ void __launch_bounds__(kJoinThreads)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int total = in.start[in.slots];
   // partial sums [from, to) of the id that begins in span s
-  auto add_parts = [&](auto& sum, int64_t s, int from, int to, int64_t c, bool whole) {
-    constexpr int N = sizeof(sum) / sizeof(float);
+  auto add_parts = [&](auto& sum, int64_t s, int from, int to, int64_t c) {
+    constexpr int M = sizeof(sum) / sizeof(float);
     for (int k0 = from; k0 < to; k0 += kJoinDepth) {
-      Pack<float, N> x[kJoinDepth];
+      Pack<float, M> x[kJoinDepth];
 #pragma unroll
       for (int u = 0; u < kJoinDepth; ++u) {
         const int k = k0 + u < to ? k0 + u : to - 1;
-        x[u] = load_slice<N>(in.partial + ((s + k) * 2 + (k == 0)) * width, c, width, whole);
+        x[u] = load<M>(in.partial + ((s + k) * 2 + (k == 0)) * width + vector_at<M>(c, width));
       }
 #pragma unroll
       for (int u = 0; u < kJoinDepth; ++u)
         if (k0 + u < to)
 #pragma unroll
-          for (int k = 0; k < N; ++k) sum[k] += x[u].v[k];
+          for (int k = 0; k < M; ++k) sum[k] += x[u].v[k];
     }
   };
   for (int64_t s0 = 0; (s0 + 1) * kSpan < n; s0 += kJoinThreads) {
@@ -469,7 +530,7 @@ __global__ void __launch_bounds__(kJoinThreads)
       const int each = (f.parts + kJoinWaves - 1) / kJoinWaves;
       const int from = wave * each, to = from + each < f.parts ? from + each : f.parts;
       float sum[1] = {0.f};
-      add_parts(sum, s, from, to, c, __all(c < width));
+      add_parts(sum, s, from, to, c);
       part[wave][lane] = sum[0];
       __syncthreads();
       if (wave == 0 && c < width) {
@@ -479,104 +540,117 @@ __global__ void __launch_bounds__(kJoinThreads)
       __syncthreads();
     }
     // from the last block on, which has the fewest of the others
-    const int64_t few = (width + 4 * kWave - 1) / (4 * kWave);
+    const int64_t few = (width + N * kWave - 1) / (N * kWave);
     const int64_t waves = static_cast<int64_t>(gridDim.x) * kJoinWaves;
     for (int64_t j = static_cast<int64_t>(wave) * gridDim.x + gridDim.x - 1 - blockIdx.x;
          j < all[0] * few; j += waves) {
       const Found f = found[0][j / few];
-      const int64_t s = f.span, id = f.id, c = (j % few) * (4 * kWave) + lane * 4;
-      const bool whole = __all(c + 4 <= width);
-      float sum[4] = {};
-      add_parts(sum, s, 0, f.parts, c, whole);
-      Pack<T, 4> y;
+      const int64_t s = f.span, id = f.id, c = (j % few) * (N * kWave) + lane * N;
+      float sum[N] = {};
+      add_parts(sum, s, 0, f.parts, c);
+      Pack<T, N> y;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) y.v[k] = narrow<T>(sum[k] * scale);
-      store_slice<4>(table + id * width, c, width, whole, y);
+      for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[k] * scale);
+      if (c < width) store<N>(table + id * width + vector_at<N>(c, width), y);
     }
   }
 }
 
 // Few tokens: every block sorts all of them for its rows of the table, in LDS.
-// A wave takes a row and a slice of the width at a time; rows of more than
-// kLight tokens are split over the waves, whose sums are added in their order.
-constexpr int kSmallTokens = 2048, kSmallRows = 64;
+// A wave takes a row with tokens and a slice of the width at a time; rows of more
+// than kLight tokens are split over the waves, whose sums are added in their
+// order.
+constexpr int kSmallTokens = 1024, kSmallRows = 64;
 
 template <typename T, int N, bool kWide, bool kPlain>
 __global__ void __launch_bounds__(kSortThreads)
     k_grad_small(ms_tokens_t ids, ms_rows_t grad, int64_t vocab, int64_t skip, float scale,
-                 int rows_each, T* __restrict__ table) {
+                 int shift, T* __restrict__ table) {
   __shared__ int count[kSortWaves][kSmallRows];
   __shared__ int wave_sum[kSortWaves];
   __shared__ int start[kSmallRows + 1];
   __shared__ uint16_t position[kSmallTokens];
   __shared__ float part[kSortWaves][kWave * N];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * rows_each, width = grad.width;
-  const int rows = static_cast<int>(vocab - lo < rows_each ? vocab - lo : rows_each);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int64_t width = grad.width;
+  const uint32_t b = blockIdx.x;
+  const int rows = static_cast<int>((vocab - 1 - b) >> shift) + 1;      // b < vocab
+  auto table_row = [&](int r) {
+    return table + ((static_cast<int64_t>(r) << shift) + b) * width;
+  };
   sort_bucket<kSmallRows, kSmallTokens / kSortThreads, kWide, kPlain>(
-      ids, Consecutive{static_cast<uint32_t>(lo)}, rows, skip, count, wave_sum, [&](int r, int p) { start[r] = p; },
+      ids, Bucket{b, (1u << shift) - 1, static_cast<uint32_t>(shift), static_cast<uint32_t>(vocab)},
+      rows, skip, count, wave_sum, [&](int r, int p) { start[r] = p; },
       [&](int p, int, int t) { position[p] = static_cast<uint16_t>(t); });
   __syncthreads();
 
   const T* g = static_cast<const T*>(grad.data);
-  constexpr int kDepth = 8;
-  auto add_rows = [&](int from, int to, int64_t c, bool whole, float (&sum)[N]) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) sum[k] = 0.f;
-    for (int p0 = from; p0 < to; p0 += kDepth) {
-      Pack<T, N> x[kDepth];
-#pragma unroll
-      for (int u = 0; u < kDepth; ++u) {
-        const int t = __builtin_amdgcn_readfirstlane(position[p0 + u < to ? p0 + u : to - 1]);
-        x[u] = load_slice<N>(g + row_start(grad, t), c, width, whole);
-      }
-#pragma unroll
-      for (int u = 0; u < kDepth; ++u)
-        if (p0 + u < to)
-#pragma unroll
-          for (int k = 0; k < N; ++k) sum[k] += widen(x[u].v[k]);
+  // the sum of the sorted tokens [from, to), 64 positions looked up at a time
+  auto add_rows = [&](int from, int to, int64_t c, float (&sum)[N]) {
+    Tile<T, N, 1> tile;
+    tile.clear();
+    for (int p0 = from; p0 < to; p0 += kWave) {
+      const int64_t offset = row_start(grad, position[p0 + lane < to ? p0 + lane : to - 1]);
+      const int n = to - p0 < kWave ? to - p0 : kWave;
+      for (int q = 0; q < n; q += kSumDepth)
+        tile.add(q, n, c, width, [&](int i) { return g + read_lane(offset, i); });
     }
+#pragma unroll
+    for (int k = 0; k < N; ++k) sum[k] = tile.sum[0][k];
   };
   const int slices = static_cast<int>((width + kWave * N - 1) / (kWave * N));
-  bool heavy = false;
-  for (int item = wave; item < rows * slices; item += kSortWaves) {
-    const int r = item / slices;
-    const int64_t c = (static_cast<int64_t>(item - r * slices) * kWave + lane) * N;
-    const int from = start[r], to = start[r + 1];
-    if (to - from > kLight) {
-      heavy = true;
-      continue;
-    }
-    const bool whole = __all(c + N <= width);
-    float sum[N];
-    add_rows(from, to, c, whole, sum);
-    Pack<T, N> y;
-#pragma unroll
-    for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[k] * scale);
-    if (from == to)                                 // +0, whatever the scale
-      for (int k = 0; k < N; ++k) y.v[k] = static_cast<T>(0.f);
-    store_slice<N>(table + (lo + r) * width, c, width, whole, y);
-  }
-  if (!__syncthreads_or(heavy)) return;
-  for (int r = 0; r < rows; ++r) {
-    const int from = start[r], each = (start[r + 1] - from + kSortWaves - 1) / kSortWaves;
-    if (start[r + 1] - from <= kLight) continue;
-    for (int slice = 0; slice < slices; ++slice) {
-      const int64_t c0 = static_cast<int64_t>(slice) * kWave * N;
-      const int64_t c = c0 + lane * N;
-      const int a = from + wave * each, b = a + each < start[r + 1] ? a + each : start[r + 1];
+  // the same in every wave: bit r for row r
+  const int row_at = lane < rows ? lane : rows - 1;
+  const int tokens = start[row_at + 1] - start[row_at];
+  const uint64_t empty = __ballot(lane < rows && tokens == 0);
+  const uint64_t heavy = __ballot(lane < rows && tokens > kLight);
+  uint64_t some = __ballot(lane < rows && tokens > 0) & ~heavy;
+
+  if (empty) clear_rows_of<T>(empty, rows, width, table_row);
+  for (int item = wave; some; item -= slices, some &= some - 1) {
+    const int r = __ffsll(static_cast<unsigned long long>(some)) - 1;
+    const int from = uniform(start[r]), to = uniform(start[r + 1]);
+    for (; item < slices; item += kSortWaves) {
+      const int64_t c = (static_cast<int64_t>(item) * kWave + lane) * N;
       float sum[N];
-      add_rows(a, b, c, __all(c + N <= width), sum);
+      add_rows(from, to, c, sum);
+      Pack<T, N> y;
 #pragma unroll
-      for (int k = 0; k < N; ++k) part[wave][lane * N + k] = sum[k];
-      __syncthreads();
-      for (int k = threadIdx.x; k < kWave * N; k += kSortThreads) {
-        float y = part[0][k];
-        for (int w = 1; w < kSortWaves; ++w) y += part[w][k];
-        if (c0 + k < width) table[(lo + r) * width + c0 + k] = narrow<T>(y * scale);
-      }
-      __syncthreads();
+      for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[k] * scale);
+      if (c < width) store<N>(table_row(r) + vector_at<N>(c, width), y);
     }
+  }
+  // the waves share a row's slices and, where these are few, its tokens
+  const int parts = slices < kSortWaves ? kSortWaves / slices : 1, jobs = slices * parts;
+  for (uint64_t left = heavy; left; left &= left - 1) {
+    const int r = __ffsll(static_cast<unsigned long long>(left)) - 1;
+    const int from = uniform(start[r]), end = uniform(start[r + 1]), each = (end - from + parts - 1) / parts;
+    for (int j = wave; j < jobs; j += kSortWaves) {
+      const int slice = j / parts, first = from + (j - slice * parts) * each;
+      const int64_t c = (static_cast<int64_t>(slice) * kWave + lane) * N;
+      float sum[N];
+      add_rows(first, first + each < end ? first + each : end, c, sum);
+      if (parts == 1) {
+        Pack<T, N> y;
+#pragma unroll
+        for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[k] * scale);
+        if (c < width) store<N>(table_row(r) + vector_at<N>(c, width), y);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) part[j][lane * N + k] = sum[k];
+      }
+    }
+    if (parts == 1) continue;
+    __syncthreads();
+    for (int k = threadIdx.x; k < slices * kWave * N; k += kSortThreads) {
+      const int slice = k / (kWave * N), at = k % (kWave * N);
+      const int64_t c = k / N * N;                   // of the lane; its vector may be earlier
+      if (c >= width) continue;
+      float y = part[slice * parts][at];
+      for (int p = 1; p < parts; ++p) y += part[slice * parts + p][at];
+      table_row(r)[vector_at<N>(c, width) + k % N] = narrow<T>(y * scale);
+    }
+    __syncthreads();
   }
 }
 
@@ -635,15 +709,16 @@ bool is_small(int64_t n, int64_t table_bytes) {
 template <typename T, int N>
 int small_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float scale,
              int64_t skip, T* table, hipStream_t s) {
-  // some 64 KB of the table to a block, but a block for each CU if it has the rows
+  // a block for each CU at least, and no more than some 64 KB of the table to one
   const int64_t row_bytes = grad.width * static_cast<int64_t>(sizeof(T));
   const int64_t most = std::min<int64_t>(kSmallRows, std::max<int64_t>(65536 / row_bytes, 1));
-  const int rows_each = static_cast<int>(std::min(most, (vocab + 255) / 256));
-  const unsigned blocks = static_cast<unsigned>((vocab + rows_each - 1) / rows_each);
+  int shift = 0;
+  while ((shift < 8 && 1 << shift < vocab) || vocab > most << shift) ++shift;
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(vocab, 1ll << shift));
   const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
 #define SMALL(W, P)                                                                          \
   k_grad_small<T, N, W, P><<<blocks, kSortThreads, 0, s>>>(ids, grad, vocab, skip, scale, \
-                                                           rows_each, table)
+                                                           shift, table)
   if (wide && plain) SMALL(true, true);
   else if (wide) SMALL(true, false);
   else if (plain) SMALL(false, true);
@@ -659,8 +734,8 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
   const int64_t row_bytes = width * static_cast<int64_t>(sizeof(T));
   T* table = static_cast<T*>(dtable);
   if (is_small(ids.n, vocab * row_bytes))
-    return width >= 2 * kWave ? small_as<T, 4>(ids, grad, vocab, scale, skip, table, s)
-                              : small_as<T, 1>(ids, grad, vocab, scale, skip, table, s);
+    return width >= 4 ? small_as<T, 4>(ids, grad, vocab, scale, skip, table, s)
+                      : small_as<T, 1>(ids, grad, vocab, scale, skip, table, s);
   const GradShape g = shape_of(ids.n, vocab, width);
   char* w = static_cast<char*>(workspace);
   Sorted sorted;
@@ -689,22 +764,19 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
   // 512 columns to a wave (256 of a narrow fp32 table), 16 bytes to a lane
   constexpr int kVec = 16 / sizeof(T);
   const int rc =
-      sizeof(T) == 4 && width > kVec * kWave
+      width < kVec ? sum_as<T, 1, 1>(grad, vocab, scale, clear_rows, g, sorted, table, s)
+      : sizeof(T) == 4 && width > kVec * kWave
           ? sum_as<T, kVec, (sizeof(T) == 4 ? 2 : 1)>(grad, vocab, scale, clear_rows, g, sorted,
                                                       table, s)
           : sum_as<T, kVec, 1>(grad, vocab, scale, clear_rows, g, sorted, table, s);
   if (rc) return rc;
   if (ids.n > kLight) {
     const int64_t lots = (width + kWave - 1) / kWave;
-    k_join_spans<T><<<static_cast<unsigned>(std::min<int64_t>(g.spans * lots, 512)), kJoinThreads,
-                      0, s>>>(ids.n, width, scale, sorted, table);
+    (width < 4 ? k_join_spans<T, 1> : k_join_spans<T, 4>)
+        <<<static_cast<unsigned>(std::min<int64_t>(g.spans * lots, 512)), kJoinThreads, 0, s>>>(
+            ids.n, width, scale, sorted, table);
   }
   return launched();
-}
-
-unsigned blocks_for(int64_t n) {
-  const int64_t most = 1 << 20;
-  return static_cast<unsigned>(n < most ? n : most);
 }
 
 }  // namespace
@@ -714,19 +786,13 @@ extern "C" int ms_embedding(const ms_tokens_t* ids, const ms_rows_t* table, floa
   if (!good_tokens(ids) || !good_rows(table)) return MS_OPS_EINVAL;
   if (ids->n == 0 || table->width == 0) return MS_OPS_OK;
   if (!out || table->n < 1) return MS_OPS_EINVAL;
+  if (table->n > 1 && table->inner < table->n) return MS_OPS_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned blocks = blocks_for(ids->n);
   switch (table->dtype) {
-    case MS_OPS_F32:
-      k_lookup<float><<<blocks, 256, 0, s>>>(*ids, *table, scale, static_cast<float*>(out));
-      break;
-    case MS_OPS_F16:
-      k_lookup<f16><<<blocks, 256, 0, s>>>(*ids, *table, scale, static_cast<f16*>(out));
-      break;
-    default:
-      k_lookup<bf16><<<blocks, 256, 0, s>>>(*ids, *table, scale, static_cast<bf16*>(out));
+    case MS_OPS_F32: return lookup_as<float>(*ids, *table, scale, out, s);
+    case MS_OPS_F16: return lookup_as<f16>(*ids, *table, scale, out, s);
+    default: return lookup_as<bf16>(*ids, *table, scale, out, s);
   }
-  return launched();
 }
 
 extern "C" int64_t ms_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t width) {

@@ -117,6 +117,10 @@ __device__ __forceinline__ void store_stream(T* p, const Pack<T, N>& x) {
   __builtin_nontemporal_store(r, reinterpret_cast<raw*>(p));
 }
 
+// A value that all lanes have, told to the compiler: branches on it leave loads
+// in flight.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 __device__ __forceinline__ int read_lane(int x, int lane) {
   return __builtin_amdgcn_readlane(x, lane);
 }
