@@ -266,6 +266,25 @@ struct Split {
   int64_t stride;
 };
 
+// 16 bytes of logits, as words until they are used: taken apart into values
+// beside a conditional load, every load is waited for before the next.
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> values_of(Words w) {
+  Pack<T, 16 / sizeof(T)> x;
+  __builtin_memcpy(&x, &w, 16);
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ Words no_values() {         // all -inf
+  Pack<T, 16 / sizeof(T)> x;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) x.v[i] = static_cast<T>(-INFINITY);
+  Words w;
+  __builtin_memcpy(&w, &x, 16);
+  return w;
+}
+
 // The largest of the values seen, in as few instructions as the type has.
 template <typename T>
 struct Largest {
@@ -326,23 +345,23 @@ __global__ void __launch_bounds__(NT, kTop ? 6 : 8)
   const T* first = x + head;
 
   // the last round's threads without a unit load the last one
-  auto load_group = [&](int k0, Unit (&p)[kGroup]) {
+  auto load_group = [&](int k0, Words (&p)[kGroup]) {
 #pragma unroll
     for (int k = 0; k < kGroup; ++k)
       if (k0 + k < rounds) {
         const int u = (k0 + k) * NT + threadIdx.x;
-        p[k] = load_stream<kVec>(first + static_cast<int64_t>(u < units ? u : units - 1) * kVec);
+        p[k] = __builtin_nontemporal_load(reinterpret_cast<const Words*>(
+            first + static_cast<int64_t>(u < units ? u : units - 1) * kVec));
       }
   };
   // ... and drop it
-  auto mask_group = [&](int k0, Unit (&p)[kGroup]) {
+  auto mask_group = [&](int k0, Words (&p)[kGroup]) {
 #pragma unroll
     for (int k = 0; k < kGroup; ++k)
       if (k0 + k >= rounds - 1 && (k0 + k) * NT + static_cast<int>(threadIdx.x) >= units)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) p[k].v[i] = static_cast<T>(-INFINITY);
+        p[k] = no_values<T>();
   };
-  Unit now[kGroup], next[kGroup];
+  Words now[kGroup], next[kGroup];
   load_group(0, now);
   // the values before and behind the units, one to a thread
   const int tid = threadIdx.x;
@@ -359,7 +378,7 @@ __global__ void __launch_bounds__(NT, kTop ? 6 : 8)
 
   Largest<T> largest;
 #pragma unroll
-  for (int k = 0; k < kGroup; ++k) largest.see(now[k]);
+  for (int k = 0; k < kGroup; ++k) largest.see(values_of<T>(now[k]));
   float seen = wave_max(fmaxf(single, largest.get())), s = 0.f, t = 0.f;
   float m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
   auto add = [&](float v) {
@@ -376,7 +395,7 @@ __global__ void __launch_bounds__(NT, kTop ? 6 : 8)
       Largest<T> here;
 #pragma unroll
       for (int k = 0; k < kGroup; ++k)
-        if (k0 + k < rounds) here.see(now[k]);
+        if (k0 + k < rounds) here.see(values_of<T>(now[k]));
       seen = wave_max(here.get());
       m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
     }
@@ -385,8 +404,8 @@ __global__ void __launch_bounds__(NT, kTop ? 6 : 8)
     for (int k = 0; k < kGroup; ++k) {
       if (k0 + k >= rounds) break;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) add(widen(now[k].v[i]));
-      if (kTop) here.see(now[k]);
+      for (int i = 0; i < kVec; ++i) add(widen(values_of<T>(now[k]).v[i]));
+      if (kTop) here.see(values_of<T>(now[k]));
     }
     if (kTop && k0) {
       const float high = here.get();
@@ -498,14 +517,15 @@ __global__ void __launch_bounds__(NT, kTop ? 6 : 8)
       __syncthreads();
       const int again = sh.look_count < 2 * NT ? sh.look_count * kGroup : 0;
       for (int i0 = tid; i0 < again; i0 += kAgain * NT) {
-        Unit p[kAgain];
+        Words p[kAgain];
         int u[kAgain];
 #pragma unroll
         for (int j = 0; j < kAgain; ++j) {
           const int i = i0 + j * NT < again ? i0 + j * NT : i0;
           const int look = sh.looks[i / kGroup];
           u[j] = ((look / NT) * kGroup + i % kGroup) * NT + look % NT;
-          p[j] = load<kVec>(first + static_cast<int64_t>(u[j] < units ? u[j] : 0) * kVec);
+          p[j] = *reinterpret_cast<const Words*>(
+              first + static_cast<int64_t>(u[j] < units ? u[j] : 0) * kVec);
           if (i0 + j * NT >= again) u[j] = units;
         }
 #pragma unroll
@@ -513,8 +533,8 @@ __global__ void __launch_bounds__(NT, kTop ? 6 : 8)
           if (u[j] < units)
 #pragma unroll
             for (int i = 0; i < kVec; ++i)
-              if (widen(p[j].v[i]) >= least_value)
-                offer(widen(p[j].v[i]), head + u[j] * kVec + i);
+              if (widen(values_of<T>(p[j]).v[i]) >= least_value)
+                offer(widen(values_of<T>(p[j]).v[i]), head + u[j] * kVec + i);
       }
       __syncthreads();
       give_up = sh.count > sh.kCandidates || sh.look_count >= 2 * NT;
@@ -607,7 +627,7 @@ __global__ void __launch_bounds__(kThreads)
 constexpr float kFarLse = 256.f;
 
 constexpr int kGradThreads = 256, kGradWaves = kGradThreads / kWave;
-constexpr int kGradGroup = 2;             // 16-byte units to a thread; 1, 2, 4: 276, 279, 282 us
+constexpr int kGradGroup = 1;             // 16-byte units to a thread; 1, 2, 4: 270, 280, 290 us
 
 // A block takes kGradGroup rounds of aligned 16-byte units of the gradient's row
 // (the logits' row may lie otherwise).  With c a whole number near lse L and
@@ -629,12 +649,15 @@ __global__ void __launch_bounds__(kGradThreads)
   const int head = off < vocab ? off : vocab;
   const int units = (vocab - head) / kVec, rest = vocab - head - units * kVec;
 
-  Pack<T, kVec> in[kGradGroup];
+  typedef typename raw_of<16>::type AnyWords;          // the logits may lie otherwise
+  Words in[kGradGroup];
+  if (units > 0)
 #pragma unroll
-  for (int i = 0; i < kGradGroup; ++i) {
-    const int u = part * kEach + i * kGradThreads + tid;
-    if (u < units) in[i] = load_stream_any<kVec>(x + head + static_cast<int64_t>(u) * kVec);
-  }
+    for (int i = 0; i < kGradGroup; ++i) {
+      const int u = part * kEach + i * kGradThreads + tid;
+      in[i] = __builtin_nontemporal_load(reinterpret_cast<const AnyWords*>(
+          x + head + static_cast<int64_t>(u < units ? u : units - 1) * kVec));
+    }
   const int64_t target = token(targets, r);
   const bool counts = grad_logprob && target != ignore;
   float g = counts ? grad_logprob[r] : 0.f;
@@ -692,7 +715,7 @@ __global__ void __launch_bounds__(kGradThreads)
     if (u < units) {
       float y[kVec];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) y[j] = one(widen(in[i].v[j]));
+      for (int j = 0; j < kVec; ++j) y[j] = one(widen(values_of<T>(in[i]).v[j]));
       const unsigned at = static_cast<unsigned>(hit - head - u * kVec);
       if (at < kVec && hit >= 0)
 #pragma unroll
