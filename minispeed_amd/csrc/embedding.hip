@@ -227,9 +227,12 @@ __device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Bucket
 
   // exclusive sum over the rows, then over the waves of each row
   const int r = threadIdx.x;
-  int mine = 0;
-  if (r < rows)
-    for (int w = 0; w < kSortWaves; ++w) mine += count[w][r];
+  int mine = 0, by_wave[kSortWaves];
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) {
+    by_wave[w] = r < rows ? count[w][r] : 0;
+    mine += by_wave[w];
+  }
   const int upto = wave_scan(mine);
   if (lane == 63) wave_sum[wave] = upto;
   __syncthreads();
@@ -237,10 +240,10 @@ __device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Bucket
   for (int w = 0; w < wave; ++w) at += wave_sum[w];
   if (r < rows) {
     begin(r, at);
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-      const int c = count[w][r];
       count[w][r] = at;
-      at += c;
+      at += by_wave[w];
     }
     if (r == rows - 1) begin(rows, at);
   }
@@ -392,26 +395,42 @@ __device__ __forceinline__ void clear_rows_of(uint64_t empty, int rows, int64_t 
   }
 }
 
-// Blocks below sum_blocks: a span and kWave * N * G columns; wave w adds the
-// span's w-th, (w + kSumWaves)-th .. run of equal ids.  The other blocks: rows
-// from clear_from on that have no tokens.  16384 x 768 bf16 into 12000 rows,
+// Block `block` of those that clear: `each` rows from `from` on, below `until`,
+// those that have no tokens.
+template <typename T>
+__device__ __forceinline__ void clear_absent(const Sorted& in, int64_t block, int64_t from,
+                                             int64_t until, int each, int64_t width, T* table) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r0 = from + block * each;
+  const int rows = static_cast<int>(until - r0 < each ? until - r0 : each);
+  const int64_t slot = in.slot(r0 + (lane < rows ? lane : rows - 1));
+  const uint64_t empty = __ballot(lane < rows && in.start[slot] == in.start[slot + 1]);
+  clear_rows_of<T>(empty, rows, width, [&](int k) { return table + (r0 + k) * width; });
+}
+
+// What is left to clear: rows [from, until), `each` to a block, in the blocks from
+// `first_block` on.
+struct Clear {
+  int64_t from, until;
+  int each;
+  unsigned first_block;
+};
+
+// Blocks below clear.first_block: a span and kWave * N * G columns; wave w adds the
+// span's w-th, (w + kSumWaves)-th .. run of equal ids.  16384 x 768 bf16 into 12000 rows,
 // uniform ids or falling off as 1 / rank: 15.5 and 16.1 us (39 and 32 MB moved).
 // A wave to a span that keeps its 16 rows in registers, the loop over them
 // unrolled: 16.5 and more; the rows set down in LDS for a short loop: 17.3
 // and 23.
 template <typename T, int N, int G>
 __global__ void __launch_bounds__(kSumThreads)
-    k_sum_spans(ms_rows_t grad, int64_t vocab, float scale, int slices, unsigned sum_blocks,
-                int64_t clear_from, int clear_rows, Sorted in, T* __restrict__ table) {
+    k_sum_spans(ms_rows_t grad, float scale, int slices, Clear clear, Sorted in,
+                T* __restrict__ table) {
   const int lane = threadIdx.x & 63;
   const int64_t width = grad.width;
-  if (blockIdx.x >= sum_blocks) {
-    // consecutive vectors of `clear_rows` rows to the block's threads
-    const int64_t r0 = clear_from + static_cast<int64_t>(blockIdx.x - sum_blocks) * clear_rows;
-    const int rows = static_cast<int>(vocab - r0 < clear_rows ? vocab - r0 : clear_rows);
-    const int64_t slot = in.slot(r0 + (lane < rows ? lane : rows - 1));
-    const uint64_t empty = __ballot(lane < rows && in.start[slot] == in.start[slot + 1]);
-    clear_rows_of<T>(empty, rows, width, [&](int k) { return table + (r0 + k) * width; });
+  if (blockIdx.x >= clear.first_block) {
+    clear_absent(in, blockIdx.x - clear.first_block, clear.from, clear.until, clear.each, width,
+                 table);
     return;
   }
   const int64_t s = blockIdx.x / slices, first = s * kSpan;
@@ -469,7 +488,13 @@ constexpr int kJoinDepth = 8;             // partial sums in flight per wave
 // each and are added in their order.  Jobs go round the waves and blocks.
 template <typename T, int N>
 __global__ void __launch_bounds__(kJoinThreads)
-    k_join_spans(int64_t n, int64_t width, float scale, Sorted in, T* __restrict__ table) {
+    k_join_spans(int64_t n, int64_t width, float scale, Clear clear, Sorted in,
+                 T* __restrict__ table) {
+  if (blockIdx.x >= clear.first_block) {
+    clear_absent(in, blockIdx.x - clear.first_block, clear.from, clear.until, clear.each, width,
+                 table);
+    return;
+  }
   struct Found {
     int span, id, parts;
   };
@@ -477,6 +502,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   __shared__ int found_by[2][kJoinWaves];
   __shared__ float part[kJoinWaves][kWave];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned blocks = clear.first_block;
   const int total = in.start[in.slots];
   // partial sums [from, to) of the id that begins in span s
   auto add_parts = [&](auto& sum, int64_t s, int from, int to, int64_t c) {
@@ -524,7 +550,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     __syncthreads();
 
     const int64_t lots = (width + kWave - 1) / kWave;
-    for (int64_t j = blockIdx.x; j < all[1] * lots; j += gridDim.x) {
+    for (int64_t j = blockIdx.x; j < all[1] * lots; j += blocks) {
       const Found f = found[1][j / lots];
       const int64_t s = f.span, id = f.id, c = (j % lots) * kWave + lane;
       const int each = (f.parts + kJoinWaves - 1) / kJoinWaves;
@@ -541,8 +567,8 @@ __global__ void __launch_bounds__(kJoinThreads)
     }
     // from the last block on, which has the fewest of the others
     const int64_t few = (width + N * kWave - 1) / (N * kWave);
-    const int64_t waves = static_cast<int64_t>(gridDim.x) * kJoinWaves;
-    for (int64_t j = static_cast<int64_t>(wave) * gridDim.x + gridDim.x - 1 - blockIdx.x;
+    const int64_t waves = static_cast<int64_t>(blocks) * kJoinWaves;
+    for (int64_t j = static_cast<int64_t>(wave) * blocks + blocks - 1 - blockIdx.x;
          j < all[0] * few; j += waves) {
       const Found f = found[0][j / few];
       const int64_t s = f.span, id = f.id, c = (j % few) * (N * kWave) + lane * N;
@@ -681,20 +707,29 @@ GradShape shape_of(int64_t n, int64_t vocab, int64_t width) {
 // What the sort's launch clears while it sorts; the sort takes some 8 us.
 constexpr int64_t kClearBesideSort = 48 << 20;
 
+// Blocks that clear rows [from, until) behind `first` others; blocks: of the launch.
+Clear clear_after(int64_t first, int64_t from, int64_t until, int64_t row_bytes, int64_t bytes,
+                  int64_t& blocks) {
+  Clear c;
+  c.from = from;
+  c.until = until;
+  c.each = static_cast<int>(std::min<int64_t>(kClearRows, std::max<int64_t>(bytes / row_bytes, 1)));
+  c.first_block = static_cast<unsigned>(first);
+  blocks = first + (until - from + c.each - 1) / c.each;
+  return c;
+}
+
 template <typename T, int N, int G>
-int sum_as(const ms_rows_t& grad, int64_t vocab, float scale, int64_t clear_from,
-           const GradShape& g, const Sorted& sorted, T* table, hipStream_t s) {
+int sum_as(const ms_rows_t& grad, float scale, int64_t from, int64_t until, const GradShape& g,
+           const Sorted& sorted, T* table, hipStream_t s) {
   const int slices = static_cast<int>((grad.width + kWave * N * G - 1) / (kWave * N * G));
-  const int64_t sums = g.spans * slices;
-  const int64_t row_bytes = grad.width * static_cast<int64_t>(sizeof(T));
-  const int clear_rows = static_cast<int>(
-      std::min<int64_t>(kClearRows, std::max<int64_t>(kClearBytes / row_bytes, 1)));
-  const int64_t clears = (vocab - clear_from + clear_rows - 1) / clear_rows;
-  if (sums + clears > INT32_MAX) return MS_OPS_EINVAL;
-  if (sums + clears == 0) return MS_OPS_OK;
-  k_sum_spans<T, N, G><<<static_cast<unsigned>(sums + clears), kSumThreads, 0, s>>>(
-      grad, vocab, scale, slices, static_cast<unsigned>(sums), clear_from, clear_rows, sorted,
-      table);
+  int64_t blocks;
+  const Clear clear = clear_after(g.spans * slices, from, until,
+                                  grad.width * static_cast<int64_t>(sizeof(T)), kClearBytes, blocks);
+  if (blocks > INT32_MAX) return MS_OPS_EINVAL;
+  if (blocks == 0) return MS_OPS_OK;
+  k_sum_spans<T, N, G><<<static_cast<unsigned>(blocks), kSumThreads, 0, s>>>(
+      grad, scale, slices, clear, sorted, table);
   return launched();
 }
 
@@ -761,21 +796,28 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
   else SORT(false, false);
 #undef SORT
   if (int rc = launched()) return rc;
+  // of what is left to clear, the last launch gets half where that is much
+  const bool joins = ids.n > kLight;
+  const int64_t left = vocab - clear_rows;
+  const int64_t until =
+      joins && left * row_bytes > 2 * kClearBesideSort ? clear_rows + left / 2 : vocab;
   // 512 columns to a wave (256 of a narrow fp32 table), 16 bytes to a lane
   constexpr int kVec = 16 / sizeof(T);
   const int rc =
-      width < kVec ? sum_as<T, 1, 1>(grad, vocab, scale, clear_rows, g, sorted, table, s)
+      width < kVec ? sum_as<T, 1, 1>(grad, scale, clear_rows, until, g, sorted, table, s)
       : sizeof(T) == 4 && width > kVec * kWave
-          ? sum_as<T, kVec, (sizeof(T) == 4 ? 2 : 1)>(grad, vocab, scale, clear_rows, g, sorted,
+          ? sum_as<T, kVec, (sizeof(T) == 4 ? 2 : 1)>(grad, scale, clear_rows, until, g, sorted,
                                                       table, s)
-          : sum_as<T, kVec, 1>(grad, vocab, scale, clear_rows, g, sorted, table, s);
-  if (rc) return rc;
-  if (ids.n > kLight) {
-    const int64_t lots = (width + kWave - 1) / kWave;
-    (width < 4 ? k_join_spans<T, 1> : k_join_spans<T, 4>)
-        <<<static_cast<unsigned>(std::min<int64_t>(g.spans * lots, 512)), kJoinThreads, 0, s>>>(
-            ids.n, width, scale, sorted, table);
-  }
+          : sum_as<T, kVec, 1>(grad, scale, clear_rows, until, g, sorted, table, s);
+  if (rc || !joins) return rc;
+  const int64_t jobs = g.spans * ((width + kWave - 1) / kWave);
+  int64_t join_blocks;
+  const Clear rest = clear_after(std::min<int64_t>(jobs, 512), until, vocab, row_bytes,
+                                 4 * kClearBytes, join_blocks);
+  if (join_blocks > INT32_MAX) return MS_OPS_EINVAL;
+  (width < 4 ? k_join_spans<T, 1> : k_join_spans<T, 4>)
+      <<<static_cast<unsigned>(join_blocks), kJoinThreads, 0, s>>>(ids.n, width, scale, rest,
+                                                                   sorted, table);
   return launched();
 }
 
