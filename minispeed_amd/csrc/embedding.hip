@@ -133,16 +133,15 @@ struct Sorted {
   }
 };
 
-// A bucket, every 2^shift-th row of the table: the rows of those before it, and a
-// row's number in it (2^32 - 1: it is none of its).
+// A bucket, every 2^shift-th row of the table.  What is no row at all is 2^32 - 1;
+// its top bit keeps it out of every bucket.
 struct Bucket {
-  uint32_t bucket, mask, shift, vocab;
-  __device__ __forceinline__ bool before(uint32_t id) const {
-    return (id & mask) < bucket && id < vocab;
+  uint32_t bucket, shift, vocab;
+
+  __device__ __forceinline__ uint32_t key(uint32_t id) const {
+    return id & ((1u << shift) - 1 | 0x80000000u);
   }
-  __device__ __forceinline__ uint32_t row(uint32_t id) const {
-    return (id & mask) == bucket && id < vocab ? id >> shift : ~0u;
-  }
+  __device__ __forceinline__ uint32_t row(uint32_t id) const { return id >> shift; }
 };
 
 __device__ __forceinline__ int wave_scan(int x) {
@@ -196,6 +195,9 @@ __device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Bucket
         if (t >= last) id[k] = ~0u;
       }
     }
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+      if (id[k] >= bucket.vocab) id[k] = ~0u;
     if (none != ~0u) {
 #pragma unroll
       for (int k = 0; k < kSteps; ++k)
@@ -213,9 +215,17 @@ __device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Bucket
     if (t0 != first) load_ids(t0, id);
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-      below += bucket.before(id[k]);
-      const uint32_t r = bucket.row(id[k]);
-      if (r < static_cast<uint32_t>(rows)) atomicAdd(&count[wave][r], 1);
+      const uint32_t key = bucket.key(id[k]);
+      below += key < bucket.bucket;
+      // most often none, one or many of one id (padding): one addition for the first
+      // id, which 64 to one address would serialise, and the rest by themselves
+      const uint64_t mine = __ballot(key == bucket.bucket);
+      if (!mine) continue;
+      const int lead = __ffsll(static_cast<unsigned long long>(mine)) - 1;
+      const uint32_t one = read_lane(static_cast<int>(id[k]), lead);
+      const uint64_t same = __ballot(id[k] == one);
+      if (lane == lead) count[wave][bucket.row(one)] += __popcll(same);
+      if (key == bucket.bucket && id[k] != one) atomicAdd(&count[wave][bucket.row(id[k])], 1);
     }
   }
   for (int k = 32; k; k >>= 1) below += __shfl_xor(below, k);
@@ -253,8 +263,9 @@ __device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Bucket
     if (part > kWave * kSteps) load_ids(t0, id);      // else they are still here
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-      const uint32_t row = bucket.row(id[k]);
-      uint64_t left = __ballot(row < static_cast<uint32_t>(rows));
+      uint64_t left = __ballot(bucket.key(id[k]) == bucket.bucket);
+      if (!left) continue;
+      const uint32_t row = left >> (threadIdx.x & 63) & 1 ? bucket.row(id[k]) : ~0u;
       while (left) {                               // once per different id
         const int lead = __ffsll(static_cast<unsigned long long>(left)) - 1;
         const uint32_t which = read_lane(static_cast<int>(row), lead);
@@ -285,8 +296,7 @@ __global__ void __launch_bounds__(kSortThreads)
     return;
   }
   const uint32_t b = blockIdx.x;
-  const Bucket bucket = {b, static_cast<uint32_t>(buckets - 1),
-                         static_cast<uint32_t>(out.shift), static_cast<uint32_t>(vocab)};
+  const Bucket bucket = {b, static_cast<uint32_t>(out.shift), static_cast<uint32_t>(vocab)};
   const int64_t slot = static_cast<int64_t>(b) * out.rows;
   sort_bucket<kSortRows, kSortSteps, kWide, kPlain>(
       ids, bucket, out.rows, skip, count, wave_sum,
@@ -605,8 +615,7 @@ __global__ void __launch_bounds__(kSortThreads)
     return table + ((static_cast<int64_t>(r) << shift) + b) * width;
   };
   sort_bucket<kSmallRows, kSmallTokens / kSortThreads, kWide, kPlain>(
-      ids, Bucket{b, (1u << shift) - 1, static_cast<uint32_t>(shift), static_cast<uint32_t>(vocab)},
-      rows, skip, count, wave_sum, [&](int r, int p) { start[r] = p; },
+      ids, Bucket{b, static_cast<uint32_t>(shift), static_cast<uint32_t>(vocab)}, rows, skip, count, wave_sum, [&](int r, int p) { start[r] = p; },
       [&](int p, int, int t) { position[p] = static_cast<uint16_t>(t); });
   __syncthreads();
 
