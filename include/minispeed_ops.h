@@ -96,7 +96,7 @@ int ms_embedding(const ms_tokens_t* ids, const ms_rows_t* table, float scale,
  * gradient's type and written whole (rows without tokens are zeros).  Sums
  * are fp32 in an order that depends on the ids alone, multiplied by scale
  * and rounded once.  Ids outside [0, vocab) and `padding_idx` (-1: none) add
- * nothing.  dtable is 16-byte aligned.
+ * nothing.  dtable is 16-byte aligned; at most 2^30 tokens.
  */
 int64_t ms_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t width);
 int ms_embedding_grad(const ms_tokens_t* ids, const ms_rows_t* grad, int64_t vocab,

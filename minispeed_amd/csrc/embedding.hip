@@ -742,6 +742,9 @@ int sum_as(const ms_rows_t& grad, float scale, int64_t from, int64_t until, cons
   return launched();
 }
 
+// Positions past the end of the list are 32-bit too.
+constexpr int64_t kMostTokens = 1 << 30;
+
 // One launch where three would mostly wait for each other: up to kSmallTokens
 // tokens and kSmallTable bytes of table.
 constexpr int64_t kSmallTable = 32 << 20;
@@ -847,7 +850,7 @@ extern "C" int ms_embedding(const ms_tokens_t* ids, const ms_rows_t* table, floa
 }
 
 extern "C" int64_t ms_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t width) {
-  if (n < 0 || vocab < 0 || width < 0 || n > INT32_MAX || vocab > INT32_MAX) return -1;
+  if (n < 0 || vocab < 0 || width < 0 || n > kMostTokens || vocab > INT32_MAX) return -1;
   if (vocab == 0 || width == 0) return 0;
   const GradShape g = shape_of(n, vocab, width);
   return g.start_bytes + 2 * g.list_bytes + g.partial_bytes;
@@ -856,8 +859,8 @@ extern "C" int64_t ms_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t
 extern "C" int ms_embedding_grad(const ms_tokens_t* ids, const ms_rows_t* grad, int64_t vocab,
                                  float scale, int64_t padding_idx, void* dtable, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
-  if (!good_tokens(ids) || !good_rows(grad) || grad->n != ids->n || vocab < 0 ||
-      vocab > INT32_MAX)
+  if (!good_tokens(ids) || !good_rows(grad) || grad->n != ids->n || ids->n > kMostTokens ||
+      vocab < 0 || vocab > INT32_MAX)
     return MS_OPS_EINVAL;
   if (vocab == 0 || grad->width == 0) return MS_OPS_OK;
   if (!dtable || (reinterpret_cast<uintptr_t>(dtable) & 15)) return MS_OPS_EINVAL;

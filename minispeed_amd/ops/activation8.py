@@ -228,4 +228,6 @@ def checkpoint8(fn, *args, preserve_rng_state: bool = True):
     ``args`` only if one of them requires a gradient, as with any reentrant
     checkpoint.
     """
+    if not torch.is_grad_enabled():
+        return fn(*args)
     return _Checkpoint.apply(fn, preserve_rng_state, *args)

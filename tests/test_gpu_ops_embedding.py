@@ -198,8 +198,8 @@ def test_autograd_and_another_stream():
     assert not ms.ops.embedding(ids, w.detach()).requires_grad
 
 
-def test_in_a_graph():
-    rows, width, n = 300, 72, 200
+@pytest.mark.parametrize("rows,width,n", [(300, 72, 200), (5000, 136, 3000)])
+def test_in_a_graph(rows, width, n):
     ids, g = _ids(n, rows, 22), _rand((n, width), "bf16", 23)
     w = _rand((rows, width), "bf16", 24)
     side = torch.cuda.Stream()

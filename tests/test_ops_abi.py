@@ -85,6 +85,10 @@ def test_argument_errors_come_back_before_a_launch(lib):
     assert g(ref(ids), ref(table), I64(10), F(1), I64(-1), P(8), P(16), I64(need), None) == -1
     assert g(ref(ids), ref(rows), I64(-1), F(1), I64(-1), P(8), P(16), I64(need), None) == -1
     assert g(ref(ids), ref(rows), I64(10), F(1), I64(-1), None, P(16), I64(need), None) == -1
+    long = Tokens(8, 2 ** 30 + 1, 2 ** 30 + 1, 0, 1, 1, 0)
+    assert lib.ms_embedding_grad_workspace(2 ** 30 + 1, 10, 16) == -1
+    assert g(ref(long), ref(Rows(8, 2 ** 30 + 1, 16, 2 ** 30 + 1, 0, 16, 1, 0)), I64(10), F(1),
+             I64(-1), P(16), P(16), I64(1 << 40), None) == -1
     if need:
         assert g(ref(ids), ref(rows), I64(10), F(1), I64(-1), P(16), P(16), I64(need - 1), None) == -2
         assert g(ref(ids), ref(rows), I64(10), F(1), I64(-1), P(16), P(8), I64(need), None) == -2
