@@ -31,7 +31,9 @@ __device__ __forceinline__ int64_t vector_at(int64_t c, int64_t width) {
 }
 
 // The output is cut into vectors of 16 bytes, which go to the lanes one after
-// the other whatever the width, kLookupEach of them in flight.
+// the other whatever the width, kLookupEach of them in flight.  Bound by memory:
+// 8192 x 2048 fp16 from 50257 rows 9.3 us, 33.5 MB written at 3.6 TB/s beside the
+// rows read, most of them more than once and from the caches.
 constexpr int kLookupThreads = 256, kLookupEach = 4;
 
 // kShort: rows of less than a vector, value by value.
@@ -428,10 +430,10 @@ struct Clear {
 
 // Blocks below clear.first_block: a span and kWave * N * G columns; wave w adds the
 // span's w-th, (w + kSumWaves)-th .. run of equal ids.  16384 x 768 bf16 into 12000 rows,
-// uniform ids or falling off as 1 / rank: 15.5 and 16.1 us (39 and 32 MB moved).
-// A wave to a span that keeps its 16 rows in registers, the loop over them
-// unrolled: 16.5 and more; the rows set down in LDS for a short loop: 17.3
-// and 23.
+// uniform ids or falling off as 1 / rank: 11.1 and 10.8 us (39 and 32 MB moved), 15.5
+// and 16.1 before the rows were loaded as words.  A wave to a span that keeps its
+// 16 rows in registers, the loop over them unrolled: 16.5 and more; the rows
+// set down in LDS for a short loop: 17.3 and 23.
 template <typename T, int N, int G>
 __global__ void __launch_bounds__(kSumThreads)
     k_sum_spans(ms_rows_t grad, float scale, int slices, Clear clear, Sorted in,
@@ -615,7 +617,8 @@ __global__ void __launch_bounds__(kSortThreads)
     return table + ((static_cast<int64_t>(r) << shift) + b) * width;
   };
   sort_bucket<kSmallRows, kSmallTokens / kSortThreads, kWide, kPlain>(
-      ids, Bucket{b, static_cast<uint32_t>(shift), static_cast<uint32_t>(vocab)}, rows, skip, count, wave_sum, [&](int r, int p) { start[r] = p; },
+      ids, Bucket{b, static_cast<uint32_t>(shift), static_cast<uint32_t>(vocab)}, rows, skip,
+      count, wave_sum, [&](int r, int p) { start[r] = p; },
       [&](int p, int, int t) { position[p] = static_cast<uint16_t>(t); });
   __syncthreads();
 
@@ -659,7 +662,8 @@ __global__ void __launch_bounds__(kSortThreads)
   const int parts = slices < kSortWaves ? kSortWaves / slices : 1, jobs = slices * parts;
   for (uint64_t left = heavy; left; left &= left - 1) {
     const int r = __ffsll(static_cast<unsigned long long>(left)) - 1;
-    const int from = uniform(start[r]), end = uniform(start[r + 1]), each = (end - from + parts - 1) / parts;
+    const int from = uniform(start[r]), end = uniform(start[r + 1]);
+    const int each = (end - from + parts - 1) / parts;
     for (int j = wave; j < jobs; j += kSortWaves) {
       const int slice = j / parts, first = from + (j - slice * parts) * each;
       const int64_t c = (static_cast<int64_t>(slice) * kWave + lane) * N;
@@ -713,7 +717,7 @@ GradShape shape_of(int64_t n, int64_t vocab, int64_t width) {
   return g;
 }
 
-// What the sort's launch clears while it sorts; the sort takes some 8 us.
+// What the sort's launch clears while it sorts, which takes it some 12 us.
 constexpr int64_t kClearBesideSort = 48 << 20;
 
 // Blocks that clear rows [from, until) behind `first` others; blocks: of the launch.
@@ -746,7 +750,9 @@ int sum_as(const ms_rows_t& grad, float scale, int64_t from, int64_t until, cons
 constexpr int64_t kMostTokens = 1 << 30;
 
 // One launch where three would mostly wait for each other: up to kSmallTokens
-// tokens and kSmallTable bytes of table.
+// tokens and kSmallTable bytes of table.  768 columns, ids that fall off as 1 / rank,
+// and with 33% and 90% of them one id: 1024 tokens 10, 18 and 31 us, 21 to 24 in three
+// launches; 2048 tokens would take 11, 26 and 53.
 constexpr int64_t kSmallTable = 32 << 20;
 
 bool is_small(int64_t n, int64_t table_bytes) {
@@ -780,6 +786,7 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
   const int64_t width = grad.width;
   const int64_t row_bytes = width * static_cast<int64_t>(sizeof(T));
   T* table = static_cast<T*>(dtable);
+  if (skip < 0 || skip >= vocab) skip = -1;                // no row: compared as 32-bit words
   if (is_small(ids.n, vocab * row_bytes))
     return width >= 4 ? small_as<T, 4>(ids, grad, vocab, scale, skip, table, s)
                       : small_as<T, 1>(ids, grad, vocab, scale, skip, table, s);

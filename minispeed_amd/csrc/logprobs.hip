@@ -131,7 +131,7 @@ struct Lists {
   Key few[256];
   alignas(16) uint32_t high[NT];
   int at[NT];
-  int looks[2 * NT];        // thread + NT * group
+  int looks[4 * NT];        // thread + NT * group
   int look_count, count;
 };
 
@@ -323,10 +323,13 @@ struct Largest<f16> {
 // that of its others.  The k-th largest of the threads' values bounds the k-th
 // largest of all from below; the few groups that may reach it are read again,
 // their values that do listed in LDS and counted against each other.
+//
+// Measured, 8192 x 50257 fp16 with entropy: 122 us, 6.7 TB/s read, of 7.3 that a
+// kernel which only reads gets; 2048 x 128256 bf16 with 8 alternatives: 98 us, 5.4.
 template <typename T, int NT, bool kTop, bool kEntropy>
-__global__ void __launch_bounds__(NT, kTop ? 6 : 8)
+__global__ void __launch_bounds__(NT, kTop && NT < 256 ? 6 : 8)      // 6 fit beside their LDS
     k_logprobs(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out, Split split) {
-  constexpr int kVec = 16 / sizeof(T), kWaves = NT / kWave, kGroup = 4;
+  constexpr int kVec = 16 / sizeof(T), kWaves = NT / kWave, kGroup = kTop ? 3 : 4;
   typedef Pack<T, kVec> Unit;
   __shared__ Sums sums[kWaves];
   __shared__ float value[kWaves];
@@ -511,33 +514,44 @@ __global__ void __launch_bounds__(NT, kTop ? 6 : 8)
               order_of(best) == least && (g * kGroup * NT + tid) * kVec + head > last;
           if ((g == best_group || order_of(others) >= least) && !out_of_reach) {
             const int at = atomicAdd(&sh.look_count, 1);
-            if (at < 2 * NT) sh.looks[at] = tid + NT * g;
+            if (at < 4 * NT) sh.looks[at] = tid + NT * g;
           }
         }
       __syncthreads();
-      const int again = sh.look_count < 2 * NT ? sh.look_count * kGroup : 0;
-      for (int i0 = tid; i0 < again; i0 += kAgain * NT) {
-        Words p[kAgain];
-        int u[kAgain];
+      if (sh.look_count <= 4 * NT) {
+        const int again = sh.look_count * kGroup;
+        for (int i0 = tid; i0 < again; i0 += kAgain * NT) {
+          Words p[kAgain];
+          int u[kAgain];
 #pragma unroll
-        for (int j = 0; j < kAgain; ++j) {
-          const int i = i0 + j * NT < again ? i0 + j * NT : i0;
-          const int look = sh.looks[i / kGroup];
-          u[j] = ((look / NT) * kGroup + i % kGroup) * NT + look % NT;
-          p[j] = *reinterpret_cast<const Words*>(
-              first + static_cast<int64_t>(u[j] < units ? u[j] : 0) * kVec);
-          if (i0 + j * NT >= again) u[j] = units;
+          for (int j = 0; j < kAgain; ++j) {
+            const int i = i0 + j * NT < again ? i0 + j * NT : i0;
+            const int look = sh.looks[i / kGroup];
+            u[j] = ((look / NT) * kGroup + i % kGroup) * NT + look % NT;
+            p[j] = *reinterpret_cast<const Words*>(
+                first + static_cast<int64_t>(u[j] < units ? u[j] : 0) * kVec);
+            if (i0 + j * NT >= again) u[j] = units;
+          }
+#pragma unroll
+          for (int j = 0; j < kAgain; ++j)
+            if (u[j] < units)
+#pragma unroll
+              for (int i = 0; i < kVec; ++i)
+                if (widen(values_of<T>(p[j]).v[i]) >= least_value)
+                  offer(widen(values_of<T>(p[j]).v[i]), head + u[j] * kVec + i);
         }
+      } else {
+        // more groups than the list takes (a long row, many alternatives): all again
+        // (1024 x 262144 bf16, 50 alternatives, with half the list: 180 us instead of 121)
+        for (int u = tid; u < units; u += NT) {
+          const Unit p = unit_of(0, u);
 #pragma unroll
-        for (int j = 0; j < kAgain; ++j)
-          if (u[j] < units)
-#pragma unroll
-            for (int i = 0; i < kVec; ++i)
-              if (widen(values_of<T>(p[j]).v[i]) >= least_value)
-                offer(widen(values_of<T>(p[j]).v[i]), head + u[j] * kVec + i);
+          for (int i = 0; i < kVec; ++i)
+            if (widen(p.v[i]) >= least_value) offer(widen(p.v[i]), head + u * kVec + i);
+        }
       }
       __syncthreads();
-      give_up = sh.count > sh.kCandidates || sh.look_count >= 2 * NT;
+      give_up = sh.count > sh.kCandidates;
     }
   }
 
@@ -570,8 +584,8 @@ __global__ void __launch_bounds__(NT, kTop ? 6 : 8)
 
 // Threads to a block.  With alternatives 256, of which more fit a CU beside their
 // LDS and end together: 8192 x 50257 bf16 with entropy, 8 and 50 alternatives
-// 143 and 187 us, 198 and 226 with 512 (and 1024 or 4096 keys to the list: 143
-// and 170).  Without, 512: 126 us, 130 with 256.  Small vocabularies: 128.
+// 149 and 181 us, 198 and 226 with 512 (and 146 and 190 with groups of 4 rounds).
+// Without, 512: 126 us, 130 with 256.  Small vocabularies: 128.
 constexpr int kThreads = 512, kTopThreads = 256, kFewThreads = 128, kFewUnits = 512;
 
 // A row's parts.
@@ -627,12 +641,13 @@ __global__ void __launch_bounds__(kThreads)
 constexpr float kFarLse = 256.f;
 
 constexpr int kGradThreads = 256, kGradWaves = kGradThreads / kWave;
-constexpr int kGradGroup = 1;             // 16-byte units to a thread; 1, 2, 4: 270, 280, 290 us
+constexpr int kGradGroup = 1;             // 16-byte units to a thread; 1, 2, 4: 263, 280, 290 us
 
 // A block takes kGradGroup rounds of aligned 16-byte units of the gradient's row
 // (the logits' row may lie otherwise).  With c a whole number near lse L and
 // p' = 2^(x L - c): dx = p' (a + b x), where a and b hold what c rounded off; the
-// target's g is added to the one value.
+// target's g is added to the one value.  8192 x 50257 fp16: 263 us, 6.3 TB/s, what
+// a copy of as many bytes gets.
 template <typename T, bool kEntropy>
 __global__ void __launch_bounds__(kGradThreads)
     k_logprobs_grad(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, const float* lse,

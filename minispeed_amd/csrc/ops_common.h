@@ -80,18 +80,7 @@ __device__ __forceinline__ void store(T* p, const Pack<T, N>& x) {
   *reinterpret_cast<raw*>(p) = r;
 }
 
-// 16 aligned bytes that are read once: not kept in the caches.
-template <int N, typename T>
-__device__ __forceinline__ Pack<T, N> load_stream(const T* p) {
-  typedef uint32_t raw __attribute__((ext_vector_type(4)));
-  static_assert(N * sizeof(T) == 16, "");
-  const raw r = __builtin_nontemporal_load(reinterpret_cast<const raw*>(p));
-  Pack<T, N> x;
-  __builtin_memcpy(&x, &r, 16);
-  return x;
-}
-
-// ... at any element alignment.
+// N values that are read once, at any element alignment: not kept in the caches.
 template <int N, typename T>
 __device__ __forceinline__ Pack<T, N> load_stream_any(const T* p) {
   typedef typename raw_of<N * sizeof(T)>::type raw;

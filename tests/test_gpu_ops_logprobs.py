@@ -207,6 +207,18 @@ def test_alternatives_of_ordered_rows(order, dtype):
         check(x, torch.zeros(2, dtype=torch.int64, device=DEV), top=top)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_many_places_to_look_again(dtype):
+    """Two far apart places of many threads hold what may be an alternative."""
+    n, v, apart = 257, 131072, 65536
+    x = _logits(n, v, dtype, 31, std=1.0)
+    high = torch.arange(0, 800, 8)
+    for start in (0, apart):
+        values = 8 + torch.randn(n, len(high), generator=torch.Generator().manual_seed(start))
+        x[:, (high + start).to(DEV)] = values.to(x.dtype).to(DEV)
+    check(x, _targets(n, v, 32), top=50)
+
+
 def test_rows_past_32_bits():
     n, v = 17_000, 131_072                        # 2.2e9 values, 4.5 GB
     x = torch.zeros(n, v, dtype=torch.bfloat16, device=DEV)
