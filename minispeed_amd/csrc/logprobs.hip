@@ -324,8 +324,8 @@ struct Largest<f16> {
 // largest of all from below; the few groups that may reach it are read again,
 // their values that do listed in LDS and counted against each other.
 //
-// Measured, 8192 x 50257 fp16 with entropy: 122 us, 6.7 TB/s read, of 7.3 that a
-// kernel which only reads gets; 2048 x 128256 bf16 with 8 alternatives: 98 us, 5.4.
+// Measured, 8192 x 50257 fp16: 123 us, 6.7 TB/s read, of 7.3 that a
+// kernel which only reads gets; 2048 x 128256 bf16, entropy, 8 alternatives: 95 us, 5.5.
 template <typename T, int NT, bool kTop, bool kEntropy>
 __global__ void __launch_bounds__(NT, kTop && NT < 256 ? 6 : 8)      // 6 fit beside their LDS
     k_logprobs(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out, Split split) {
