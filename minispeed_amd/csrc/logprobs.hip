@@ -120,6 +120,7 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t r, const R
   out.logprob[r] = target == ignore ? 0.f : good ? row.logprob(given) : quiet_nan();
 }
 
+constexpr float kMostSum = 0x1p100f;
 constexpr int kMost = MS_OPS_MAX_TOP;
 static_assert(kMost <= kWave, "");
 
@@ -194,7 +195,7 @@ __device__ __forceinline__ void select_top(Lists<NT, C>& sh, int n, int k, Put p
 // A row by itself whatever it holds: the maximum first, then the sums, then one
 // pass for each alternative.  (Inlined: a call's stack alone took the whole
 // kernel from 126 to 190 us for 8192 x 50257.)  For rows that the fast way gives up: NaN, +inf,
-// logits beyond 2^20 or 88 above all that the first look saw.
+// logits beyond 2^19, or 69 above all that the first look saw.
 template <int NT, typename T>
 __device__ __forceinline__ void slow_row(float* value, Key* keys, const T* x, int64_t vocab, int64_t r,
                                       const Outputs& out, int64_t target, int64_t ignore) {
@@ -253,10 +254,22 @@ __device__ __forceinline__ void slow_row(float* value, Key* keys, const T* x, in
   }
 }
 
+// A wave's whole m2 for the largest logit it has seen.  A mask's lowest values, for
+// which seen * L may overflow, get 0: they add nothing, which is right beside
+// logits above kFarBelow / 2 and nowhere else.
+constexpr float kFarBelow = -524288.f;        // -2^19
+// Below this the first look may have met only masked values, -1e4 for one.
+constexpr float kLow = -64.f;
+__device__ __forceinline__ float reference(float seen) {
+  return seen < kFarBelow ? 0.f : rintf(seen * kLog2e);
+}
+// ... whether leaving them out was wrong
+__device__ __forceinline__ bool needed(Sums all) { return all.s == 0.f || all.m2 < kFarBelow / 2; }
+
 // What a part of a split row leaves for k_join_parts, its keys behind it.
 struct Part {
   Sums sums;
-  int given_up;
+  int given_up;         // 2: values were left out
 };
 
 struct Split {
@@ -316,8 +329,9 @@ struct Largest<f16> {
 // TB/s instead of 6.8.)
 //
 // The first group gives a reference, one per wave, so that no running maximum
-// is kept: s only overflows where later logits are 88 above all the wave saw,
-// and the row is then done again by slow_row.
+// is kept but for waves that may have seen only masked values.  Where later logits
+// are 69 above all that the wave saw the row is done again by slow_row: s < 2^100
+// keeps t, up to 100 s, in range too.
 //
 // For the alternatives each thread keeps the largest value of its best group and
 // that of its others.  The k-th largest of the threads' values bounds the k-th
@@ -333,6 +347,7 @@ __global__ void __launch_bounds__(NT, kTop && NT < 256 ? 6 : 8)      // 6 fit be
   typedef Pack<T, kVec> Unit;
   __shared__ Sums sums[kWaves];
   __shared__ float value[kWaves];
+  __shared__ int out_of[kWaves];
   __shared__ Lists<(kTop ? NT : 1), (kTop ? 1024 : kMost)> sh;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r = blockIdx.x / split.parts, vocab = logits.width;
@@ -383,7 +398,8 @@ __global__ void __launch_bounds__(NT, kTop && NT < 256 ? 6 : 8)      // 6 fit be
 #pragma unroll
   for (int k = 0; k < kGroup; ++k) largest.see(values_of<T>(now[k]));
   float seen = wave_max(fmaxf(single, largest.get())), s = 0.f, t = 0.f;
-  float m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
+  float m2 = reference(seen);
+  bool left_out = seen < kFarBelow && seen != -INFINITY;
   auto add = [&](float v) {
     const float y = fmaf(v, kLog2e, -m2), e = exp2_fast(y);
     s += e;
@@ -393,14 +409,24 @@ __global__ void __launch_bounds__(NT, kTop && NT < 256 ? 6 : 8)      // 6 fit be
   float best = largest.get(), others = -INFINITY;
   int best_group = 0;
   for (int k0 = 0;;) {
-    if (k0 && seen == -INFINITY) {
-      // a wave that has seen nothing but -inf looks again
+    if (k0 && seen < kLow) {
+      // a wave that may have seen nothing but what is masked looks again
       Largest<T> here;
 #pragma unroll
       for (int k = 0; k < kGroup; ++k)
         if (k0 + k < rounds) here.see(values_of<T>(now[k]));
-      seen = wave_max(here.get());
-      m2 = seen == -INFINITY ? 0.f : rintf(seen * kLog2e);
+      const float high = wave_max(here.get());
+      left_out |= high < kFarBelow && high != -INFINITY;
+      if (high > seen) {
+        const float to = reference(high);
+        if (seen >= kFarBelow) {
+          const float d = m2 - to, k = exp2_fast(d);
+          if (kEntropy) t = fmaf(d, s, t) * k;
+          s *= k;
+        }
+        seen = high;
+        m2 = to;
+      }
     }
     Largest<T> here;
 #pragma unroll
@@ -427,20 +453,23 @@ __global__ void __launch_bounds__(NT, kTop && NT < 256 ? 6 : 8)      // 6 fit be
 
   s = wave_sum(s);
   if (kEntropy) t = wave_sum(t);
-  if (lane == 0) sums[wave] = Sums{m2, s, t};
+  if (lane == 0) sums[wave] = Sums{m2, s, t}, out_of[wave] = left_out;
   const float most = fmaxf(single, best);
   if constexpr (kTop) {
     sh.high[tid] = tid < units || alone >= 0 ? order_of(most) : 0;
     if (tid == 0) sh.count = sh.look_count = 0;
   }
   __syncthreads();
-  bool give_up = false;
+  bool give_up = false, some_out = false;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    give_up |= !(sums[w].s < INFINITY) || !(fabsf(sums[w].m2) <= 1 << 20);
-  if (!kTop && !give_up && wave) return;
+  for (int w = 0; w < kWaves; ++w) {
+    give_up |= !(sums[w].s < kMostSum) || !(sums[w].m2 <= 1 << 20);
+    some_out |= out_of[w];
+  }
+  if (!kTop && !give_up && !some_out && wave) return;
   Sums all = sums[0];
   for (int w = 1; w < kWaves; ++w) all = join(all, sums[w]);
+  if (split.parts == 1) give_up |= some_out && needed(all);
   const float given = widen(given_raw);
 
   if constexpr (kTop) {
@@ -570,7 +599,7 @@ __global__ void __launch_bounds__(NT, kTop && NT < 256 ? 6 : 8)      // 6 fit be
     return;
   }
   char* left = split.work + blockIdx.x * split.stride;
-  if (tid == 0) *reinterpret_cast<Part*>(left) = Part{all, give_up};
+  if (tid == 0) *reinterpret_cast<Part*>(left) = Part{all, give_up ? 1 : some_out ? 2 : 0};
   if constexpr (kTop) {
     if (give_up) return;
     Key* keys = reinterpret_cast<Key*>(left + sizeof(Part));
@@ -610,7 +639,8 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = threadIdx.x & 63;
   Part mine{{0.f, 0.f, 0.f}, 0};
   if (lane < split.parts) mine = *reinterpret_cast<const Part*>(work + lane * split.stride);
-  const bool give_up = __any(mine.given_up);
+  bool give_up = __any(mine.given_up == 1);
+  const bool some_out = __any(mine.given_up == 2);
   Sums all = mine.sums;
   for (int k = 1; k < kWave; k <<= 1) {
     Sums other;
@@ -620,6 +650,7 @@ __global__ void __launch_bounds__(kThreads)
     all = lane & k ? join(other, all) : join(all, other);
   }
   __syncthreads();
+  give_up |= some_out && needed(all);
   if (give_up) {
     slow_row<kThreads>(value, sh.list, row, vocab, r, out, target, ignore);
     return;

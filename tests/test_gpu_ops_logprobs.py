@@ -168,6 +168,39 @@ def test_masks(dtype, v):
     check_grad(x, t, entropy=False)
 
 
+@pytest.mark.parametrize("n", [3, 257])             # rows that are split, and that are not
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_masked_stretches(dtype, n):
+    """A mask that leaves the last values, one in the middle, or a few."""
+    v = 33_000
+    low = torch.finfo(ref.DTYPES[dtype]).min
+    for fill in (-INF, low, -1e4, -70.0, -6e5 if dtype != "fp16" else -6e4):
+        x, t = _logits(n, v, dtype, 41), _targets(n, v, 42)
+        x[0, :-5] = fill
+        x[1, :20_000] = fill
+        x[2, : v // 2], x[2, v // 2 + 1:] = fill, fill
+        if n > 3:
+            x[3:9, torch.arange(v, device=DEV) % 3001 != 17] = fill
+            x[9, : v // 2], x[9, v // 2:] = low, fill
+            x[10] = fill
+            x[10, ::2] = fill - 1 if -1e6 < fill else fill
+        check(x, t, top=8)
+        check(x, t, entropy=False)
+        check_grad(x, t)
+
+
+@pytest.mark.parametrize("n", [2, 257])
+@pytest.mark.parametrize("above", [60.0, 68.0, 75.0, 84.0, 86.0, 88.0, 89.0, 300.0])
+def test_one_far_above_the_others(above, n):
+    v = 50_257
+    x = _logits(n, v, "fp32", 43)
+    x[:, 40_000] = above
+    x[0, -1] = above
+    t = torch.full((n,), 40_000, device=DEV)
+    check(x, t, top=3)
+    check(x, t)
+
+
 def test_nan_and_infinity():
     v = 700
     x, t = _logits(6, v, "fp32", 11), _targets(6, v, 12, 0.0)
