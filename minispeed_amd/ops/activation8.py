@@ -95,7 +95,7 @@ class _ActivationLinear(torch.autograd.Function):
         a, saved = activation8(h, kind, up)
         ctx.kind, ctx.meta = kind, [(s.shape, s.dtype) for s in saved]
         ctx.save_for_backward(weight, *(t for s in saved for t in (s.codes, s.exponents)))
-        ctx.has_bias = bias is not None
+        ctx.bias_dtype = None if bias is None else bias.dtype
         return F.linear(a, weight, bias)
 
     @staticmethod
@@ -107,12 +107,14 @@ class _ActivationLinear(torch.autograd.Function):
         dh = dup = dw = db = None
         flat = grad.reshape(-1, grad.shape[-1])
         if need[0] or need[1] or need[2]:
-            grads, a = activation8_grad(saved, grad.matmul(weight), ctx.kind, again=need[2])
+            # (the types differ under autocast only)
+            da = grad.matmul(weight.to(grad.dtype)).to(saved[0].dtype)
+            grads, a = activation8_grad(saved, da, ctx.kind, again=need[2])
             dh, dup = grads if len(grads) == 2 else (grads[0], None)
             if need[2]:
-                dw = flat.t().mm(a.reshape(-1, a.shape[-1]))
-        if ctx.has_bias and need[3]:
-            db = flat.sum(0)
+                dw = flat.t().mm(a.reshape(-1, a.shape[-1]).to(grad.dtype)).to(weight.dtype)
+        if ctx.bias_dtype is not None and need[3]:
+            db = flat.sum(0, dtype=ctx.bias_dtype)
         return dh, dup, dw, db, None
 
 
@@ -141,7 +143,7 @@ class _Checkpoint(torch.autograd.Function):
         for arg in args:
             if not isinstance(arg, torch.Tensor):
                 ctx.slots.append(("value", arg, False))
-            elif arg.is_floating_point() and arg.dim() > 0 and arg.dtype in _HELD:
+            elif arg.is_cuda and arg.dim() > 0 and arg.dtype in _HELD:
                 packed = pack8(arg)
                 ctx.slots.append(("held", (packed.shape, packed.dtype), arg.requires_grad))
                 held += [packed.codes, packed.exponents]
@@ -218,8 +220,8 @@ def checkpoint8(fn, *args, preserve_rng_state: bool = True):
     """``fn(*args)`` whose activations are computed again in the backward pass, from
     arguments held in 8 bits.
 
-    The floating tensors among ``args`` are kept in their 8-bit form (other
-    tensors as they are), and ``fn`` runs again on the values they stand for when
+    The float32, float16 and bfloat16 tensors on the GPU among ``args`` are kept in
+    their 8-bit form (other tensors as they are), and ``fn`` runs again on the values they stand for when
     the gradients come: the use of minispeed's ``checkpoint``
     (minispeed/activation_checkpointing.py:17-20) with a quarter to a half of its
     memory.  The first run sees the arguments themselves.  Parameters that ``fn``

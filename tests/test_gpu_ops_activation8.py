@@ -221,6 +221,37 @@ def test_activation_linear_autograd(kind):
     assert abs(slope - float(prod.sum())) <= 1e-4 * float(prod.abs().sum())
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("half_h", [False, True])
+def test_activation_linear_under_autocast(dtype, half_h):
+    """fp32 parameters, products in half precision: a product of 64 terms is off by
+    at most a rounding of each operand, the sum and the result (2^-8 for bf16)."""
+    kind, n, f, d = "silu", 24, 64, 48
+    w, b = _rand((d, f), "fp32", 17, 0.1).requires_grad_(), _rand((d,), "fp32", 18).requires_grad_()
+    h0 = _rand((n, f), dtype if half_h else "fp32", 19)
+    gy = _rand((n, d), dtype, 20)
+    h = h0.clone().requires_grad_()
+    with torch.autocast("cuda", ref.DTYPES[dtype]):
+        y = ms.ops.activation8_linear(h, w, b, kind)
+    y.backward(gy)
+    assert y.dtype == gy.dtype and h.grad.dtype == h.dtype
+    assert w.grad.dtype == b.grad.dtype == torch.float32
+    hv = ref.held(h0)[2].view(n, f).requires_grad_()
+    wv = w.detach().cpu().double().requires_grad_()
+    (F.silu(hv) @ wv.t()).backward(gy.cpu().double())
+    unit = 2.0 ** (-11 if dtype == "fp16" else -8)
+    size = (gy.cpu().double().abs() @ wv.detach().abs()) * 1.1
+    assert bool(((h.grad.cpu().double() - hv.grad).abs() <= 5 * unit * size).all())
+    size = gy.cpu().double().abs().t() @ F.silu(hv.detach()).abs()
+    assert bool(((w.grad.cpu().double() - wv.grad).abs() <= 5 * unit * size + 1e-6).all())
+
+
+def test_checkpoint_of_a_host_tensor():
+    x, host = _rand((4, 32), "fp32", 21).requires_grad_(), torch.arange(4.0)
+    ms.ops.checkpoint8(lambda z, c: (z * c.to(DEV)[:, None]).sum(), x, host).backward()
+    assert torch.equal(x.grad, host.to(DEV)[:, None].expand(4, 32))
+
+
 def test_checkpoint_runs_again_on_the_held_values():
     torch.manual_seed(0)
     layer = torch.nn.Sequential(torch.nn.Linear(64, 96), torch.nn.GELU(), torch.nn.Dropout(0.5),
