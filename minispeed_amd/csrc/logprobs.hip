@@ -614,8 +614,11 @@ __global__ void __launch_bounds__(NT, kTop && NT < 256 ? 6 : 8)      // 6 fit be
 // Threads to a block.  With alternatives 256, of which more fit a CU beside their
 // LDS and end together: 8192 x 50257 bf16 with entropy, 8 and 50 alternatives
 // 149 and 181 us, 198 and 226 with 512 (and 146 and 190 with groups of 4 rounds).
-// Without, 512: 126 us, 130 with 256.  Small vocabularies: 128.
-constexpr int kThreads = 512, kTopThreads = 256, kFewThreads = 128, kFewUnits = 512;
+// Without, 512: 126 us, 130 with 256.  Rows of up to kMidUnits units (half of that with
+// alternatives) are over soon, so 128, more rows beside each other: 32768 x 4097 and
+// 8192, 16384 x 16384 bf16 61, 86 and 86 us, 156, 171 and 127 with 512; 8 alternatives
+// 116, 145 and 121, 134, 172 and 121 with 256.
+constexpr int kThreads = 512, kTopThreads = 256, kMidThreads = 128, kMidUnits = 2048;
 
 // A row's parts.
 template <typename T>
@@ -664,6 +667,216 @@ __global__ void __launch_bounds__(kThreads)
     });
 }
 
+// -- short rows -----------------------------------------------------------------
+
+// Rows of up to kShortUnits units: a wave to a row, which it holds in registers, R
+// units to a lane; the blocks that fit beside each other go through all rows.
+// With entropy, bf16: 65536 x 512 25 us, 65536 x 4096 86 us (6.2 TB/s), with 8 alternatives 57 and
+// 149.  (A block of 128 threads to a row: 65536 x 512 56 and 140 us, which is what
+// starting the blocks takes.)
+constexpr int kShortThreads = 256, kShortWaves = kShortThreads / kWave;
+constexpr int kShortUnits = 8 * kWave;
+constexpr int kShortBlocks = 2048;               // 8 to a CU
+constexpr int kShortList = 256;
+
+// Where a row's units lie, and the value before or behind them that a lane takes.
+template <typename T>
+struct ShortRow {
+  static constexpr int kVec = 16 / sizeof(T);
+  const T* x;
+  int head, units, alone;
+
+  // aligned_to: the address whose 16-byte units are taken
+  __device__ __forceinline__ ShortRow(const T* row, const T* aligned_to, int vocab, int lane) {
+    x = row;
+    const int off =
+        static_cast<int>(-(reinterpret_cast<uintptr_t>(aligned_to) / sizeof(T)) & (kVec - 1));
+    head = off < vocab ? off : vocab;
+    units = (vocab - head) / kVec;
+    const int rest = vocab - head - units * kVec;
+    alone = lane < head                             ? lane
+            : lane >= kVec && lane - kVec < rest ? head + units * kVec + lane - kVec
+                                                    : -1;
+  }
+  // kAny: the units lie at any address.  Lanes without a unit load the last one.
+  template <bool kAny, int R>
+  __device__ __forceinline__ void load(Words (&w)[R], int lane) const {
+    typedef typename raw_of<16>::type AnyWords;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int u = k * kWave + lane;
+      const T* at = x + head + static_cast<int64_t>(u < units ? u : units - 1) * kVec;
+      if (units > 0)
+        w[k] = kAny ? __builtin_nontemporal_load(reinterpret_cast<const AnyWords*>(at))
+                    : __builtin_nontemporal_load(reinterpret_cast<const Words*>(at));
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+      if (k * kWave + lane >= units) w[k] = no_values<T>();
+  }
+  __device__ __forceinline__ float load_alone() const {
+    const T raw = x[alone >= 0 ? alone : 0];
+    return alone >= 0 ? widen(raw) : -INFINITY;
+  }
+};
+
+// A wave's values: f(value, index) for each that it has.
+template <typename T, int R, typename F>
+__device__ __forceinline__ void each_value(const ShortRow<T>& row, const Words (&w)[R], float single,
+                                           int lane, F f) {
+  constexpr int kVec = 16 / sizeof(T);
+  if (row.alone >= 0) f(single, row.alone);
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+    if (k * kWave + lane < row.units)
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        f(widen(values_of<T>(w[k]).v[i]), row.head + (k * kWave + lane) * kVec + i);
+}
+
+__device__ __forceinline__ int wave_count(int x) {
+  for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k);
+  return uniform(x);
+}
+
+// The `top` first of a row in key order, into `list`, whatever it holds: of the
+// values that equal the last one those with the lowest indices.  At least `top`
+// values are as large as `least`.  (The row is read again for each step: its words
+// taken apart in registers cost every row its place.)
+template <typename T>
+__device__ __forceinline__ void list_exactly(const T* x, int vocab, int lane, int top,
+                                             uint32_t least, Key* list) {
+  auto count = [&](auto test) {
+    int n = 0;
+    for (int j = lane; j < vocab; j += kWave) n += test(order_of(widen(x[j])));
+    return wave_count(n);
+  };
+  int above = count([&](uint32_t o) { return o > least; });
+  if (above >= top) {
+    uint32_t bound = 0;                       // the largest word that `top` are as large as
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t more = bound | 1u << bit;
+      if (more <= least || count([&](uint32_t o) { return o >= more; }) >= top) bound = more;
+    }
+    least = bound;
+    above = count([&](uint32_t o) { return o > least; });
+  }
+  int to = 0, equal = 0;
+  const uint64_t lower = (1ull << lane) - 1;
+  for (int j0 = 0; j0 < vocab; j0 += kWave) {
+    const int j = j0 + lane;
+    const float v = j < vocab ? widen(x[j]) : 0.f;
+    const uint32_t o = j < vocab ? order_of(v) : 0;
+    const uint64_t same = __ballot(j < vocab && o == least);
+    const bool in = j < vocab && (o > least || (o == least && equal + __popcll(same & lower) <
+                                                                   top - above));
+    const uint64_t all = __ballot(in);
+    if (in) list[to + __popcll(all & lower)] = key_of(v, j);
+    to += __popcll(all);
+    equal += __popcll(same);
+  }
+}
+
+template <typename T, int R, bool kTop, bool kEntropy>
+__global__ void __launch_bounds__(kShortThreads)
+    k_logprobs_short(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, Outputs out) {
+  constexpr int kVec = 16 / sizeof(T);
+  __shared__ Key lists[kTop ? kShortWaves : 1][kTop ? kShortList : 1];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int vocab = static_cast<int>(logits.width);
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kShortWaves + wave; r < logits.n;
+       r += static_cast<int64_t>(gridDim.x) * kShortWaves) {
+    const int64_t target = token(targets, r);
+    const T* x = static_cast<const T*>(logits.data) + row_start(logits, r);
+    const ShortRow<T> row(x, x, vocab, lane);
+    Words w[R];
+    row.template load<false>(w, lane);
+    const float single = row.load_alone();
+    const bool good = target >= 0 && target < vocab;
+    const float given = widen(x[good ? target : 0]);
+    Largest<T> largest[2];                             // of each half of the units
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      Pack<T, kVec / 2> half[2];
+      __builtin_memcpy(half, &w[k], 16);
+      largest[0].see(half[0]);
+      largest[1].see(half[1]);
+    }
+    const float mine = fmaxf(single, largest[0].get()), other = largest[1].get();
+    const float most = wave_max(fmaxf(mine, other)), base = most == -INFINITY ? 0.f : most;
+    float s = 0.f, t = 0.f;
+    auto add = [&](float v) {
+      const float y = (v - base) * kLog2e, e = exp2_fast(y);
+      s += e;
+      if (kEntropy) t = fmaf(e, fmaxf(y, -1e30f), t);
+    };
+    add(single);
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) add(widen(values_of<T>(w[k]).v[i]));
+    s = wave_sum(s);
+    if (kEntropy) t = wave_sum(t);
+    const bool empty = s == 0.f;
+    const float ls = log2_fast(s) * kLn2;
+    auto logprob = [&](float v) { return empty ? -INFINITY : (v - base) - ls; };
+    if (lane == 0) {
+      out.lse[r] = empty ? -INFINITY : base + ls;
+      if (kEntropy) out.entropy[r] = empty ? 0.f : ls - t / s * kLn2;
+      out.logprob[r] = target == ignore ? 0.f : good ? logprob(given) : quiet_nan();
+    }
+    if constexpr (kTop) {
+      // the k-th largest of the 128 half lanes' largest bounds the k-th largest from
+      // below; what reaches it is listed and counted against each other
+      constexpr int kSkip = sizeof(T) == 2 ? 13 : 0;
+      Key* list = lists[wave];
+      const bool unit = lane < row.units;
+      const uint32_t least = kth_largest<kSkip>(unit || row.alone >= 0 ? order_of(mine) : 0,
+                                                unit ? order_of(other) : 0, out.top);
+      int found = kShortList + 1;
+      if (least == 0 && vocab <= kShortList) {           // fewer than that: all of them
+        for (int j = lane; j < vocab; j += kWave) list[j] = key_of(widen(x[j]), j);
+        found = vocab;
+      } else if (s < INFINITY && least > 0x007FFFFFu) {
+        const float least_value = value_of(least);
+        int to = 0;
+        auto offer = [&](float v, int j) {
+          const uint64_t hits = __ballot(v >= least_value);
+          if (!hits) return;
+          const int at = to + __popcll(hits & ((1ull << lane) - 1));
+          if (v >= least_value && at < kShortList) list[at] = key_of(v, j);
+          to += __popcll(hits);
+        };
+        offer(single, row.alone);
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+#pragma unroll
+          for (int i = 0; i < kVec; ++i)
+            offer(widen(values_of<T>(w[k]).v[i]), row.head + (k * kWave + lane) * kVec + i);
+        found = to;
+      }
+      if (found > kShortList) {
+        list_exactly(x, vocab, lane, out.top, least, list);
+        found = out.top;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (int i = lane; i < found; i += kWave) {
+        const Key key = list[i];
+        int above = 0;
+#pragma unroll 4
+        for (int j = 0; j < found; ++j) above += list[j] > key;
+        if (above < out.top) {
+          out.top_id[r * out.top + above] = index_of(key);
+          out.top_logprob[r * out.top + above] = logprob(value_of(key));
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
 // -- gradient -----------------------------------------------------------------
 
 // Beyond this an fp32 lse no longer tells logits from each other (a row masked
@@ -679,6 +892,24 @@ constexpr int kGradGroup = 1;             // 16-byte units to a thread; 1, 2, 4:
 // p' = 2^(x L - c): dx = p' (a + b x), where a and b hold what c rounded off; the
 // target's g is added to the one value.  8192 x 50257 fp16: 263 us, 6.3 TB/s, what
 // a copy of as many bytes gets.
+// A value's gradient but for the target's g; lse within kFarLse.
+template <bool kEntropy>
+struct RowGrad {
+  float c, a, b;
+
+  __device__ __forceinline__ RowGrad(float lse, float entropy, float g, float h) {
+    c = rintf(lse * kLog2e);
+    const float k = exp2_fast(-fmaf(lse, kLog2e, -c));
+    b = -h * k;
+    a = -(g + h * (entropy - lse)) * k;
+  }
+  __device__ __forceinline__ float operator()(float v) const {
+    const float p = exp2_fast(fmaf(v, kLog2e, -c));
+    if (!kEntropy) return p * a;
+    return p * fmaf(b, fmaxf(v, -1e6f), a);        // -inf: p is 0, and 0 * inf must not be
+  }
+};
+
 template <typename T, bool kEntropy>
 __global__ void __launch_bounds__(kGradThreads)
     k_logprobs_grad(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, const float* lse,
@@ -748,13 +979,7 @@ __global__ void __launch_bounds__(kGradThreads)
     return;
   }
 
-  const float c = rintf(l * kLog2e), k = exp2_fast(-fmaf(l, kLog2e, -c));
-  const float b = -h * k, a = -(g + h * (big_h - l)) * k;
-  auto one = [&](float v) {
-    const float p = exp2_fast(fmaf(v, kLog2e, -c));
-    if (!kEntropy) return p * a;
-    return p * fmaf(b, fmaxf(v, -1e6f), a);        // -inf: p is 0, and 0 * inf must not be
-  };
+  const RowGrad<kEntropy> one(l, big_h, g, h);
 #pragma unroll
   for (int i = 0; i < kGradGroup; ++i) {
     const int u = part * kEach + i * kGradThreads + tid;
@@ -780,14 +1005,79 @@ __global__ void __launch_bounds__(kGradThreads)
   if (alone >= 0) d[alone] = narrow<T>(one(widen(x[alone])) + (alone == hit ? g : 0.f));
 }
 
-// How a row is split: not at all from 512 rows on, two blocks to a CU; else so
-// that there are as many blocks, each with a unit to every thread at least.
+// Short rows: a wave to each, as forward, by the units of the gradient's row.  65536 x
+// 512 and 4096 bf16 29 and 190 us (4.6 and 5.6 TB/s), 55 us for the first with a
+// block to each.
+template <typename T, int R, bool kEntropy>
+__global__ void __launch_bounds__(kShortThreads)
+    k_logprobs_grad_short(ms_rows_t logits, ms_tokens_t targets, int64_t ignore, const float* lse,
+                          const float* entropy, const float* grad_logprob,
+                          const float* grad_entropy, T* __restrict__ out) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int vocab = static_cast<int>(logits.width);
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kShortWaves + wave; r < logits.n;
+       r += static_cast<int64_t>(gridDim.x) * kShortWaves) {
+    const int64_t target = token(targets, r);
+    const T* x = static_cast<const T*>(logits.data) + row_start(logits, r);
+    T* d = out + r * vocab;
+    const ShortRow<T> row(x, d, vocab, lane);
+    Words w[R];
+    row.template load<true>(w, lane);
+    const float single = row.load_alone();
+    const bool counts = grad_logprob && target != ignore;
+    float g = counts ? grad_logprob[r] : 0.f;
+    if (counts && (target < 0 || target >= vocab)) g = quiet_nan();
+    const int hit = target >= 0 && target < vocab ? static_cast<int>(target) : -1;
+    const float h = kEntropy ? grad_entropy[r] : 0.f, big_h = kEntropy ? entropy[r] : 0.f;
+    const float l = lse[r];
+    auto write = [&](auto one) {
+      if (row.alone >= 0) d[row.alone] = narrow<T>(one(single) + (row.alone == hit ? g : 0.f));
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int j0 = row.head + (k * kWave + lane) * kVec;
+        if (k * kWave + lane >= row.units) continue;
+        Pack<T, kVec> z;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          z.v[i] = narrow<T>(one(widen(values_of<T>(w[k]).v[i])) + (j0 + i == hit ? g : 0.f));
+        store_stream<kVec>(d + j0, z);
+      }
+    };
+    if (l == -INFINITY) {
+      g = 0.f;
+      write([](float) { return 0.f; });
+    } else if (fabsf(l) > kFarLse) {
+      float most = single, s = 0.f;
+      each_value(row, w, single, lane, [&](float v, int) { most = fmaxf(most, v); });
+      most = wave_max(most);
+      each_value(row, w, single, lane,
+                 [&](float v, int) { s += exp2_fast((v - most) * kLog2e); });
+      const float ls = log2_fast(wave_sum(s)) * kLn2;
+      write([&](float v) {
+        const float logp = (v - most) - ls, p = exp2_fast(logp * kLog2e);
+        float y = -g * p;
+        if (kEntropy && p != 0.f) y -= h * p * (logp + big_h);
+        return y;
+      });
+    } else {
+      write(RowGrad<kEntropy>(l, big_h, g, h));
+    }
+  }
+}
+
+bool is_short(int64_t vocab, int32_t dtype) {
+  return vocab * dtype_bytes(dtype) <= kShortUnits * 16;
+}
+// How a row is split: short ones not at all, others not from 512 rows on, two
+// blocks to a CU; else so that there are as many blocks, each with a unit to every
+// thread at least.
 Split split_of(int64_t n, int64_t vocab, int32_t dtype, int32_t top) {
   const int64_t least = (top ? kTopThreads : kThreads) * (16 / dtype_bytes(dtype));
   Split s;
   const int64_t wanted = std::min<int64_t>(kWave, 512 / std::max<int64_t>(n, 1));
   s.length = vocab;
-  if (wanted > 1 && vocab > least) {
+  if (wanted > 1 && vocab > least && !is_short(vocab, dtype)) {
     s.length = (vocab + wanted - 1) / wanted;
     s.length = std::max(least, (s.length + 63) / 64 * 64);
   }
@@ -807,15 +1097,37 @@ void launch_rows(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ig
     k_logprobs<T, NT, kTop, false><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
 }
 
+template <typename T, int R>
+void launch_short(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
+                  const Outputs& out, hipStream_t s) {
+  const unsigned blocks = static_cast<unsigned>(
+      std::min<int64_t>(kShortBlocks, (logits.n + kShortWaves - 1) / kShortWaves));
+#define SHORT(TOP, ENTROPY)                                    \
+  k_logprobs_short<T, R, TOP, ENTROPY><<<blocks, kShortThreads, 0, s>>>(logits, targets, ignore, out)
+  if (out.top && out.entropy) SHORT(true, true);
+  else if (out.top) SHORT(true, false);
+  else if (out.entropy) SHORT(false, true);
+  else SHORT(false, false);
+#undef SHORT
+}
+
 template <typename T>
 int logprobs_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
                 const Outputs& out, const Split& split, hipStream_t s) {
-  constexpr int kVec = 16 / sizeof(T);
-  const bool few = logits.width <= kFewUnits * kVec;
-  if (few && out.top)
-    launch_rows<T, kFewThreads, true>(logits, targets, ignore, out, split, s);
-  else if (few)
-    launch_rows<T, kFewThreads, false>(logits, targets, ignore, out, split, s);
+  const int64_t lane_units = (logits.width * static_cast<int64_t>(sizeof(T)) + 1023) / 1024;
+  if (is_short(logits.width, logits.dtype)) {
+    if (lane_units <= 1) launch_short<T, 1>(logits, targets, ignore, out, s);
+    else if (lane_units <= 2) launch_short<T, 2>(logits, targets, ignore, out, s);
+    else if (lane_units <= 4) launch_short<T, 4>(logits, targets, ignore, out, s);
+    else launch_short<T, 8>(logits, targets, ignore, out, s);
+    return launched();
+  }
+  const bool mid = logits.width * static_cast<int64_t>(sizeof(T)) <=
+                   kMidUnits * 16 / (out.top ? 2 : 1);
+  if (out.top && mid)
+    launch_rows<T, kMidThreads, true>(logits, targets, ignore, out, split, s);
+  else if (mid)
+    launch_rows<T, kMidThreads, false>(logits, targets, ignore, out, split, s);
   else if (out.top)
     launch_rows<T, kTopThreads, true>(logits, targets, ignore, out, split, s);
   else
@@ -831,6 +1143,21 @@ template <typename T>
 int grad_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore, const float* lse,
             const float* entropy, const float* grad_logprob, const float* grad_entropy,
             void* dlogits, hipStream_t s) {
+  if (is_short(logits.width, logits.dtype)) {
+    const int64_t lane_units = (logits.width * static_cast<int64_t>(sizeof(T)) + 1023) / 1024;
+    const unsigned short_blocks = static_cast<unsigned>(
+        std::min<int64_t>(kShortBlocks, (logits.n + kShortWaves - 1) / kShortWaves));
+#define SHORT(R)                                                                        \
+  (grad_entropy ? k_logprobs_grad_short<T, R, true> : k_logprobs_grad_short<T, R, false>) \
+      <<<short_blocks, kShortThreads, 0, s>>>(logits, targets, ignore, lse, entropy,      \
+                                              grad_logprob, grad_entropy, static_cast<T*>(dlogits))
+    if (lane_units <= 1) SHORT(1);
+    else if (lane_units <= 2) SHORT(2);
+    else if (lane_units <= 4) SHORT(4);
+    else SHORT(8);
+#undef SHORT
+    return launched();
+  }
   constexpr int64_t kEach = kGradGroup * kGradThreads * (16 / sizeof(T));
   const int64_t per_row = std::max<int64_t>((logits.width + kEach - 1) / kEach, 1);
   if (logits.n * per_row > INT32_MAX) return MS_OPS_EINVAL;

@@ -119,6 +119,34 @@ def test_grad(dtype, n, v):
     check_grad(x, t, entropy=True)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("v", [64, 250, 300, 600, 1030, 2048, 4090, 4096])
+def test_short_rows(v, dtype):
+    """Rows that a wave holds: any contents, orders and starts."""
+    n, low = 24, torch.finfo(ref.DTYPES[dtype]).min
+    wide = _logits(n, v + 3, dtype, 51)
+    x = wide[:, 3:]                               # rows 3 values off, one after the other
+    ramp = torch.linspace(-4, 4, v).to(x.dtype).to(DEV)
+    x[1], x[2], x[3] = ramp, ramp.flip(0), (torch.arange(v, device=DEV) % 3).to(x.dtype)
+    x[4], x[5], x[6] = -INF, low, 0.0
+    x[7, 5:], x[8, 5:], x[9, : v - 5] = -INF, low, -1e4
+    x[10], x[11] = torch.finfo(x.dtype).max / 2, -3000.0
+    x[12, v // 2], x[13, v // 3], x[14] = INF, NAN, NAN
+    x[15] = torch.where(torch.arange(v, device=DEV) // 64 == 2, 5.0 + ramp.float(), -1.0).to(x.dtype)
+    t = _targets(n, v, 52)
+    for top in (0, 1, 20, min(v, 64)):
+        check(x, t, top=top, entropy=top != 20)
+    good = [r for r in range(n) if r not in (12, 13, 14)]
+    check_grad(x[good], t[good])
+    check_grad(wide[:12, 3:], t[:12], entropy=False)
+
+
+def test_more_short_rows_than_waves():
+    x, t = _logits(20_000, 40, "bf16", 53), _targets(20_000, 40, 54)
+    check(x, t, top=3)
+    check_grad(x, t)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_many_rows(dtype):
     x, t = _logits(2100, 1030, dtype, 5), _targets(2100, 1030, 6)
