@@ -594,27 +594,31 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
 }
 
-// Few tokens: every block sorts all of them for its rows of the table, in LDS.
-// A wave takes a row with tokens and a slice of the width at a time; rows of more
-// than kLight tokens are split over the waves, whose sums are added in their
-// order.
-constexpr int kSmallTokens = 1024, kSmallRows = 64;
+// Few tokens: every block sorts all of them for its rows of the table, in LDS, and
+// makes those rows' columns [part * columns, .. + columns).  A wave takes a row with tokens and
+// a slice of the columns at a time; rows of more than kLight tokens are split over
+// the waves, whose sums are added in their order.
+constexpr int kSmallTokens = 1024, kSmallRows = 64, kSmallParts = 8;
+constexpr int64_t kSmallBlocks = 256, kSmallBytes = 262144;
 
 template <typename T, int N, bool kWide, bool kPlain>
 __global__ void __launch_bounds__(kSortThreads)
     k_grad_small(ms_tokens_t ids, ms_rows_t grad, int64_t vocab, int64_t skip, float scale,
-                 int shift, T* __restrict__ table) {
+                 int shift, int column_parts, int columns, T* __restrict__ table) {
   __shared__ int count[kSortWaves][kSmallRows];
   __shared__ int wave_sum[kSortWaves];
   __shared__ int start[kSmallRows + 1];
   __shared__ uint16_t position[kSmallTokens];
   __shared__ float part[kSortWaves][kWave * N];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int64_t width = grad.width;
-  const uint32_t b = blockIdx.x;
+  const uint32_t b = blockIdx.x / column_parts;
+  const int64_t column = static_cast<int64_t>(blockIdx.x - b * column_parts) * columns;
+  // from here on a row is its columns of this block.  (A last vector that ends with them
+  // may begin in the part before, which it then writes as that does.)
+  const int64_t width = grad.width - column < columns ? grad.width - column : columns;
   const int rows = static_cast<int>((vocab - 1 - b) >> shift) + 1;      // b < vocab
   auto table_row = [&](int r) {
-    return table + ((static_cast<int64_t>(r) << shift) + b) * width;
+    return table + ((static_cast<int64_t>(r) << shift) + b) * grad.width + column;
   };
   sort_bucket<kSmallRows, kSmallTokens / kSortThreads, kWide, kPlain>(
       ids, Bucket{b, static_cast<uint32_t>(shift), static_cast<uint32_t>(vocab)}, rows, skip,
@@ -622,7 +626,7 @@ __global__ void __launch_bounds__(kSortThreads)
       [&](int p, int, int t) { position[p] = static_cast<uint16_t>(t); });
   __syncthreads();
 
-  const T* g = static_cast<const T*>(grad.data);
+  const T* g = static_cast<const T*>(grad.data) + column;
   // the sum of the sorted tokens [from, to), 64 positions looked up at a time
   auto add_rows = [&](int from, int to, int64_t c, float (&sum)[N]) {
     Tile<T, N, 1> tile;
@@ -750,10 +754,11 @@ int sum_as(const ms_rows_t& grad, float scale, int64_t from, int64_t until, cons
 constexpr int64_t kMostTokens = 1 << 30;
 
 // One launch where three would mostly wait for each other: up to kSmallTokens
-// tokens and kSmallTable bytes of table.  768 columns, ids that fall off as 1 / rank,
-// and with 33% and 90% of them one id: 1024 tokens 10, 18 and 31 us, 21 to 24 in three
-// launches; 2048 tokens would take 11, 26 and 53.
-constexpr int64_t kSmallTable = 32 << 20;
+// tokens and kSmallTable bytes of table.  50257 x 768 bf16, ids that fall off as 1 / rank,
+// and with 33% and 90% of them one id: 316 tokens 18, 19 and 19 us, 24, 25 and 25 in three
+// launches, 1024 tokens 19, 20 and 32, 29, 29 and 28; 2048 tokens of 12000 rows would
+// take up to 53.  100000 x 1024: 41 and 42 to 68, 40 and 44 in three.
+constexpr int64_t kSmallTable = 96 << 20;
 
 bool is_small(int64_t n, int64_t table_bytes) {
   return n <= kSmallTokens && table_bytes <= kSmallTable;
@@ -762,16 +767,26 @@ bool is_small(int64_t n, int64_t table_bytes) {
 template <typename T, int N>
 int small_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float scale,
              int64_t skip, T* table, hipStream_t s) {
-  // a block for each CU at least, and no more than some 64 KB of the table to one
-  const int64_t row_bytes = grad.width * static_cast<int64_t>(sizeof(T));
-  const int64_t most = std::min<int64_t>(kSmallRows, std::max<int64_t>(65536 / row_bytes, 1));
+  // A block for each CU at least, and no more than some 256 KB of the table to one
+  // (50257 x 768 bf16 18 us, 24 with 64 KB).  Where the table is small, several take the
+  // columns of its rows, or one had all tokens of a frequent id: 316 and 1024 tokens
+  // of 1588 x 1344 bf16, 90% one id, 10.9 and 16.5 us, 19.8 and 46.9 without.
+  const int64_t slices = (grad.width + kWave * N - 1) / (kWave * N);
+  int64_t most_parts = kSmallParts;
+  while (most_parts > 1 && vocab * most_parts > kSmallBlocks * kSmallRows) most_parts /= 2;
+  const int64_t each = (slices + most_parts - 1) / most_parts;
+  const int parts = static_cast<int>((slices + each - 1) / each);
+  const int64_t columns = each * kWave * N;
+  const int64_t bytes = std::min(columns, grad.width) * static_cast<int64_t>(sizeof(T));
+  const int64_t most = std::min<int64_t>(kSmallRows, std::max<int64_t>(kSmallBytes / bytes, 1));
   int shift = 0;
-  while ((shift < 8 && 1 << shift < vocab) || vocab > most << shift) ++shift;
-  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(vocab, 1ll << shift));
+  while (((parts << shift) < 256 && 1 << shift < vocab) || vocab > most << shift) ++shift;
+  const unsigned blocks =
+      static_cast<unsigned>(std::min<int64_t>(vocab, 1ll << shift)) * parts;
   const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
 #define SMALL(W, P)                                                                          \
-  k_grad_small<T, N, W, P><<<blocks, kSortThreads, 0, s>>>(ids, grad, vocab, skip, scale, \
-                                                           shift, table)
+  k_grad_small<T, N, W, P><<<blocks, kSortThreads, 0, s>>>(                                  \
+      ids, grad, vocab, skip, scale, shift, parts, static_cast<int>(columns), table)
   if (wide && plain) SMALL(true, true);
   else if (wide) SMALL(true, false);
   else if (plain) SMALL(false, true);

@@ -102,6 +102,20 @@ def test_grad(dtype, kind, rows, width, n):
     check_grad(_rand((n, width), dtype, 7, 0.1), _ids(n, rows, 8, kind), rows, scale=1.5)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["same", "zipf", "uniform"])
+@pytest.mark.parametrize("width", [257, 513, 1025, 1344, 2050, 4099])
+def test_grad_of_wide_rows(dtype, kind, width):
+    """Rows that several blocks share; the last part of one may be a single column."""
+    for rows, n in ((2, 1000), (77, 300), (700, 1024)):
+        check_grad(_rand((n, width), dtype, 29, 0.1), _ids(n, rows, 30, kind), rows)
+        dirty = torch.full((rows, width), float("nan"), dtype=ref.DTYPES[dtype], device=DEV)
+        del dirty                                 # the allocator hands it out again
+        assert not bool(torch.isnan(ms.ops.embedding_grad(
+            torch.ones(3, width, dtype=ref.DTYPES[dtype], device=DEV),
+            torch.tensor([0, 1, 1], device=DEV), rows)).any())
+
+
 @pytest.mark.parametrize("kind", ["same", "zipf"])
 def test_grad_of_many_tokens(kind):
     check_grad(_rand((70_000, 72), "bf16", 9, 0.1), _ids(70_000, 5000, 10, kind), 5000)
