@@ -322,8 +322,8 @@ __global__ void __launch_bounds__(kThreads)
     unpack_block<false, T>(codes, exponents, n, out);
 }
 
-// Rows that are not one after the other: units within a row (kRows 1), or value
-// by value (2).
+// Rows that are not one after the other: units within a row (kRows 1), or any of
+// which may lie across rows (2).
 template <bool kWhole, typename T, int kRows>
 __device__ __forceinline__ typename Units<T>::Unit fetch_rows(const ms_rows_t& m, int64_t i,
                                                               int64_t n) {
@@ -339,10 +339,14 @@ __device__ __forceinline__ typename Units<T>::Unit fetch_rows(const ms_rows_t& m
       for (int j = 0; j < N; ++j) u.v[j] = static_cast<T>(0.f);
     return u;
   }
+  const int64_t at = kWhole || i < n ? i : 0;
+  int64_t r = at / m.width, c = at - r * m.width;
+  if (c + N <= m.width && (kWhole || i + N <= n))
+    return load_stream_any<N>(x + row_start(m, r) + c);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int64_t at = i + j < n ? i + j : 0, r = at / m.width;
-    u.v[j] = i + j < n ? x[row_start(m, r) + (at - r * m.width)] : static_cast<T>(0.f);
+    u.v[j] = i + j < n ? x[row_start(m, r) + c] : static_cast<T>(0.f);
+    if (++c == m.width && i + j + 1 < n) c = 0, ++r;
   }
   return u;
 }
