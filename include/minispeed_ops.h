@@ -22,7 +22,8 @@
  *     elements; elements of a row are consecutive.  Token lists are the same
  *     with one element per row.  A plain list has inner = its length.
  *     Lists, rows and vocabularies hold fewer than 2^31 entries; offsets are
- *     64-bit.
+ *     64-bit.  A launch has fewer than 2^32 threads: a call that would take
+ *     more (some 2^35 values) is refused with MS_OPS_EINVAL.
  */
 #ifndef MINISPEED_OPS_H
 #define MINISPEED_OPS_H

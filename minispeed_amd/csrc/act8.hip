@@ -149,7 +149,8 @@ __device__ __forceinline__ uint32_t block_max(const Pack<T, 8>& x) {
 // Codes of N values: adding 1.5 * 2^23 rounds x / step to nearest even and
 // leaves it in the low byte; an infinity or NaN (inverse step 0) leaves 0.
 template <int N>
-__device__ __forceinline__ void encode(const float (&x)[N], float inverse, uint32_t (&codes)[N / 4]) {
+__device__ __forceinline__ void encode(const float (&x)[N], float inverse,
+                                       uint32_t (&codes)[N / 4]) {
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) {
     uint32_t k[4];
@@ -276,7 +277,8 @@ __device__ __forceinline__ int64_t unit_at(int k) {
 }
 
 template <bool kWhole, typename T>
-__device__ __forceinline__ void pack_block(const T* x, int64_t n, int8_t* codes, uint8_t* exponents) {
+__device__ __forceinline__ void pack_block(const T* x, int64_t n, int8_t* codes,
+                                           uint8_t* exponents) {
   constexpr int kEach = 2;
   constexpr int N = Units<T>::kVec;
   typename Units<T>::Unit u[kEach];
@@ -300,12 +302,14 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <bool kWhole, typename T>
-__device__ __forceinline__ void unpack_block(const int8_t* codes, const uint8_t* exponents, int64_t n, T* out) {
+__device__ __forceinline__ void unpack_block(const int8_t* codes, const uint8_t* exponents,
+                                             int64_t n, T* out) {
   constexpr int kEach = 1;
   constexpr int N = Units<T>::kVec;
   uint32_t c[kEach][N / 4], e[kEach];
 #pragma unroll
-  for (int k = 0; k < kEach; ++k) fetch<kWhole, T>(codes, exponents, unit_at<T, kEach>(k), n, c[k], e[k]);
+  for (int k = 0; k < kEach; ++k)
+    fetch<kWhole, T>(codes, exponents, unit_at<T, kEach>(k), n, c[k], e[k]);
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
     float v[N];
@@ -352,8 +356,9 @@ __device__ __forceinline__ typename Units<T>::Unit fetch_rows(const ms_rows_t& m
 }
 
 template <bool kWhole, typename T, int K, int kRows>
-__device__ __forceinline__ void act8_block(ms_rows_t h, ms_rows_t up, T* a, int8_t* codes, uint8_t* exponents, int8_t* up_codes,
-         uint8_t* up_exponents) {
+__device__ __forceinline__ void act8_block(ms_rows_t h, ms_rows_t up, T* a, int8_t* codes,
+                                           uint8_t* exponents, int8_t* up_codes,
+                                           uint8_t* up_exponents) {
   constexpr int kEach = kEachOf<K>;
   constexpr int N = Units<T>::kVec;
   constexpr bool kGated = K == MS_ACT_SWIGLU;
@@ -395,8 +400,10 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <bool kWhole, typename T, int K, bool kAgain>
-__device__ __forceinline__ void act8_grad_block(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
-              const uint8_t* up_exponents, const T* grad, int64_t n, T* dh, T* dup, T* a) {
+__device__ __forceinline__ void act8_grad_block(const int8_t* codes, const uint8_t* exponents,
+                                                const int8_t* up_codes,
+                                                const uint8_t* up_exponents, const T* grad,
+                                                int64_t n, T* dh, T* dup, T* a) {
   constexpr int kEach = kEachOf<K>;
   constexpr int N = Units<T>::kVec;
   constexpr bool kGated = K == MS_ACT_SWIGLU;
@@ -438,9 +445,11 @@ __global__ void __launch_bounds__(kThreads)
     k_act8_grad(const int8_t* codes, const uint8_t* exponents, const int8_t* up_codes,
                 const uint8_t* up_exponents, const T* grad, int64_t n, T* dh, T* dup, T* a) {
   if (block_within<T, kEachOf<K>>(n))
-    act8_grad_block<true, T, K, kAgain>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup, a);
+    act8_grad_block<true, T, K, kAgain>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup,
+                                        a);
   else
-    act8_grad_block<false, T, K, kAgain>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup, a);
+    act8_grad_block<false, T, K, kAgain>(codes, exponents, up_codes, up_exponents, grad, n, dh, dup,
+                                         a);
 }
 
 // Blocks for n values; 0: too many.
@@ -448,7 +457,7 @@ template <typename T, int kEach>
 unsigned blocks_for(int64_t n) {
   constexpr int64_t kValues = kThreads * kEach * Units<T>::kVec;
   const int64_t blocks = (n + kValues - 1) / kValues;
-  return blocks > INT32_MAX ? 0 : static_cast<unsigned>(blocks);
+  return fits(blocks, kThreads) ? static_cast<unsigned>(blocks) : 0;
 }
 
 template <typename T, int K>

@@ -83,7 +83,7 @@ int lookup_as(const ms_tokens_t& ids, const ms_rows_t& table, float scale, void*
   const int64_t vectors = (table.width + n - 1) / n, each = kLookupThreads * kLookupEach;
   if (vectors > INT32_MAX) return MS_OPS_EINVAL;
   const int64_t blocks = (ids.n * vectors + each - 1) / each;
-  if (blocks > INT32_MAX) return MS_OPS_EINVAL;
+  if (!fits(blocks, kLookupThreads)) return MS_OPS_EINVAL;
   const bool plain = ids.inner >= ids.n && ids.inner_stride == 1;
 #define LOOKUP(W, P)                                                                        \
   (brief ? k_lookup<T, W, P, true> : k_lookup<T, W, P, false>)                             \
@@ -392,7 +392,8 @@ __device__ __forceinline__ void clear_rows_of(uint64_t empty, int rows, int64_t 
   constexpr int kVec = 16 / sizeof(T);
   if (width < kVec) {
     for (int64_t i = threadIdx.x; i < width * rows; i += blockDim.x)
-      if (empty >> (i / width) & 1) row(static_cast<int>(i / width))[i % width] = static_cast<T>(0.f);
+      if (empty >> (i / width) & 1)
+        row(static_cast<int>(i / width))[i % width] = static_cast<T>(0.f);
     return;
   }
   Pack<T, kVec> zero;
@@ -736,20 +737,6 @@ Clear clear_after(int64_t first, int64_t from, int64_t until, int64_t row_bytes,
   return c;
 }
 
-template <typename T, int N, int G>
-int sum_as(const ms_rows_t& grad, float scale, int64_t from, int64_t until, const GradShape& g,
-           const Sorted& sorted, T* table, hipStream_t s) {
-  const int slices = static_cast<int>((grad.width + kWave * N * G - 1) / (kWave * N * G));
-  int64_t blocks;
-  const Clear clear = clear_after(g.spans * slices, from, until,
-                                  grad.width * static_cast<int64_t>(sizeof(T)), kClearBytes, blocks);
-  if (blocks > INT32_MAX) return MS_OPS_EINVAL;
-  if (blocks == 0) return MS_OPS_OK;
-  k_sum_spans<T, N, G><<<static_cast<unsigned>(blocks), kSumThreads, 0, s>>>(
-      grad, scale, slices, clear, sorted, table);
-  return launched();
-}
-
 // Positions past the end of the list are 32-bit too.
 constexpr int64_t kMostTokens = 1 << 30;
 
@@ -820,6 +807,24 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
   const int64_t clear_bytes = clear_rows * row_bytes;
   const int64_t clear = (clear_bytes / 16 + kSortThreads) / kSortThreads;
   const unsigned blocks = static_cast<unsigned>(buckets + std::min<int64_t>(clear, 1024));
+  // of what is left to clear, the last launch gets half where that is much
+  const bool joins = ids.n > kLight;
+  const int64_t left = vocab - clear_rows;
+  const int64_t until =
+      joins && left * row_bytes > 2 * kClearBesideSort ? clear_rows + left / 2 : vocab;
+  // 512 columns to a wave (256 of a narrow fp32 table), 16 bytes to a lane
+  constexpr int kVec = 16 / sizeof(T), kPair = sizeof(T) == 4 ? 2 : 1;
+  const bool brief = width < kVec, pair = kPair == 2 && width > kVec * kWave;
+  const int64_t columns = kWave * (brief ? 1 : pair ? kVec * kPair : kVec);
+  const int64_t slices = (width + columns - 1) / columns;
+  int64_t sum_blocks, join_blocks;
+  const Clear first =
+      clear_after(g.spans * slices, clear_rows, until, row_bytes, kClearBytes, sum_blocks);
+  const int64_t jobs = g.spans * ((width + kWave - 1) / kWave);
+  const Clear rest = clear_after(std::min<int64_t>(jobs, 512), until, vocab, row_bytes,
+                                 4 * kClearBytes, join_blocks);
+  if (!fits(sum_blocks, kSumThreads) || !fits(join_blocks, kJoinThreads)) return MS_OPS_EINVAL;
+
   const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
 #define SORT(W, P)                                                                     \
   k_sort_tokens<W, P><<<blocks, kSortThreads, 0, s>>>(ids, vocab, skip, buckets, sorted, \
@@ -830,25 +835,14 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
   else SORT(false, false);
 #undef SORT
   if (int rc = launched()) return rc;
-  // of what is left to clear, the last launch gets half where that is much
-  const bool joins = ids.n > kLight;
-  const int64_t left = vocab - clear_rows;
-  const int64_t until =
-      joins && left * row_bytes > 2 * kClearBesideSort ? clear_rows + left / 2 : vocab;
-  // 512 columns to a wave (256 of a narrow fp32 table), 16 bytes to a lane
-  constexpr int kVec = 16 / sizeof(T);
-  const int rc =
-      width < kVec ? sum_as<T, 1, 1>(grad, scale, clear_rows, until, g, sorted, table, s)
-      : sizeof(T) == 4 && width > kVec * kWave
-          ? sum_as<T, kVec, (sizeof(T) == 4 ? 2 : 1)>(grad, scale, clear_rows, until, g, sorted,
-                                                      table, s)
-          : sum_as<T, kVec, 1>(grad, scale, clear_rows, until, g, sorted, table, s);
-  if (rc || !joins) return rc;
-  const int64_t jobs = g.spans * ((width + kWave - 1) / kWave);
-  int64_t join_blocks;
-  const Clear rest = clear_after(std::min<int64_t>(jobs, 512), until, vocab, row_bytes,
-                                 4 * kClearBytes, join_blocks);
-  if (join_blocks > INT32_MAX) return MS_OPS_EINVAL;
+  if (sum_blocks) {
+    (brief  ? k_sum_spans<T, 1, 1>
+     : pair ? k_sum_spans<T, kVec, kPair>
+            : k_sum_spans<T, kVec, 1>)<<<static_cast<unsigned>(sum_blocks), kSumThreads, 0, s>>>(
+        grad, scale, static_cast<int>(slices), first, sorted, table);
+    if (int rc = launched()) return rc;
+  }
+  if (!joins) return MS_OPS_OK;
   (width < 4 ? k_join_spans<T, 1> : k_join_spans<T, 4>)
       <<<static_cast<unsigned>(join_blocks), kJoinThreads, 0, s>>>(ids.n, width, scale, rest,
                                                                    sorted, table);

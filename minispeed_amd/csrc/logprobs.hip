@@ -197,8 +197,9 @@ __device__ __forceinline__ void select_top(Lists<NT, C>& sh, int n, int k, Put p
 // kernel from 126 to 190 us for 8192 x 50257.)  For rows that the fast way gives up: NaN, +inf,
 // logits beyond 2^19, or 69 above all that the first look saw.
 template <int NT, typename T>
-__device__ __forceinline__ void slow_row(float* value, Key* keys, const T* x, int64_t vocab, int64_t r,
-                                      const Outputs& out, int64_t target, int64_t ignore) {
+__device__ __forceinline__ void slow_row(float* value, Key* keys, const T* x, int64_t vocab,
+                                         int64_t r, const Outputs& out, int64_t target,
+                                         int64_t ignore) {
   constexpr int kThreads = NT, kWaves = NT / kWave;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   auto block = [&](float v, auto op) {
@@ -722,8 +723,8 @@ struct ShortRow {
 
 // A wave's values: f(value, index) for each that it has.
 template <typename T, int R, typename F>
-__device__ __forceinline__ void each_value(const ShortRow<T>& row, const Words (&w)[R], float single,
-                                           int lane, F f) {
+__device__ __forceinline__ void each_value(const ShortRow<T>& row, const Words (&w)[R],
+                                           float single, int lane, F f) {
   constexpr int kVec = 16 / sizeof(T);
   if (row.alone >= 0) f(single, row.alone);
 #pragma unroll
@@ -1088,13 +1089,15 @@ Split split_of(int64_t n, int64_t vocab, int32_t dtype, int32_t top) {
 }
 
 template <typename T, int NT, bool kTop>
-void launch_rows(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
-                 const Outputs& out, const Split& split, hipStream_t s) {
+int launch_rows(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
+                const Outputs& out, const Split& split, hipStream_t s) {
+  if (!fits(logits.n * split.parts, NT)) return MS_OPS_EINVAL;
   const unsigned blocks = static_cast<unsigned>(logits.n * split.parts);
   if (out.entropy)
     k_logprobs<T, NT, kTop, true><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
   else
     k_logprobs<T, NT, kTop, false><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
+  return launched();
 }
 
 template <typename T, int R>
@@ -1103,7 +1106,8 @@ void launch_short(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t i
   const unsigned blocks = static_cast<unsigned>(
       std::min<int64_t>(kShortBlocks, (logits.n + kShortWaves - 1) / kShortWaves));
 #define SHORT(TOP, ENTROPY)                                    \
-  k_logprobs_short<T, R, TOP, ENTROPY><<<blocks, kShortThreads, 0, s>>>(logits, targets, ignore, out)
+  k_logprobs_short<T, R, TOP, ENTROPY>                                   \
+      <<<blocks, kShortThreads, 0, s>>>(logits, targets, ignore, out)
   if (out.top && out.entropy) SHORT(true, true);
   else if (out.top) SHORT(true, false);
   else if (out.entropy) SHORT(false, true);
@@ -1124,15 +1128,12 @@ int logprobs_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ign
   }
   const bool mid = logits.width * static_cast<int64_t>(sizeof(T)) <=
                    kMidUnits * 16 / (out.top ? 2 : 1);
-  if (out.top && mid)
-    launch_rows<T, kMidThreads, true>(logits, targets, ignore, out, split, s);
-  else if (mid)
-    launch_rows<T, kMidThreads, false>(logits, targets, ignore, out, split, s);
-  else if (out.top)
-    launch_rows<T, kTopThreads, true>(logits, targets, ignore, out, split, s);
-  else
-    launch_rows<T, kThreads, false>(logits, targets, ignore, out, split, s);
-  if (int rc = launched()) return rc;
+  const int rc =
+      out.top && mid ? launch_rows<T, kMidThreads, true>(logits, targets, ignore, out, split, s)
+      : mid     ? launch_rows<T, kMidThreads, false>(logits, targets, ignore, out, split, s)
+      : out.top ? launch_rows<T, kTopThreads, true>(logits, targets, ignore, out, split, s)
+                : launch_rows<T, kThreads, false>(logits, targets, ignore, out, split, s);
+  if (rc) return rc;
   if (split.parts > 1)
     k_join_parts<T><<<static_cast<unsigned>(logits.n), kThreads, 0, s>>>(logits, targets, ignore,
                                                                          out, split);
@@ -1160,7 +1161,7 @@ int grad_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
   }
   constexpr int64_t kEach = kGradGroup * kGradThreads * (16 / sizeof(T));
   const int64_t per_row = std::max<int64_t>((logits.width + kEach - 1) / kEach, 1);
-  if (logits.n * per_row > INT32_MAX) return MS_OPS_EINVAL;
+  if (!fits(logits.n * per_row, kGradThreads)) return MS_OPS_EINVAL;
   const unsigned blocks = static_cast<unsigned>(logits.n * per_row);
   if (grad_entropy)
     k_logprobs_grad<T, true><<<blocks, kGradThreads, 0, s>>>(

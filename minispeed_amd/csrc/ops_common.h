@@ -55,8 +55,12 @@ __device__ __forceinline__ int64_t row_start(const ms_rows_t& m, int64_t r) {
 template <int B> struct raw_of;
 template <> struct raw_of<2> { typedef uint16_t type; };
 template <> struct raw_of<4> { typedef uint32_t type __attribute__((aligned(2))); };
-template <> struct raw_of<8> { typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2))); };
-template <> struct raw_of<16> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct raw_of<8> {
+  typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2)));
+};
+template <> struct raw_of<16> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+};
 
 template <typename T, int N>
 struct Pack {
@@ -126,9 +130,12 @@ inline bool good_tokens(const ms_tokens_t* t) {
   return t && t->n >= 0 && t->n <= INT32_MAX && t->inner >= 1 && (t->n == 0 || t->data);
 }
 inline bool good_rows(const ms_rows_t* m) {
-  return m && m->n >= 0 && m->n <= INT32_MAX && m->width >= 0 && m->inner >= 1 && good_dtype(m->dtype) &&
-         (m->n == 0 || m->width == 0 || m->data);
+  return m && m->n >= 0 && m->n <= INT32_MAX && m->width >= 0 && m->inner >= 1 &&
+         good_dtype(m->dtype) && (m->n == 0 || m->width == 0 || m->data);
 }
+
+// A launch has fewer than 2^32 threads.
+inline bool fits(int64_t blocks, int threads) { return blocks <= UINT32_MAX / threads; }
 
 // The launch's own status; errors that earlier work left are not reported here
 // as ours.

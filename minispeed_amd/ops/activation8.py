@@ -221,8 +221,8 @@ def checkpoint8(fn, *args, preserve_rng_state: bool = True):
     arguments held in 8 bits.
 
     The float32, float16 and bfloat16 tensors on the GPU among ``args`` are kept in
-    their 8-bit form (other tensors as they are), and ``fn`` runs again on the values they stand for when
-    the gradients come: the use of minispeed's ``checkpoint``
+    their 8-bit form (other tensors as they are), and ``fn`` runs again on the values
+    they stand for when the gradients come: the use of minispeed's ``checkpoint``
     (minispeed/activation_checkpointing.py:17-20) with a quarter to a half of its
     memory.  The first run sees the arguments themselves.  Parameters that ``fn``
     reaches by itself get their gradients; with ``preserve_rng_state`` random

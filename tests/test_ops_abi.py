@@ -148,3 +148,20 @@ def test_a_missing_build_is_reported(monkeypatch):
     monkeypatch.setattr(_native.importlib, "import_module", missing)
     with pytest.raises(NativeLibraryError, match="minispeed_amd.build"):
         _native.load()
+
+
+def test_calls_beyond_one_launch_are_refused(lib):
+    ref, n = ctypes.byref, 2 ** 36
+    assert lib.ms_pack8(P(16), I32(1), I64(n * 2), P(16), P(16), None) == -1
+    assert lib.ms_unpack8(P(16), P(16), I64(n), I32(1), P(16), None) == -1
+    ids = Tokens(16, 2 ** 30, 2 ** 30, 0, 1, 1, 0)
+    table, logits = Rows(16, 10, 4096, 10, 0, 4096, 1, 0), Rows(16, 2 ** 30, 40000, 2 ** 30, 0,
+                                                                40000, 1, 0)
+    assert lib.ms_embedding(ref(ids), ref(table), F(1), P(16), None) == -1
+    assert lib.ms_logprobs(ref(logits), ref(ids), I64(-100), I32(0), P(16), None, P(16), None,
+                           None, None, I64(0), None) == -1
+    assert lib.ms_logprobs_grad(ref(logits), ref(ids), I64(-100), P(16), None, P(16), None, P(16),
+                                None) == -1
+    rows = Rows(16, 2 ** 30, 4096, 2 ** 30, 0, 4096, 1, 0)
+    assert lib.ms_embedding_grad(ref(ids), ref(rows), I64(10), F(1), I64(-1), P(16), P(16),
+                                 I64(2 ** 62), None) == -1
