@@ -118,7 +118,6 @@ int lookup_as(const ms_tokens_t& ids, const ms_rows_t& table, float scale, void*
 //   k_join_spans   adds up the partial sums.
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kSortRows = 1024;
-constexpr int kSortSteps = 16;            // groups of 64 tokens in flight per wave
 
 struct Sorted {
   int32_t* start;       // [buckets * rows + 1]: where each id's tokens begin, by slot
@@ -283,7 +282,9 @@ __device__ __forceinline__ void sort_bucket(const ms_tokens_t& ids, const Bucket
   }
 }
 
-template <bool kWide, bool kPlain>
+// kSteps: groups of 64 tokens in flight per wave.  No more than there are, as all are gone
+// through: 4096 tokens (three launches) 23 us with 4 or 8, 27 with 16.
+template <int kSteps, bool kWide, bool kPlain>
 __global__ void __launch_bounds__(kSortThreads)
     k_sort_tokens(ms_tokens_t ids, int64_t vocab, int64_t skip, int buckets, Sorted out,
                   uint4* table, int64_t clear_bytes) {
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(kSortThreads)
   const uint32_t b = blockIdx.x;
   const Bucket bucket = {b, static_cast<uint32_t>(out.shift), static_cast<uint32_t>(vocab)};
   const int64_t slot = static_cast<int64_t>(b) * out.rows;
-  sort_bucket<kSortRows, kSortSteps, kWide, kPlain>(
+  sort_bucket<kSortRows, kSteps, kWide, kPlain>(
       ids, bucket, out.rows, skip, count, wave_sum,
       [&](int r, int p) {
         if (r < out.rows || b == static_cast<uint32_t>(buckets) - 1) out.start[slot + r] = p;
@@ -723,7 +724,7 @@ GradShape shape_of(int64_t n, int64_t vocab, int64_t width) {
 }
 
 // What the sort's launch clears while it sorts, which takes it some 12 us.
-constexpr int64_t kClearBesideSort = 48 << 20;
+constexpr int64_t kClearBesideSort = 40 << 20;
 
 // Blocks that clear rows [from, until) behind `first` others; blocks: of the launch.
 Clear clear_after(int64_t first, int64_t from, int64_t until, int64_t row_bytes, int64_t bytes,
@@ -741,10 +742,10 @@ Clear clear_after(int64_t first, int64_t from, int64_t until, int64_t row_bytes,
 constexpr int64_t kMostTokens = 1 << 30;
 
 // One launch where three would mostly wait for each other: up to kSmallTokens
-// tokens and kSmallTable bytes of table.  50257 x 768 bf16, ids that fall off as 1 / rank,
-// and with 33% and 90% of them one id: 316 tokens 18, 19 and 19 us, 24, 25 and 25 in three
-// launches, 1024 tokens 19, 20 and 32, 29, 29 and 28; 2048 tokens of 12000 rows would
-// take up to 53.  100000 x 1024: 41 and 42 to 68, 40 and 44 in three.
+// tokens and kSmallTable bytes of table.  Ids that fall off as 1 / rank, and with 33% and
+// 90% of them one id, bf16, in three launches in brackets: 12000 x 768, 316 tokens 9, 11
+// and 15 us (16), 1024 tokens 11, 16 and 29 (17); 50257 x 768, 19, 20 and 19 (20 to 22), 20,
+// 20 and 33 (22); 100000 x 1024, 41, 43 and 49 (37), 43, 52 and 68 (37).
 constexpr int64_t kSmallTable = 96 << 20;
 
 bool is_small(int64_t n, int64_t table_bytes) {
@@ -821,14 +822,17 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
   const Clear first =
       clear_after(g.spans * slices, clear_rows, until, row_bytes, kClearBytes, sum_blocks);
   const int64_t jobs = g.spans * ((width + kWave - 1) / kWave);
-  const Clear rest = clear_after(std::min<int64_t>(jobs, 512), until, vocab, row_bytes,
+  // (a block to a CU: 16384 tokens of 50257 x 768 bf16 35.1 us, 37.2 with two)
+  const Clear rest = clear_after(std::min<int64_t>(jobs, 256), until, vocab, row_bytes,
                                  4 * kClearBytes, join_blocks);
   if (!fits(sum_blocks, kSumThreads) || !fits(join_blocks, kJoinThreads)) return MS_OPS_EINVAL;
 
   const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
-#define SORT(W, P)                                                                     \
-  k_sort_tokens<W, P><<<blocks, kSortThreads, 0, s>>>(ids, vocab, skip, buckets, sorted, \
-                                                      static_cast<uint4*>(dtable), clear_bytes)
+#define SORT(W, P)                                                                       \
+  (ids.n <= 4 * kSortThreads   ? k_sort_tokens<4, W, P>                                  \
+   : ids.n <= 8 * kSortThreads ? k_sort_tokens<8, W, P>                                  \
+                               : k_sort_tokens<16, W, P>)<<<blocks, kSortThreads, 0, s>>>( \
+      ids, vocab, skip, buckets, sorted, static_cast<uint4*>(dtable), clear_bytes)
   if (wide && plain) SORT(true, true);
   else if (wide) SORT(true, false);
   else if (plain) SORT(false, true);
