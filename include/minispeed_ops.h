@@ -127,7 +127,8 @@ int ms_logprobs(const ms_rows_t* logits, const ms_tokens_t* targets, int64_t ign
  *   dlogits[j] = g (1[j = target] - p_j) - h p_j (log p_j + entropy)
  * with g = grad_logprob of the row (0 where target == ignore_index, and where
  * NULL) and h = grad_entropy (NULL: 0; then `entropy` is not read).  lse and entropy are
- * those that ms_logprobs gave.  Rows of -inf get zeros; a target outside
+ * those that ms_logprobs gave.  Rows of -inf get zeros, a NaN logit NaN
+ * whatever lse is; a target outside
  * [0, vocab) that is not ignore_index makes g NaN.
  */
 int ms_logprobs_grad(const ms_rows_t* logits, const ms_tokens_t* targets, int64_t ignore_index,

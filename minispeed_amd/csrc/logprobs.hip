@@ -969,9 +969,10 @@ __global__ void __launch_bounds__(kGradThreads)
     const int begin = part ? head + part * kEach * kVec : 0;
     const int end = part == blocks_per_row - 1 ? vocab : head + (part + 1) * kEach * kVec;
     for (int j = begin + tid; j < end; j += kGradThreads) {
-      float dj = 0.f;
+      const float v = widen(x[j]);
+      float dj = v != v ? v : 0.f;                     // a NaN says so whatever lse is
       if (l != -INFINITY) {
-        const float logp = (widen(x[j]) - most) - ls, p = exp2_fast(logp * kLog2e);
+        const float logp = (v - most) - ls, p = exp2_fast(logp * kLog2e);
         dj = j == hit ? g - g * p : -g * p;
         if (kEntropy && p != 0.f) dj -= h * p * (logp + big_h);
       }
@@ -1047,7 +1048,7 @@ __global__ void __launch_bounds__(kShortThreads)
     };
     if (l == -INFINITY) {
       g = 0.f;
-      write([](float) { return 0.f; });
+      write([](float v) { return v != v ? v : 0.f; });
     } else if (fabsf(l) > kFarLse) {
       float most = single, s = 0.f;
       each_value(row, w, single, lane, [&](float v, int) { most = fmaxf(most, v); });

@@ -245,6 +245,20 @@ def test_nan_and_infinity():
     assert bool(torch.isnan(d[:5]).all()) and bool(torch.isfinite(d[5]).all())
 
 
+@pytest.mark.parametrize("v", [65, 4096, 50257])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_gradient_of_nan_logits_beside_an_empty_lse(dtype, v):
+    """A row whose lse says that nothing is left, and a NaN that has come into it since."""
+    x = torch.full((3, v), -INF, dtype=ref.DTYPES[dtype], device=DEV)
+    x[0, v // 2], x[1] = NAN, NAN
+    lse, one = torch.full((3,), -INF, device=DEV), torch.ones(3, device=DEV)
+    t = torch.zeros(3, dtype=torch.int64, device=DEV)
+    for h in (None, one):
+        d = ms.ops.token_logprobs_grad(x, t, lse, one, one, h)
+        assert torch.equal(torch.isnan(d), torch.isnan(x))
+        assert not bool(d.nan_to_num(0.0).any())
+
+
 def test_targets_outside_the_vocabulary():
     x = _logits(5, 100, "bf16", 13)
     t = torch.tensor([100, -1, 7, 2 ** 40, -100], device=DEV)
