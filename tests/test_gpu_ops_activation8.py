@@ -139,6 +139,28 @@ def test_activation_over_its_range(kind, dtype):
     check_act(x, kind, torch.ones_like(x) if kind == "swiglu" else None)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_activation_in_32_bits_is_as_exact_as_its_operations(kind):
+    """fp32: in units of 2^-24 of the terms, the exponential and the reciprocal are off by 2
+    each, the exponential's argument (reduced to less than 1) and 1 + e by 1 each, the
+    polynomial and what it is of by 4, and some 5 products and sums by 1 each: 16 at
+    most, wherever the argument lies.  (gelu_tanh's argument is a product of its own, two
+    roundings, which its exponential multiplies by its magnitude.)"""
+    x = torch.cat([torch.linspace(-12.5, 12.5, 6001), torch.linspace(-0.05, 0.05, 800)]
+                  + ([torch.linspace(-80, 80, 3001)] if kind in ("silu", "swiglu") else []))
+    x = F.pad(x[:, None], (0, 31)).to(DEV)
+    up = torch.ones_like(x) if kind == "swiglu" else None
+    a, saved = ms.ops.activation8(x, kind, up=up)
+    grads, again = ms.ops.activation8_grad(saved, torch.ones_like(x), kind)
+    at = ref.held(x)[2].view(x.shape)
+    for z, got_f, got_df in ((x.cpu().double(), a, None), (at, again, grads[0])):
+        f, df, scale, size = ref.act(z, kind)
+        unit = 2.0 ** -24 * (16 + (2 * scale if kind == "gelu_tanh" else 0))
+        ref.close(got_f, f, unit * f.abs() + 2.0 ** -149, f"{kind} f")
+        if got_df is not None:
+            ref.close(got_df, df, unit * size + 2.0 ** -149, f"{kind} f'")
+
+
 def test_activation_of_views():
     both = _rand((24, 2 * 96), "bf16", 6)
     gate, up = both.chunk(2, -1)
