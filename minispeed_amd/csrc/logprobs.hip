@@ -965,9 +965,11 @@ __global__ void __launch_bounds__(kGradThreads)
       s = block(wave_sum(s), [](float a, float b) { return a + b; });
     }
     const float ls = log2_fast(s) * kLn2;
-    // the first block takes the head too, the last one what is behind the units
+    // the first block takes the head too, the last one what is behind the units; with
+    // the head before them the last block but one may already reach the row's end
     const int begin = part ? head + part * kEach * kVec : 0;
-    const int end = part == blocks_per_row - 1 ? vocab : head + (part + 1) * kEach * kVec;
+    const int behind = head + (part + 1) * kEach * kVec;
+    const int end = part == blocks_per_row - 1 || behind > vocab ? vocab : behind;
     for (int j = begin + tid; j < end; j += kGradThreads) {
       const float v = widen(x[j]);
       float dj = v != v ? v : 0.f;                     // a NaN says so whatever lse is

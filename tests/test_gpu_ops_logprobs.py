@@ -12,13 +12,16 @@ log s - t / s, each off by rel of its magnitudes.
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import minispeed_amd as ms
+from minispeed_amd import build
 from tests import ops_reference as ref
+from tests.test_ops_abi import Rows, Tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -257,6 +260,48 @@ def test_gradient_of_nan_logits_beside_an_empty_lse(dtype, v):
         d = ms.ops.token_logprobs_grad(x, t, lse, one, one, h)
         assert torch.equal(torch.isnan(d), torch.isnan(x))
         assert not bool(d.nan_to_num(0.0).any())
+
+
+# a few values more than a whole number of blocks of the gradient (2048 values of 2 bytes,
+# 1024 of 4), in rows that begin anywhere within 16 bytes
+@pytest.mark.parametrize("dtype,v", [("fp32", 2049), ("fp32", 4097), ("fp32", 4098), ("fp16", 4097),
+                                     ("bf16", 4102), ("bf16", 8193), ("fp16", 32769)])
+def test_gradient_of_odd_rows_between_others(dtype, v):
+    """Rows with nothing left and rows far from 0 before ordinary ones and at the end."""
+    x, t = _logits(17, v, dtype, 61), _targets(17, v, 62)
+    x[1::4] = -INF
+    x[3::4] = (x[3::4].float() - 3000.0).to(x.dtype)
+    x[16] = -INF
+    check_grad(x, t)
+    check_grad(x, t, entropy=False)
+    x[16] = (_logits(1, v, dtype, 63)[0].float() + 900.0).to(x.dtype)
+    check_grad(x, t)
+
+
+@pytest.mark.parametrize("dtype,v", [("fp32", 2049), ("bf16", 4097), ("fp16", 8193)])
+@pytest.mark.parametrize("fill", [-INF, -3000.0])
+def test_gradient_stays_within_its_rows(dtype, v, fill):
+    """What lies before and behind the gradient is not written, and what lies before and
+    behind the logits is not used."""
+    n, edge = 9, 64
+    whole = torch.full((n * v + 2 * edge,), NAN, dtype=ref.DTYPES[dtype], device=DEV)
+    x = whole[edge:-edge].view(n, v).fill_(fill)
+    out = torch.full_like(whole, 7.0)
+    t = torch.zeros(n, dtype=torch.int64, device=DEV)
+    lse, g = torch.logsumexp(x.float(), 1), torch.ones(n, device=DEV)
+    lib = ctypes.CDLL(build.OPS_OUTPUT)
+    rows = Rows(x.data_ptr(), n, v, n, 0, v, ["fp32", "fp16", "bf16"].index(dtype), 0)
+    ids = Tokens(t.data_ptr(), n, n, 0, 1, 1, 0)
+    ptr = ctypes.c_void_p
+    assert lib.ms_logprobs_grad(ctypes.byref(rows), ctypes.byref(ids), ctypes.c_int64(-100),
+                                ptr(lse.data_ptr()), None, ptr(g.data_ptr()), None,
+                                ptr(out[edge:].data_ptr()),
+                                ptr(torch.cuda.current_stream().cuda_stream)) == 0
+    assert bool((out[:edge] == 7.0).all()) and bool((out[-edge:] == 7.0).all())
+    d = out[edge:-edge].view(n, v).float()
+    p = 0.0 if fill == -INF else 1.0 / v
+    assert torch.allclose(d[:, 1:], torch.full_like(d[:, 1:], -p), rtol=0.01, atol=0.0)
+    assert torch.allclose(d[:, 0], torch.full_like(d[:, 0], 1.0 - p if p else 0.0), rtol=0.01)
 
 
 def test_targets_outside_the_vocabulary():
