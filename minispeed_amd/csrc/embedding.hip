@@ -597,16 +597,16 @@ __global__ void __launch_bounds__(kJoinThreads)
 }
 
 // Few tokens: every block sorts all of them for its rows of the table, in LDS, and
-// makes those rows' columns [part * columns, .. + columns).  A wave takes a row with tokens and
-// a slice of the columns at a time; rows of more than kLight tokens are split over
-// the waves, whose sums are added in their order.
+// makes those rows' columns from part * columns on, the last part all that are left.  A wave
+// takes a row with tokens and a slice of the columns at a time; the tokens of rows with more
+// than kLight are cut into `pieces`, as many in every block, whose sums are added in their order.
 constexpr int kSmallTokens = 1024, kSmallRows = 64, kSmallParts = 8;
 constexpr int64_t kSmallBlocks = 256, kSmallBytes = 262144;
 
 template <typename T, int N, bool kWide, bool kPlain>
 __global__ void __launch_bounds__(kSortThreads)
     k_grad_small(ms_tokens_t ids, ms_rows_t grad, int64_t vocab, int64_t skip, float scale,
-                 int shift, int column_parts, int columns, T* __restrict__ table) {
+                 int shift, int column_parts, int columns, int pieces, T* __restrict__ table) {
   __shared__ int count[kSortWaves][kSmallRows];
   __shared__ int wave_sum[kSortWaves];
   __shared__ int start[kSmallRows + 1];
@@ -614,10 +614,10 @@ __global__ void __launch_bounds__(kSortThreads)
   __shared__ float part[kSortWaves][kWave * N];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const uint32_t b = blockIdx.x / column_parts;
-  const int64_t column = static_cast<int64_t>(blockIdx.x - b * column_parts) * columns;
-  // from here on a row is its columns of this block.  (A last vector that ends with them
-  // may begin in the part before, which it then writes as that does.)
-  const int64_t width = grad.width - column < columns ? grad.width - column : columns;
+  const int column_part = static_cast<int>(blockIdx.x - b * column_parts);
+  const int64_t column = static_cast<int64_t>(column_part) * columns;
+  // from here on a row is its columns of this block, N or more
+  const int64_t width = column_part == column_parts - 1 ? grad.width - column : columns;
   const int rows = static_cast<int>((vocab - 1 - b) >> shift) + 1;      // b < vocab
   auto table_row = [&](int r) {
     return table + ((static_cast<int64_t>(r) << shift) + b) * grad.width + column;
@@ -665,17 +665,17 @@ __global__ void __launch_bounds__(kSortThreads)
     }
   }
   // the waves share a row's slices and, where these are few, its tokens
-  const int parts = slices < kSortWaves ? kSortWaves / slices : 1, jobs = slices * parts;
+  const int jobs = slices * pieces;                  // no more than `part` has, unless pieces is 1
   for (uint64_t left = heavy; left; left &= left - 1) {
     const int r = __ffsll(static_cast<unsigned long long>(left)) - 1;
     const int from = uniform(start[r]), end = uniform(start[r + 1]);
-    const int each = (end - from + parts - 1) / parts;
+    const int each = (end - from + pieces - 1) / pieces;
     for (int j = wave; j < jobs; j += kSortWaves) {
-      const int slice = j / parts, first = from + (j - slice * parts) * each;
+      const int slice = j / pieces, first = from + (j - slice * pieces) * each;
       const int64_t c = (static_cast<int64_t>(slice) * kWave + lane) * N;
       float sum[N];
       add_rows(first, first + each < end ? first + each : end, c, sum);
-      if (parts == 1) {
+      if (pieces == 1) {
         Pack<T, N> y;
 #pragma unroll
         for (int k = 0; k < N; ++k) y.v[k] = narrow<T>(sum[k] * scale);
@@ -685,14 +685,14 @@ __global__ void __launch_bounds__(kSortThreads)
         for (int k = 0; k < N; ++k) part[j][lane * N + k] = sum[k];
       }
     }
-    if (parts == 1) continue;
+    if (pieces == 1) continue;
     __syncthreads();
     for (int k = threadIdx.x; k < slices * kWave * N; k += kSortThreads) {
       const int slice = k / (kWave * N), at = k % (kWave * N);
       const int64_t c = k / N * N;                   // of the lane; its vector may be earlier
       if (c >= width) continue;
-      float y = part[slice * parts][at];
-      for (int p = 1; p < parts; ++p) y += part[slice * parts + p][at];
+      float y = part[slice * pieces][at];
+      for (int p = 1; p < pieces; ++p) y += part[slice * pieces + p][at];
       table_row(r)[vector_at<N>(c, width) + k % N] = narrow<T>(y * scale);
     }
     __syncthreads();
@@ -763,9 +763,15 @@ int small_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float
   int64_t most_parts = kSmallParts;
   while (most_parts > 1 && vocab * most_parts > kSmallBlocks * kSmallRows) most_parts /= 2;
   const int64_t each = (slices + most_parts - 1) / most_parts;
-  const int parts = static_cast<int>((slices + each - 1) / each);
   const int64_t columns = each * kWave * N;
-  const int64_t bytes = std::min(columns, grad.width) * static_cast<int64_t>(sizeof(T));
+  int parts = static_cast<int>((slices + each - 1) / each);
+  // no part of less than a vector: that would begin in the one before
+  if (parts > 1 && grad.width - (parts - 1) * columns < N) --parts;
+  const int64_t widest = std::max(std::min(columns, grad.width), grad.width - (parts - 1) * columns);
+  const int most_slices = static_cast<int>(
+      std::min<int64_t>((widest + kWave * N - 1) / (kWave * N), kSortWaves));
+  const int pieces = kSortWaves / most_slices;
+  const int64_t bytes = widest * static_cast<int64_t>(sizeof(T));
   const int64_t most = std::min<int64_t>(kSmallRows, std::max<int64_t>(kSmallBytes / bytes, 1));
   int shift = 0;
   while (((parts << shift) < 256 && 1 << shift < vocab) || vocab > most << shift) ++shift;
@@ -774,7 +780,7 @@ int small_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float
   const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
 #define SMALL(W, P)                                                                          \
   k_grad_small<T, N, W, P><<<blocks, kSortThreads, 0, s>>>(                                  \
-      ids, grad, vocab, skip, scale, shift, parts, static_cast<int>(columns), table)
+      ids, grad, vocab, skip, scale, shift, parts, static_cast<int>(columns), pieces, table)
   if (wide && plain) SMALL(true, true);
   else if (wide) SMALL(true, false);
   else if (plain) SMALL(false, true);

@@ -116,6 +116,21 @@ def test_grad_of_wide_rows(dtype, kind, width):
             torch.tensor([0, 1, 1], device=DEV), rows)).any())
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("width", [4, 5, 255, 257, 259, 260, 513, 514, 515, 516, 1025, 1027, 1344, 2049,
+                                   2050, 2051, 2052, 2305, 4099, 8193])
+def test_grad_adds_every_column_in_the_same_order(dtype, width):
+    """Few tokens, whose columns several blocks may share: gradients that are alike in
+    all columns have sums that are, bit for bit, on every call."""
+    for rows, n, kind in ((2, 1000, "same"), (700, 1024, "same"), (1500, 777, "zipf"),
+                          (3000, 1000, "same"), (8000, 333, "same")):
+        ids = _ids(n, rows, 31, kind)
+        g = _rand((n, 1), dtype, 32).expand(n, width).contiguous()
+        first = ms.ops.embedding_grad(g, ids, rows)
+        assert torch.equal(first, first[:, :1].expand(rows, width))
+        assert torch.equal(ms.ops.embedding_grad(g, ids, rows), first)
+
+
 @pytest.mark.parametrize("kind", ["same", "zipf"])
 def test_grad_of_many_tokens(kind):
     check_grad(_rand((70_000, 72), "bf16", 9, 0.1), _ids(70_000, 5000, 10, kind), 5000)
