@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -10,6 +11,18 @@ if ROOT not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a ROCm GPU and the built HIP library")
+
+
+def pytest_collection_finish(session):
+    # what the imports made stays: the collections between the tests then look at little
+    gc.collect()
+    gc.freeze()
+
+
+def pytest_runtest_setup(item):
+    """What an earlier test left in reference cycles goes now, not somewhere inside the
+    next test: several compare the device allocator's counts."""
+    gc.collect()
 
 
 @pytest.fixture(autouse=True)
