@@ -498,16 +498,10 @@ int act8_kind(const ms_rows_t& h, const ms_rows_t& up, void* a, int8_t* codes, u
     return m.n <= 1 || (m.inner >= m.n && m.inner_stride == m.width);
   };
   const bool gated = K == MS_ACT_SWIGLU;
-  if (dense(h) && (!gated || dense(up)))
-    k_act8<T, K, 0><<<blocks, kThreads, 0, s>>>(h, up, out, codes, exponents, up_codes,
-                                                up_exponents);
-  else if (h.width % Units<T>::kVec == 0)
-    k_act8<T, K, 1><<<blocks, kThreads, 0, s>>>(h, up, out, codes, exponents, up_codes,
-                                                up_exponents);
-  else
-    k_act8<T, K, 2><<<blocks, kThreads, 0, s>>>(h, up, out, codes, exponents, up_codes,
-                                                up_exponents);
-  return launched();
+  return launch(dense(h) && (!gated || dense(up))  ? k_act8<T, K, 0>
+                : h.width % Units<T>::kVec == 0 ? k_act8<T, K, 1>
+                                                : k_act8<T, K, 2>,
+                blocks, kThreads, s, h, up, out, codes, exponents, up_codes, up_exponents);
 }
 
 template <typename T>
@@ -533,13 +527,8 @@ int grad_kind(const int8_t* codes, const uint8_t* exponents, const int8_t* up_co
   if (!blocks) return MS_OPS_EINVAL;
   const T* g = static_cast<const T*>(grad);
   T *d = static_cast<T*>(dh), *du = static_cast<T*>(dup), *out = static_cast<T*>(a);
-  if (out)
-    k_act8_grad<T, K, true><<<blocks, kThreads, 0, s>>>(codes, exponents, up_codes, up_exponents,
-                                                        g, n, d, du, out);
-  else
-    k_act8_grad<T, K, false><<<blocks, kThreads, 0, s>>>(codes, exponents, up_codes, up_exponents,
-                                                         g, n, d, du, out);
-  return launched();
+  return launch(out ? k_act8_grad<T, K, true> : k_act8_grad<T, K, false>, blocks, kThreads, s, codes,
+                exponents, up_codes, up_exponents, g, n, d, du, out);
 }
 
 template <typename T>
@@ -568,16 +557,14 @@ template <typename T>
 int pack_as(const void* x, int64_t n, int8_t* codes, uint8_t* exponents, hipStream_t s) {
   const unsigned blocks = blocks_for<T, 2>(n);
   if (!blocks) return MS_OPS_EINVAL;
-  k_pack<T><<<blocks, kThreads, 0, s>>>(static_cast<const T*>(x), n, codes, exponents);
-  return launched();
+  return launch(k_pack<T>, blocks, kThreads, s, static_cast<const T*>(x), n, codes, exponents);
 }
 template <typename T>
 int unpack_as(const int8_t* codes, const uint8_t* exponents, int64_t n, void* out,
               hipStream_t s) {
   const unsigned blocks = blocks_for<T, 1>(n);
   if (!blocks) return MS_OPS_EINVAL;
-  k_unpack<T><<<blocks, kThreads, 0, s>>>(codes, exponents, n, static_cast<T*>(out));
-  return launched();
+  return launch(k_unpack<T>, blocks, kThreads, s, codes, exponents, n, static_cast<T*>(out));
 }
 
 }  // namespace

@@ -85,16 +85,13 @@ int lookup_as(const ms_tokens_t& ids, const ms_rows_t& table, float scale, void*
   const int64_t blocks = (ids.n * vectors + each - 1) / each;
   if (!fits(blocks, kLookupThreads)) return MS_OPS_EINVAL;
   const bool plain = ids.inner >= ids.n && ids.inner_stride == 1;
-#define LOOKUP(W, P)                                                                        \
-  (brief ? k_lookup<T, W, P, true> : k_lookup<T, W, P, false>)                             \
-      <<<static_cast<unsigned>(blocks), kLookupThreads, 0, s>>>(                            \
-          ids, table, scale, static_cast<uint32_t>(vectors), static_cast<T*>(out))
-  if (ids.wide && plain) LOOKUP(true, true);
-  else if (ids.wide) LOOKUP(true, false);
-  else if (plain) LOOKUP(false, true);
-  else LOOKUP(false, false);
+#define LOOKUP(W, P) (brief ? k_lookup<T, W, P, true> : k_lookup<T, W, P, false>)
+  return launch(ids.wide ? plain ? LOOKUP(true, true) : LOOKUP(true, false)
+                : plain  ? LOOKUP(false, true)
+                         : LOOKUP(false, false),
+                blocks, kLookupThreads, s, ids, table, scale, static_cast<uint32_t>(vectors),
+                static_cast<T*>(out));
 #undef LOOKUP
-  return launched();
 }
 
 // The gradient's table.  Tokens are sorted by (id, t) on the device, then each
@@ -775,18 +772,13 @@ int small_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float
   const int64_t most = std::min<int64_t>(kSmallRows, std::max<int64_t>(kSmallBytes / bytes, 1));
   int shift = 0;
   while (((parts << shift) < 256 && 1 << shift < vocab) || vocab > most << shift) ++shift;
-  const unsigned blocks =
-      static_cast<unsigned>(std::min<int64_t>(vocab, 1ll << shift)) * parts;
-  const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
-#define SMALL(W, P)                                                                          \
-  k_grad_small<T, N, W, P><<<blocks, kSortThreads, 0, s>>>(                                  \
-      ids, grad, vocab, skip, scale, shift, parts, static_cast<int>(columns), pieces, table)
-  if (wide && plain) SMALL(true, true);
-  else if (wide) SMALL(true, false);
-  else if (plain) SMALL(false, true);
-  else SMALL(false, false);
-#undef SMALL
-  return launched();
+  const int64_t blocks = std::min<int64_t>(vocab, 1ll << shift) * parts;
+  const bool plain = ids.inner >= ids.n && ids.inner_stride == 1;
+  return launch(ids.wide ? plain ? k_grad_small<T, N, true, true> : k_grad_small<T, N, true, false>
+                : plain  ? k_grad_small<T, N, false, true>
+                         : k_grad_small<T, N, false, false>,
+                blocks, kSortThreads, s, ids, grad, vocab, skip, scale, shift, parts,
+                static_cast<int>(columns), pieces, table);
 }
 
 template <typename T>
@@ -813,7 +805,7 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
   const int64_t clear_rows = std::min<int64_t>(vocab, kClearBesideSort / row_bytes);
   const int64_t clear_bytes = clear_rows * row_bytes;
   const int64_t clear = (clear_bytes / 16 + kSortThreads) / kSortThreads;
-  const unsigned blocks = static_cast<unsigned>(buckets + std::min<int64_t>(clear, 1024));
+  const int64_t blocks = buckets + std::min<int64_t>(clear, 1024);
   // of what is left to clear, the last launch gets half where that is much
   const bool joins = ids.n > kLight;
   const int64_t left = vocab - clear_rows;
@@ -833,30 +825,27 @@ int grad_as(const ms_tokens_t& ids, const ms_rows_t& grad, int64_t vocab, float 
                                  4 * kClearBytes, join_blocks);
   if (!fits(sum_blocks, kSumThreads) || !fits(join_blocks, kJoinThreads)) return MS_OPS_EINVAL;
 
-  const bool wide = ids.wide, plain = ids.inner >= ids.n && ids.inner_stride == 1;
-#define SORT(W, P)                                                                       \
-  (ids.n <= 4 * kSortThreads   ? k_sort_tokens<4, W, P>                                  \
-   : ids.n <= 8 * kSortThreads ? k_sort_tokens<8, W, P>                                  \
-                               : k_sort_tokens<16, W, P>)<<<blocks, kSortThreads, 0, s>>>( \
-      ids, vocab, skip, buckets, sorted, static_cast<uint4*>(dtable), clear_bytes)
-  if (wide && plain) SORT(true, true);
-  else if (wide) SORT(true, false);
-  else if (plain) SORT(false, true);
-  else SORT(false, false);
+  const bool plain = ids.inner >= ids.n && ids.inner_stride == 1;
+#define SORT(W, P)                                         \
+  (ids.n <= 4 * kSortThreads   ? k_sort_tokens<4, W, P>    \
+   : ids.n <= 8 * kSortThreads ? k_sort_tokens<8, W, P>    \
+                               : k_sort_tokens<16, W, P>)
+  int rc = launch(ids.wide ? plain ? SORT(true, true) : SORT(true, false)
+                  : plain  ? SORT(false, true)
+                           : SORT(false, false),
+                  blocks, kSortThreads, s, ids, vocab, skip, buckets, sorted,
+                  static_cast<uint4*>(dtable), clear_bytes);
 #undef SORT
-  if (int rc = launched()) return rc;
-  if (sum_blocks) {
-    (brief  ? k_sum_spans<T, 1, 1>
-     : pair ? k_sum_spans<T, kVec, kPair>
-            : k_sum_spans<T, kVec, 1>)<<<static_cast<unsigned>(sum_blocks), kSumThreads, 0, s>>>(
-        grad, scale, static_cast<int>(slices), first, sorted, table);
-    if (int rc = launched()) return rc;
-  }
-  if (!joins) return MS_OPS_OK;
-  (width < 4 ? k_join_spans<T, 1> : k_join_spans<T, 4>)
-      <<<static_cast<unsigned>(join_blocks), kJoinThreads, 0, s>>>(ids.n, width, scale, rest,
-                                                                   sorted, table);
-  return launched();
+  if (!rc && sum_blocks)
+    rc = launch(brief  ? k_sum_spans<T, 1, 1>
+                : pair ? k_sum_spans<T, kVec, kPair>
+                       : k_sum_spans<T, kVec, 1>,
+                sum_blocks, kSumThreads, s, grad, scale, static_cast<int>(slices), first, sorted,
+                table);
+  if (!rc && joins)
+    rc = launch(width < 4 ? k_join_spans<T, 1> : k_join_spans<T, 4>, join_blocks, kJoinThreads, s,
+                ids.n, width, scale, rest, sorted, table);
+  return rc;
 }
 
 }  // namespace

@@ -1095,27 +1095,20 @@ template <typename T, int NT, bool kTop>
 int launch_rows(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
                 const Outputs& out, const Split& split, hipStream_t s) {
   if (!fits(logits.n * split.parts, NT)) return MS_OPS_EINVAL;
-  const unsigned blocks = static_cast<unsigned>(logits.n * split.parts);
-  if (out.entropy)
-    k_logprobs<T, NT, kTop, true><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
-  else
-    k_logprobs<T, NT, kTop, false><<<blocks, NT, 0, s>>>(logits, targets, ignore, out, split);
-  return launched();
+  return launch(out.entropy ? k_logprobs<T, NT, kTop, true> : k_logprobs<T, NT, kTop, false>,
+                logits.n * split.parts, NT, s, logits, targets, ignore, out, split);
 }
 
 template <typename T, int R>
-void launch_short(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
+int launch_short(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
                   const Outputs& out, hipStream_t s) {
-  const unsigned blocks = static_cast<unsigned>(
-      std::min<int64_t>(kShortBlocks, (logits.n + kShortWaves - 1) / kShortWaves));
-#define SHORT(TOP, ENTROPY)                                    \
-  k_logprobs_short<T, R, TOP, ENTROPY>                                   \
-      <<<blocks, kShortThreads, 0, s>>>(logits, targets, ignore, out)
-  if (out.top && out.entropy) SHORT(true, true);
-  else if (out.top) SHORT(true, false);
-  else if (out.entropy) SHORT(false, true);
-  else SHORT(false, false);
-#undef SHORT
+  const int64_t blocks =
+      std::min<int64_t>(kShortBlocks, (logits.n + kShortWaves - 1) / kShortWaves);
+  return launch(out.top ? out.entropy ? k_logprobs_short<T, R, true, true>
+                                      : k_logprobs_short<T, R, true, false>
+                : out.entropy ? k_logprobs_short<T, R, false, true>
+                              : k_logprobs_short<T, R, false, false>,
+                blocks, kShortThreads, s, logits, targets, ignore, out);
 }
 
 template <typename T>
@@ -1123,11 +1116,10 @@ int logprobs_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ign
                 const Outputs& out, const Split& split, hipStream_t s) {
   const int64_t lane_units = (logits.width * static_cast<int64_t>(sizeof(T)) + 1023) / 1024;
   if (is_short(logits.width, logits.dtype)) {
-    if (lane_units <= 1) launch_short<T, 1>(logits, targets, ignore, out, s);
-    else if (lane_units <= 2) launch_short<T, 2>(logits, targets, ignore, out, s);
-    else if (lane_units <= 4) launch_short<T, 4>(logits, targets, ignore, out, s);
-    else launch_short<T, 8>(logits, targets, ignore, out, s);
-    return launched();
+    return (lane_units <= 1   ? launch_short<T, 1>
+            : lane_units <= 2 ? launch_short<T, 2>
+            : lane_units <= 4 ? launch_short<T, 4>
+                              : launch_short<T, 8>)(logits, targets, ignore, out, s);
   }
   const bool mid = logits.width * static_cast<int64_t>(sizeof(T)) <=
                    kMidUnits * 16 / (out.top ? 2 : 1);
@@ -1136,11 +1128,8 @@ int logprobs_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ign
       : mid     ? launch_rows<T, kMidThreads, false>(logits, targets, ignore, out, split, s)
       : out.top ? launch_rows<T, kTopThreads, true>(logits, targets, ignore, out, split, s)
                 : launch_rows<T, kThreads, false>(logits, targets, ignore, out, split, s);
-  if (rc) return rc;
-  if (split.parts > 1)
-    k_join_parts<T><<<static_cast<unsigned>(logits.n), kThreads, 0, s>>>(logits, targets, ignore,
-                                                                         out, split);
-  return launched();
+  if (rc || split.parts == 1) return rc;
+  return launch(k_join_parts<T>, logits.n, kThreads, s, logits, targets, ignore, out, split);
 }
 
 template <typename T>
@@ -1149,32 +1138,23 @@ int grad_as(const ms_rows_t& logits, const ms_tokens_t& targets, int64_t ignore,
             void* dlogits, hipStream_t s) {
   if (is_short(logits.width, logits.dtype)) {
     const int64_t lane_units = (logits.width * static_cast<int64_t>(sizeof(T)) + 1023) / 1024;
-    const unsigned short_blocks = static_cast<unsigned>(
-        std::min<int64_t>(kShortBlocks, (logits.n + kShortWaves - 1) / kShortWaves));
-#define SHORT(R)                                                                        \
-  (grad_entropy ? k_logprobs_grad_short<T, R, true> : k_logprobs_grad_short<T, R, false>) \
-      <<<short_blocks, kShortThreads, 0, s>>>(logits, targets, ignore, lse, entropy,      \
-                                              grad_logprob, grad_entropy, static_cast<T*>(dlogits))
-    if (lane_units <= 1) SHORT(1);
-    else if (lane_units <= 2) SHORT(2);
-    else if (lane_units <= 4) SHORT(4);
-    else SHORT(8);
+    const int64_t short_blocks =
+        std::min<int64_t>(kShortBlocks, (logits.n + kShortWaves - 1) / kShortWaves);
+#define SHORT(R) (grad_entropy ? k_logprobs_grad_short<T, R, true> : k_logprobs_grad_short<T, R, false>)
+    return launch(lane_units <= 1   ? SHORT(1)
+                  : lane_units <= 2 ? SHORT(2)
+                  : lane_units <= 4 ? SHORT(4)
+                                    : SHORT(8),
+                  short_blocks, kShortThreads, s, logits, targets, ignore, lse, entropy,
+                  grad_logprob, grad_entropy, static_cast<T*>(dlogits));
 #undef SHORT
-    return launched();
   }
   constexpr int64_t kEach = kGradGroup * kGradThreads * (16 / sizeof(T));
   const int64_t per_row = std::max<int64_t>((logits.width + kEach - 1) / kEach, 1);
   if (!fits(logits.n * per_row, kGradThreads)) return MS_OPS_EINVAL;
-  const unsigned blocks = static_cast<unsigned>(logits.n * per_row);
-  if (grad_entropy)
-    k_logprobs_grad<T, true><<<blocks, kGradThreads, 0, s>>>(
-        logits, targets, ignore, lse, entropy, grad_logprob, grad_entropy,
-        static_cast<int>(per_row), static_cast<T*>(dlogits));
-  else
-    k_logprobs_grad<T, false><<<blocks, kGradThreads, 0, s>>>(
-        logits, targets, ignore, lse, entropy, grad_logprob, grad_entropy,
-        static_cast<int>(per_row), static_cast<T*>(dlogits));
-  return launched();
+  return launch(grad_entropy ? k_logprobs_grad<T, true> : k_logprobs_grad<T, false>,
+                logits.n * per_row, kGradThreads, s, logits, targets, ignore, lse, entropy,
+                grad_logprob, grad_entropy, static_cast<int>(per_row), static_cast<T*>(dlogits));
 }
 
 }  // namespace

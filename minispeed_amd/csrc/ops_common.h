@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <tuple>
+
 #include "minispeed_ops.h"
 
 namespace ops {
@@ -137,8 +139,22 @@ inline bool good_rows(const ms_rows_t* m) {
 // A launch has fewer than 2^32 threads.
 inline bool fits(int64_t blocks, int threads) { return blocks <= UINT32_MAX / threads; }
 
-// The launch's own status; errors that earlier work left are not reported here
-// as ours.
-inline int launched() { return static_cast<int>(hipGetLastError()); }
+// Launches a kernel and returns the launch's own status.  (After <<<>>> only
+// hipGetLastError() tells, and that is the last error of any call of the thread:
+// one that earlier work left would be taken for the launch's, and taken away from those who
+// look for it.)
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), int64_t blocks, int threads, hipStream_t s, A... a) {
+  static_assert(sizeof...(P) == sizeof...(A), "");
+  std::tuple<P...> values(static_cast<P>(a)...);
+  return std::apply(
+      [&](P&... v) {
+        void* args[] = {static_cast<void*>(&v)...};
+        return static_cast<int>(hipLaunchKernel(reinterpret_cast<const void*>(kernel),
+                                                dim3(static_cast<unsigned>(blocks)), dim3(threads),
+                                                args, 0, s));
+      },
+      values);
+}
 
 }  // namespace ops

@@ -8,11 +8,15 @@ the last place of the result.
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import minispeed_amd as ms
+from minispeed_amd import build
 from tests import ops_reference as ref
+from tests.test_ops_abi import Rows, Tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -275,3 +279,31 @@ def test_refusals():
         ms.ops.embedding_grad(g.double(), ids, 10)
     with pytest.raises(RuntimeError, match="cpu"):
         ms.ops.embedding_grad(g.cpu(), ids, 10)
+
+
+def test_an_error_that_earlier_work_left_is_not_taken_for_the_launchs():
+    """The thread's last HIP error (here of a device number that there is not) is neither
+    reported by the operators nor taken away."""
+    rows, width, n = 3000, 64, 2000                      # three launches
+    w, ids, g = _rand((rows, width), "fp32", 33), _ids(n, rows, 34), _rand((n, width), "fp32", 35)
+    out, dw = torch.empty(n, width, device=DEV), torch.empty(rows, width, device=DEV)
+    lib, hip = ctypes.CDLL(build.OPS_OUTPUT), ctypes.CDLL("libamdhip64.so.7")
+    lib.ms_embedding_grad_workspace.restype = ctypes.c_int64
+    i64, ptr, ref_of = ctypes.c_int64, ctypes.c_void_p, ctypes.byref
+    size = lib.ms_embedding_grad_workspace(i64(n), i64(rows), i64(width))
+    work = torch.empty(size, dtype=torch.uint8, device=DEV)
+    table, grad = Rows(w.data_ptr(), rows, width, rows, 0, width, 0, 0), Rows(g.data_ptr(), n, width, n,
+                                                                              0, width, 0, 0)
+    tokens = Tokens(ids.data_ptr(), n, n, 0, 1, 1, 0)
+    stream = ptr(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    hip.hipGetLastError()
+    bad = hip.hipSetDevice(9999)
+    codes = [lib.ms_embedding(ref_of(tokens), ref_of(table), ctypes.c_float(1), ptr(out.data_ptr()),
+                              stream),
+             lib.ms_embedding_grad(ref_of(tokens), ref_of(grad), i64(rows), ctypes.c_float(1),
+                                   i64(-1), ptr(dw.data_ptr()), ptr(work.data_ptr()), i64(size),
+                                   stream)]
+    left = hip.hipGetLastError()
+    assert bad != 0 and codes == [0, 0] and left == bad
+    assert torch.equal(out, w[ids]) and torch.equal(dw, ms.ops.embedding_grad(g, ids, rows))
