@@ -143,7 +143,7 @@ class _Checkpoint(torch.autograd.Function):
         for arg in args:
             if not isinstance(arg, torch.Tensor):
                 ctx.slots.append(("value", arg, False))
-            elif arg.is_cuda and arg.dim() > 0 and arg.dtype in _HELD:
+            elif _is_activation(arg):
                 packed = pack8(arg)
                 ctx.slots.append(("held", (packed.shape, packed.dtype), arg.requires_grad))
                 held += [packed.codes, packed.exponents]
@@ -184,6 +184,12 @@ class _Checkpoint(torch.autograd.Function):
 _HELD = (torch.float32, torch.float16, torch.bfloat16)
 
 
+def _is_activation(arg):
+    """What is held in 8 bits: gradients flow through it, to something that is no parameter."""
+    return (arg.is_cuda and arg.dim() > 0 and arg.dtype in _HELD and arg.requires_grad
+            and not isinstance(arg, torch.nn.Parameter))
+
+
 def _rng_state(args):
     device = next((a.device for a in args if isinstance(a, torch.Tensor) and a.is_cuda), None)
     return (torch.get_rng_state(), device,
@@ -220,11 +226,13 @@ def checkpoint8(fn, *args, preserve_rng_state: bool = True):
     """``fn(*args)`` whose activations are computed again in the backward pass, from
     arguments held in 8 bits.
 
-    The float32, float16 and bfloat16 tensors on the GPU among ``args`` are kept in
-    their 8-bit form (other tensors as they are), and ``fn`` runs again on the values
+    The float32, float16 and bfloat16 tensors on the GPU among ``args`` that require a
+    gradient are kept in their 8-bit form, and ``fn`` runs again on the values
     they stand for when the gradients come: the use of minispeed's ``checkpoint``
     (minispeed/activation_checkpointing.py:17-20) with a quarter to a half of its
-    memory.  The first run sees the arguments themselves.  Parameters that ``fn``
+    memory.  Parameters, which are there anyway, and tensors without a gradient (masks,
+    whose infinities no 8-bit form has, and tables) are kept as they are.  The first run
+    sees the arguments themselves.  Parameters that ``fn``
     reaches by itself get their gradients; with ``preserve_rng_state`` random
     operations (dropout) draw the same numbers in both runs.  Gradients reach
     ``args`` only if one of them requires a gradient, as with any reentrant

@@ -316,6 +316,29 @@ def test_checkpoint_of_half_precision_and_of_nothing():
     assert not ms.ops.checkpoint8(lambda a: a * 2, x.detach()).requires_grad
 
 
+def test_checkpoint_keeps_masks_tables_and_parameters_as_they_are():
+    torch.manual_seed(1)
+    x = _rand((2, 12, 32), "fp32", 22).requires_grad_()
+    mask = torch.full((12, 12), -math.inf, device=DEV).triu(1)
+    table = _rand((12, 32), "fp32", 23)
+    w = torch.nn.Parameter(_rand((32, 32), "fp32", 24, 0.1))
+    seen = []
+
+    def fn(z, mask, table, w):
+        seen.append((mask.detach().clone(), table.detach().clone(), w.detach().clone()))
+        return torch.softmax((z * table) @ z.transpose(1, 2) + mask, -1) @ (z @ w)
+
+    y = ms.ops.checkpoint8(fn, x, mask, table, w)
+    y.backward(torch.ones_like(y))
+    for a, b in zip(*seen):
+        assert torch.equal(a, b)
+    z, v = x.detach().clone(), w.detach().clone().requires_grad_()
+    z = ref.held(z)[2].view(z.shape).float().to(DEV).requires_grad_()
+    fn(z, mask, table, v).backward(torch.ones_like(y))
+    assert torch.equal(x.grad, z.grad) and torch.equal(w.grad, v.grad)
+    assert bool(torch.isfinite(x.grad).all()) and bool(x.grad.any())
+
+
 def test_in_a_graph():
     h, up, g = (_rand((40, 200), "bf16", s) for s in (18, 19, 20))
 
