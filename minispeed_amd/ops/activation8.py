@@ -234,10 +234,10 @@ def checkpoint8(fn, *args, preserve_rng_state: bool = True):
     whose infinities no 8-bit form has, and tables) are kept as they are.  The first run
     sees the arguments themselves.  Parameters that ``fn``
     reaches by itself get their gradients; with ``preserve_rng_state`` random
-    operations (dropout) draw the same numbers in both runs.  Gradients reach
-    ``args`` only if one of them requires a gradient, as with any reentrant
-    checkpoint.
+    operations (dropout) draw the same numbers in both runs.  If none of ``args``
+    requires a gradient there is nothing to hold, and ``fn`` runs as it would by itself.
     """
-    if not torch.is_grad_enabled():
+    if not torch.is_grad_enabled() or not any(isinstance(a, torch.Tensor) and a.requires_grad
+                                              for a in args):
         return fn(*args)
     return _Checkpoint.apply(fn, preserve_rng_state, *args)

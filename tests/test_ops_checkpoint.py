@@ -1,0 +1,19 @@
+"""checkpoint8 on the host: its autograd, with tensors that no kernel touches (what is
+not on a GPU is kept as it is)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import minispeed_amd as ms
+
+
+def test_parameters_get_gradients_when_no_argument_requires_one():
+    layer = torch.nn.Linear(4, 3)
+    x = torch.arange(8.0).view(2, 4)
+    y = ms.ops.checkpoint8(layer, x)
+    assert y.requires_grad
+    y.sum().backward()
+    assert torch.equal(layer.weight.grad, x.sum(0).expand(3, 4))
+    assert not ms.ops.checkpoint8(lambda a: a * 2, x).requires_grad
