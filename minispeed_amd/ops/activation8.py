@@ -152,7 +152,12 @@ class _Checkpoint(torch.autograd.Function):
                 held.append(arg)
         ctx.save_for_backward(*held)
         with torch.no_grad():
-            return fn(*args)
+            out = fn(*args)
+        for o in out if isinstance(out, tuple) else (out,):
+            if isinstance(o, (tuple, list, dict)):       # autograd would not see what is in it
+                raise TypeError(f"fn gives a {type(o).__name__}; expected a tensor or a tuple "
+                                "of tensors")
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -232,7 +237,8 @@ def checkpoint8(fn, *args, preserve_rng_state: bool = True):
     (minispeed/activation_checkpointing.py:17-20) with a quarter to a half of its
     memory.  Parameters, which are there anyway, and tensors without a gradient (masks,
     whose infinities no 8-bit form has, and tables) are kept as they are.  The first run
-    sees the arguments themselves.  Parameters that ``fn``
+    sees the arguments themselves.  ``fn`` gives a tensor or a tuple of them (and of
+    other things, which are passed on).  Parameters that ``fn``
     reaches by itself get their gradients; with ``preserve_rng_state`` random
     operations (dropout) draw the same numbers in both runs.  If none of ``args``
     requires a gradient there is nothing to hold, and ``fn`` runs as it would by itself.

@@ -17,3 +17,15 @@ def test_parameters_get_gradients_when_no_argument_requires_one():
     y.sum().backward()
     assert torch.equal(layer.weight.grad, x.sum(0).expand(3, 4))
     assert not ms.ops.checkpoint8(lambda a: a * 2, x).requires_grad
+
+
+@pytest.mark.parametrize("wrap", [lambda y: [y], lambda y: {"y": y}, lambda y: (y, (y, y)),
+                                  lambda y: (y, [y])])
+def test_results_whose_gradients_would_be_lost_are_refused(wrap):
+    x = torch.ones(3, requires_grad=True)
+    with pytest.raises(TypeError, match="tuple"):
+        ms.ops.checkpoint8(lambda a: wrap(a * 2), x)
+    y, n, none = ms.ops.checkpoint8(lambda a: (a * 2, 7, None), x)
+    assert n == 7 and none is None
+    y.sum().backward()
+    assert torch.equal(x.grad, torch.full((3,), 2.0))
