@@ -14,6 +14,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
+from torch.utils._pytree import tree_leaves
 
 from . import _native
 
@@ -154,7 +155,9 @@ class _Checkpoint(torch.autograd.Function):
         with torch.no_grad():
             out = fn(*args)
         for o in out if isinstance(out, tuple) else (out,):
-            if isinstance(o, (tuple, list, dict)):       # autograd would not see what is in it
+            # autograd would not see tensors in it
+            if not isinstance(o, torch.Tensor) and any(isinstance(t, torch.Tensor)
+                                                       for t in tree_leaves([o]) if t is not o):
                 raise TypeError(f"fn gives a {type(o).__name__}; expected a tensor or a tuple "
                                 "of tensors")
         return out

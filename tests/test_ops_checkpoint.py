@@ -25,7 +25,7 @@ def test_results_whose_gradients_would_be_lost_are_refused(wrap):
     x = torch.ones(3, requires_grad=True)
     with pytest.raises(TypeError, match="tuple"):
         ms.ops.checkpoint8(lambda a: wrap(a * 2), x)
-    y, n, none = ms.ops.checkpoint8(lambda a: (a * 2, 7, None), x)
-    assert n == 7 and none is None
+    y, n, none, sizes = ms.ops.checkpoint8(lambda a: (a * 2, 7, None, [1, 2]), x)
+    assert n == 7 and none is None and sizes == [1, 2]
     y.sum().backward()
     assert torch.equal(x.grad, torch.full((3,), 2.0))
