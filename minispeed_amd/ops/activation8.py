@@ -157,7 +157,7 @@ class _Checkpoint(torch.autograd.Function):
         for o in out if isinstance(out, tuple) else (out,):
             # autograd would not see tensors in it
             if not isinstance(o, torch.Tensor) and any(isinstance(t, torch.Tensor)
-                                                       for t in tree_leaves([o]) if t is not o):
+                                                       for t in tree_leaves(o)):
                 raise TypeError(f"fn gives a {type(o).__name__}; expected a tensor or a tuple "
                                 "of tensors")
         return out
