@@ -12,6 +12,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -44,6 +45,13 @@ void need_hip(const Tensor& t, const char* what) {
     throw std::runtime_error(std::string(what) + " is on " + t.device().str() +
                              "; minispeed_amd.ops runs HIP kernels and needs tensors on a ROCm "
                              "GPU (device 'cuda')");
+}
+
+// The kernels have no forward-mode derivatives; run below autograd they would drop a tangent.
+void need_no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), what,
+      " has a tangent; minispeed_amd.ops has no forward-mode derivatives");
 }
 
 void need_device(const Tensor& t, const Tensor& like, const char* what) {
@@ -163,6 +171,7 @@ const float* per_row(const std::optional<Tensor>& t, const Tensor& logits, int64
 // ---------------------------------------------------------------------------
 
 Tensor embedding(const Tensor& ids, const Tensor& weight, double scale) {
+  need_no_tangent(weight, "weight");
   need_hip(weight, "weight");
   need_device(ids, weight, "ids");
   if (weight.dim() != 2) bad_value("weight has shape " + shape_of(weight) + ", expected [rows, width]");
@@ -182,6 +191,7 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale) {
 
 Tensor embedding_grad(const Tensor& grad, const Tensor& ids, int64_t rows, double scale,
                       int64_t padding_idx) {
+  need_no_tangent(grad, "grad");
   need_hip(grad, "grad");
   need_device(ids, grad, "ids");
   if (rows < 0) bad_value("rows is " + std::to_string(rows));
@@ -205,6 +215,7 @@ Tensor embedding_grad(const Tensor& grad, const Tensor& ids, int64_t rows, doubl
 }
 
 void need_targets(const Tensor& logits, const Tensor& targets) {
+  need_no_tangent(logits, "logits");
   need_hip(logits, "logits");
   need_device(targets, logits, "targets");
   bool match = logits.dim() >= 1 && targets.dim() == logits.dim() - 1;
@@ -257,6 +268,10 @@ Tensor token_logprobs_grad(const Tensor& logits, const Tensor& targets, const Te
                            const std::optional<Tensor>& grad_logprob,
                            const std::optional<Tensor>& entropy,
                            const std::optional<Tensor>& grad_entropy, int64_t ignore_index) {
+  need_no_tangent(lse, "lse");
+  if (grad_logprob) need_no_tangent(*grad_logprob, "grad_logprob");
+  if (entropy) need_no_tangent(*entropy, "entropy");
+  if (grad_entropy) need_no_tangent(*grad_entropy, "grad_entropy");
   need_targets(logits, targets);
   if (grad_entropy && !entropy) bad_value("grad_entropy needs entropy");
   at::AutoDispatchBelowADInplaceOrView below;
@@ -277,6 +292,7 @@ Tensor token_logprobs_grad(const Tensor& logits, const Tensor& targets, const Te
 int64_t blocks_of(int64_t n) { return (n + MS_OPS_BLOCK - 1) / MS_OPS_BLOCK; }
 
 py::tuple pack8(const Tensor& x) {
+  need_no_tangent(x, "x");
   need_hip(x, "x");
   const int32_t type = dtype_of(x.scalar_type(), "x");
   at::AutoDispatchBelowADInplaceOrView below;
@@ -320,6 +336,8 @@ Tensor unpack8(const Tensor& codes, const Tensor& exponents, const std::vector<i
 }
 
 py::tuple act8(const Tensor& h, const std::optional<Tensor>& up, int64_t kind) {
+  need_no_tangent(h, "h");
+  if (up) need_no_tangent(*up, "up");
   need_hip(h, "h");
   if ((kind == MS_ACT_SWIGLU) != up.has_value())
     bad_value(up ? "up is for the gated kind only" : "the gated kind needs up");
@@ -356,6 +374,7 @@ py::tuple act8_grad(const Tensor& codes, const Tensor& exponents,
                     const std::optional<Tensor>& up_codes,
                     const std::optional<Tensor>& up_exponents, const Tensor& grad, int64_t kind,
                     bool again) {
+  need_no_tangent(grad, "grad");
   need_hip(grad, "grad");
   const int32_t type = dtype_of(grad.scalar_type(), "grad");
   const bool gated = kind == MS_ACT_SWIGLU;

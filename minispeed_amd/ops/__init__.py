@@ -11,8 +11,9 @@
 
 ``embedding``, ``token_logprobs``, ``checkpoint8`` and ``activation8_linear`` take
 part in autograd; the ``_grad`` functions are the same backward passes for a
-program that calls them itself.  All of them run on the current stream, allocate
-through torch's caching allocator and return before the kernels have finished.
+program that calls them itself.  Forward-mode derivatives are refused.  All of them
+run on the current stream, allocate through torch's caching allocator and return before
+the kernels have finished.
 """
 
 from .activation8 import (Checkpoint8, activation8, activation8_grad, activation8_linear,
