@@ -9,9 +9,9 @@
   :func:`activation8_grad`, :func:`activation8_linear` — activations held in 8
   bits between forward and backward.
 
-``embedding``, ``token_logprobs``, ``checkpoint8`` and ``activation8_linear`` take
-part in autograd; the ``_grad`` functions are the same backward passes for a
-program that calls them itself.  Forward-mode derivatives are refused.  All of them
+``embedding``, ``token_logprobs``, ``activation8``, ``checkpoint8`` and
+``activation8_linear`` take part in autograd; the ``_grad`` functions are the same backward
+passes for a program that calls them itself, and are not differentiable again.  Forward-mode derivatives are refused.  All of them
 run on the current stream, allocate through torch's caching allocator and return before
 the kernels have finished.
 """

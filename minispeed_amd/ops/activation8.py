@@ -38,7 +38,8 @@ class Checkpoint8:
 
 
 def pack8(x: torch.Tensor) -> Checkpoint8:
-    """The 8-bit form of ``x`` (float32 / float16 / bfloat16)."""
+    """The 8-bit form of ``x`` (float32 / float16 / bfloat16).  Its whole numbers carry no
+    gradient, and neither does what :func:`unpack8` makes of them."""
     codes, exponents = _native.pack8(x)
     return Checkpoint8(codes, exponents, x.shape, x.dtype)
 
@@ -55,15 +56,40 @@ def _kind(kind: str) -> int:
         raise ValueError(f"unknown activation {kind!r}; expected one of {sorted(KINDS)}") from None
 
 
+class _Activation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, up, kind):
+        a, *held = _native.act8(h, up, _kind(kind))
+        ctx.kind, ctx.meta, ctx.gated = kind, (h.shape, h.dtype), up is not None
+        ctx.save_for_backward(*held)
+        ctx.mark_non_differentiable(*(t for t in held if t is not None))
+        ctx.set_materialize_grads(False)
+        return a, *held
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, *_):
+        if grad is None:
+            return None, None, None
+        held = ctx.saved_tensors
+        saved = [Checkpoint8(held[k], held[k + 1], *ctx.meta) for k in ((0, 2) if ctx.gated else (0,))]
+        grads, _ = activation8_grad(saved, grad, ctx.kind, again=False)
+        return grads[0], grads[1] if ctx.gated else None, None
+
+
 def activation8(h: torch.Tensor, kind: str = "gelu", up: Optional[torch.Tensor] = None
                 ) -> Tuple[torch.Tensor, Tuple[Checkpoint8, ...]]:
     """``(a, saved)``: the activation of ``h`` and its input in 8 bits, in one pass.
 
     ``kind`` is ``"gelu"`` (with the error function), ``"gelu_tanh"``, ``"silu"`` or
     ``"swiglu"`` (``silu(h) * up``).  ``a`` is computed from ``h`` itself; ``saved``
-    (one checkpoint, two for ``"swiglu"``) is what :func:`activation8_grad` takes.
+    (one checkpoint, two for ``"swiglu"``) is what :func:`activation8_grad` takes.  ``a``
+    is differentiable, by the held values.
     """
-    a, codes, exponents, up_codes, up_exponents = _native.act8(h, up, _kind(kind))
+    if torch.is_grad_enabled() and (h.requires_grad or (up is not None and up.requires_grad)):
+        a, codes, exponents, up_codes, up_exponents = _Activation.apply(h, up, kind)
+    else:
+        a, codes, exponents, up_codes, up_exponents = _native.act8(h, up, _kind(kind))
     saved = (Checkpoint8(codes, exponents, h.shape, h.dtype),)
     if up is not None:
         saved += (Checkpoint8(up_codes, up_exponents, h.shape, h.dtype),)

@@ -243,6 +243,31 @@ def test_activation_linear_autograd(kind):
     assert abs(slope - float(prod.sum())) <= 1e-4 * float(prod.abs().sum())
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_activation_autograd(kind):
+    """The activation's gradients are those of its backward pass, for whichever inputs want them."""
+    h0, g = _rand((3, 70), "bf16", 25), _rand((3, 70), "bf16", 27, 0.1)
+    up0 = _rand((3, 70), "bf16", 26) if kind == "swiglu" else None
+    plain, saved = ms.ops.activation8(h0, kind, up=up0)
+    grads, _ = ms.ops.activation8_grad(saved, g, kind)
+    for want_h, want_up in ((True, True), (True, False), (False, True)):
+        h, up = h0.clone().requires_grad_(want_h), None
+        if kind == "swiglu":
+            up = up0.clone().requires_grad_(want_up)
+        elif not want_h:
+            continue
+        a, held = ms.ops.activation8(h, kind, up=up)
+        assert a.requires_grad and torch.equal(a.detach(), plain)
+        assert all(torch.equal(x.codes, y.codes) and torch.equal(x.exponents, y.exponents)
+                   and not x.codes.requires_grad for x, y in zip(held, saved))
+        a.backward(g)
+        assert torch.equal(h.grad, grads[0]) if want_h else h.grad is None
+        if up is not None:
+            assert torch.equal(up.grad, grads[1]) if want_up else up.grad is None
+    with torch.no_grad():
+        assert not ms.ops.activation8(h, kind, up=up)[0].requires_grad
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("half_h", [False, True])
 def test_activation_linear_under_autocast(dtype, half_h):
