@@ -134,8 +134,12 @@ class _ActivationLinear(torch.autograd.Function):
         dh = dup = dw = db = None
         flat = grad.reshape(-1, grad.shape[-1])
         if need[0] or need[1] or need[2]:
-            # (the types differ under autocast only)
-            da = grad.matmul(weight.to(grad.dtype)).to(saved[0].dtype)
+            if need[0] or need[1]:
+                # (the types differ under autocast only)
+                da = grad.matmul(weight.to(grad.dtype)).to(saved[0].dtype)
+            else:
+                # only the activation again is used, on which these values have no bearing
+                da = torch.empty(saved[0].shape, dtype=saved[0].dtype, device=grad.device)
             grads, a = activation8_grad(saved, da, ctx.kind, again=need[2])
             dh, dup = grads if len(grads) == 2 else (grads[0], None)
             if need[2]:

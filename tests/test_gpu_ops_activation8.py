@@ -14,6 +14,7 @@ import math
 import pytest
 import torch
 import torch.nn.functional as F
+from torch.utils._python_dispatch import TorchDispatchMode
 
 import minispeed_amd as ms
 from tests import ops_reference as ref
@@ -266,6 +267,35 @@ def test_activation_autograd(kind):
             assert torch.equal(up.grad, grads[1]) if want_up else up.grad is None
     with torch.no_grad():
         assert not ms.ops.activation8(h, kind, up=up)[0].requires_grad
+
+
+class _Products(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.n = 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.n += func.overloadpacket in (torch.ops.aten.mm, torch.ops.aten.addmm, torch.ops.aten.bmm)
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("kind", ["gelu", "swiglu"])
+def test_activation_linear_computes_no_product_that_nobody_wants(kind):
+    h, w0 = _rand((2, 9, 64), "bf16", 28), _rand((32, 64), "bf16", 29, 0.1)
+    up = _rand((2, 9, 64), "bf16", 30) if kind == "swiglu" else None
+    gy, got = _rand((2, 9, 32), "bf16", 31), {}
+    for want_h, want_w, products in ((True, True, 2), (False, True, 1), (True, False, 1)):
+        x, w = h.clone().requires_grad_(want_h), w0.clone().requires_grad_(want_w)
+        y = ms.ops.activation8_linear(x, w, None, kind, up)
+        # the backward pass runs in autograd's own thread: called here for the mode to see it
+        node, count = y.grad_fn, _Products()
+        with count, torch.no_grad():
+            grads = type(node)._forward_cls.backward(node, gy)
+        assert count.n == products, (want_h, want_w, count.n)
+        y.backward(gy)
+        for name, t, g in (("h", x, grads[0]), ("w", w, grads[2])):
+            if t.requires_grad:
+                assert torch.equal(t.grad, got.setdefault(name, t.grad)) and torch.equal(t.grad, g)
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
