@@ -320,6 +320,9 @@ void need_held(const Tensor& codes, const Tensor& exponents, int64_t n) {
 
 Tensor unpack8(const Tensor& codes, const Tensor& exponents, const std::vector<int64_t>& shape,
                py::object dtype) {
+  if (!THPDtype_Check(dtype.ptr()))
+    throw py::type_error("the checkpoint's dtype is " + std::string(py::repr(dtype)) +
+                         ", expected a torch.dtype");
   const at::ScalarType as = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
   const int32_t type = dtype_of(as, "the checkpoint");
   at::AutoDispatchBelowADInplaceOrView below;

@@ -165,3 +165,11 @@ def test_calls_beyond_one_launch_are_refused(lib):
     rows = Rows(16, 2 ** 30, 4096, 2 ** 30, 0, 4096, 1, 0)
     assert lib.ms_embedding_grad(ref(ids), ref(rows), I64(10), F(1), I64(-1), P(16), P(16),
                                  I64(2 ** 62), None) == -1
+
+
+@pytest.mark.parametrize("dtype", ["float32", None, 5, torch.zeros(1)])
+def test_a_checkpoint_of_no_dtype_is_refused(dtype):
+    held = ms.ops.Checkpoint8(torch.zeros(32, dtype=torch.int8), torch.ones(1, dtype=torch.uint8),
+                              (32,), dtype)
+    with pytest.raises(TypeError, match="torch.dtype"):
+        ms.ops.unpack8(held)
