@@ -107,9 +107,10 @@ def activation8_grad(saved: Sequence[Checkpoint8], grad: torch.Tensor, kind: str
     """
     if not 1 <= len(saved) <= 2:
         raise ValueError(f"{len(saved)} checkpoints, expected one or two")
-    if saved[0].dtype != grad.dtype or saved[0].shape != tuple(grad.shape):
-        raise ValueError(f"grad is {grad.dtype} {tuple(grad.shape)}, the checkpoint "
-                         f"{saved[0].dtype} {saved[0].shape}")
+    for s in saved:
+        if s.dtype != grad.dtype or s.shape != tuple(grad.shape):
+            raise ValueError(f"grad is {grad.dtype} {tuple(grad.shape)}, the checkpoint "
+                             f"{s.dtype} {s.shape}")
     up = saved[1] if len(saved) == 2 else None
     dh, dup, a = _native.act8_grad(saved[0].codes, saved[0].exponents, up and up.codes,
                                    up and up.exponents, grad, _kind(kind), again)

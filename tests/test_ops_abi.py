@@ -173,3 +173,14 @@ def test_a_checkpoint_of_no_dtype_is_refused(dtype):
                               (32,), dtype)
     with pytest.raises(TypeError, match="torch.dtype"):
         ms.ops.unpack8(held)
+
+
+def test_two_checkpoints_of_different_tensors_are_refused():
+    held = [ms.ops.Checkpoint8(torch.zeros(32, dtype=torch.int8), torch.ones(1, dtype=torch.uint8),
+                               shape, dtype)
+            for shape, dtype in (((4, 8), torch.float32), ((8, 4), torch.float32),
+                                 ((4, 8), torch.float16))]
+    grad = torch.zeros(4, 8)
+    for up in held[1:]:
+        with pytest.raises(ValueError, match="checkpoint"):
+            ms.ops.activation8_grad((held[0], up), grad, "swiglu")
