@@ -571,7 +571,7 @@ int unpack_as(const int8_t* codes, const uint8_t* exponents, int64_t n, void* ou
 
 extern "C" int ms_pack8(const void* x, int32_t dtype, int64_t n, int8_t* codes, uint8_t* exponents,
                         void* stream) {
-  if (!good_dtype(dtype) || n < 0) return MS_OPS_EINVAL;
+  if (!good_dtype(dtype) || n < 0 || !countable(n)) return MS_OPS_EINVAL;
   if (n == 0) return MS_OPS_OK;
   if (!x || !codes || !exponents) return MS_OPS_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -584,7 +584,7 @@ extern "C" int ms_pack8(const void* x, int32_t dtype, int64_t n, int8_t* codes, 
 
 extern "C" int ms_unpack8(const int8_t* codes, const uint8_t* exponents, int64_t n, int32_t dtype,
                           void* out, void* stream) {
-  if (!good_dtype(dtype) || n < 0) return MS_OPS_EINVAL;
+  if (!good_dtype(dtype) || n < 0 || !countable(n)) return MS_OPS_EINVAL;
   if (n == 0) return MS_OPS_OK;
   if (!out || !codes || !exponents) return MS_OPS_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -620,7 +620,7 @@ extern "C" int ms_act8_grad(const int8_t* codes, const uint8_t* exponents, const
                             const uint8_t* up_exponents, const void* grad, int32_t dtype,
                             int32_t kind, int64_t n, void* dh, void* dup, void* a, void* stream) {
   const bool gated = kind == MS_ACT_SWIGLU;
-  if (!good_kind(kind) || !good_dtype(dtype) || n < 0) return MS_OPS_EINVAL;
+  if (!good_kind(kind) || !good_dtype(dtype) || n < 0 || !countable(n)) return MS_OPS_EINVAL;
   if (n == 0) return MS_OPS_OK;
   if (!codes || !exponents || !grad || !dh) return MS_OPS_EINVAL;
   if (gated != (up_codes != nullptr) || gated != (up_exponents != nullptr) ||

@@ -854,7 +854,7 @@ extern "C" int ms_embedding(const ms_tokens_t* ids, const ms_rows_t* table, floa
                             void* stream) {
   if (!good_tokens(ids) || !good_rows(table)) return MS_OPS_EINVAL;
   if (ids->n == 0 || table->width == 0) return MS_OPS_OK;
-  if (!out || table->n < 1) return MS_OPS_EINVAL;
+  if (!out || table->n < 1 || !countable(ids->n, table->width)) return MS_OPS_EINVAL;
   if (table->n > 1 && table->inner < table->n) return MS_OPS_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (table->dtype) {
@@ -865,7 +865,9 @@ extern "C" int ms_embedding(const ms_tokens_t* ids, const ms_rows_t* table, floa
 }
 
 extern "C" int64_t ms_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t width) {
-  if (n < 0 || vocab < 0 || width < 0 || n > kMostTokens || vocab > INT32_MAX) return -1;
+  if (n < 0 || vocab < 0 || width < 0 || n > kMostTokens || vocab > INT32_MAX ||
+      !countable(std::max(n, vocab), width))
+    return -1;
   if (vocab == 0 || width == 0) return 0;
   const GradShape g = shape_of(n, vocab, width);
   return g.start_bytes + 2 * g.list_bytes + g.partial_bytes;
@@ -875,7 +877,7 @@ extern "C" int ms_embedding_grad(const ms_tokens_t* ids, const ms_rows_t* grad, 
                                  float scale, int64_t padding_idx, void* dtable, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   if (!good_tokens(ids) || !good_rows(grad) || grad->n != ids->n || ids->n > kMostTokens ||
-      vocab < 0 || vocab > INT32_MAX)
+      vocab < 0 || vocab > INT32_MAX || !countable(vocab, grad->width))
     return MS_OPS_EINVAL;
   if (vocab == 0 || grad->width == 0) return MS_OPS_OK;
   if (!dtable || (reinterpret_cast<uintptr_t>(dtable) & 15)) return MS_OPS_EINVAL;

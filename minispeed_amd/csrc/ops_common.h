@@ -128,12 +128,18 @@ __device__ __forceinline__ int64_t read_lane(int64_t x, int lane) {
 inline bool good_dtype(int32_t d) { return d >= MS_OPS_F32 && d <= MS_OPS_BF16; }
 inline int64_t dtype_bytes(int32_t d) { return d == MS_OPS_F32 ? 4 : 2; }
 
+// Whether a * b values, as many bytes and some times that, can be counted in 64 bits.
+inline bool countable(int64_t a, int64_t b = 1) {
+  int64_t product;
+  return !__builtin_mul_overflow(a, b, &product) && product < int64_t{1} << 56;
+}
+
 inline bool good_tokens(const ms_tokens_t* t) {
   return t && t->n >= 0 && t->n <= INT32_MAX && t->inner >= 1 && (t->n == 0 || t->data);
 }
 inline bool good_rows(const ms_rows_t* m) {
   return m && m->n >= 0 && m->n <= INT32_MAX && m->width >= 0 && m->inner >= 1 &&
-         good_dtype(m->dtype) && (m->n == 0 || m->width == 0 || m->data);
+         countable(m->n, m->width) && good_dtype(m->dtype) && (m->n == 0 || m->width == 0 || m->data);
 }
 
 // A launch has fewer than 2^32 threads.

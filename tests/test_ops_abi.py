@@ -184,3 +184,26 @@ def test_two_checkpoints_of_different_tensors_are_refused():
     for up in held[1:]:
         with pytest.raises(ValueError, match="checkpoint"):
             ms.ops.activation8_grad((held[0], up), grad, "swiglu")
+
+
+def test_sizes_whose_products_pass_64_bits_are_refused(lib):
+    """Products that come out small or negative would make a small launch over rows of any length."""
+    ref, most = ctypes.byref, 2 ** 63 - 1
+    assert lib.ms_pack8(P(16), I32(1), I64(most), P(16), P(16), None) == -1
+    assert lib.ms_unpack8(P(16), P(16), I64(most - 3), I32(1), P(16), None) == -1
+    assert lib.ms_act8_grad(P(16), P(16), None, None, P(16), I32(1), I32(0), I64(most), P(16), None,
+                            None, None) == -1
+    for n, width in ((2 ** 31 - 1, 2 ** 33), (2 ** 31 - 1, 2 ** 34), (2 ** 30, 2 ** 34 + 2)):
+        assert lib.ms_act8(ref(Rows(16, n, width, n, 0, width, 1, 0)), None, I32(0), P(16), P(16),
+                           P(16), None, None, None) == -1
+    ids = Tokens(16, 4, 4, 0, 1, 1, 0)
+    for vocab, width in ((2 ** 31 - 1, 2 ** 32), (2 ** 31 - 1, 2 ** 33), (5, 2 ** 61), (5, 2 ** 62),
+                         (1, most)):
+        assert lib.ms_embedding_grad_workspace(4, vocab, width) == -1
+        assert lib.ms_embedding_grad(ref(ids), ref(Rows(16, 4, width, 4, 0, width, 1, 0)), I64(vocab),
+                                     F(1), I64(-1), P(16), P(16), I64(most), None) == -1
+        assert lib.ms_embedding(ref(ids), ref(Rows(16, vocab, width, vocab, 0, width, 1, 0)), F(1),
+                                P(16), None) == -1
+    many = Tokens(16, 2 ** 31 - 1, 2 ** 31 - 1, 0, 1, 1, 0)
+    assert lib.ms_embedding(ref(many), ref(Rows(16, 1, 2 ** 34, 1, 0, 0, 1, 0)), F(1), P(16),
+                            None) == -1
