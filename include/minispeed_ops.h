@@ -16,7 +16,8 @@
  *     launch.  ms_ops_error_string() names both kinds.
  *   - The same call gives the same bits: no floating-point atomics, every sum
  *     in a fixed order.  (That of a row of logits follows from the row's
- *     address modulo 16; nothing else depends on addresses.)
+ *     address modulo 16, and of its gradient's where lse is beyond +-256; nothing
+ *     else depends on addresses.)
  *   - Row-strided operands are given as (inner, outer_stride, inner_stride):
  *     row r starts at (r / inner) * outer_stride + (r % inner) * inner_stride
  *     elements; elements of a row are consecutive.  Token lists are the same

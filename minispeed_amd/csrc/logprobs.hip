@@ -886,6 +886,7 @@ __global__ void __launch_bounds__(kShortThreads)
 constexpr float kFarLse = 256.f;
 
 constexpr int kGradThreads = 256, kGradWaves = kGradThreads / kWave;
+constexpr int kFarUnits = 4;              // units to a thread in flight, rows beyond kFarLse
 constexpr int kGradGroup = 1;             // 16-byte units to a thread; 1, 2, 4: 263, 280, 290 us
 
 // A block takes kGradGroup rounds of aligned 16-byte units of the gradient's row
@@ -944,8 +945,57 @@ __global__ void __launch_bounds__(kGradThreads)
   const float h = kEntropy ? grad_entropy[r] : 0.f, big_h = kEntropy ? entropy[r] : 0.f;
   const float l = lse[r];
 
-  if (l == -INFINITY || fabsf(l) > kFarLse) {
-    // every block of the row finds the maximum and the sum for itself
+  if (l == -INFINITY) {
+    // the first block takes the head too, the last one what is behind the units; with
+    // the head before them the last block but one may already reach the row's end
+    const int begin = part ? head + part * kEach * kVec : 0;
+    const int behind = head + (part + 1) * kEach * kVec;
+    const int end = part == blocks_per_row - 1 || behind > vocab ? vocab : behind;
+    for (int j = begin + tid; j < end; j += kGradThreads) {
+      const float v = widen(x[j]);
+      d[j] = narrow<T>(v != v ? v : 0.f);              // a NaN says so whatever lse is
+    }
+    return;
+  }
+  // the value of this thread before or behind the units, if `head` and `rest` are the block's
+  const int alone_head = tid < head ? tid : -1;
+  const int alone_rest = tid >= kVec && tid - kVec < rest ? head + units * kVec + tid - kVec : -1;
+  if (fabsf(l) > kFarLse) {
+    // One block for the whole row: the maximum and the sum first, then the gradient.
+    // 8192 x 50257 fp16, all rows so 496 us, one of them 317, none 266; where every block
+    // of a row went through all of it 13250 us and 340.
+    if (part) return;
+    const int alone = alone_head >= 0 ? alone_head : alone_rest;
+    const float single = alone >= 0 ? widen(x[alone]) : -INFINITY;
+    auto load_far = [&](int u0, Words (&w)[kFarUnits]) {
+#pragma unroll
+      for (int i = 0; i < kFarUnits; ++i) {
+        const int u = u0 + i * kGradThreads + tid;
+        w[i] = *reinterpret_cast<const AnyWords*>(
+            x + head + static_cast<int64_t>(u < units ? u : units - 1) * kVec);
+      }
+#pragma unroll
+      for (int i = 0; i < kFarUnits; ++i)
+        if (u0 + i * kGradThreads + tid >= units) w[i] = no_values<T>();
+    };
+    float most = single, s = single == -INFINITY ? 0.f : 1.f;
+    if (single != single || single == INFINITY) s = quiet_nan();
+    for (int u0 = 0; u0 < units; u0 += kFarUnits * kGradThreads) {
+      Words w[kFarUnits];
+      load_far(u0, w);
+      Largest<T> largest;
+#pragma unroll
+      for (int i = 0; i < kFarUnits; ++i) largest.see(values_of<T>(w[i]));
+      const float to = fmaxf(most, largest.get());
+      if (to > most) s *= exp2_fast((most - to) * kLog2e);
+      most = to;
+      const float base = most == -INFINITY ? 0.f : most;
+#pragma unroll
+      for (int i = 0; i < kFarUnits; ++i)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          s += exp2_fast((widen(values_of<T>(w[i]).v[j]) - base) * kLog2e);
+    }
     auto block = [&](float v, auto op) {
       __syncthreads();
       if ((tid & 63) == 0) slot[tid >> 6] = v;
@@ -954,31 +1004,30 @@ __global__ void __launch_bounds__(kGradThreads)
       for (int w = 1; w < kGradWaves; ++w) y = op(y, slot[w]);
       return y;
     };
-    float most = 0.f, s = 1.f;
-    if (l != -INFINITY) {
-      most = -INFINITY;
-      for (int j = tid; j < vocab; j += kGradThreads) most = fmaxf(most, widen(x[j]));
-      most = block(wave_max(most), [](float a, float b) { return fmaxf(a, b); });
-      s = 0.f;
-      for (int j = tid; j < vocab; j += kGradThreads)
-        s += exp2_fast((widen(x[j]) - most) * kLog2e);
-      s = block(wave_sum(s), [](float a, float b) { return a + b; });
-    }
-    const float ls = log2_fast(s) * kLn2;
-    // the first block takes the head too, the last one what is behind the units; with
-    // the head before them the last block but one may already reach the row's end
-    const int begin = part ? head + part * kEach * kVec : 0;
-    const int behind = head + (part + 1) * kEach * kVec;
-    const int end = part == blocks_per_row - 1 || behind > vocab ? vocab : behind;
-    for (int j = begin + tid; j < end; j += kGradThreads) {
-      const float v = widen(x[j]);
-      float dj = v != v ? v : 0.f;                     // a NaN says so whatever lse is
-      if (l != -INFINITY) {
-        const float logp = (v - most) - ls, p = exp2_fast(logp * kLog2e);
-        dj = j == hit ? g - g * p : -g * p;
-        if (kEntropy && p != 0.f) dj -= h * p * (logp + big_h);
+    const float mine = most;
+    most = block(wave_max(most), [](float a, float b) { return fmaxf(a, b); });
+    s *= exp2_fast((mine - most) * kLog2e);
+    const float ls =
+        log2_fast(block(wave_sum(s), [](float a, float b) { return a + b; })) * kLn2;
+    auto one = [&](float v, int j) {
+      const float logp = (v - most) - ls, p = exp2_fast(logp * kLog2e);
+      float dj = j == hit ? g - g * p : -g * p;
+      if (kEntropy && p != 0.f) dj -= h * p * (logp + big_h);
+      return narrow<T>(dj);
+    };
+    if (alone >= 0) d[alone] = one(single, alone);
+    for (int u0 = 0; u0 < units; u0 += kFarUnits * kGradThreads) {
+      Words w[kFarUnits];
+      load_far(u0, w);
+#pragma unroll
+      for (int i = 0; i < kFarUnits; ++i) {
+        const int u = u0 + i * kGradThreads + tid, j0 = head + u * kVec;
+        if (u >= units) continue;
+        Pack<T, kVec> z;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) z.v[j] = one(widen(values_of<T>(w[i]).v[j]), j0 + j);
+        store_stream<kVec>(d + j0, z);
       }
-      d[j] = narrow<T>(dj);
     }
     return;
   }
@@ -1001,11 +1050,9 @@ __global__ void __launch_bounds__(kGradThreads)
       store_stream<kVec>(d + head + static_cast<int64_t>(u) * kVec, z);
     }
   }
-  // the values before and behind the units
-  const int alone = part == 0 && tid < head ? tid
-                    : part == blocks_per_row - 1 && tid >= kVec && tid - kVec < rest
-                        ? head + units * kVec + tid - kVec
-                        : -1;
+  const int alone = part == 0 && alone_head >= 0           ? alone_head
+                    : part == blocks_per_row - 1 ? alone_rest
+                                                 : -1;
   if (alone >= 0) d[alone] = narrow<T>(one(widen(x[alone])) + (alone == hit ? g : 0.f));
 }
 

@@ -304,6 +304,26 @@ def test_gradient_stays_within_its_rows(dtype, v, fill):
     assert torch.allclose(d[:, 0], torch.full_like(d[:, 0], 1.0 - p if p else 0.0), rtol=0.01)
 
 
+def test_gradient_of_rows_far_from_zero_is_no_order_slower():
+    """Logits that share a large offset cost a pass more, not one for every block of a row."""
+    n, v = 2048, 50257
+    near, t = _logits(n, v, "bf16", 64), _targets(n, v, 65)
+    far = (near.float() + 4096.0).to(near.dtype)
+    g, us = torch.ones(n, device=DEV), []
+    for x in (near, far):
+        lse = ms.ops.token_logprobs(x, t).lse
+        times = []
+        for _ in range(5):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            ms.ops.token_logprobs_grad(x, t, lse, g)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        us.append(min(times))
+    assert us[1] < 8 * us[0], us
+
+
 def test_targets_outside_the_vocabulary():
     x = _logits(5, 100, "bf16", 13)
     t = torch.tensor([100, -1, 7, 2 ** 40, -100], device=DEV)
