@@ -55,7 +55,7 @@ constexpr bool kFineOf = sizeof(T) == 4 || K == MS_ACT_SWIGLU;
 // rounded by itself, is 4e-7 for m of some units and 1e-6 from 50 on.
 template <bool kFine>
 __device__ __forceinline__ float lifted_exp2(float hi, float lo, float l, float l_lo) {
-  if (!kFine) return __builtin_amdgcn_exp2f(fmaf(hi, -l, kLift));
+  if (!kFine) return __builtin_amdgcn_exp2f(hi * -l + kLift);
   const float n = rintf(hi * -l);
   const float part = fmaf(hi, -l_lo, fmaf(lo, -l, fmaf(hi, -l, -n)));
   return ldexpf(__builtin_amdgcn_exp2f(part), static_cast<int>(n) + static_cast<int>(kLift));
@@ -89,21 +89,36 @@ __device__ __forceinline__ Act logistic_act(float x, float z, float dz) {
 template <int K, bool kFine>
 __device__ __forceinline__ Act act(float x) {
   if (K == MS_ACT_GELU) {
-    // Phi(-a) = exp(-a^2 / 2) Q(a), Q = erfcx(a / sqrt 2) / 2 = r P(a r) with
-    // r = 1 / (a + 3.75): P by a weighted fit (least squares, reweighted towards the
-    // least largest relative error, 4e-8 with these coefficients) over [0, 15].  Near 0
-    // only its first terms count; the tail needs no difference.
+    // Phi(-a) = exp(-a^2 / 2) Q(a), Q = erfcx(a / sqrt 2) / 2, by weighted fits over
+    // [0, 15] (least squares, reweighted towards the least largest relative error), so that
+    // the tail needs no difference.  Fine: r P(a r) with r = 1 / (a + 3.75), 4e-8; near 0
+    // only P's first terms count.  Else t P(t) with t = 1 / (1 + 0.37 a), 2e-7, 5e-7 as
+    // evaluated, one operation fewer: 8192 x 8192 bf16 forward 57 us, 59 with the other.
     const float a = __builtin_elementwise_minimum(fabsf(x), 15.f);      // NaN stays
-    const float r = __builtin_amdgcn_rcpf(a + 3.75f), u = a * r;
-    float q = 0.113523148f;
-    q = fmaf(q, u, -0.388860106f);
-    q = fmaf(q, u, 0.299531192f);
-    q = fmaf(q, u, 0.386662275f);
-    q = fmaf(q, u, -0.285418391f);
-    q = fmaf(q, u, -1.70484757f);
-    q = fmaf(q, u, 3.83854222f);
-    q = fmaf(q, u, -3.7351315f);
-    q = fmaf(q, u, 1.875f) * r;
+    float q;
+    if (kFine) {
+      const float r = __builtin_amdgcn_rcpf(a + 3.75f), u = a * r;
+      q = 0.113523148f;
+      q = fmaf(q, u, -0.388860106f);
+      q = fmaf(q, u, 0.299531192f);
+      q = fmaf(q, u, 0.386662275f);
+      q = fmaf(q, u, -0.285418391f);
+      q = fmaf(q, u, -1.70484757f);
+      q = fmaf(q, u, 3.83854222f);
+      q = fmaf(q, u, -3.7351315f);
+      q = fmaf(q, u, 1.875f) * r;
+    } else {
+      const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.37f, 1.f));
+      q = -0.0313271917f;
+      q = fmaf(q, t, 0.135133371f);
+      q = fmaf(q, t, -0.194299534f);
+      q = fmaf(q, t, 0.0645160899f);
+      q = fmaf(q, t, 0.0134064732f);
+      q = fmaf(q, t, 0.0901831239f);
+      q = fmaf(q, t, 0.127163798f);
+      q = fmaf(q, t, 0.147615328f);
+      q = fmaf(q, t, 0.147608608f) * t;
+    }
     const float a2 = a * a;
     const float e =                                                     // log2 e / 2
         lifted_exp2<kFine>(a2, fmaf(a, a, -a2), 0.721347511f, 9.62981495e-9f);
