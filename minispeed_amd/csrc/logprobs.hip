@@ -740,20 +740,22 @@ __device__ __forceinline__ int wave_count(int x) {
   return uniform(x);
 }
 
-// The `top` first of a row in key order, into `list`, whatever it holds: of the
-// values that equal the last one those with the lowest indices.  At least `top`
-// values are as large as `least`.  (The row is read again for each step: its words
-// taken apart in registers cost every row its place.)
+// The `top` first of a row in key order, into `list`, whatever it holds, and perhaps
+// others, kShortList at most; how many.  Of the values that equal the last one those with
+// the lowest indices.  At least `top` values are as large as `least`.  (The row is read again
+// for each step: its words taken apart in registers cost every row its place.)
 template <typename T>
-__device__ __forceinline__ void list_exactly(const T* x, int vocab, int lane, int top,
-                                             uint32_t least, Key* list) {
+__device__ __forceinline__ int list_exactly(const T* x, int vocab, int lane, int top,
+                                            uint32_t least, Key* list) {
   auto count = [&](auto test) {
     int n = 0;
     for (int j = lane; j < vocab; j += kWave) n += test(order_of(widen(x[j])));
     return wave_count(n);
   };
   int above = count([&](uint32_t o) { return o > least; });
-  if (above >= top) {
+  // (a mask that leaves little has that little in few lanes: `least` is what is masked, and
+  // what is above fits the list.  With the search for it a row took 116 us.)
+  if (above > kShortList) {
     uint32_t bound = 0;                       // the largest word that `top` are as large as
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t more = bound | 1u << bit;
@@ -762,6 +764,7 @@ __device__ __forceinline__ void list_exactly(const T* x, int vocab, int lane, in
     least = bound;
     above = count([&](uint32_t o) { return o > least; });
   }
+  const int missing = above < top ? top - above : 0;      // of those that equal `least`
   int to = 0, equal = 0;
   const uint64_t lower = (1ull << lane) - 1;
   for (int j0 = 0; j0 < vocab; j0 += kWave) {
@@ -769,13 +772,14 @@ __device__ __forceinline__ void list_exactly(const T* x, int vocab, int lane, in
     const float v = j < vocab ? widen(x[j]) : 0.f;
     const uint32_t o = j < vocab ? order_of(v) : 0;
     const uint64_t same = __ballot(j < vocab && o == least);
-    const bool in = j < vocab && (o > least || (o == least && equal + __popcll(same & lower) <
-                                                                   top - above));
+    const int before = equal + static_cast<int>(__popcll(same & lower));
+    const bool in = j < vocab && (o > least || (o == least && before < missing));
     const uint64_t all = __ballot(in);
     if (in) list[to + __popcll(all & lower)] = key_of(v, j);
     to += __popcll(all);
     equal += __popcll(same);
   }
+  return to;
 }
 
 template <typename T, int R, bool kTop, bool kEntropy>
@@ -832,8 +836,11 @@ __global__ void __launch_bounds__(kShortThreads)
       constexpr int kSkip = sizeof(T) == 2 ? 13 : 0;
       Key* list = lists[wave];
       const bool unit = lane < row.units;
-      const uint32_t least = kth_largest<kSkip>(unit || row.alone >= 0 ? order_of(mine) : 0,
-                                                unit ? order_of(other) : 0, out.top);
+      uint32_t least = kth_largest<kSkip>(unit || row.alone >= 0 ? order_of(mine) : 0,
+                                          unit ? order_of(other) : 0, out.top);
+      // the last bits of a 2-byte type's word, which are not searched, are 1 in a negative
+      // value's: without them all of a masked row's values would lie above
+      if (least && !(least >> 31)) least |= (1u << kSkip) - 1;
       int found = kShortList + 1;
       if (least == 0 && vocab <= kShortList) {           // fewer than that: all of them
         for (int j = lane; j < vocab; j += kWave) list[j] = key_of(widen(x[j]), j);
@@ -857,8 +864,7 @@ __global__ void __launch_bounds__(kShortThreads)
         found = to;
       }
       if (found > kShortList) {
-        list_exactly(x, vocab, lane, out.top, least, list);
-        found = out.top;
+        found = list_exactly(x, vocab, lane, out.top, least, list);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();

@@ -324,6 +324,31 @@ def test_gradient_of_rows_far_from_zero_is_no_order_slower():
     assert us[1] < 8 * us[0], us
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_alternatives_of_short_rows_with_little_left(dtype):
+    """Rows that a mask leaves nothing, or less than there are alternatives: the first
+    indices of what is masked follow, in a pass or two over the row."""
+    n, v = 8, 3001
+    plain, t = _logits(n, v, dtype, 66), _targets(n, v, 67)
+    x = plain.clone()
+    x[3], x[4, 7:], x[5, : v - 9] = -INF, -INF, torch.finfo(x.dtype).min
+    x[6], x[7, ::2] = -1.5, -INF
+    for top in (1, 4, 5, 7, 8, 20, 64):
+        check(x, t, top=top)
+    us = []
+    for z in (plain, x):
+        times = []
+        for _ in range(20):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            ms.ops.token_logprobs(z, t, top=5)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        us.append(1e3 * min(times))
+    assert us[1] < us[0] + 60.0, us
+
+
 def test_targets_outside_the_vocabulary():
     x = _logits(5, 100, "bf16", 13)
     t = torch.tensor([100, -1, 7, 2 ** 40, -100], device=DEV)
