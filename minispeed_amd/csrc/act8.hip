@@ -41,13 +41,13 @@ struct Act {
 // the far tails are right down to the smallest denormal.
 constexpr float kLift = 32.f, kDrop = 2.3283064e-10f;   // 2^-32
 
-// kFine in what follows: for results of 32 bits, and for swiglu, where it costs nothing
-// (4096 x 14336 bf16 backward 96 us either way) and its products come closer to the
-// nearest 2-byte values.  Other 2-byte results hide it, and it costs: 8192 x 8192 fp16,
+// kFine in what follows: for results of 32 bits, and in swiglu's backward pass, where it
+// costs nothing (4096 x 14336 bf16 96 us either way) and its products of three come closer to
+// the nearest 2-byte values.  Other 2-byte results hide it, and it costs: 8192 x 8192 fp16,
 // forward and backward, gelu 77 and 83 us, 63 and 78 without; gelu_tanh 66 and 83, 56 and 78; silu
-// 58 and 79, 56 and 79.
-template <typename T, int K>
-constexpr bool kFineOf = sizeof(T) == 4 || K == MS_ACT_SWIGLU;
+// 58 and 79, 56 and 79; swiglu forward 88 and 87, of views 109 and 102.
+template <typename T, int K, bool kBackward>
+constexpr bool kFineOf = sizeof(T) == 4 || (kBackward && K == MS_ACT_SWIGLU);
 
 // 2^(32 - m L) for m = hi + lo >= 0 and L = l + l_lo.  Fine: of the exponent's
 // whole and broken parts only the second goes through v_exp_f32, so that its rounding
@@ -420,7 +420,7 @@ __device__ __forceinline__ void act8_block(ms_rows_t h, ms_rows_t up, T* a, int8
     for (int j = 0; j < N; ++j) v[j] = widen(x[k].v[j]);
     hold<kWhole, T>(x[k], v, i, n, codes, exponents);
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = act<K, kFineOf<T, K>>(v[j]).f;
+    for (int j = 0; j < N; ++j) f[j] = act<K, kFineOf<T, K, false>>(v[j]).f;
     if constexpr (kGated) {
 #pragma unroll
       for (int j = 0; j < N; ++j) v[j] = widen(u[k].v[j]);
@@ -467,7 +467,7 @@ __device__ __forceinline__ void act8_grad_block(const int8_t* codes, const uint8
     if constexpr (kGated) decode(uc[k], step_of(ue[k]), u);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const Act y = act<K, kFineOf<T, K>>(x[j]);
+      const Act y = act<K, kFineOf<T, K, true>>(x[j]);
       const float gj = widen(g[k].v[j]);
       if constexpr (kGated) {
         d[j] = gj * u[j] * y.df;
