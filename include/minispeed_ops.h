@@ -96,8 +96,8 @@ int ms_embedding(const ms_tokens_t* ids, const ms_rows_t* table, float scale,
  * Its gradient: dtable[v, :] = scale * sum over the tokens t with id_t = v, in
  * increasing t, of grad[t, :]; dtable is dense [vocab, width] of the
  * gradient's type and written whole (rows without tokens are zeros).  Sums
- * are fp32 in an order that depends on the ids alone, multiplied by scale
- * and rounded once.  Ids outside [0, vocab) and `padding_idx` (-1: none) add
+ * are fp32 in an order that follows from the ids, the sizes and the type, and
+ * is the same for every column; they are multiplied by scale and rounded once.  Ids outside [0, vocab) and `padding_idx` (-1: none) add
  * nothing.  dtable is 16-byte aligned; at most 2^30 tokens.
  */
 int64_t ms_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t width);
@@ -130,7 +130,9 @@ int ms_logprobs(const ms_rows_t* logits, const ms_tokens_t* targets, int64_t ign
  * NULL) and h = grad_entropy (NULL: 0; then `entropy` is not read).  lse and entropy are
  * those that ms_logprobs gave.  Rows of -inf get zeros, a NaN logit NaN
  * whatever lse is; a target outside
- * [0, vocab) that is not ignore_index makes g NaN.
+ * [0, vocab) that is not ignore_index makes g NaN.  A row whose lse is beyond
+ * +-256 costs another pass over its logits: its maximum and sum are found again,
+ * as an fp32 lse no longer tells them from each other.
  */
 int ms_logprobs_grad(const ms_rows_t* logits, const ms_tokens_t* targets, int64_t ignore_index,
                      const float* lse, const float* entropy, const float* grad_logprob,

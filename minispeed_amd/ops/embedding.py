@@ -55,8 +55,8 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: floa
 
     ``grad`` (``[*ids.shape, width]``) is the gradient of the embedding's output.
     Row ``v`` is ``scale`` times the sum of the rows of ``grad`` whose id is
-    ``v``, added in 32 bits in an order that depends on ``ids`` alone, and
-    rounded once: the same inputs give the same bits.  The whole table is
+    ``v``, added in 32 bits in an order that follows from ``ids``, the sizes and
+    the type, and rounded once: the same inputs give the same bits.  The whole table is
     written; rows without tokens are zeros.
     """
     return _native.embedding_grad(grad, ids, rows, scale, _padding(padding_idx, rows))

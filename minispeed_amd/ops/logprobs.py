@@ -52,7 +52,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
     64) the ``k`` likeliest tokens as ``top_logprob`` and ``top_id``, in falling
     order, equal ones by rising index.  ``logprob`` and ``entropy`` are
     differentiable, so that ``-token_logprobs(logits, targets).logprob.mean()`` is
-    a cross-entropy loss.
+    a cross-entropy loss.  ``lse`` and the alternatives are not: a loss on them adds
+    nothing to the gradients.  (``logits.gather(-1, targets[..., None])[..., 0] - logprob``
+    is an ``lse`` that has a gradient.)
 
     A row that a mask left nothing (all ``-inf``) has log probability ``-inf``,
     entropy 0 and a gradient of zeros.  A row with NaN or ``+inf`` gives NaN, and
