@@ -173,6 +173,36 @@ int ms_act8_grad(const int8_t* codes, const uint8_t* exponents, const int8_t* up
                  const uint8_t* up_exponents, const void* grad, int32_t dtype, int32_t kind,
                  int64_t n, void* dh, void* dup, void* a, void* stream);
 
+/*
+ * Log probabilities of given tokens under softmax(x), x = scale * hidden * weight^T, without
+ * the logits x ever being stored.  `hidden` [n, width] and `weight` [vocab, width] have one
+ * element type, width 1 to 2^20, vocab >= 1.  Outputs as of ms_logprobs, fp32, dense:
+ * lse, and logprob (0 where target == ignore_index, NaN where it is outside of [0, vocab)).
+ * A token whose logits hold NaN or +inf has NaN in both, one whose logits are all -inf
+ * has -inf in both.
+ */
+int64_t ms_linear_logprobs_workspace(const ms_rows_t* hidden, const ms_rows_t* weight);
+int ms_linear_logprobs(const ms_rows_t* hidden, const ms_rows_t* weight,
+                       const ms_tokens_t* targets, float scale, int64_t ignore_index,
+                       float* logprob, float* lse, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
+/*
+ * Its gradients, dense, of the operands' type:
+ *   d = g 1[v = target] + (l - g) exp(x - lse),  dhidden = scale d weight,
+ *   dweight = scale d^T hidden
+ * with g = grad_logprob (0 where target == ignore_index, and where NULL) and l = grad_lse
+ * (0 where NULL); lse is the forward pass's.  dhidden or dweight may be NULL: not
+ * computed.  d is rounded to the operands' type (three times, for fp32: 24 bits).
+ * Tokens whose lse is -inf, and those with g = l = 0, have d = 0.
+ */
+int64_t ms_linear_logprobs_grad_workspace(const ms_rows_t* hidden, const ms_rows_t* weight);
+int ms_linear_logprobs_grad(const ms_rows_t* hidden, const ms_rows_t* weight,
+                            const ms_tokens_t* targets, float scale, int64_t ignore_index,
+                            const float* lse, const float* grad_logprob, const float* grad_lse,
+                            void* dhidden, void* dweight, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

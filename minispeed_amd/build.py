@@ -32,7 +32,7 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 OUTPUT = os.path.join(PKG_DIR, "libminispeed_boundary.so")
 ARCH = "gfx950"
 OPS_SOURCES = [os.path.join(PKG_DIR, "csrc", f"{name}.hip")
-               for name in ("embedding", "logprobs", "act8")]
+               for name in ("embedding", "logprobs", "act8", "linear")]
 OPS_OUTPUT = os.path.join(PKG_DIR, "libminispeed_ops.so")
 
 # -ffp-contract=off: every a*b+c the kernels do not write as fmaf stays two
@@ -63,7 +63,7 @@ def command(output: str = OUTPUT) -> List[str]:
 
 
 def ops_command(output: str = OPS_OUTPUT) -> List[str]:
-    return [hipcc(), *HIP_FLAGS, "-parallel-jobs=3", f"-I{INCLUDE}", *OPS_SOURCES, "-o", output]
+    return [hipcc(), *HIP_FLAGS, "-parallel-jobs=6", f"-I{INCLUDE}", *OPS_SOURCES, "-o", output]
 
 
 def _compile_hip(cmd: List[str], tmp: str, output: str, verbose: bool) -> str:

@@ -1,0 +1,715 @@
+// Log probabilities of given tokens under softmax(scale * hidden * weight^T),
+// and their gradients, without storing the logits.
+//
+//   x[t, v] = scale * hidden[t] . weight[v],  lse[t] = log sum over v of exp x[t, v]
+//   logprob[t] = x[t, y] - lse[t]
+//   d[t, v] = g[t] 1[v = y] + (l[t] - g[t]) p[t, v],   p = exp(x - lse),
+//             g, l the gradients of logprob and lse
+//   dhidden = scale * d weight,   dweight = scale * d^T hidden
+//
+// Forward, one product (product.h) with the vocabulary along m: its epilogue takes each
+// token's maximum and sum of exponentials over the wave's rows, and a second kernel
+// joins those partial sums.  Backward, the vocabulary is gone through in pieces: the
+// piece's logits are computed again and left as d, in the operands' 16-bit type; then
+// come the two products with d.  Four products' work in all for what needs at least
+// three, and one piece of d (kPiece bytes at most) in place of the logits.
+//
+// Numbers.  Products of 16-bit values are exact in the fp32 sums.  d is rounded once
+// to the operands' type, as the products take it: an error of half an ulp of each
+// term, which the sums average.  In fp16 a row of d is scaled by a power of two that
+// brings its bound to 2^14 (p reaches down to 2^-20 over large vocabularies, and g is
+// an inverse count of tokens); dhidden's rows are scaled back, and dweight takes its
+// scales from a copy of hidden multiplied by them, exactly but for underflow of
+// rows whose gradients are 2^14 times smaller than the largest.
+// 32-bit operands are split into three bf16 planes of 8 bits each (x = a + b + c,
+// exactly), and six products of planes are summed; what is left out is below 2^-22 of
+// the terms.  The matrix units' own 32-bit products have a sixteenth of the bf16 rate.
+//
+// exp and log are taken in units of log 2.
+#include "product.h"
+
+#include <algorithm>
+
+namespace ops {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int64_t kMaxWidth = 1 << 20;
+constexpr int64_t kPiece = int64_t{256} << 20;     // bytes of d at a time
+
+// What a token's row of d is made of, by k_rows.
+struct __attribute__((aligned(16))) row_t {
+  float lse2;       // lse in units of log 2
+  float soft;       // (l - g) * up: the factor of p
+  float given;      // g * up: what the token's own column has more
+  float down;       // 1 / up, a power of two
+};
+
+__device__ __forceinline__ float swap_halves(float x) { return __shfl_xor(x, 32); }
+
+// ---------------------------------------------------------------------------
+// Epilogues.  acc[i][j][r] is C[m0 + 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4,
+// n0 + 32 j + lane % 32].
+
+// Per token: maximum and sum over the wave's rows of the vocabulary.
+struct sum_epilogue {
+  float2* parts;       // [part][tokens]: maximum in units of log 2, sum relative to it
+  float* picked;       // [tokens]: the given token's logit
+  ms_tokens_t targets;
+  float scale;
+
+  template <int MI, int NI>
+  __device__ void store(const f32x16 (&acc)[MI][NI], int m0, int n0, int part, int, int lane, int m,
+                        int n) const {
+    const int half = 4 * (lane >> 5), left = m - m0;
+    const float unit = scale * kLog2e;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int t = n0 + j * 32 + (lane & 31);
+      const int64_t y = t < n ? token(targets, t) - m0 : -1;
+      if (y >= 0 && y < MI * 32 && (static_cast<int>(y) & 4) == half) {
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (i * 32 + 8 * (r / 4) + half + r % 4 == y) x = acc[i][j][r];
+        picked[t] = x * scale;
+      }
+      // the scale can be negative, so the largest product need not be the largest logit
+      float most = -__builtin_inff(), sum = 0.0f;
+      if (left >= MI * 32) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, acc[i][j][r] * unit);
+        most = fmaxf(most, swap_halves(most));
+        const float base = most == -__builtin_inff() ? 0.0f : most;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], unit, -base));
+      } else {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (i * 32 + 8 * (r / 4) + half + r % 4 < left) most = fmaxf(most, acc[i][j][r] * unit);
+        most = fmaxf(most, swap_halves(most));
+        const float base = most == -__builtin_inff() ? 0.0f : most;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (i * 32 + 8 * (r / 4) + half + r % 4 < left)
+              sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], unit, -base));
+      }
+      sum += swap_halves(sum);
+      if (lane < 32 && t < n) parts[static_cast<int64_t>(part) * n + t] = make_float2(most, sum);
+    }
+  }
+};
+
+// A piece's columns of d: d[t, m], dense rows of ld elements; planes of bf16 for fp32.
+template <typename T, int Planes>
+struct soft_epilogue {
+  T* d;
+  int64_t ld, plane;
+  const row_t* rows;
+  ms_tokens_t targets;
+  float scale;
+  int32_t first;         // the piece's first token of the vocabulary
+
+  template <int MI, int NI>
+  __device__ void store(const f32x16 (&acc)[MI][NI], int m0, int n0, int, int, int lane, int m,
+                        int n) const {
+    const int half = 4 * (lane >> 5);
+    const float unit = scale * kLog2e;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int t = n0 + j * 32 + (lane & 31);
+      if (t >= n) continue;
+      const row_t row = rows[t];
+      const int64_t y = token(targets, t) - first - m0;
+      T* out = d + t * ld + m0 + half;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          Pack<T, 4> o[Planes];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = i * 32 + q * 8 + e;
+            float v = __builtin_amdgcn_exp2f(fmaf(acc[i][j][q * 4 + e], unit, -row.lse2)) * row.soft;
+            if (at + half == y) v += row.given;
+            if (row.soft == 0.0f && row.given == 0.0f) v = 0.0f;
+            if (m0 + at + half >= m) v = 0.0f;
+#pragma unroll
+            for (int s = 0; s < Planes; ++s) {
+              o[s].v[e] = narrow<T>(v);
+              v -= widen(o[s].v[e]);
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < Planes; ++s) store_words(out + s * plane + i * 32 + q * 8, o[s]);
+        }
+    }
+  }
+
+  __device__ static void store_words(T* p, const Pack<T, 4>& x) {
+    typedef uint32_t raw __attribute__((ext_vector_type(2)));
+    raw r;
+    __builtin_memcpy(&r, &x, 8);
+    *reinterpret_cast<raw*>(p) = r;
+  }
+};
+
+// out[n, m]: final values of type T, or fp32 partial sums, one buffer for each split.
+template <typename T>
+struct out_epilogue {
+  T* out;                // final where `parts` is null
+  float* parts;          // [split][n][m]
+  const row_t* rows;     // final: each n's factor, or null
+  const float* factor;   // final: one factor, or null
+  float scale;
+  int32_t add;           // parts: to what is there
+
+  template <int MI, int NI>
+  __device__ void store(const f32x16 (&acc)[MI][NI], int m0, int n0, int, int split, int lane, int m,
+                        int n) const {
+    const int half = 4 * (lane >> 5);
+    const float all = factor ? *factor * scale : scale;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int t = n0 + j * 32 + (lane & 31);
+      if (t >= n) continue;
+      const float by = rows ? rows[t].down * all : all;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int at = m0 + i * 32 + q * 8 + half;
+          if (at >= m) continue;
+          if (parts) {
+            float* p = parts + (static_cast<int64_t>(split) * n + t) * m + at;
+            if (at + 4 <= m) {
+              Pack<float, 4> x;
+              if (add) x = load<4>(p);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x.v[e] = (add ? x.v[e] : 0.0f) + acc[i][j][q * 4 + e];
+              store_any(p, x);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (at + e < m) p[e] = (add ? p[e] : 0.0f) + acc[i][j][q * 4 + e];
+            }
+          } else {
+            T* p = out + static_cast<int64_t>(t) * m + at;
+            Pack<T, 4> x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.v[e] = narrow<T>(acc[i][j][q * 4 + e] * by);
+            if (at + 4 <= m) {
+              store_any(p, x);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (at + e < m) p[e] = x.v[e];
+            }
+          }
+        }
+    }
+  }
+  template <typename U>
+  __device__ static void store_any(U* p, const Pack<U, 4>& x) { ops::store<4>(p, x); }
+};
+
+// ---------------------------------------------------------------------------
+// Around the products.
+
+// Joins a token's partial sums.  `lanes` threads (a power of two up to 256) to a token.
+__global__ __launch_bounds__(256) void k_join(const float2* parts, const float* picked, int64_t count,
+                                              int64_t n, int lanes, ms_tokens_t targets, int64_t vocab,
+                                              int64_t ignore_index, float* logprob, float* lse) {
+  __shared__ float2 held[256];
+  const int each = 256 / lanes, which = threadIdx.x % each, lane = threadIdx.x / each;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * each + which;
+  float most = -__builtin_inff(), sum = 0.0f;
+  if (t < n) {
+    for (int64_t k = lane; k < count; k += lanes) {
+      const float2 x = parts[k * n + t];
+      const float top = fmaxf(most, x.x), base = top == -__builtin_inff() ? 0.0f : top;
+      sum = sum * __builtin_amdgcn_exp2f(most - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
+      most = top;
+    }
+  }
+  held[threadIdx.x] = make_float2(most, sum);
+  for (int step = lanes / 2; step; step /= 2) {
+    __syncthreads();
+    if (lane < step) {
+      const float2 x = held[threadIdx.x + step * each];
+      const float top = fmaxf(most, x.x), base = top == -__builtin_inff() ? 0.0f : top;
+      sum = sum * __builtin_amdgcn_exp2f(most - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
+      most = top;
+      held[threadIdx.x] = make_float2(most, sum);
+    }
+  }
+  if (lane == 0 && t < n) {
+    const float base = most == -__builtin_inff() ? 0.0f : most;
+    const float l = (base + __builtin_amdgcn_logf(sum)) * kLn2;
+    const int64_t y = token(targets, t);
+    float p;
+    if (y == ignore_index) {
+      p = 0.0f;
+    } else if (y < 0 || y >= vocab) {
+      p = quiet_nan();
+    } else {
+      p = l == -__builtin_inff() ? l : picked[t] - l;
+    }
+    logprob[t] = p;
+    lse[t] = l;
+  }
+}
+
+// The exponent of a row's bound on |d|, such that bound * 2^up < 2^15; 0 for zero rows.
+__device__ __forceinline__ int lift(float bound) {
+  const int e = static_cast<int>(__float_as_uint(bound) >> 23 & 255);
+  // (the smallest numbers, infinities and NaN are left as they are)
+  return e == 0 || e == 255 ? 0 : min(max(14 + 127 - e, -100), 100);
+}
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((e + 127) << 23); }
+
+// Row numbers for the backward pass.  With `lifted` (fp16) one block does all rows and
+// leaves the least power of two of any row's scale in factor[0].
+__global__ __launch_bounds__(1024) void k_rows(const float* lse, const float* grad_logprob,
+                                               const float* grad_lse, ms_tokens_t targets,
+                                               int64_t vocab, int64_t ignore_index, int lifted,
+                                               row_t* rows, float* factor) {
+  __shared__ int least[16];
+  int low = 100;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; t < targets.n;
+       t += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t y = token(targets, t);
+    float g = grad_logprob && y != ignore_index ? grad_logprob[t] : 0.0f;
+    float l = grad_lse ? grad_lse[t] : 0.0f;
+    const float of = lse[t];
+    if (y != ignore_index && (y < 0 || y >= vocab) && grad_logprob) g = quiet_nan();
+    if (of == -__builtin_inff()) g = l = 0.0f;
+    const float soft = l - g;
+    int up = 0;
+    if (lifted) {
+      const float bound = fabsf(soft) + fabsf(g);
+      up = lift(bound);
+      if (bound > 0.0f) low = min(low, up);
+    }
+    rows[t] = {of == -__builtin_inff() ? 0.0f : of * kLog2e, soft * pow2(up), g * pow2(up), pow2(-up)};
+  }
+  if (!lifted) return;
+#pragma unroll
+  for (int s = 32; s; s /= 2) low = min(low, __shfl_xor(low, s));
+  if ((threadIdx.x & 63) == 0) least[threadIdx.x >> 6] = low;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (unsigned w = 0; w < blockDim.x / 64; ++w) low = min(low, least[w]);
+    factor[0] = pow2(-low);
+  }
+}
+
+// A matrix as the products take it: rows at `ld`, zeros behind `width`; times a row's
+// scale relative to the largest (fp16), or as three planes (fp32).
+template <typename T>
+__global__ __launch_bounds__(256) void k_layout(ms_rows_t from, int64_t ld, const row_t* rows,
+                                                const float* factor, T* to) {
+  const int64_t chunks = ld / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= from.n * chunks) return;
+  const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+  const T* p = static_cast<const T*>(from.data) + row_start(from, r) + c;
+  Pack<T, 8> x;
+  if (c + 8 <= from.width) {
+    x = load<8>(p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.v[e] = c + e < from.width ? p[e] : static_cast<T>(0.0f);
+  }
+  if (rows) {
+    // a row without a gradient keeps the scale 1 that it was given: its d is zero
+    const float by = rows[r].soft == 0.0f && rows[r].given == 0.0f ? 1.0f : rows[r].down / *factor;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.v[e] = narrow<T>(widen(x.v[e]) * by);
+  }
+  ops::store<8>(to + r * ld + c, x);
+}
+
+// Three planes of bf16: the leading 8 bits of each value, the next 8, the rest.  Cut off
+// instead of rounded, so that nothing overflows and the rest is exact.
+__global__ __launch_bounds__(256) void k_planes(ms_rows_t from, int64_t ld, int64_t plane,
+                                                uint16_t* to) {
+  const int64_t chunks = ld / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= from.n * chunks) return;
+  const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+  const float* p = static_cast<const float*>(from.data) + row_start(from, r) + c;
+  Pack<uint16_t, 8> out[3];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float x = c + e < from.width ? p[e] : 0.0f;
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+      const uint32_t cut = __float_as_uint(x) & 0xffff0000u;
+      out[s].v[e] = static_cast<uint16_t>(cut >> 16);
+      // (an infinity or NaN has nothing behind it)
+      x = (cut & 0x7f800000u) == 0x7f800000u ? 0.0f : x - __uint_as_float(cut);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < 3; ++s) ops::store<8>(to + s * plane + r * ld + c, out[s]);
+}
+
+// Sums of `count` partial buffers, scaled and rounded.
+template <typename T>
+__global__ __launch_bounds__(256) void k_fold(const float* parts, int count, int64_t n, int64_t width,
+                                              const row_t* rows, const float* factor, float scale,
+                                              T* out) {
+  const int64_t all = n * width;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= all) return;
+  const float by = factor ? *factor * scale : scale;
+  if (i + 4 <= all) {
+    Pack<float, 4> sum = load<4>(parts + i);
+    for (int s = 1; s < count; ++s) {
+      const Pack<float, 4> x = load<4>(parts + s * all + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum.v[e] += x.v[e];
+    }
+    Pack<T, 4> o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o.v[e] = narrow<T>(sum.v[e] * (rows ? rows[(i + e) / width].down * by : by));
+    ops::store<4>(out + i, o);
+  } else {
+    for (int64_t j = i; j < all; ++j) {
+      float sum = parts[j];
+      for (int s = 1; s < count; ++s) sum += parts[s * all + j];
+      out[j] = narrow<T>(sum * (rows ? rows[j / width].down * by : by));
+    }
+  }
+}
+
+// No tokens: a gradient of zeros.
+__global__ __launch_bounds__(256) void k_zero(uint16_t* to, int64_t n) {
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
+  for (int e = 0; e < 4; ++e, i += 256)
+    if (i < n) to[i] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// Host.
+
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int64_t ceil_div(int64_t x, int64_t by) { return (x + by - 1) / by; }
+
+// How the products' tiles are cut: 256 x 256 by 8 waves, 128 x 128 or 128 x 32 by 4.
+struct Cut {
+  int m, n, wm;
+};
+constexpr Cut kLarge{256, 256, 2}, kMedium{128, 128, 2}, kFew{128, 32, 4};
+
+// The tile for an M x N product: few columns waste what a wide tile computes beyond them;
+// below two large tiles to a CU the medium ones spread better.
+Cut cut_of(int64_t m, int64_t n) {
+  if (n <= 64) return kFew;
+  if (ceil_div(m, 256) * ceil_div(n, 256) < 256) return kMedium;
+  return kLarge;
+}
+
+// Parts of k that give every CU a block, each of 8 steps or more.
+int splits_of(int64_t m, int64_t n, int64_t steps, Cut c) {
+  const int64_t tiles = ceil_div(m, c.m) * ceil_div(n, c.n);
+  const int64_t want = c.m == 256 ? 256 : 512;
+  if (tiles * 2 > want) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(want, tiles), steps / 8)));
+}
+
+template <typename T, Side SA, Side SB, typename E>
+int run_product(Cut c, const product_args& args, const E& epilogue, hipStream_t s) {
+  product_args p = args;
+  p.tiles_m = static_cast<int32_t>(ceil_div(p.a.rows, c.m));
+  p.tiles_n = static_cast<int32_t>(ceil_div(p.b.rows, c.n));
+  const int64_t blocks = int64_t{p.tiles_m} * p.tiles_n * p.splits;
+  const int threads = c.m == 256 ? 512 : 256;
+  if (!fits(blocks, threads)) return MS_OPS_EINVAL;
+  if (c.m == 256) return launch(k_product<T, 256, 256, 2, 4, SA, SB, E>, blocks, threads, s, p, epilogue);
+  if (c.n == 128) return launch(k_product<T, 128, 128, 2, 2, SA, SB, E>, blocks, threads, s, p, epilogue);
+  return launch(k_product<T, 128, 32, 4, 1, SA, SB, E>, blocks, threads, s, p, epilogue);
+}
+
+// Space cut from the workspace, or only counted while `at` is null.
+struct Space {
+  char* at;
+  int64_t used = 0;
+  template <typename T>
+  T* take(int64_t n) {
+    T* p = at ? reinterpret_cast<T*>(at + used) : nullptr;
+    used += round_up(n * static_cast<int64_t>(sizeof(T)), 256);
+    return p;
+  }
+};
+
+bool good_sizes(const ms_rows_t* hidden, const ms_rows_t* weight) {
+  return good_rows(hidden) && good_rows(weight) && hidden->dtype == weight->dtype &&
+         hidden->width == weight->width && hidden->width >= 1 && hidden->width <= kMaxWidth &&
+         weight->n >= 1 && countable(hidden->n, weight->n);
+}
+
+// Whether the products can take the matrix as it lies.
+bool lies_well(const ms_rows_t& m) {
+  return m.dtype != MS_OPS_F32 && m.inner >= m.n && m.inner_stride % 8 == 0 &&
+         m.inner_stride >= m.width && m.inner_stride <= kMaxWidth && m.width % 8 == 0 &&
+         reinterpret_cast<uintptr_t>(m.data) % 16 == 0;
+}
+
+int planes_of(const ms_rows_t& m) { return m.dtype == MS_OPS_F32 ? 3 : 1; }
+int pairs_of(const ms_rows_t& m) { return m.dtype == MS_OPS_F32 ? 6 : 1; }
+
+// The matrix as an operand, laid out in the workspace where it does not lie well.
+operand prepare(const ms_rows_t& m, Space& space, int& rc, hipStream_t s, bool run) {
+  operand o;
+  o.rows = static_cast<int32_t>(m.n);
+  if (lies_well(m)) {
+    o.data = static_cast<const uint16_t*>(m.data);
+    o.ld = m.inner_stride;
+    o.plane = 0;
+    return o;
+  }
+  o.ld = round_up(m.width, 8);
+  o.plane = round_up(m.n * o.ld, 128);
+  uint16_t* to = space.take<uint16_t>(o.plane * planes_of(m));
+  o.data = to;
+  if (!run || rc) return o;
+  const int64_t blocks = ceil_div(m.n * (o.ld / 8), 256);
+  if (!fits(blocks, 256)) {
+    rc = MS_OPS_EINVAL;
+  } else if (m.dtype == MS_OPS_F32) {
+    rc = launch(k_planes, blocks, 256, s, m, o.ld, o.plane, to);
+  } else if (m.dtype == MS_OPS_F16) {
+    rc = launch(k_layout<f16>, blocks, 256, s, m, o.ld, nullptr, nullptr, reinterpret_cast<f16*>(to));
+  } else {
+    rc = launch(k_layout<bf16>, blocks, 256, s, m, o.ld, nullptr, nullptr,
+                reinterpret_cast<bf16*>(to));
+  }
+  return o;
+}
+
+// The forward pass, or with run = false what workspace it takes.
+int forward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t* targets, float scale,
+            int64_t ignore_index, float* logprob, float* lse, Space& space, hipStream_t s, bool run) {
+  int rc = 0;
+  const int64_t n = hidden.n, vocab = weight.n;
+  product_args p{};
+  p.b = prepare(hidden, space, rc, s, run);
+  p.a = prepare(weight, space, rc, s, run);
+  p.k = static_cast<int32_t>(hidden.width);
+  p.pairs = pairs_of(hidden);
+  p.splits = 1;
+  const Cut c = cut_of(vocab, n);
+  const int64_t count = ceil_div(vocab, c.m) * c.wm;
+  sum_epilogue e{};
+  e.parts = space.take<float2>(count * n);
+  e.picked = space.take<float>(n);
+  if (!run || rc) return rc;
+  e.targets = *targets;
+  e.scale = scale;
+  rc = hidden.dtype == MS_OPS_F16 ? run_product<f16, kAlong, kAlong>(c, p, e, s)
+                                  : run_product<bf16, kAlong, kAlong>(c, p, e, s);
+  if (rc) return rc;
+  // few tokens: more threads to each, as one after the other they would wait for memory
+  int lanes = 8;
+  while (lanes < 256 && n * lanes < 65536 && lanes * 2 <= count) lanes *= 2;
+  return launch(k_join, ceil_div(n, 256 / lanes), 256, s, e.parts, e.picked, count, n, lanes, *targets,
+                vocab, ignore_index, logprob, lse);
+}
+
+template <typename T>
+int fold(const float* parts, int count, int64_t n, int64_t width, const row_t* rows,
+         const float* factor, float scale, void* out, hipStream_t s) {
+  const int64_t blocks = ceil_div(ceil_div(n * width, 4), 256);
+  if (!fits(blocks, 256)) return MS_OPS_EINVAL;
+  return launch(k_fold<T>, blocks, 256, s, parts, count, n, width, rows, factor, scale,
+                static_cast<T*>(out));
+}
+
+// T: the products' type; Out: the results'; Planes: 3 for 32 bits.
+template <typename T, typename Out, int Planes>
+int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t* targets,
+             float scale, int64_t ignore_index, const float* lse, const float* grad_logprob,
+             const float* grad_lse, void* dhidden, void* dweight, Space& space, hipStream_t s,
+             bool run) {
+  int rc = 0;
+  const int64_t n = hidden.n, vocab = weight.n, width = hidden.width;
+  const int pairs = pairs_of(hidden);
+  const bool lifted = hidden.dtype == MS_OPS_F16;
+  row_t* rows = space.take<row_t>(n);
+  float* factor = space.take<float>(1);
+  if (run)
+    rc = launch(k_rows, lifted ? 1 : std::min<int64_t>(ceil_div(n, 1024), 1024), 1024, s, lse,
+                grad_logprob, grad_lse, *targets, vocab, ignore_index, lifted ? 1 : 0, rows, factor);
+  const operand h = prepare(hidden, space, rc, s, run), w = prepare(weight, space, rc, s, run);
+  operand scaled = h;
+  if (lifted && dweight) {
+    scaled.ld = round_up(width, 8);
+    f16* to = space.take<f16>(n * scaled.ld);
+    scaled.data = reinterpret_cast<const uint16_t*>(to);
+    const int64_t blocks = ceil_div(n * (scaled.ld / 8), 256);
+    if (!fits(blocks, 256)) return MS_OPS_EINVAL;
+    if (run && !rc)
+      rc = launch(k_layout<f16>, blocks, 256, s, hidden, scaled.ld, rows, factor, to);
+  }
+  // A piece of the vocabulary: whole large tiles, as many as kPiece holds
+  int64_t piece = kPiece / (n * 2 * Planes) / 256 * 256;
+  piece = std::min(std::max<int64_t>(piece, 256), round_up(vocab, 256));
+  piece = std::min(piece, kMaxWidth);
+  const int64_t pieces = ceil_div(vocab, piece);
+  const int64_t plane = round_up(n * piece, 128);
+  T* d = space.take<T>(plane * Planes);
+  // dhidden sums over the pieces in fp32
+  const Cut cut_h = cut_of(width, n);
+  const int splits_h = dhidden ? splits_of(width, n, ceil_div(piece, kStep) * pairs, cut_h) : 1;
+  float* parts_h = dhidden && (splits_h > 1 || pieces > 1) ? space.take<float>(splits_h * n * width)
+                                                           : nullptr;
+  const Cut cut_w = cut_of(width, std::min(piece, vocab));
+  const int splits_w =
+      dweight ? splits_of(width, std::min(piece, vocab), ceil_div(n, kStep) * pairs, cut_w) : 1;
+  float* parts_w = splits_w > 1 ? space.take<float>(splits_w * std::min(piece, vocab) * width) : nullptr;
+  if (!run || rc) return rc;
+
+  for (int64_t first = 0; first < vocab; first += piece) {
+    const int64_t here = std::min(piece, vocab - first);
+    operand w_here = w;
+    w_here.data += first * w.ld;
+    w_here.rows = static_cast<int32_t>(here);
+
+    product_args p{w_here, h, static_cast<int32_t>(width), pairs, 0, 0, 1};
+    soft_epilogue<T, Planes> soft{d, piece, plane, rows, *targets, scale, static_cast<int32_t>(first)};
+    rc = run_product<T, kAlong, kAlong>(cut_of(here, n), p, soft, s);
+    if (rc) return rc;
+
+    if (dhidden) {
+      operand a = w_here, b{reinterpret_cast<const uint16_t*>(d), piece, plane,
+                            static_cast<int32_t>(n)};
+      a.rows = static_cast<int32_t>(width);
+      product_args q{a, b, static_cast<int32_t>(here), pairs, 0, 0, splits_h};
+      out_epilogue<Out> out{static_cast<Out*>(dhidden), parts_h, rows, nullptr, scale, first > 0};
+      rc = run_product<T, kAcross, kAlong>(cut_h, q, out, s);
+      if (rc) return rc;
+    }
+    if (dweight) {
+      operand a = scaled, b{reinterpret_cast<const uint16_t*>(d), piece, plane,
+                            static_cast<int32_t>(here)};
+      a.rows = static_cast<int32_t>(width);
+      product_args q{a, b, static_cast<int32_t>(n), pairs, 0, 0, splits_w};
+      Out* to = static_cast<Out*>(dweight) + first * width;
+      const float* by = lifted ? factor : nullptr;
+      out_epilogue<Out> out{to, parts_w, nullptr, by, scale, 0};
+      rc = run_product<T, kAcross, kAcross>(cut_w, q, out, s);
+      if (rc) return rc;
+      if (parts_w) {
+        rc = fold<Out>(parts_w, splits_w, here, width, nullptr, by, scale, to, s);
+        if (rc) return rc;
+      }
+    }
+  }
+  if (parts_h) return fold<Out>(parts_h, splits_h, n, width, rows, nullptr, scale, dhidden, s);
+  return 0;
+}
+
+int backward_of(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t* targets,
+                float scale, int64_t ignore_index, const float* lse, const float* grad_logprob,
+                const float* grad_lse, void* dhidden, void* dweight, Space& space, hipStream_t s,
+                bool run) {
+  switch (hidden.dtype) {
+    case MS_OPS_F16:
+      return backward<f16, f16, 1>(hidden, weight, targets, scale, ignore_index, lse, grad_logprob,
+                                   grad_lse, dhidden, dweight, space, s, run);
+    case MS_OPS_BF16:
+      return backward<bf16, bf16, 1>(hidden, weight, targets, scale, ignore_index, lse, grad_logprob,
+                                     grad_lse, dhidden, dweight, space, s, run);
+    default:
+      return backward<bf16, float, 3>(hidden, weight, targets, scale, ignore_index, lse, grad_logprob,
+                                      grad_lse, dhidden, dweight, space, s, run);
+  }
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+}  // namespace ops
+
+extern "C" {
+
+int64_t ms_linear_logprobs_workspace(const ms_rows_t* hidden, const ms_rows_t* weight) {
+  using namespace ops;
+  if (!good_sizes(hidden, weight)) return MS_OPS_EINVAL;
+  if (hidden->n == 0) return 0;
+  Space space{nullptr};
+  forward(*hidden, *weight, nullptr, 1.0f, 0, nullptr, nullptr, space, nullptr, false);
+  return space.used;
+}
+
+int ms_linear_logprobs(const ms_rows_t* hidden, const ms_rows_t* weight, const ms_tokens_t* targets,
+                       float scale, int64_t ignore_index, float* logprob, float* lse, void* workspace,
+                       int64_t workspace_bytes, void* stream) {
+  using namespace ops;
+  if (!good_sizes(hidden, weight) || !good_tokens(targets) || targets->n != hidden->n)
+    return MS_OPS_EINVAL;
+  if (hidden->n == 0) return MS_OPS_OK;
+  if (!logprob || !lse) return MS_OPS_EINVAL;
+  if (workspace_bytes < ms_linear_logprobs_workspace(hidden, weight) || !workspace ||
+      !aligned(workspace))
+    return MS_OPS_EWORKSPACE;
+  Space space{static_cast<char*>(workspace)};
+  return forward(*hidden, *weight, targets, scale, ignore_index, logprob, lse, space,
+                 static_cast<hipStream_t>(stream), true);
+}
+
+int64_t ms_linear_logprobs_grad_workspace(const ms_rows_t* hidden, const ms_rows_t* weight) {
+  using namespace ops;
+  if (!good_sizes(hidden, weight)) return MS_OPS_EINVAL;
+  if (hidden->n == 0) return 0;
+  Space space{nullptr};
+  // (any address: both gradients)
+  char some;
+  backward_of(*hidden, *weight, nullptr, 1.0f, 0, nullptr, nullptr, nullptr, &some, &some, space,
+              nullptr, false);
+  return space.used;
+}
+
+int ms_linear_logprobs_grad(const ms_rows_t* hidden, const ms_rows_t* weight,
+                            const ms_tokens_t* targets, float scale, int64_t ignore_index,
+                            const float* lse, const float* grad_logprob, const float* grad_lse,
+                            void* dhidden, void* dweight, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  using namespace ops;
+  if (!good_sizes(hidden, weight) || !good_tokens(targets) || targets->n != hidden->n)
+    return MS_OPS_EINVAL;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (hidden->n == 0) {
+    if (!dweight) return MS_OPS_OK;
+    const int64_t words = ceil_div(weight->n * weight->width * dtype_bytes(weight->dtype), 2);
+    const int64_t blocks = ceil_div(words, 1024);
+    if (!fits(blocks, 256)) return MS_OPS_EINVAL;
+    return launch(k_zero, blocks, 256, s, static_cast<uint16_t*>(dweight), words);
+  }
+  if (!lse) return MS_OPS_EINVAL;
+  if (!dhidden && !dweight) return MS_OPS_OK;
+  if (workspace_bytes < ms_linear_logprobs_grad_workspace(hidden, weight) || !workspace ||
+      !aligned(workspace))
+    return MS_OPS_EWORKSPACE;
+  Space space{static_cast<char*>(workspace)};
+  return backward_of(*hidden, *weight, targets, scale, ignore_index, lse, grad_logprob, grad_lse,
+                     dhidden, dweight, space, s, true);
+}
+
+}  // extern "C"

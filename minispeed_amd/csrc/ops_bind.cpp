@@ -405,6 +405,75 @@ py::tuple act8_grad(const Tensor& codes, const Tensor& exponents,
   return py::make_tuple(wrap(dh), wrap(dup), wrap(a));
 }
 
+void need_head(const Tensor& hidden, const Tensor& weight, const Tensor& targets) {
+  need_no_tangent(hidden, "hidden");
+  need_no_tangent(weight, "weight");
+  need_hip(hidden, "hidden");
+  need_device(weight, hidden, "weight");
+  need_device(targets, hidden, "targets");
+  if (weight.dim() != 2 || hidden.dim() < 1 || weight.size(1) != hidden.size(-1))
+    bad_value("weight has shape " + shape_of(weight) + ", expected [vocab, width] for hidden " +
+              shape_of(hidden));
+  if (weight.scalar_type() != hidden.scalar_type())
+    throw py::type_error(std::string("weight has dtype ") + c10::toString(weight.scalar_type()) +
+                         ", hidden " + c10::toString(hidden.scalar_type()));
+  if (weight.size(0) < 1 || weight.size(0) > std::numeric_limits<int32_t>::max() ||
+      weight.size(1) < 1 || weight.size(1) > int64_t{1} << 20)
+    bad_value("weight has shape " + shape_of(weight) +
+              ", expected a vocabulary of 1 to 2^31 - 1 and a width of 1 to 2^20");
+  bool match = targets.dim() == hidden.dim() - 1;
+  for (int64_t d = 0; match && d < targets.dim(); ++d) match = targets.size(d) == hidden.size(d);
+  if (!match)
+    bad_value("targets has shape " + shape_of(targets) + ", expected the leading dimensions of hidden " +
+              shape_of(hidden));
+}
+
+py::tuple linear_logprobs(const Tensor& hidden, const Tensor& weight, const Tensor& targets,
+                          double scale, int64_t ignore_index) {
+  need_head(hidden, weight, targets);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(hidden.device());
+  Tensor hold_h, hold_w, hold_t;
+  const ms_rows_t h = rows_of(hidden, "hidden", hold_h), w = rows_of(weight, "weight", hold_w);
+  const ms_tokens_t y = tokens_of(targets, "targets", hold_t);
+  const Tensor logprob = make(hidden, targets.sizes(), at::kFloat);
+  const Tensor lse = make(hidden, targets.sizes(), at::kFloat);
+  const int64_t bytes = ms_linear_logprobs_workspace(&h, &w);
+  const Tensor work = scratch(hidden, bytes);
+  check(ms_linear_logprobs(&h, &w, &y, static_cast<float>(scale), ignore_index,
+                           static_cast<float*>(logprob.data_ptr()),
+                           static_cast<float*>(lse.data_ptr()), data_of(work), bytes,
+                           stream_of(hidden)),
+        "ms_linear_logprobs");
+  return py::make_tuple(wrap(logprob), wrap(lse));
+}
+
+py::tuple linear_logprobs_grad(const Tensor& hidden, const Tensor& weight, const Tensor& targets,
+                               const Tensor& lse, const std::optional<Tensor>& grad_logprob,
+                               const std::optional<Tensor>& grad_lse, double scale,
+                               int64_t ignore_index, bool want_hidden, bool want_weight) {
+  need_no_tangent(lse, "lse");
+  if (grad_logprob) need_no_tangent(*grad_logprob, "grad_logprob");
+  if (grad_lse) need_no_tangent(*grad_lse, "grad_lse");
+  need_head(hidden, weight, targets);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(hidden.device());
+  Tensor hold_h, hold_w, hold_t, hold[3];
+  const ms_rows_t h = rows_of(hidden, "hidden", hold_h), w = rows_of(weight, "weight", hold_w);
+  const ms_tokens_t y = tokens_of(targets, "targets", hold_t);
+  const float* l = per_row(lse, hidden, h.n, "lse", hold[0]);
+  const float* g = per_row(grad_logprob, hidden, h.n, "grad_logprob", hold[1]);
+  const float* gl = per_row(grad_lse, hidden, h.n, "grad_lse", hold[2]);
+  const Tensor dh = want_hidden ? make(hidden, hidden.sizes(), hidden.scalar_type()) : Tensor();
+  const Tensor dw = want_weight ? make(weight, weight.sizes(), weight.scalar_type()) : Tensor();
+  const int64_t bytes = ms_linear_logprobs_grad_workspace(&h, &w);
+  const Tensor work = scratch(hidden, bytes);
+  check(ms_linear_logprobs_grad(&h, &w, &y, static_cast<float>(scale), ignore_index, l, g, gl,
+                                data_of(dh), data_of(dw), data_of(work), bytes, stream_of(hidden)),
+        "ms_linear_logprobs_grad");
+  return py::make_tuple(wrap(dh), wrap(dw));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ops, m) {
@@ -419,4 +488,6 @@ PYBIND11_MODULE(_ops, m) {
   m.def("unpack8", wrap_pybind_function(unpack8));
   m.def("act8", wrap_pybind_function(act8));
   m.def("act8_grad", wrap_pybind_function(act8_grad));
+  m.def("linear_logprobs", wrap_pybind_function(linear_logprobs));
+  m.def("linear_logprobs_grad", wrap_pybind_function(linear_logprobs_grad));
 }

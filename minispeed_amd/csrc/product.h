@@ -1,0 +1,259 @@
+// Matrix products with an epilogue of their own, for operators that use the
+// product's values where they arise instead of storing them (linear.hip).
+//
+//   C[m, n] = sum over k of A[m, k] B[n, k],   2-byte elements, fp32 sums
+//
+// A block computes a tile of C; its waves hold it as 32 x 32 squares of matrix
+// instructions (v_mfma_f32_32x32x16).  Of such a square a lane has one column
+// n = lane % 32 and the rows m = 8 (i / 4) + 4 (lane / 32) + i % 4, i < 16: an
+// epilogue that reduces over m stays within two lanes, and one that stores has four
+// consecutive m of one n.
+//
+// Tiles of 64 k go from memory to LDS by loads that write LDS themselves, so that
+// no register holds them; two of them take turns.  LDS is written in the order of the
+// lanes, so each lane chooses which 16 bytes it fetches such that the reads of a
+// fragment meet all banks:
+//   along  k (rows of A or B lie along k): chunk c of row r lies at c ^ (r / 2 % 8);
+//   across k (rows lie along m or n, one for each k): chunk c of row k at c ^ 4 (k % 4),
+//            read by the transposing LDS load, 4 k of one m to a lane.
+// Chunks beyond an operand's edge are fetched from beyond the buffer's range, which
+// gives zeros.
+#pragma once
+
+#include "ops_common.h"
+
+namespace ops {
+
+constexpr int kStep = 64;                 // k of one tile
+constexpr uint32_t kBeyond = 0x7f000000;  // an offset outside of every buffer
+constexpr uint32_t kRange = 0x40000000;   // bytes that a tile's offsets stay within
+
+enum Side { kAlong, kAcross };
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+#define MS_LDS __attribute__((address_space(3)))
+
+template <typename T> struct frag_of;
+template <> struct frag_of<f16> { typedef f16x8 type; };
+template <> struct frag_of<bf16> { typedef bf16x8 type; };
+
+__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// One operand: `rows` of m or n against k.  Along k: row r starts at r * ld, and ld and
+// the address are multiples of 16 bytes.  Across k: k starts at k * ld, the same.
+// A 32-bit operand is three planes of bf16 whose sum it is (plane: elements from one to
+// the next); the product then runs over the six pairs of planes whose product is not
+// below the last bit, as if k were six times as long.
+struct operand {
+  const uint16_t* data;
+  int64_t ld;
+  int64_t plane;
+  int32_t rows;
+};
+
+struct product_args {
+  operand a, b;
+  int32_t k;
+  int32_t pairs;                   // 1, or 6 pairs of planes
+  int32_t tiles_m, tiles_n, splits;
+};
+
+// Which pair of planes: (0,0) (0,1) (1,0) (1,1) (0,2) (2,0), two bits each.
+__device__ __forceinline__ int plane_a(int pair) { return 0x850 >> (2 * pair) & 3; }
+__device__ __forceinline__ int plane_b(int pair) { return 0x244 >> (2 * pair) & 3; }
+
+// One operand's tile of R rows, fetched by NT threads.
+template <int R, int NT, Side S>
+struct Fetch {
+  static constexpr int kIssues = R * kStep * 2 / (NT * 16);
+  static constexpr int kChunks = R / 8;              // across: 16-byte chunks of a row
+  static constexpr int kRowsPer = S == kAlong ? NT / 8 : NT / kChunks;
+  static constexpr int kTurn = kChunks >= 16 ? 3 : 0;
+  static_assert(kIssues >= 1 && R * kStep * 2 % (NT * 16) == 0, "");
+  static_assert(S == kAlong ? kRowsPer % 16 == 0 : kRowsPer % 4 == 0, "");
+
+  const char* base;
+  int64_t ld_bytes;
+  uint32_t offset[kIssues];
+  int first_k;        // k of this thread's first chunk, within the tile
+
+  __device__ Fetch(const operand& o, int row0, int tid) {
+    ld_bytes = o.ld * 2;
+    if (S == kAlong) {
+      base = reinterpret_cast<const char*>(o.data) + row0 * ld_bytes;
+      const int r = tid >> 3, chunk = (tid & 7) ^ (r >> 1 & 7);
+      first_k = chunk * 8;
+#pragma unroll
+      for (int i = 0; i < kIssues; ++i) {
+        const int row = r + i * kRowsPer;
+        offset[i] = row0 + row < o.rows
+                        ? static_cast<uint32_t>(row * static_cast<int>(ld_bytes)) + chunk * 16
+                        : kBeyond;
+      }
+    } else {
+      base = reinterpret_cast<const char*>(o.data) + static_cast<int64_t>(row0) * 2;
+      first_k = tid / kChunks;
+      const int chunk = tid % kChunks ^ (first_k & kTurn) << 2;
+#pragma unroll
+      for (int i = 0; i < kIssues; ++i)
+        offset[i] = row0 + chunk * 8 < o.rows
+                        ? static_cast<uint32_t>((first_k + i * kRowsPer) * static_cast<int>(ld_bytes)) +
+                              chunk * 16
+                        : kBeyond;
+    }
+  }
+
+  // The tile at k0 of plane `shift` elements further, into LDS at `to`; `left` is k - k0.
+  __device__ void issue(int64_t shift, int k0, int left, char MS_LDS* to, int wave) const {
+    const char* p = base + shift * 2 + (S == kAlong ? static_cast<int64_t>(k0) * 2 : k0 * ld_bytes);
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(p), 0, kRange, 0x00027000);
+    char MS_LDS* dst = to + wave * 1024;
+    if (left >= kStep) {
+#pragma unroll
+      for (int i = 0; i < kIssues; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, dst + i * NT * 16, 16, offset[i], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kIssues; ++i) {
+        const int k = S == kAlong ? first_k : first_k + i * kRowsPer;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, dst + i * NT * 16, 16,
+                                                 k < left ? offset[i] : kBeyond, 0, 0, 0);
+      }
+    }
+  }
+};
+
+// Fragments of one operand: kept addresses of a lane, then one read for each square.
+template <typename T, int R, Side S>
+struct Frags {
+  typedef typename frag_of<T>::type frag;
+  uint32_t at[4];
+
+  // first: the wave's first row of the tile.
+  __device__ Frags(int first, int lane) {
+    if (S == kAlong) {
+      const int r = lane & 31;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        at[ks] = (first + r) * 128 + (((ks * 2 + (lane >> 5)) ^ (r >> 1 & 7)) << 4);
+    } else {
+      constexpr int kTurn = R / 8 >= 16 ? 3 : 0;
+      const int k = (lane >> 5) * 8 + ((lane & 15) >> 2);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int m = first + q * 32 + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+        at[q] = k * R * 2 + (((m >> 3) ^ (k & kTurn) << 2) << 4) + (m & 7) * 2;
+      }
+    }
+  }
+
+  // Square q (32 rows further each), 16 k from 16 ks.
+  __device__ frag read(const char MS_LDS* tile, int q, int ks) const {
+    if (S == kAlong)
+      return *reinterpret_cast<const frag MS_LDS*>(tile + at[ks] + q * 32 * 128);
+    union { s16x4 half[2]; frag whole; } u;
+    const char MS_LDS* p = tile + at[q & 3] + (q >> 2) * 256 + ks * 16 * R * 2;
+    u.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<s16x4 MS_LDS*>(const_cast<char MS_LDS*>(p)));
+    u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<s16x4 MS_LDS*>(const_cast<char MS_LDS*>(p + 4 * R * 2)));
+    return u.whole;
+  }
+};
+
+// Block b's place: neighbours in a tile order to one XCD (blocks go round the 8 XCDs),
+// in that order bands of 8 columns of tiles, so that what runs at a time on an XCD shares
+// its operands in the XCD's cache.
+__device__ __forceinline__ void place(uint32_t b, uint32_t total, int tiles_m, int tiles_n,
+                                      int& tm, int& tn, int& split) {
+  const uint32_t q = total / 8, r = total % 8, x = b % 8;
+  uint32_t t = x * q + min(x, r) + b / 8;
+  const uint32_t each = static_cast<uint32_t>(tiles_m) * tiles_n;
+  split = t / each;
+  t -= split * each;
+  const uint32_t band = t / (8 * tiles_m), first = band * 8;
+  const uint32_t wide = min(8u, tiles_n - first);
+  t -= first * tiles_m;
+  tm = t / wide;
+  tn = first + t % wide;
+}
+
+namespace {
+template <typename T, int BM, int BN, int WM, int WN, Side SA, Side SB, typename Epilogue>
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_product(product_args p, Epilogue epilogue) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host has none of the built-in functions)
+  constexpr int NT = WM * WN * 64, MI = BM / WM / 32, NI = BN / WN / 32;
+  constexpr int kTileA = BM * kStep * 2, kTile = kTileA + BN * kStep * 2;
+  static_assert(BM % (WM * 32) == 0 && BN % (WN * 32) == 0, "");
+  __shared__ __attribute__((aligned(1024))) char memory[2 * kTile];
+  char MS_LDS* const lds = (char MS_LDS*)memory;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  int tm, tn, split;
+  place(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn, split);
+
+  const Fetch<BM, NT, SA> fetch_a(p.a, tm * BM, tid);
+  const Fetch<BN, NT, SB> fetch_b(p.b, tn * BN, tid);
+  const Frags<T, BM, SA> frags_a(wm * MI * 32, lane);
+  const Frags<T, BN, SB> frags_b(wn * NI * 32, lane);
+
+  const int steps = (p.k + kStep - 1) / kStep;
+  const int64_t all = static_cast<int64_t>(steps) * p.pairs;
+  const int begin = static_cast<int>(all * split / p.splits);
+  const int end = static_cast<int>(all * (split + 1) / p.splits);
+
+  f32x16 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) acc[i][j] = f32x16{};
+
+  int pair = begin / steps, k0 = (begin - pair * steps) * kStep;
+  auto issue = [&](int buffer) {
+    char MS_LDS* to = lds + buffer * kTile;
+    fetch_a.issue(plane_a(pair) * p.a.plane, k0, p.k - k0, to, wave);
+    fetch_b.issue(plane_b(pair) * p.b.plane, k0, p.k - k0, to + kTileA, wave);
+    k0 += kStep;
+    if (k0 >= p.k) k0 = 0, ++pair;
+  };
+
+  if (begin < end) issue(0);
+  for (int s = begin; s < end; ++s) {
+    const int buffer = (s - begin) & 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (s + 1 < end) issue(buffer ^ 1);
+    const char MS_LDS* tile = lds + buffer * kTile;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      typename frag_of<T>::type a[MI], b[NI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) a[i] = frags_a.read(tile, i, ks);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) b[j] = frags_b.read(tile + kTileA, j, ks);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j]);
+    }
+    // the fragments of this tile are in registers before any wave fetches into it again
+    asm volatile("" ::: "memory");
+  }
+
+  epilogue.template store<MI, NI>(acc, tm * BM + wm * MI * 32, tn * BN + wn * NI * 32,
+                                  tm * WM + wm, split, lane, p.a.rows, p.b.rows);
+#endif
+}
+
+}  // namespace
+}  // namespace ops

@@ -19,10 +19,12 @@ the kernels have finished.
 from .activation8 import (Checkpoint8, activation8, activation8_grad, activation8_linear,
                           checkpoint8, pack8, unpack8)
 from .embedding import embedding, embedding_grad
+from .linear import LinearLogprobs, linear_logprobs, linear_logprobs_grad
 from .logprobs import TokenLogprobs, token_logprobs, token_logprobs_grad
 
 __all__ = [
     "Checkpoint8",
+    "LinearLogprobs",
     "TokenLogprobs",
     "activation8",
     "activation8_grad",
@@ -30,6 +32,8 @@ __all__ = [
     "checkpoint8",
     "embedding",
     "embedding_grad",
+    "linear_logprobs",
+    "linear_logprobs_grad",
     "pack8",
     "token_logprobs",
     "token_logprobs_grad",
