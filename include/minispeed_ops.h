@@ -203,6 +203,46 @@ int ms_linear_logprobs_grad(const ms_rows_t* hidden, const ms_rows_t* weight,
                             void* dhidden, void* dweight, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
+enum {
+  MS_NORM_RMS = 0,        /* x / sqrt(mean(x^2) + eps)                    */
+  MS_NORM_LAYER = 1       /* (x - mean) / sqrt(mean((x - mean)^2) + eps)  */
+};
+
+/*
+ * Between two blocks of a model: the norm after the one, its gate and residual scale, the
+ * residual sum and the norm before the next.
+ *   u    = norm(block) * block_weight + block_bias   (block itself without block_weight)
+ *   next = residual + scale * gate * u
+ *   out  = norm(next) * weight + bias
+ * `block` NULL: out = norm(residual) * weight + bias, and `next` is not written.  Rows have
+ * 1 to 16384 elements; weights, biases [width] and `gate` [gates, width] are dense and of the
+ * rows' type; gates divides the number of rows, and that many neighbouring rows share one (0: no
+ * gate, gate NULL).  Biases go with MS_NORM_LAYER, block_bias with block_weight.  `out`
+ * comes from the sums before they are rounded into `next`.  stats (NULL: not
+ * wanted) gets mean and reciprocal deviation of next, then of block where it has a norm: 2
+ * or 4 floats for each row.  Outputs are dense.
+ */
+int ms_norm(const ms_rows_t* residual, const ms_rows_t* block, int32_t kind, const void* weight,
+            const void* bias, const void* block_weight, const void* block_bias, const void* gate,
+            int64_t gates, float scale, float eps, void* next, void* out, float* stats,
+            void* stream);
+
+/*
+ * Its gradients.  dout and dnext are those of `out` and `next` (one may be NULL: zeros);
+ * next, stats and block are the forward pass's (next: the residual itself where there is no
+ * block).  Written whole: dresidual, dblock (with block) [n, width]; dweight, and unless NULL
+ * dbias, dblock_weight (required with block_weight), dblock_bias [width]; dgate (with gate)
+ * [gates, width].  Sums over rows are fp32 in an order that follows from the sizes.
+ */
+int64_t ms_norm_grad_workspace(int64_t n, int64_t width, int32_t dtype, int32_t kind, int32_t post,
+                               int64_t gates);
+int ms_norm_grad(const ms_rows_t* dout, const ms_rows_t* dnext, const ms_rows_t* next,
+                 const float* stats, const ms_rows_t* block, int32_t kind, const void* weight,
+                 const void* block_weight, const void* block_bias, const void* gate, int64_t gates,
+                 float scale, void* dresidual, void* dblock, void* dweight, void* dbias,
+                 void* dblock_weight, void* dblock_bias, void* dgate, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -474,6 +474,156 @@ py::tuple linear_logprobs_grad(const Tensor& hidden, const Tensor& weight, const
   return py::make_tuple(wrap(dh), wrap(dw));
 }
 
+// A dense vector that goes with rows like x, or null.
+const void* vector_of(const std::optional<Tensor>& t, const Tensor& x, const char* what, Tensor& hold) {
+  if (!t) return nullptr;
+  need_no_tangent(*t, what);
+  need_device(*t, x, what);
+  if (t->scalar_type() != x.scalar_type())
+    throw py::type_error(std::string(what) + " has dtype " + c10::toString(t->scalar_type()) +
+                         ", expected " + c10::toString(x.scalar_type()));
+  if (t->dim() != 1 || t->size(0) != x.size(-1))
+    bad_value(std::string(what) + " has shape " + shape_of(*t) + ", expected [" +
+              std::to_string(x.size(-1)) + "]");
+  hold = t->contiguous();
+  return hold.data_ptr();
+}
+
+// How many gates there are: one for all rows, or the leading dimensions of x up to where
+// the gate's are 1.
+int64_t gates_of(const Tensor& gate, const Tensor& x) {
+  const int64_t dims = x.dim() - 1;
+  if (gate.dim() == 1 && gate.size(0) == x.size(-1)) return 1;
+  int64_t gates = 1, d = 0;
+  bool fits = gate.dim() == x.dim() && gate.size(-1) == x.size(-1);
+  if (fits) {
+    while (d < dims && gate.size(d) == x.size(d)) gates *= gate.size(d++);
+    while (d < dims && gate.size(d) == 1) ++d;
+    fits = d == dims;
+  }
+  if (!fits)
+    bad_value("gate has shape " + shape_of(gate) + ", expected [width], or that of rows " + shape_of(x) +
+              " with a size of 1 in the last of the leading dimensions");
+  return gates;
+}
+
+void need_like(const Tensor& t, const Tensor& x, const char* what) {
+  need_no_tangent(t, what);
+  need_device(t, x, what);
+  if (t.scalar_type() != x.scalar_type())
+    throw py::type_error(std::string(what) + " has dtype " + c10::toString(t.scalar_type()) +
+                         ", expected " + c10::toString(x.scalar_type()));
+  if (t.sizes() != x.sizes())
+    bad_value(std::string(what) + " has shape " + shape_of(t) + ", expected " + shape_of(x));
+}
+
+// The operands that both passes have.
+struct norm_operands {
+  ms_rows_t x{}, block{};
+  const void *weight, *bias, *block_weight, *block_bias, *gate = nullptr;
+  int64_t gates = 0;
+  Tensor hold[7];
+
+  norm_operands(const Tensor& rows, const char* what, const std::optional<Tensor>& block_of,
+                const Tensor& weight_of, const std::optional<Tensor>& bias_of,
+                const std::optional<Tensor>& block_weight_of,
+                const std::optional<Tensor>& block_bias_of, const std::optional<Tensor>& gate_of,
+                int64_t kind) {
+    need_no_tangent(rows, what);
+    need_hip(rows, what);
+    dtype_of(rows.scalar_type(), what);
+    if (rows.dim() < 1 || rows.size(-1) < 1 || rows.size(-1) > 16384)
+      bad_value(std::string(what) + " has shape " + shape_of(rows) + ", expected rows of 1 to 16384");
+    if (block_of) need_like(*block_of, rows, "block");
+    if (!block_of && (block_weight_of || gate_of)) bad_value("block_weight and gate need block");
+    if (block_bias_of && !block_weight_of) bad_value("block_bias needs block_weight");
+    if (kind != MS_NORM_LAYER && (bias_of || block_bias_of)) bad_value("biases go with kind 'layer'");
+    weight = vector_of(weight_of, rows, "weight", hold[0]);
+    bias = vector_of(bias_of, rows, "bias", hold[1]);
+    block_weight = vector_of(block_weight_of, rows, "block_weight", hold[2]);
+    block_bias = vector_of(block_bias_of, rows, "block_bias", hold[3]);
+    if (gate_of) {
+      need_no_tangent(*gate_of, "gate");
+      need_device(*gate_of, rows, "gate");
+      if (gate_of->scalar_type() != rows.scalar_type())
+        throw py::type_error(std::string("gate has dtype ") + c10::toString(gate_of->scalar_type()) +
+                             ", expected " + c10::toString(rows.scalar_type()));
+      gates = gates_of(*gate_of, rows);
+      hold[4] = gate_of->contiguous();
+      gate = hold[4].data_ptr();
+    }
+    x = rows_of(rows, what, hold[5]);
+    if (block_of) block = rows_of(*block_of, "block", hold[6]);
+  }
+};
+
+py::tuple norm(const Tensor& residual, const std::optional<Tensor>& block, const Tensor& weight,
+               const std::optional<Tensor>& bias, const std::optional<Tensor>& block_weight,
+               const std::optional<Tensor>& block_bias, const std::optional<Tensor>& gate,
+               double scale, double eps, int64_t kind) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(residual.device());
+  const norm_operands o(residual, "residual", block, weight, bias, block_weight, block_bias, gate, kind);
+  const Tensor next = block ? make(residual, residual.sizes(), residual.scalar_type()) : Tensor();
+  const Tensor out = make(residual, residual.sizes(), residual.scalar_type());
+  std::vector<int64_t> shape(residual.sizes().begin(), residual.sizes().end());
+  shape.back() = block_weight ? 4 : 2;
+  const Tensor stats = make(residual, shape, at::kFloat);
+  // (a gate of no rows stands for none: there is nothing that it would multiply)
+  check(ms_norm(&o.x, block ? &o.block : nullptr, static_cast<int32_t>(kind), o.weight, o.bias,
+                o.block_weight, o.block_bias, o.gates ? o.gate : nullptr, o.gates,
+                static_cast<float>(scale), static_cast<float>(eps), data_of(next), out.data_ptr(),
+                static_cast<float*>(stats.data_ptr()), stream_of(residual)),
+        "ms_norm");
+  return py::make_tuple(wrap(next), wrap(out), wrap(stats));
+}
+
+py::tuple norm_grad(const std::optional<Tensor>& grad_out, const std::optional<Tensor>& grad_residual,
+                    const Tensor& residual, const Tensor& stats, const std::optional<Tensor>& block,
+                    const Tensor& weight, const std::optional<Tensor>& bias,
+                    const std::optional<Tensor>& block_weight,
+                    const std::optional<Tensor>& block_bias, const std::optional<Tensor>& gate,
+                    double scale, int64_t kind) {
+  if (!grad_out && !grad_residual) bad_value("grad_out and grad_residual are both None");
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(residual.device());
+  const norm_operands o(residual, "residual", block, weight, bias, block_weight, block_bias, gate, kind);
+  if (grad_out) need_like(*grad_out, residual, "grad_out");
+  if (grad_residual) need_like(*grad_residual, residual, "grad_residual");
+  need_no_tangent(stats, "stats");
+  need_device(stats, residual, "stats");
+  const int64_t fields = block_weight ? 4 : 2;
+  bool match = stats.scalar_type() == at::kFloat && stats.dim() == residual.dim() &&
+               stats.size(-1) == fields;
+  for (int64_t d = 0; match && d + 1 < stats.dim(); ++d) match = stats.size(d) == residual.size(d);
+  if (!match)
+    bad_value("stats has shape " + shape_of(stats) + " and dtype " + c10::toString(stats.scalar_type()) +
+              ", expected float32 and " + std::to_string(fields) + " for each row of " +
+              shape_of(residual));
+  Tensor hold_o, hold_r;
+  const ms_rows_t dout = grad_out ? rows_of(*grad_out, "grad_out", hold_o) : ms_rows_t{};
+  const ms_rows_t dnext = grad_residual ? rows_of(*grad_residual, "grad_residual", hold_r) : ms_rows_t{};
+  const Tensor dense = stats.contiguous();
+  const auto like = [&](const std::optional<Tensor>& t) {
+    return t ? make(residual, t->sizes(), residual.scalar_type()) : Tensor();
+  };
+  const Tensor dx = make(residual, residual.sizes(), residual.scalar_type());
+  const Tensor db = like(block), dw = like(weight), dbias = like(bias), dbw = like(block_weight),
+               dbb = like(block_bias), dg = like(gate);
+  const int32_t post = block_weight ? 1 : 0;
+  const int64_t bytes = ms_norm_grad_workspace(o.x.n, o.x.width, o.x.dtype, static_cast<int32_t>(kind),
+                                               post, o.gates);
+  const Tensor work = scratch(residual, bytes);
+  check(ms_norm_grad(grad_out ? &dout : nullptr, grad_residual ? &dnext : nullptr, &o.x,
+                     static_cast<const float*>(dense.data_ptr()), block ? &o.block : nullptr,
+                     static_cast<int32_t>(kind), o.weight, o.block_weight, o.block_bias,
+                     o.gates ? o.gate : nullptr, o.gates, static_cast<float>(scale), data_of(dx),
+                     data_of(db), data_of(dw), data_of(dbias), data_of(dbw), data_of(dbb),
+                     o.gates ? data_of(dg) : nullptr, data_of(work), bytes, stream_of(residual)),
+        "ms_norm_grad");
+  return py::make_tuple(wrap(dx), wrap(db), wrap(dw), wrap(dbias), wrap(dbw), wrap(dbb), wrap(dg));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ops, m) {
@@ -488,6 +638,8 @@ PYBIND11_MODULE(_ops, m) {
   m.def("unpack8", wrap_pybind_function(unpack8));
   m.def("act8", wrap_pybind_function(act8));
   m.def("act8_grad", wrap_pybind_function(act8_grad));
+  m.def("norm", wrap_pybind_function(norm));
+  m.def("norm_grad", wrap_pybind_function(norm_grad));
   m.def("linear_logprobs", wrap_pybind_function(linear_logprobs));
   m.def("linear_logprobs_grad", wrap_pybind_function(linear_logprobs_grad));
 }

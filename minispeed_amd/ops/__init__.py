@@ -21,10 +21,13 @@ from .activation8 import (Checkpoint8, activation8, activation8_grad, activation
 from .embedding import embedding, embedding_grad
 from .linear import LinearLogprobs, linear_logprobs, linear_logprobs_grad
 from .logprobs import TokenLogprobs, token_logprobs, token_logprobs_grad
+from .norm import (ResidualNorm, ResidualNormGrads, norm, residual_norm, residual_norm_grad)
 
 __all__ = [
     "Checkpoint8",
     "LinearLogprobs",
+    "ResidualNorm",
+    "ResidualNormGrads",
     "TokenLogprobs",
     "activation8",
     "activation8_grad",
@@ -34,7 +37,10 @@ __all__ = [
     "embedding_grad",
     "linear_logprobs",
     "linear_logprobs_grad",
+    "norm",
     "pack8",
+    "residual_norm",
+    "residual_norm_grad",
     "token_logprobs",
     "token_logprobs_grad",
     "unpack8",
