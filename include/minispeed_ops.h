@@ -1,8 +1,9 @@
 /*
  * minispeed_ops.h — C ABI of the language-model operators around the boundary
  * step on MI355X (gfx950): the token embedding and its gradient, log
- * probabilities of given tokens and their gradient, and activations held in
- * 8 bits between forward and backward.
+ * probabilities of given tokens and their gradient (of logits, or straight from the
+ * hidden states), activations held in 8 bits between forward and backward, the norms
+ * around a block with its gate and residual sum, and the relative position bias.
  *
  * Conventions (as minispeed_boundary.h)
  *   - Every pointer is caller-owned device memory [dev]; scalars are read
@@ -242,6 +243,33 @@ int ms_norm_grad(const ms_rows_t* dout, const ms_rows_t* dnext, const ms_rows_t*
                  float scale, void* dresidual, void* dblock, void* dweight, void* dbias,
                  void* dblock_weight, void* dblock_bias, void* dgate, void* workspace,
                  int64_t workspace_bytes, void* stream);
+
+/*
+ * Relative position bias of attention: out[h, i, j] = table[bucket(j - i - first), h], dense
+ * [heads, queries, keys] of the table's type; bucket b of head h is at b * bucket_stride +
+ * h * head_stride.  A side has n = buckets / 2 buckets (all of them, causal; n >= 2, an even
+ * number of buckets unless causal, 512 at most): distances below n / 2 one each, and bucket
+ * n / 2 + s from the least distance a on for which (a / (n/2))^(n - n/2) >=
+ * (max_distance / (n/2))^s.  Keys up to the query come first, then those behind it; causal,
+ * keys behind the query get -inf.  max_distance lies above n / 2, |first| within 2^40.
+ */
+int ms_position_bias(const void* table, int32_t dtype, int64_t buckets, int64_t bucket_stride,
+                     int64_t head_stride, int64_t heads, int64_t queries, int64_t keys, int64_t first,
+                     int64_t max_distance, int32_t causal, void* out, void* stream);
+
+/*
+ * The table's gradient, dense [buckets, heads], written whole: sums over the batch and all
+ * pairs of a bucket, in fp32, in an order that follows from the sizes.  grad's rows of `keys`
+ * elements lie at batch_stride, head_stride, row_stride; causal, what lies at keys behind
+ * the query is not looked at.
+ */
+int64_t ms_position_bias_grad_workspace(int32_t dtype, int64_t buckets, int64_t batch, int64_t heads,
+                                        int64_t queries, int64_t keys);
+int ms_position_bias_grad(const void* grad, int32_t dtype, int64_t batch, int64_t batch_stride,
+                          int64_t heads, int64_t head_stride, int64_t queries, int64_t row_stride,
+                          int64_t keys, int64_t first, int64_t buckets, int64_t max_distance,
+                          int32_t causal, void* dtable, void* workspace, int64_t workspace_bytes,
+                          void* stream);
 
 #ifdef __cplusplus
 }

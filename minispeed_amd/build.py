@@ -32,7 +32,7 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 OUTPUT = os.path.join(PKG_DIR, "libminispeed_boundary.so")
 ARCH = "gfx950"
 OPS_SOURCES = [os.path.join(PKG_DIR, "csrc", f"{name}.hip")
-               for name in ("embedding", "logprobs", "act8", "linear", "norm")]
+               for name in ("embedding", "logprobs", "act8", "linear", "norm", "posbias")]
 OPS_OUTPUT = os.path.join(PKG_DIR, "libminispeed_ops.so")
 
 # -ffp-contract=off: every a*b+c the kernels do not write as fmaf stays two

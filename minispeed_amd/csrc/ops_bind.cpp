@@ -624,6 +624,70 @@ py::tuple norm_grad(const std::optional<Tensor>& grad_out, const std::optional<T
   return py::make_tuple(wrap(dx), wrap(db), wrap(dw), wrap(dbias), wrap(dbw), wrap(dbb), wrap(dg));
 }
 
+void need_buckets(int64_t buckets, int64_t first, int64_t max_distance, bool causal) {
+  const int64_t side = causal ? buckets : buckets / 2;
+  if (buckets > 512 || side < 2 || (!causal && buckets % 2))
+    bad_value("there are " + std::to_string(buckets) + " buckets, expected " +
+              (causal ? "2 to 512" : "an even number from 4 to 512"));
+  if (max_distance <= side / 2 || max_distance > std::numeric_limits<int32_t>::max())
+    bad_value("max_distance is " + std::to_string(max_distance) + ", expected " +
+              std::to_string(side / 2 + 1) + " to 2^31 - 1");
+  if (first < -(int64_t{1} << 40) || first > int64_t{1} << 40)
+    bad_value("first is " + std::to_string(first) + ", expected -2^40 to 2^40");
+}
+
+Tensor position_bias(const Tensor& table, int64_t queries, int64_t keys, int64_t first,
+                     int64_t max_distance, bool causal) {
+  need_no_tangent(table, "table");
+  need_hip(table, "table");
+  const int32_t type = dtype_of(table.scalar_type(), "table");
+  if (table.dim() != 2) bad_value("table has shape " + shape_of(table) + ", expected [buckets, heads]");
+  need_buckets(table.size(0), first, max_distance, causal);
+  if (queries < 0 || keys < 0)
+    bad_value("there are " + std::to_string(queries) + " queries and " + std::to_string(keys) + " keys");
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(table.device());
+  const Tensor out = make(table, {table.size(1), queries, keys}, table.scalar_type());
+  check(ms_position_bias(table.data_ptr(), type, table.size(0), table.stride(0), table.stride(1),
+                         table.size(1), queries, keys, first, max_distance, causal ? 1 : 0,
+                         out.data_ptr(), stream_of(table)),
+        "ms_position_bias");
+  return out;
+}
+
+Tensor position_bias_grad(const Tensor& grad, int64_t buckets, int64_t first, int64_t max_distance,
+                          bool causal) {
+  need_no_tangent(grad, "grad");
+  need_hip(grad, "grad");
+  const int32_t type = dtype_of(grad.scalar_type(), "grad");
+  if (grad.dim() < 3)
+    bad_value("grad has shape " + shape_of(grad) + ", expected [..., heads, queries, keys]");
+  need_buckets(buckets, first, max_distance, causal);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(grad.device());
+  const int64_t lead = grad.dim() - 3, heads = grad.size(lead), queries = grad.size(lead + 1),
+                keys = grad.size(lead + 2);
+  Tensor hold = grad;
+  int64_t inner, outer_stride, batch_stride;
+  const auto fits = [&] {
+    return (keys <= 1 || hold.stride(lead + 2) == 1) &&
+           two_strides(hold, lead, inner, outer_stride, batch_stride) && outer_stride == 0;
+  };
+  if (!fits()) {
+    hold = grad.contiguous();
+    fits();
+  }
+  const int64_t batch = product(grad, lead);
+  const Tensor out = make(grad, {buckets, heads}, grad.scalar_type());
+  const int64_t bytes = ms_position_bias_grad_workspace(type, buckets, batch, heads, queries, keys);
+  const Tensor work = scratch(grad, bytes);
+  check(ms_position_bias_grad(hold.data_ptr(), type, batch, batch_stride, heads, hold.stride(lead),
+                              queries, hold.stride(lead + 1), keys, first, buckets, max_distance,
+                              causal ? 1 : 0, out.data_ptr(), data_of(work), bytes, stream_of(grad)),
+        "ms_position_bias_grad");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ops, m) {
@@ -640,6 +704,8 @@ PYBIND11_MODULE(_ops, m) {
   m.def("act8_grad", wrap_pybind_function(act8_grad));
   m.def("norm", wrap_pybind_function(norm));
   m.def("norm_grad", wrap_pybind_function(norm_grad));
+  m.def("position_bias", wrap_pybind_function(position_bias));
+  m.def("position_bias_grad", wrap_pybind_function(position_bias_grad));
   m.def("linear_logprobs", wrap_pybind_function(linear_logprobs));
   m.def("linear_logprobs_grad", wrap_pybind_function(linear_logprobs_grad));
 }

@@ -22,6 +22,7 @@ from .embedding import embedding, embedding_grad
 from .linear import LinearLogprobs, linear_logprobs, linear_logprobs_grad
 from .logprobs import TokenLogprobs, token_logprobs, token_logprobs_grad
 from .norm import (ResidualNorm, ResidualNormGrads, norm, residual_norm, residual_norm_grad)
+from .posbias import position_bias, position_bias_grad
 
 __all__ = [
     "Checkpoint8",
@@ -39,6 +40,8 @@ __all__ = [
     "linear_logprobs_grad",
     "norm",
     "pack8",
+    "position_bias",
+    "position_bias_grad",
     "residual_norm",
     "residual_norm_grad",
     "token_logprobs",
