@@ -177,7 +177,8 @@ int ms_act8_grad(const int8_t* codes, const uint8_t* exponents, const int8_t* up
 /*
  * Log probabilities of given tokens under softmax(x), x = scale * hidden * weight^T, without
  * the logits x ever being stored.  `hidden` [n, width] and `weight` [vocab, width] have one
- * element type, width 1 to 2^20, vocab >= 1.  Outputs as of ms_logprobs, fp32, dense:
+ * element type, width 1 to 2^20, vocab >= 1,
+ * both of at most 2^31 - 1025 rows.  Outputs as of ms_logprobs, fp32, dense:
  * lse, and logprob (0 where target == ignore_index, NaN where it is outside of [0, vocab)).
  * A token whose logits hold NaN or +inf has NaN in both, one whose logits are all -inf
  * has -inf in both.

@@ -35,6 +35,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kMaxWidth = 1 << 20;
+constexpr int64_t kMaxRows = INT32_MAX - 1024;     // a tile behind the last row stays in 32 bits
 constexpr int64_t kPiece = int64_t{256} << 20;     // bytes of d at a time
 
 // What a token's row of d is made of, by k_rows.
@@ -461,7 +462,7 @@ struct Space {
 bool good_sizes(const ms_rows_t* hidden, const ms_rows_t* weight) {
   return good_rows(hidden) && good_rows(weight) && hidden->dtype == weight->dtype &&
          hidden->width == weight->width && hidden->width >= 1 && hidden->width <= kMaxWidth &&
-         weight->n >= 1 && countable(hidden->n, weight->n);
+         weight->n >= 1 && hidden->n <= kMaxRows && weight->n <= kMaxRows && countable(hidden->n, weight->n);
 }
 
 // Whether the products can take the matrix as it lies.

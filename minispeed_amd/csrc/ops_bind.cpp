@@ -417,10 +417,10 @@ void need_head(const Tensor& hidden, const Tensor& weight, const Tensor& targets
   if (weight.scalar_type() != hidden.scalar_type())
     throw py::type_error(std::string("weight has dtype ") + c10::toString(weight.scalar_type()) +
                          ", hidden " + c10::toString(hidden.scalar_type()));
-  if (weight.size(0) < 1 || weight.size(0) > std::numeric_limits<int32_t>::max() ||
+  if (weight.size(0) < 1 || weight.size(0) > std::numeric_limits<int32_t>::max() - 1024 ||
       weight.size(1) < 1 || weight.size(1) > int64_t{1} << 20)
     bad_value("weight has shape " + shape_of(weight) +
-              ", expected a vocabulary of 1 to 2^31 - 1 and a width of 1 to 2^20");
+              ", expected a vocabulary of 1 to 2^31 - 1025 and a width of 1 to 2^20");
   bool match = targets.dim() == hidden.dim() - 1;
   for (int64_t d = 0; match && d < targets.dim(); ++d) match = targets.size(d) == hidden.size(d);
   if (!match)
