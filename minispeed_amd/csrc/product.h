@@ -70,6 +70,19 @@ struct product_args {
 __device__ __forceinline__ int plane_a(int pair) { return 0x850 >> (2 * pair) & 3; }
 __device__ __forceinline__ int plane_b(int pair) { return 0x244 >> (2 * pair) & 3; }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes from each lane's offset to `to` + 16 lane in LDS.  In assembly, as the compiler
+// would wait for it before the next read of LDS, of the other tile too; the wait is wait_loads().
+// (An instruction between setting m0 and its use is required.)
+__device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t offset, uint32_t to) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset),
+      "s"(rsrc)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // One operand's tile of R rows, fetched by NT threads.
 template <int R, int NT, Side S>
 struct Fetch {
@@ -112,21 +125,20 @@ struct Fetch {
   }
 
   // The tile at k0 of plane `shift` elements further, into LDS at `to`; `left` is k - k0.
-  __device__ void issue(int64_t shift, int k0, int left, char MS_LDS* to, int wave) const {
+  __device__ void issue(int64_t shift, int k0, int left, uint32_t to, int wave) const {
     const char* p = base + shift * 2 + (S == kAlong ? static_cast<int64_t>(k0) * 2 : k0 * ld_bytes);
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(p), 0, kRange, 0x00027000);
-    char MS_LDS* dst = to + wave * 1024;
+    const u32x4 rsrc = {static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)),
+                        static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) >> 32) & 0xffff, kRange,
+                        0x00027000};
+    const uint32_t dst = to + wave * 1024;
     if (left >= kStep) {
 #pragma unroll
-      for (int i = 0; i < kIssues; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, dst + i * NT * 16, 16, offset[i], 0, 0, 0);
+      for (int i = 0; i < kIssues; ++i) load_to_lds(rsrc, offset[i], dst + i * NT * 16);
     } else {
 #pragma unroll
       for (int i = 0; i < kIssues; ++i) {
         const int k = S == kAlong ? first_k : first_k + i * kRowsPer;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, dst + i * NT * 16, 16,
-                                                 k < left ? offset[i] : kBeyond, 0, 0, 0);
+        load_to_lds(rsrc, k < left ? offset[i] : kBeyond, dst + i * NT * 16);
       }
     }
   }
@@ -220,34 +232,50 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product(product_args p, Epi
 
   int pair = begin / steps, k0 = (begin - pair * steps) * kStep;
   auto issue = [&](int buffer) {
-    char MS_LDS* to = lds + buffer * kTile;
+    const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + buffer * kTile;
     fetch_a.issue(plane_a(pair) * p.a.plane, k0, p.k - k0, to, wave);
     fetch_b.issue(plane_b(pair) * p.b.plane, k0, p.k - k0, to + kTileA, wave);
     k0 += kStep;
     if (k0 >= p.k) k0 = 0, ++pair;
   };
-
-  if (begin < end) issue(0);
-  for (int s = begin; s < end; ++s) {
-    const int buffer = (s - begin) & 1;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    if (s + 1 < end) issue(buffer ^ 1);
+  typedef typename frag_of<T>::type frag;
+  frag a[2][MI], b[2][NI];
+  auto read = [&](int buffer, int ks, int set) {
     const char MS_LDS* tile = lds + buffer * kTile;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      typename frag_of<T>::type a[MI], b[NI];
+    for (int i = 0; i < MI; ++i) a[set][i] = frags_a.read(tile, i, ks);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = frags_a.read(tile, i, ks);
+    for (int j = 0; j < NI; ++j) b[set][j] = frags_b.read(tile + kTileA, j, ks);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](int set) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) b[j] = frags_b.read(tile + kTileA, j, ks);
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int j = 0; j < NI; ++j) acc[i][j] = mfma(a[set][i], b[set][j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  if (begin < end) {
+    issue(0);
+    wait_loads();
+    __syncthreads();
+    if (begin + 1 < end) issue(1);
+    read(0, 0, 0);
+  }
+  for (int s = begin; s < end; ++s) {
+    const int buffer = (s - begin) & 1;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j]);
+    for (int ks = 0; ks < 3; ++ks) {
+      read(buffer, ks + 1, (ks + 1) & 1);
+      multiply(ks & 1);
     }
-    // the fragments of this tile are in registers before any wave fetches into it again
-    asm volatile("" ::: "memory");
+    // This tile's fragments are in registers and the next tile is in LDS, in all waves
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (s + 2 < end) issue(buffer);
+    if (s + 1 < end) read(buffer ^ 1, 0, 0);
+    multiply(1);
   }
 
   epilogue.template store<MI, NI>(acc, tm * BM + wm * MI * 32, tn * BN + wn * NI * 32,
