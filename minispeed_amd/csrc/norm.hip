@@ -32,45 +32,47 @@ namespace {
 
 constexpr int64_t kMaxWidth = 16384;
 
-// The sum over a wave's lanes, in every lane.
-__device__ __forceinline__ float wave_sum(float x) {
+// The sum over each N neighbouring lanes (up to 16), in every lane.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float x) {
 #define MS_DPP_ADD(ctrl) \
   x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, 0xf, 0xf, true))
-  MS_DPP_ADD(0xB1);    // lanes 1 0 3 2
-  MS_DPP_ADD(0x4E);    // lanes 2 3 0 1
-  MS_DPP_ADD(0x141);   // each 8 lanes mirrored
-  MS_DPP_ADD(0x140);   // each 16 lanes mirrored
+  if (N > 1) MS_DPP_ADD(0xB1);    // lanes 1 0 3 2
+  if (N > 2) MS_DPP_ADD(0x4E);    // lanes 2 3 0 1
+  if (N > 4) MS_DPP_ADD(0x141);   // each 8 lanes mirrored
+  if (N > 8) MS_DPP_ADD(0x140);   // each 16 lanes mirrored
 #undef MS_DPP_ADD
+  return x;
+}
+
+// The sum over a wave's lanes, in every lane.
+__device__ __forceinline__ float wave_sum(float x) {
+  x = lanes_sum<16>(x);
   const int b = __float_as_int(x);
   return (__int_as_float(read_lane(b, 0)) + __int_as_float(read_lane(b, 16))) +
          (__int_as_float(read_lane(b, 32)) + __int_as_float(read_lane(b, 48)));
 }
 
-// Sums over a team of W waves.  Two places take turns, so that one barrier is enough: a
-// wave reaches the second next sum only after all have read this one.
+// Sums over a team of W waves (a power of two).  Two places take turns, so that one barrier is
+// enough: a wave reaches the second next sum only after all have read this one.
 template <int W>
 struct Team {
   float2 (*place)[16];
-  int turn = 0, wave, first;
+  int turn = 0, wave, slot;
 
-  __device__ Team(float2 (*p)[16], int wave_of_block) : place(p), wave(wave_of_block) {
-    first = wave / W * W;
-  }
+  __device__ Team(float2 (*p)[16], int wave_of_block)
+      : place(p), wave(wave_of_block), slot(wave_of_block / W * W + threadIdx.x % W) {}
   __device__ float2 sum(float2 x, bool both) {
     x.x = wave_sum(x.x);
     if (both) x.y = wave_sum(x.y);
     if (W == 1) return x;
     place[turn][wave] = x;
     __syncthreads();
-    float2 s = place[turn][first];
-#pragma unroll
-    for (int k = 1; k < W; ++k) {
-      const float2 o = place[turn][first + k];
-      s.x += o.x;
-      s.y += o.y;
-    }
+    x = place[turn][slot];
+    x.x = lanes_sum<W>(x.x);
+    if (both) x.y = lanes_sum<W>(x.y);
     turn ^= 1;
-    return s;
+    return x;
   }
   __device__ float sum(float x) { return sum(make_float2(x, 0.0f), false).x; }
 };
@@ -129,8 +131,15 @@ __device__ __forceinline__ float2 row_stats(const float (&x)[C][V], const int64_
   return make_float2(mean, 1.0f / sqrtf(var + eps));
 }
 
-// A team of W waves to a row; blocks of at least 4 waves.
-template <typename T, int W, int C, bool Layer>
+// A vector's columns; zeros where there is none.
+template <int V, typename T>
+__device__ __forceinline__ Pack<T, V> vector_columns(const void* p, int64_t c, int64_t width) {
+  return p ? load_columns<V>(static_cast<const T*>(p), c, width) : Pack<T, V>{};
+}
+
+// A team of W waves to a row; blocks of at least 4 waves.  Everything is loaded before the first
+// sum, which all would wait for.
+template <typename T, int W, int C, bool Layer, bool Post>
 __global__ __launch_bounds__(W < 4 ? 256 : W * 64) void k_norm(forward_args a) {
   constexpr int V = 16 / sizeof(T), kWaves = W < 4 ? 4 : W;
   __shared__ float2 place[2][16];
@@ -143,42 +152,53 @@ __global__ __launch_bounds__(W < 4 ? 256 : W * 64) void k_norm(forward_args a) {
   Team<W> team(place, wave);
   int64_t col[C];
   float x[C][V];
-  Pack<T, V> raw[C], more[C];
+  Pack<T, V> raw[C], more[C], weight[C], bias[C], gate[C], block_weight[C], block_bias[C];
   const T* residual = static_cast<const T*>(a.residual.data) + row_start(a.residual, row);
-  const T* block = static_cast<const T*>(a.block.data) + (a.block.data ? row_start(a.block, row) : 0);
+  const T* block =
+      a.block.data ? static_cast<const T*>(a.block.data) + row_start(a.block, row) : nullptr;
+  const T* gates = a.gate ? static_cast<const T*>(a.gate) + row / a.gate_rows * width : nullptr;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     col[c] = (static_cast<int64_t>(c) * W * 64 + lane) * V;
     raw[c] = load_columns<V>(residual, col[c], width);
-    if (a.block.data) more[c] = load_columns<V>(block, col[c], width);
+  }
+  if (block) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) more[c] = load_columns<V>(block, col[c], width);
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    weight[c] = load_columns<V>(static_cast<const T*>(a.weight), col[c], width);
+    if (Layer) bias[c] = vector_columns<V, T>(a.bias, col[c], width);
+    if (Post) {
+      block_weight[c] = load_columns<V>(static_cast<const T*>(a.block_weight), col[c], width);
+      if (Layer) block_bias[c] = vector_columns<V, T>(a.block_bias, col[c], width);
+    }
+  }
+  if (gates) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) gate[c] = load_columns<V>(gates, col[c], width);
   }
   float2 post = make_float2(0.0f, 1.0f);
-  const T* gate = static_cast<const T*>(a.gate) + (a.gate ? row / a.gate_rows * width : 0);
-  if (a.block.data) {
+  if (block) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < V; ++e) x[c][e] = widen(more[c].v[e]);
-    if (a.block_weight) {
+    if (Post) {
       post = row_stats<Layer>(x, col, width, a.eps, team);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const Pack<T, V> w = load_columns<V>(static_cast<const T*>(a.block_weight), col[c], width);
-        Pack<T, V> b{};
-        if (Layer && a.block_bias)
-          b = load_columns<V>(static_cast<const T*>(a.block_bias), col[c], width);
+      for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          x[c][e] = fmaf((x[c][e] - post.x) * post.y, widen(w.v[e]), widen(b.v[e]));
-      }
+          x[c][e] = fmaf((x[c][e] - post.x) * post.y, widen(block_weight[c].v[e]),
+                         Layer ? widen(block_bias[c].v[e]) : 0.0f);
     }
-    if (a.gate) {
+    if (gates) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const Pack<T, V> g = load_columns<V>(gate, col[c], width);
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[c][e] *= widen(g.v[e]);
-      }
+        for (int e = 0; e < V; ++e) x[c][e] *= widen(gate[c].v[e]);
     }
     T* next = static_cast<T*>(a.next) + row * width;
 #pragma unroll
@@ -201,20 +221,18 @@ __global__ __launch_bounds__(W < 4 ? 256 : W * 64) void k_norm(forward_args a) {
   T* out = static_cast<T*>(a.out) + row * width;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const Pack<T, V> w = load_columns<V>(static_cast<const T*>(a.weight), col[c], width);
-    Pack<T, V> b{}, o;
-    if (Layer && a.bias) b = load_columns<V>(static_cast<const T*>(a.bias), col[c], width);
+    Pack<T, V> o;
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      o.v[e] = narrow<T>(fmaf((x[c][e] - pre.x) * pre.y, widen(w.v[e]), widen(b.v[e])));
+      o.v[e] = narrow<T>(fmaf((x[c][e] - pre.x) * pre.y, widen(weight[c].v[e]),
+                              Layer ? widen(bias[c].v[e]) : 0.0f));
     store_columns<V>(out, col[c], width, o);
   }
   if (a.stats && lane == 0) {
-    const int fields = a.block.data && a.block_weight ? 4 : 2;
-    float* s = a.stats + row * fields;
+    float* s = a.stats + row * (Post ? 4 : 2);
     s[0] = pre.x;
     s[1] = pre.y;
-    if (fields == 4) {
+    if (Post) {
       s[2] = post.x;
       s[3] = post.y;
     }
@@ -238,77 +256,140 @@ struct backward_args {
 // Waves of a block: eight, so that two blocks of a CU wait at different barriers, or a row's.
 constexpr int block_waves(int w) { return w < 8 ? 8 : w; }
 
-// What a thread has of a row: 4 neighbouring columns C times, so that the sums and the
-// next row's values fit in the registers beside it.
-constexpr int kOwn = 4;
-template <typename T, int C>
-struct Row {
-  Pack<T, kOwn> dy[C], dx[C], x[C], b[C];
-  float mean, rstd, block_mean, block_rstd;
-  bool live;
+// What a thread has of a row, 16 bytes at a time, kept as they were loaded until they are used:
+// taken apart earlier, they would be waited for.
+template <typename T>
+struct Words {
+  uint32_t w[4];
+  __device__ float operator[](int e) const {
+    Pack<T, 16 / sizeof(T)> x;
+    __builtin_memcpy(&x, w, 16);
+    return widen(x.v[e]);
+  }
+};
+
+// The columns of a thread: 16 bytes at each of C byte offsets in a row.  Where the rows are whole
+// 16 bytes long, those behind the end are not loaded, and zeros.
+template <typename T, int W, int C>
+struct Columns {
+  static constexpr int V = 16 / sizeof(T);
+  uint32_t at[C];
+  int width;
+  bool even;
+
+  __device__ Columns(int lane, int width_of) : width(width_of), even(width_of % V == 0) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) at[c] = (c * W * 64 + lane) * 16;
+  }
+  __device__ int column(int c, int e) const { return static_cast<int>(at[c] / sizeof(T)) + e; }
+  __device__ bool in(int c, int e = 0) const { return column(c, e) < width; }
+  __device__ Words<T> load(const T* row, int c) const {
+    Words<T> x = {{0, 0, 0, 0}};
+    typedef typename raw_of<16>::type raw;
+    if (even) {
+      if (in(c)) {
+        const raw r = *reinterpret_cast<const raw*>(reinterpret_cast<const char*>(row) + at[c]);
+        __builtin_memcpy(x.w, &r, 16);
+      }
+    } else {
+      const Pack<T, V> p = load_columns<V>(row, column(c, 0), width);
+      __builtin_memcpy(x.w, &p, 16);
+    }
+    return x;
+  }
+  __device__ void store(T* row, int c, const Pack<T, V>& x) const {
+    if (even) {
+      if (in(c)) {
+        typedef typename raw_of<16>::type raw;
+        raw r;
+        __builtin_memcpy(&r, &x, 16);
+        *reinterpret_cast<raw*>(reinterpret_cast<char*>(row) + at[c]) = r;
+      }
+    } else {
+      store_columns<V>(row, column(c, 0), width, x);
+    }
+  }
 };
 
 // Teams of W waves.  An item is up to item_rows neighbouring rows that share a gate;
 // teams take items in turn, all the same number of rows, since the barriers are the
-// block's.  A row's loads are under way while the one before is worked on.
+// block's.  Rows of up to 16 bytes a thread (C = 1): a row's loads are under way while
+// the one before is worked on, and all sums are in registers.  Longer ones have neither
+// registers: operands are loaded where they are used, and the first two sums are in LDS.
 template <typename T, int W, int C, bool Layer, bool Post>
 __global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args a) {
-  constexpr int V = kOwn, kTeams = block_waves(W) / W;
+  constexpr int V = 16 / sizeof(T), kTeams = block_waves(W) / W;
+  constexpr bool kShort = C == 1;
   constexpr int kVectors = (Layer ? 2 : 1) * (Post ? 2 : 1);
+  constexpr int kInLds = kShort ? 0 : kVectors < 2 ? kVectors : 2, kInRegs = kVectors - kInLds;
   // weight, bias, block weight, block bias, as far as there are any
   constexpr int kWeight = 0, kBias = Layer, kBlockWeight = Post ? 1 + Layer : 0,
                 kBlockBias = Layer && Post ? 3 : 0;
   __shared__ float2 place[2][16];
-  __shared__ float joined[kTeams > 1 ? W * 64 * C * V : 1];
+  __shared__ float joined[kShort ? (kTeams > 1 ? W * 64 * V : 1) : kInLds * W * 64 * C * V];
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid % (W * 64);
-  const int64_t width = a.next.width;
+  const int width = static_cast<int>(a.next.width);
   const float inverse = 1.0f / static_cast<float>(width);
   Team<W> team(place, wave);
-  int64_t col[C];
-  Pack<T, V> weight[C], block_weight[C], block_bias[C], gate[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    col[c] = (static_cast<int64_t>(c) * W * 64 + lane) * V;
-    weight[c] = load_columns<V>(static_cast<const T*>(a.weight), col[c], width);
-    if (Post) {
-      block_weight[c] = load_columns<V>(static_cast<const T*>(a.block_weight), col[c], width);
-      block_bias[c] = Pack<T, V>{};
-      if (Layer && a.block_bias)
-        block_bias[c] = load_columns<V>(static_cast<const T*>(a.block_bias), col[c], width);
-    }
+  const Columns<T, W, C> cols(lane, width);
+  const T* const weights = static_cast<const T*>(a.weight);
+  const T* const block_weights = static_cast<const T*>(a.block_weight);
+  const T* const block_biases = static_cast<const T*>(a.block_bias);
+  Words<T> weight[C], block_weight[C], block_bias[C], gate[C];
+  if (kShort) {
+    weight[0] = cols.load(weights, 0);
+    if (Post) block_weight[0] = cols.load(block_weights, 0);
+    if (Post && Layer && block_biases) block_bias[0] = cols.load(block_biases, 0);
   }
-  float sums[kVectors][C][V] = {}, gate_sum[C][V] = {};
+  float sums[kInRegs > 0 ? kInRegs : 1][C][V] = {}, gate_sum[C][V] = {};
+  if (!kShort) {
+    for (int k = tid; k < kInLds * W * 64 * C * V; k += W * 64) joined[k] = 0.0f;
+  }
+  // (a thread's own places of it, so that no barrier is needed)
+  auto add = [&](int k, int c, int e, float x) {
+    if (k < kInLds)
+      joined[((k * C + c) * V + e) * W * 64 + lane] += x;
+    else
+      sums[k - kInLds][c][e] += x;
+  };
   const bool block_there = a.block.data != nullptr, gated = a.gate != nullptr;
+  const bool dout_there = a.dout.data != nullptr, dnext_there = a.dnext.data != nullptr;
   constexpr int kFields = Post ? 4 : 2;
 
-  const int64_t teams = static_cast<int64_t>(gridDim.x) * kTeams;
-  const int64_t rounds = (a.items + teams - 1) / teams;
-  const int64_t first_item = static_cast<int64_t>(blockIdx.x) * kTeams + wave / W;
-
-  // row k of the team's item of a round; not live where there is none
-  auto place_of = [&](int64_t round, int64_t k, bool& live) {
-    const int64_t item = round * teams + first_item;
-    const int64_t group = item / a.parts, part = item - group * a.parts;
-    const int64_t in = part * a.item_rows + k;
-    live = round < rounds && item < a.items && in < a.gate_rows && k < a.item_rows;
-    return group * a.gate_rows + in;
+  const int teams = static_cast<int>(gridDim.x) * kTeams, items = static_cast<int>(a.items);
+  const int rounds = (items + teams - 1) / teams;
+  const int parts = static_cast<int>(a.parts), item_rows = static_cast<int>(a.item_rows);
+  // The rows [row, end) of the team's item of a round: none where it has no item.
+  auto place_of = [&](int round, int& item, int& group, int& row, int& end) {
+    item = uniform(round * teams + static_cast<int>(blockIdx.x) * kTeams + wave / W);
+    const bool live = round < rounds && item < items;
+    group = live ? item / parts : 0;
+    const int begin = group * static_cast<int>(a.gate_rows);
+    row = begin + (live ? item - group * parts : 0) * item_rows;
+    end = live ? min(row + item_rows, begin + static_cast<int>(a.gate_rows)) : row;
   };
-  auto fetch = [&](int64_t round, int64_t k, Row<T, C>& r) {
-    const int64_t row = place_of(round, k, r.live);
-    if (!r.live) return;
-    const T* px = static_cast<const T*>(a.next.data) + row_start(a.next, row);
-    const T* py = a.dout.data ? static_cast<const T*>(a.dout.data) + row_start(a.dout, row) : nullptr;
-    const T* pn = a.dnext.data ? static_cast<const T*>(a.dnext.data) + row_start(a.dnext, row) : nullptr;
-    const T* pb = block_there ? static_cast<const T*>(a.block.data) + row_start(a.block, row) : nullptr;
+
+  auto row_of = [](const ms_rows_t& m, int row) {
+    return static_cast<const T*>(m.data) + row_start(m, row);
+  };
+  struct Row {
+    Words<T> dy[C], dx[C], x[C], b[C];
+    float mean, rstd, block_mean, block_rstd;
+  };
+  // The loads of a row, without branches that depend on it: row 0's, in the place of none
+  auto fetch = [&](int row, Row& r) {
+    const T *px = row_of(a.next, row), *py = dout_there ? row_of(a.dout, row) : px;
+    const T *pn = dnext_there ? row_of(a.dnext, row) : px, *pb = block_there ? row_of(a.block, row) : px;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      r.x[c] = load_columns<V>(px, col[c], width);
-      r.dy[c] = r.dx[c] = r.b[c] = Pack<T, V>{};
-      if (py) r.dy[c] = load_columns<V>(py, col[c], width);
-      if (pn) r.dx[c] = load_columns<V>(pn, col[c], width);
-      if (pb) r.b[c] = load_columns<V>(pb, col[c], width);
+      r.x[c] = cols.load(px, c);
+      r.dy[c] = cols.load(py, c);
+      if (kShort) {
+        r.dx[c] = cols.load(pn, c);
+        r.b[c] = cols.load(pb, c);
+      }
     }
-    const float* s = a.stats + row * kFields;
+    const float* s = a.stats + static_cast<int64_t>(row) * kFields;
     r.mean = s[0];
     r.rstd = s[1];
     if (Post) {
@@ -317,84 +398,101 @@ __global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args
     }
   };
 
-  Row<T, C> now, then;
-  fetch(0, 0, then);
-  for (int64_t round = 0; round < rounds; ++round) {
-    const int64_t item = round * teams + first_item;
-    const int64_t group = item / a.parts;
-    if (gated && item < a.items) {
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        gate[c] = load_columns<V>(static_cast<const T*>(a.gate) + group * width, col[c], width);
-    }
-    for (int64_t k = 0; k < a.item_rows; ++k) {
-      now = then;
-      const bool last = k + 1 == a.item_rows;
-      fetch(last ? round + 1 : round, last ? 0 : k + 1, then);
-      bool live;
-      const int64_t row = place_of(round, k, live);
+  Row now, then;
+  int item, group, row, end;
+  place_of(0, item, group, row, end);
+  if (kShort) fetch(row < end ? row : 0, then);
+  for (int round = 0; round < rounds; ++round) {
+    int next_item, next_group, next_row, next_end;
+    place_of(round + 1, next_item, next_group, next_row, next_end);
+    const T* gates = static_cast<const T*>(a.gate) + static_cast<int64_t>(group) * width;
+    if (gated && kShort) gate[0] = cols.load(gates, 0);
+    for (int k = 0; k < item_rows; ++k, ++row) {
+      const bool live = row < end;
+      if (kShort) {
+        now = then;
+        const int following = k + 1 == item_rows ? (next_row < next_end ? next_row : 0)
+                                                 : (row + 1 < end ? row + 1 : 0);
+        fetch(following, then);
+      } else {
+        fetch(live ? row : 0, now);
+      }
       float2 s = make_float2(0.0f, 0.0f);
-      if (live) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) {
+        if (!kShort) weight[c] = cols.load(weights, c);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float v = (widen(now.x[c].v[e]) - now.mean) * now.rstd;
-            const float t = widen(now.dy[c].v[e]) * widen(weight[c].v[e]);
-            s.x = fmaf(t, v, s.x);
-            s.y += t;
-          }
+        for (int e = 0; e < V; ++e) {
+          const float v = (now.x[c][e] - now.mean) * now.rstd;
+          const float t = (dout_there ? now.dy[c][e] : 0.0f) * weight[c][e];
+          s.x = fmaf(t, v, s.x);
+          if (Layer) s.y += t;
+        }
       }
       s = team.sum(s, Layer);
       float d[C][V];
       float2 s2 = make_float2(0.0f, 0.0f);
       if (live) {
         const float along = s.x * inverse, level = Layer ? s.y * inverse : 0.0f;
+        T* out = static_cast<T*>(a.dresidual) + static_cast<int64_t>(row) * width;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
+          if (!kShort) {
+            now.dx[c] = dnext_there ? cols.load(row_of(a.dnext, row), c) : Words<T>{};
+            weight[c] = cols.load(weights, c);
+          }
           Pack<T, V> o;
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float v = (widen(now.x[c].v[e]) - now.mean) * now.rstd, g = widen(now.dy[c].v[e]);
-            const float t = g * widen(weight[c].v[e]);
-            sums[kWeight][c][e] = fmaf(g, v, sums[kWeight][c][e]);
-            if (Layer) sums[kBias][c][e] += g;
-            float r = fmaf(-v, along, t);
+            const float v = (now.x[c][e] - now.mean) * now.rstd;
+            const float g = dout_there ? now.dy[c][e] : 0.0f;
+            add(kWeight, c, e, g * v);
+            if (Layer) add(kBias, c, e, g);
+            float r = fmaf(-v, along, g * weight[c][e]);
             if (Layer) r -= level;
-            d[c][e] = fmaf(r, now.rstd, widen(now.dx[c].v[e]));
+            d[c][e] = fmaf(r, now.rstd, dnext_there ? now.dx[c][e] : 0.0f);
             o.v[e] = narrow<T>(d[c][e]);
           }
-          store_columns<V>(static_cast<T*>(a.dresidual) + row * width, col[c], width, o);
+          cols.store(out, c, o);
         }
         if (block_there) {
 #pragma unroll
-          for (int c = 0; c < C; ++c)
+          for (int c = 0; c < C; ++c) {
+            if (!kShort) {
+              now.b[c] = cols.load(row_of(a.block, row), c);
+              if (Post) block_weight[c] = cols.load(block_weights, c);
+              if (Post && Layer && block_biases) block_bias[c] = cols.load(block_biases, c);
+              if (gated) gate[c] = cols.load(gates, c);
+            }
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              float q = d[c][e] * a.scale, u = widen(now.b[c].v[e]), w = 0.0f;
+              float q = d[c][e] * a.scale, u = now.b[c][e], w = 0.0f;
               if (Post) {
                 w = (u - now.block_mean) * now.block_rstd;
-                u = fmaf(w, widen(block_weight[c].v[e]), widen(block_bias[c].v[e]));
+                if (gated)
+                  u = fmaf(w, block_weight[c][e], Layer && block_biases ? block_bias[c][e] : 0.0f);
               }
               if (gated) {
                 gate_sum[c][e] = fmaf(q, u, gate_sum[c][e]);
-                q *= widen(gate[c].v[e]);
+                q *= gate[c][e];
               }
               if (Post) {
-                sums[kBlockWeight][c][e] = fmaf(q, w, sums[kBlockWeight][c][e]);
-                if (Layer) sums[kBlockBias][c][e] += q;
+                add(kBlockWeight, c, e, q * w);
+                if (Layer) add(kBlockBias, c, e, q);
                 // (the weight is 0 behind the row's end)
-                q *= widen(block_weight[c].v[e]);
+                q *= block_weight[c][e];
                 s2.x = fmaf(q, w, s2.x);
-                s2.y += q;
+                if (Layer) s2.y += q;
               }
               d[c][e] = q;
             }
+          }
         }
       }
       if (Post) s2 = team.sum(s2, Layer);
       if (live && block_there) {
         const float along = s2.x * inverse, level = Layer ? s2.y * inverse : 0.0f;
+        T* out = static_cast<T*>(a.dblock) + static_cast<int64_t>(row) * width;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           Pack<T, V> o;
@@ -402,34 +500,39 @@ __global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args
           for (int e = 0; e < V; ++e) {
             float q = d[c][e];
             if (Post) {
-              const float w = (widen(now.b[c].v[e]) - now.block_mean) * now.block_rstd;
+              const float w = (now.b[c][e] - now.block_mean) * now.block_rstd;
               q = fmaf(-w, along, q);
               if (Layer) q -= level;
               q *= now.block_rstd;
             }
             o.v[e] = narrow<T>(q);
           }
-          store_columns<V>(static_cast<T*>(a.dblock) + row * width, col[c], width, o);
+          cols.store(out, c, o);
         }
       }
     }
-    if (gated && item < a.items) {
+    if (gated && item < items) {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         if (a.gate_sums) {
+          float* out = a.gate_sums + static_cast<int64_t>(item) * width;
 #pragma unroll
           for (int e = 0; e < V; ++e)
-            if (col[c] + e < width) a.gate_sums[item * width + col[c] + e] = gate_sum[c][e];
+            if (cols.in(c, e)) out[cols.column(c, e)] = gate_sum[c][e];
         } else {
           Pack<T, V> o;
 #pragma unroll
           for (int e = 0; e < V; ++e) o.v[e] = narrow<T>(gate_sum[c][e]);
-          store_columns<V>(static_cast<T*>(a.dgate) + group * width, col[c], width, o);
+          cols.store(static_cast<T*>(a.dgate) + static_cast<int64_t>(group) * width, c, o);
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) gate_sum[c][e] = 0.0f;
       }
     }
+    item = next_item;
+    group = next_group;
+    row = next_row;
+    end = next_end;
   }
 
   // The block's sums: one team after the other adds in LDS.
@@ -441,13 +544,11 @@ __global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args
         __syncthreads();
         if (which != t) continue;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            float* p = &joined[(c * V + e) * W * 64 + lane];
-            if (t > 0) sums[k][c][e] += *p;
-            *p = sums[k][c][e];
-          }
+        for (int e = 0; e < V; ++e) {
+          float* p = &joined[e * W * 64 + lane];
+          if (t > 0) sums[k < kInRegs ? k : 0][0][e] += *p;
+          *p = sums[k < kInRegs ? k : 0][0][e];
+        }
       }
     }
     if (which == kTeams - 1) {
@@ -456,7 +557,9 @@ __global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if (col[c] + e < width) out[col[c] + e] = sums[k][c][e];
+          if (cols.in(c, e))
+            out[cols.column(c, e)] = k < kInLds ? joined[((k * C + c) * V + e) * W * 64 + lane]
+                                                : sums[k - kInLds][c][e];
     }
   }
 }
@@ -532,21 +635,26 @@ int run_forward(const forward_args& a, bool layer, hipStream_t s) {
   constexpr int kWaves = W < 4 ? 4 : W;
   const int64_t blocks = ceil_div(a.residual.n, kWaves / W);
   if (!fits(blocks, kWaves * 64)) return MS_OPS_EINVAL;
-  return layer ? launch(k_norm<T, W, C, true>, blocks, kWaves * 64, s, a)
-               : launch(k_norm<T, W, C, false>, blocks, kWaves * 64, s, a);
+  if (a.block_weight)
+    return layer ? launch(k_norm<T, W, C, true, true>, blocks, kWaves * 64, s, a)
+                 : launch(k_norm<T, W, C, false, true>, blocks, kWaves * 64, s, a);
+  return layer ? launch(k_norm<T, W, C, true, false>, blocks, kWaves * 64, s, a)
+               : launch(k_norm<T, W, C, false, false>, blocks, kWaves * 64, s, a);
 }
 
-// A wave to a row as long as it holds it in 64 bytes a lane, as no barrier is needed then.
+// A wave to a row while it holds it in 32 bytes a lane, as no barrier is needed then; more
+// waves rather than more registers for longer ones (2048 fp16: 64 bytes a lane 41.6 us).
 template <typename T>
 int choose_forward(const forward_args& a, bool layer, hipStream_t s) {
   const int64_t chunks = ceil_div(a.residual.width, 16 / static_cast<int>(sizeof(T)) * 64);
   if (chunks <= 1) return run_forward<T, 1, 1>(a, layer, s);
   if (chunks <= 2) return run_forward<T, 1, 2>(a, layer, s);
-  if (chunks <= 4) return run_forward<T, 1, 4>(a, layer, s);
-  if (chunks <= 8) return run_forward<T, 4, 2>(a, layer, s);
-  if (chunks <= 16) return run_forward<T, 4, 4>(a, layer, s);
+  if (chunks <= 4) return run_forward<T, 4, 1>(a, layer, s);
+  if (chunks <= 8) return run_forward<T, 8, 1>(a, layer, s);
+  if (chunks <= 16) return run_forward<T, 16, 1>(a, layer, s);
   if (chunks <= 32) return run_forward<T, 16, 2>(a, layer, s);
-  return run_forward<T, 16, 4>(a, layer, s);
+  if constexpr (sizeof(T) == 4) return run_forward<T, 16, 4>(a, layer, s);
+  return MS_OPS_EINVAL;       // (no 2-byte row is that long)
 }
 
 // How backward cuts the rows: teams of `waves`, `blocks` of them, items of a gate's rows.
@@ -555,9 +663,9 @@ struct Shares {
   int64_t blocks, parts, item_rows, items;
 };
 
-Shares shares_of(int64_t n, int64_t width, int64_t gates) {
+Shares shares_of(int64_t n, int64_t width, int64_t bytes, int64_t gates) {
   Shares s{};
-  const int64_t chunks = ceil_div(width, kOwn * 64);
+  const int64_t chunks = ceil_div(width * bytes, 16 * 64);
   s.waves = 1;
   while (s.waves < 16 && s.waves < chunks) s.waves *= 2;
   const int64_t teams_of_block = block_waves(s.waves) / s.waves;
@@ -594,7 +702,7 @@ int run_backward(const backward_args& a, bool layer, bool post, int64_t blocks, 
 
 template <typename T>
 int choose_backward(const backward_args& a, bool layer, bool post, const Shares& sh, hipStream_t s) {
-  const int64_t chunks = ceil_div(a.next.width, kOwn * 64);
+  const int64_t chunks = ceil_div(a.next.width * static_cast<int64_t>(sizeof(T)), 16 * 64);
   switch (sh.waves) {
     case 1: return run_backward<T, 1, 1>(a, layer, post, sh.blocks, s);
     case 2: return run_backward<T, 2, 1>(a, layer, post, sh.blocks, s);
@@ -603,7 +711,8 @@ int choose_backward(const backward_args& a, bool layer, bool post, const Shares&
   }
   if (chunks <= 16) return run_backward<T, 16, 1>(a, layer, post, sh.blocks, s);
   if (chunks <= 32) return run_backward<T, 16, 2>(a, layer, post, sh.blocks, s);
-  return run_backward<T, 16, 4>(a, layer, post, sh.blocks, s);
+  if constexpr (sizeof(T) == 4) return run_backward<T, 16, 4>(a, layer, post, sh.blocks, s);
+  return MS_OPS_EINVAL;
 }
 
 template <typename T>
@@ -665,7 +774,7 @@ int64_t ms_norm_grad_workspace(int64_t n, int64_t width, int32_t dtype, int32_t 
       (gates && n % gates))
     return MS_OPS_EINVAL;
   if (n == 0) return 0;
-  return grad_workspace(shares_of(n, width, gates), width, kind == MS_NORM_LAYER,
+  return grad_workspace(shares_of(n, width, dtype_bytes(dtype), gates), width, kind == MS_NORM_LAYER,
                         post != 0, gates != 0);
 }
 
@@ -697,7 +806,7 @@ int ms_norm_grad(const ms_rows_t* dout, const ms_rows_t* dnext, const ms_rows_t*
                                      : run_zeros<f16>(zeros, count, width, s);
   }
   if ((!dout && !dnext) || !stats || !dresidual || (block && !dblock)) return MS_OPS_EINVAL;
-  const Shares sh = shares_of(n, width, gates);
+  const Shares sh = shares_of(n, width, dtype_bytes(next->dtype), gates);
   if (workspace_bytes < grad_workspace(sh, width, layer, post, gate) || !workspace ||
       reinterpret_cast<uintptr_t>(workspace) % 16)
     return MS_OPS_EWORKSPACE;
