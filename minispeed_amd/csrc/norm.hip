@@ -77,25 +77,84 @@ struct Team {
   __device__ float sum(float x) { return sum(make_float2(x, 0.0f), false).x; }
 };
 
-// V values at column c of a row of `width`; those behind its end are zeros.
-template <int V, typename T>
-__device__ __forceinline__ Pack<T, V> load_columns(const T* p, int64_t c, int64_t width) {
-  if (c + V <= width) return load<V>(p + c);
-  Pack<T, V> x;
-#pragma unroll
-  for (int e = 0; e < V; ++e) x.v[e] = c + e < width ? p[c + e] : static_cast<T>(0.0f);
-  return x;
-}
-template <int V, typename T>
-__device__ __forceinline__ void store_columns(T* p, int64_t c, int64_t width, const Pack<T, V>& x) {
-  if (c + V <= width) {
-    store<V>(p + c, x);
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (c + e < width) p[c + e] = x.v[e];
+// What a thread has of a row, 16 bytes at a time, kept as they were loaded until they are used:
+// taken apart earlier, they would be waited for.
+template <typename T>
+struct Words {
+  uint32_t w[4];
+  __device__ float operator[](int e) const {
+    Pack<T, 16 / sizeof(T)> x;
+    __builtin_memcpy(&x, w, 16);
+    return widen(x.v[e]);
   }
-}
+};
+
+// The columns of a thread: 16 bytes at each of C byte offsets in a row.  Rows are reached as
+// buffers that end with them, so that what lies behind the end is neither loaded (zeros) nor
+// stored, by words and without a branch: behind a branch a wave could no longer tell its
+// loads from its stores, which are counted together, and would wait for both.  The last value
+// of a row of an odd number of 2-byte ones is moved by itself.
+typedef uint32_t words4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t kNowhere = 0x7ffffff0;
+
+template <typename T, int W, int C>
+struct Columns {
+  static constexpr int V = 16 / sizeof(T);
+  uint32_t at[C], last_at, last_word;
+  int width;
+  bool odd;
+
+  __device__ Columns(int lane, int width_of) : width(width_of) {
+    odd = sizeof(T) == 2 && width % 2 != 0;
+    const uint32_t end = (width - 1) * sizeof(T);
+    last_at = kNowhere;
+    last_word = 4;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      at[c] = (c * W * 64 + lane) * 16;
+      if (odd && end >= at[c] && end < at[c] + 16) last_at = end, last_word = c * 4 + (end - at[c]) / 4;
+    }
+    if (last_at == kNowhere) last_word = 4 * C;
+  }
+  __device__ int column(int c, int e) const { return static_cast<int>(at[c] / sizeof(T)) + e; }
+  __device__ bool in(int c, int e = 0) const { return column(c, e) < width; }
+  // A row's buffer, or with there = false one of nothing.
+  __device__ __amdgpu_buffer_rsrc_t buffer(const T* row, bool there = true) const {
+    const int bytes = width * static_cast<int>(sizeof(T));
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row), 0, there ? bytes : 0, 0x00027000);
+  }
+  __device__ void load(const T* row, Words<T> (&x)[C], bool there = true) const {
+    const __amdgpu_buffer_rsrc_t b = buffer(row, there);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const words4 r = __builtin_amdgcn_raw_buffer_load_b128(b, at[c], 0, 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[c].w[k] = r[k];
+    }
+    if (odd) {
+      const uint32_t last = __builtin_amdgcn_raw_buffer_load_b16(b, last_at, 0, 0);
+#pragma unroll
+      for (int k = 0; k < 4 * C; ++k)
+        if (last_word == static_cast<uint32_t>(k)) x[k / 4].w[k % 4] = last;
+    }
+  }
+  __device__ void store(T* row, const Pack<T, V> (&x)[C], bool there = true) const {
+    const __amdgpu_buffer_rsrc_t b = buffer(row, there);
+    uint32_t last = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      words4 r;
+      __builtin_memcpy(&r, &x[c], 16);
+      __builtin_amdgcn_raw_buffer_store_b128(r, b, at[c], 0, 0);
+      if (odd) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (last_word == static_cast<uint32_t>(c * 4 + k)) last = r[k];
+      }
+    }
+    if (odd) __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(last), b, last_at, 0, 0);
+  }
+};
 
 struct forward_args {
   ms_rows_t residual, block;           // block.data NULL: none
@@ -107,9 +166,10 @@ struct forward_args {
 };
 
 // Mean and reciprocal deviation of the team's row, held as C groups of V.
-template <bool Layer, int C, int V, typename Of>
-__device__ __forceinline__ float2 row_stats(const float (&x)[C][V], const int64_t (&col)[C],
-                                            int64_t width, float eps, Of& team) {
+template <bool Layer, int C, int V, typename Cols, typename Of>
+__device__ __forceinline__ float2 row_stats(const float (&x)[C][V], const Cols& cols, float eps,
+                                            Of& team) {
+  const float width = static_cast<float>(cols.width);
   float mean = 0.0f, sq = 0.0f;
   if (Layer) {
     float s = 0.0f;
@@ -117,7 +177,7 @@ __device__ __forceinline__ float2 row_stats(const float (&x)[C][V], const int64_
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < V; ++e) s += x[c][e];
-    mean = team.sum(s) / static_cast<float>(width);
+    mean = team.sum(s) / width;
   }
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -125,16 +185,10 @@ __device__ __forceinline__ float2 row_stats(const float (&x)[C][V], const int64_
     for (int e = 0; e < V; ++e) {
       const float d = x[c][e] - mean;
       // (columns behind the end are zeros, but for the mean)
-      if (!Layer || col[c] + e < width) sq = fmaf(d, d, sq);
+      if (!Layer || cols.in(c, e)) sq = fmaf(d, d, sq);
     }
-  const float var = team.sum(sq) / static_cast<float>(width);
+  const float var = team.sum(sq) / width;
   return make_float2(mean, 1.0f / sqrtf(var + eps));
-}
-
-// A vector's columns; zeros where there is none.
-template <int V, typename T>
-__device__ __forceinline__ Pack<T, V> vector_columns(const void* p, int64_t c, int64_t width) {
-  return p ? load_columns<V>(static_cast<const T*>(p), c, width) : Pack<T, V>{};
 }
 
 // A team of W waves to a row; blocks of at least 4 waves.  Everything is loaded before the first
@@ -147,87 +201,72 @@ __global__ __launch_bounds__(W < 4 ? 256 : W * 64) void k_norm(forward_args a) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kWaves / W) + wave / W;
   if (W == 1 && row >= a.residual.n) return;
   static_assert(W == 1 || W >= 4, "the waves of a block belong to one row, or each has its own");
-  const int64_t width = a.residual.width;
+  const int width = static_cast<int>(a.residual.width);
   const int lane = tid % (W * 64);
   Team<W> team(place, wave);
-  int64_t col[C];
+  const Columns<T, W, C> cols(lane, width);
+  Words<T> residual[C], more[C], weight[C], bias[C], gate[C], block_weight[C], block_bias[C];
+  const bool block_there = a.block.data != nullptr, gated = a.gate != nullptr;
+  auto vector = [&](const void* p, Words<T>(&x)[C]) {
+    const T* some = static_cast<const T*>(p ? p : a.weight);
+    cols.load(some, x, p != nullptr);
+  };
+  cols.load(static_cast<const T*>(a.residual.data) + row_start(a.residual, row), residual);
+  const T* rows = static_cast<const T*>(block_there ? a.block.data : a.residual.data);
+  cols.load(rows + (block_there ? row_start(a.block, row) : 0), more, block_there);
+  vector(a.weight, weight);
+  if (Layer) vector(a.bias, bias);
+  if (Post) vector(a.block_weight, block_weight);
+  if (Post && Layer) vector(a.block_bias, block_bias);
+  if (gated)
+    cols.load(static_cast<const T*>(a.gate) +
+                  static_cast<uint32_t>(row) / static_cast<uint32_t>(a.gate_rows) *
+                      static_cast<int64_t>(width),
+              gate);
   float x[C][V];
-  Pack<T, V> raw[C], more[C], weight[C], bias[C], gate[C], block_weight[C], block_bias[C];
-  const T* residual = static_cast<const T*>(a.residual.data) + row_start(a.residual, row);
-  const T* block =
-      a.block.data ? static_cast<const T*>(a.block.data) + row_start(a.block, row) : nullptr;
-  const T* gates = a.gate ? static_cast<const T*>(a.gate) + row / a.gate_rows * width : nullptr;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    col[c] = (static_cast<int64_t>(c) * W * 64 + lane) * V;
-    raw[c] = load_columns<V>(residual, col[c], width);
-  }
-  if (block) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) more[c] = load_columns<V>(block, col[c], width);
-  }
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    weight[c] = load_columns<V>(static_cast<const T*>(a.weight), col[c], width);
-    if (Layer) bias[c] = vector_columns<V, T>(a.bias, col[c], width);
-    if (Post) {
-      block_weight[c] = load_columns<V>(static_cast<const T*>(a.block_weight), col[c], width);
-      if (Layer) block_bias[c] = vector_columns<V, T>(a.block_bias, col[c], width);
-    }
-  }
-  if (gates) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) gate[c] = load_columns<V>(gates, col[c], width);
-  }
+  Pack<T, V> o[C];
   float2 post = make_float2(0.0f, 1.0f);
-  if (block) {
+  if (block_there) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[c][e] = widen(more[c].v[e]);
+      for (int e = 0; e < V; ++e) x[c][e] = more[c][e];
     if (Post) {
-      post = row_stats<Layer>(x, col, width, a.eps, team);
+      post = row_stats<Layer>(x, cols, a.eps, team);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          x[c][e] = fmaf((x[c][e] - post.x) * post.y, widen(block_weight[c].v[e]),
-                         Layer ? widen(block_bias[c].v[e]) : 0.0f);
+          x[c][e] = fmaf((x[c][e] - post.x) * post.y, block_weight[c][e], Layer ? block_bias[c][e] : 0.0f);
     }
-    if (gates) {
+    if (gated) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[c][e] *= widen(gate[c].v[e]);
+        for (int e = 0; e < V; ++e) x[c][e] *= gate[c][e];
     }
-    T* next = static_cast<T*>(a.next) + row * width;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      Pack<T, V> o;
+    for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        x[c][e] = fmaf(x[c][e], a.scale, widen(raw[c].v[e]));
-        o.v[e] = narrow<T>(x[c][e]);
+        x[c][e] = fmaf(x[c][e], a.scale, residual[c][e]);
+        o[c].v[e] = narrow<T>(x[c][e]);
       }
-      store_columns<V>(next, col[c], width, o);
-    }
+    cols.store(static_cast<T*>(a.next) + row * width, o);
   } else {
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[c][e] = widen(raw[c].v[e]);
+      for (int e = 0; e < V; ++e) x[c][e] = residual[c][e];
   }
-  const float2 pre = row_stats<Layer>(x, col, width, a.eps, team);
-  T* out = static_cast<T*>(a.out) + row * width;
+  const float2 pre = row_stats<Layer>(x, cols, a.eps, team);
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    Pack<T, V> o;
+  for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      o.v[e] = narrow<T>(fmaf((x[c][e] - pre.x) * pre.y, widen(weight[c].v[e]),
-                              Layer ? widen(bias[c].v[e]) : 0.0f));
-    store_columns<V>(out, col[c], width, o);
-  }
+      o[c].v[e] =
+          narrow<T>(fmaf((x[c][e] - pre.x) * pre.y, weight[c][e], Layer ? bias[c][e] : 0.0f));
+  cols.store(static_cast<T*>(a.out) + row * width, o);
   if (a.stats && lane == 0) {
     float* s = a.stats + row * (Post ? 4 : 2);
     s[0] = pre.x;
@@ -256,68 +295,13 @@ struct backward_args {
 // Waves of a block: eight, so that two blocks of a CU wait at different barriers, or a row's.
 constexpr int block_waves(int w) { return w < 8 ? 8 : w; }
 
-// What a thread has of a row, 16 bytes at a time, kept as they were loaded until they are used:
-// taken apart earlier, they would be waited for.
-template <typename T>
-struct Words {
-  uint32_t w[4];
-  __device__ float operator[](int e) const {
-    Pack<T, 16 / sizeof(T)> x;
-    __builtin_memcpy(&x, w, 16);
-    return widen(x.v[e]);
-  }
-};
-
-// The columns of a thread: 16 bytes at each of C byte offsets in a row.  Where the rows are whole
-// 16 bytes long, those behind the end are not loaded, and zeros.
-template <typename T, int W, int C>
-struct Columns {
-  static constexpr int V = 16 / sizeof(T);
-  uint32_t at[C];
-  int width;
-  bool even;
-
-  __device__ Columns(int lane, int width_of) : width(width_of), even(width_of % V == 0) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) at[c] = (c * W * 64 + lane) * 16;
-  }
-  __device__ int column(int c, int e) const { return static_cast<int>(at[c] / sizeof(T)) + e; }
-  __device__ bool in(int c, int e = 0) const { return column(c, e) < width; }
-  __device__ Words<T> load(const T* row, int c) const {
-    Words<T> x = {{0, 0, 0, 0}};
-    typedef typename raw_of<16>::type raw;
-    if (even) {
-      if (in(c)) {
-        const raw r = *reinterpret_cast<const raw*>(reinterpret_cast<const char*>(row) + at[c]);
-        __builtin_memcpy(x.w, &r, 16);
-      }
-    } else {
-      const Pack<T, V> p = load_columns<V>(row, column(c, 0), width);
-      __builtin_memcpy(x.w, &p, 16);
-    }
-    return x;
-  }
-  __device__ void store(T* row, int c, const Pack<T, V>& x) const {
-    if (even) {
-      if (in(c)) {
-        typedef typename raw_of<16>::type raw;
-        raw r;
-        __builtin_memcpy(&r, &x, 16);
-        *reinterpret_cast<raw*>(reinterpret_cast<char*>(row) + at[c]) = r;
-      }
-    } else {
-      store_columns<V>(row, column(c, 0), width, x);
-    }
-  }
-};
-
 // Teams of W waves.  An item is up to item_rows neighbouring rows that share a gate;
 // teams take items in turn, all the same number of rows, since the barriers are the
 // block's.  Rows of up to 16 bytes a thread (C = 1): a row's loads are under way while
 // the one before is worked on, and all sums are in registers.  Longer ones have neither
 // registers: operands are loaded where they are used, and the first two sums are in LDS.
 template <typename T, int W, int C, bool Layer, bool Post>
-__global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args a) {
+__global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 4) void k_norm_grad(backward_args a) {
   constexpr int V = 16 / sizeof(T), kTeams = block_waves(W) / W;
   constexpr bool kShort = C == 1;
   constexpr int kVectors = (Layer ? 2 : 1) * (Post ? 2 : 1);
@@ -336,10 +320,13 @@ __global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args
   const T* const block_weights = static_cast<const T*>(a.block_weight);
   const T* const block_biases = static_cast<const T*>(a.block_bias);
   Words<T> weight[C], block_weight[C], block_bias[C], gate[C];
+  auto load_block_vectors = [&] {
+    if (Post) cols.load(block_weights, block_weight);
+    if (Post && Layer) cols.load(block_biases ? block_biases : weights, block_bias, block_biases);
+  };
   if (kShort) {
-    weight[0] = cols.load(weights, 0);
-    if (Post) block_weight[0] = cols.load(block_weights, 0);
-    if (Post && Layer && block_biases) block_bias[0] = cols.load(block_biases, 0);
+    cols.load(weights, weight);
+    load_block_vectors();
   }
   float sums[kInRegs > 0 ? kInRegs : 1][C][V] = {}, gate_sum[C][V] = {};
   if (!kShort) {
@@ -376,20 +363,15 @@ __global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args
     Words<T> dy[C], dx[C], x[C], b[C];
     float mean, rstd, block_mean, block_rstd;
   };
-  // The loads of a row, without branches that depend on it: row 0's, in the place of none
-  auto fetch = [&](int row, Row& r) {
-    const T *px = row_of(a.next, row), *py = dout_there ? row_of(a.dout, row) : px;
-    const T *pn = dnext_there ? row_of(a.dnext, row) : px, *pb = block_there ? row_of(a.block, row) : px;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      r.x[c] = cols.load(px, c);
-      r.dy[c] = cols.load(py, c);
-      if (kShort) {
-        r.dx[c] = cols.load(pn, c);
-        r.b[c] = cols.load(pb, c);
-      }
+  // The loads of a row, of nothing where there is none
+  auto fetch = [&](int row, bool live, Row& r) {
+    cols.load(row_of(a.next, row), r.x, live);
+    cols.load(dout_there ? row_of(a.dout, row) : weights, r.dy, live && dout_there);
+    if (kShort) {
+      cols.load(dnext_there ? row_of(a.dnext, row) : weights, r.dx, live && dnext_there);
+      cols.load(block_there ? row_of(a.block, row) : weights, r.b, live && block_there);
     }
-    const float* s = a.stats + static_cast<int64_t>(row) * kFields;
+    const float* s = a.stats + (live ? static_cast<int64_t>(row) * kFields : 0);
     r.mean = s[0];
     r.rstd = s[1];
     if (Post) {
@@ -401,133 +383,120 @@ __global__ __launch_bounds__(block_waves(W) * 64) void k_norm_grad(backward_args
   Row now, then;
   int item, group, row, end;
   place_of(0, item, group, row, end);
-  if (kShort) fetch(row < end ? row : 0, then);
+  Pack<T, V> o[C];
+  if (kShort) {
+    fetch(row, row < end, then);
+    // Two stores of nothing: as many follow the loads of every later row, so that the wait
+    // for loads is known not to be one for those stores.
+    cols.store(static_cast<T*>(a.dresidual), o, false);
+    cols.store(static_cast<T*>(a.dresidual), o, false);
+  }
   for (int round = 0; round < rounds; ++round) {
     int next_item, next_group, next_row, next_end;
     place_of(round + 1, next_item, next_group, next_row, next_end);
     const T* gates = static_cast<const T*>(a.gate) + static_cast<int64_t>(group) * width;
-    if (gated && kShort) gate[0] = cols.load(gates, 0);
+    if (gated && kShort) cols.load(gates, gate);
     for (int k = 0; k < item_rows; ++k, ++row) {
       const bool live = row < end;
       if (kShort) {
         now = then;
-        const int following = k + 1 == item_rows ? (next_row < next_end ? next_row : 0)
-                                                 : (row + 1 < end ? row + 1 : 0);
-        fetch(following, then);
+        const bool last = k + 1 == item_rows;
+        fetch(last ? next_row : row + 1, last ? next_row < next_end : row + 1 < end, then);
       } else {
-        fetch(live ? row : 0, now);
+        fetch(row, live, now);
+        cols.load(weights, weight);
       }
       float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (!kShort) weight[c] = cols.load(weights, c);
+      for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float v = (now.x[c][e] - now.mean) * now.rstd;
-          const float t = (dout_there ? now.dy[c][e] : 0.0f) * weight[c][e];
+          const float v = (now.x[c][e] - now.mean) * now.rstd, t = now.dy[c][e] * weight[c][e];
           s.x = fmaf(t, v, s.x);
           if (Layer) s.y += t;
         }
-      }
       s = team.sum(s, Layer);
+      if (!kShort) {
+        cols.load(weights, weight);
+        cols.load(dnext_there ? row_of(a.dnext, row) : weights, now.dx, live && dnext_there);
+      }
+      // (a row that is none has zeros for gradients, and adds them)
       float d[C][V];
       float2 s2 = make_float2(0.0f, 0.0f);
-      if (live) {
-        const float along = s.x * inverse, level = Layer ? s.y * inverse : 0.0f;
-        T* out = static_cast<T*>(a.dresidual) + static_cast<int64_t>(row) * width;
+      const float along = s.x * inverse, level = Layer ? s.y * inverse : 0.0f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          if (!kShort) {
-            now.dx[c] = dnext_there ? cols.load(row_of(a.dnext, row), c) : Words<T>{};
-            weight[c] = cols.load(weights, c);
-          }
-          Pack<T, V> o;
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float v = (now.x[c][e] - now.mean) * now.rstd;
-            const float g = dout_there ? now.dy[c][e] : 0.0f;
-            add(kWeight, c, e, g * v);
-            if (Layer) add(kBias, c, e, g);
-            float r = fmaf(-v, along, g * weight[c][e]);
-            if (Layer) r -= level;
-            d[c][e] = fmaf(r, now.rstd, dnext_there ? now.dx[c][e] : 0.0f);
-            o.v[e] = narrow<T>(d[c][e]);
-          }
-          cols.store(out, c, o);
+        for (int e = 0; e < V; ++e) {
+          const float v = (now.x[c][e] - now.mean) * now.rstd, g = now.dy[c][e];
+          add(kWeight, c, e, live ? g * v : 0.0f);
+          if (Layer) add(kBias, c, e, g);
+          float r = fmaf(-v, along, g * weight[c][e]);
+          if (Layer) r -= level;
+          d[c][e] = fmaf(r, now.rstd, now.dx[c][e]);
+          o[c].v[e] = narrow<T>(d[c][e]);
         }
-        if (block_there) {
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            if (!kShort) {
-              now.b[c] = cols.load(row_of(a.block, row), c);
-              if (Post) block_weight[c] = cols.load(block_weights, c);
-              if (Post && Layer && block_biases) block_bias[c] = cols.load(block_biases, c);
-              if (gated) gate[c] = cols.load(gates, c);
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              float q = d[c][e] * a.scale, u = now.b[c][e], w = 0.0f;
-              if (Post) {
-                w = (u - now.block_mean) * now.block_rstd;
-                if (gated)
-                  u = fmaf(w, block_weight[c][e], Layer && block_biases ? block_bias[c][e] : 0.0f);
-              }
-              if (gated) {
-                gate_sum[c][e] = fmaf(q, u, gate_sum[c][e]);
-                q *= gate[c][e];
-              }
-              if (Post) {
-                add(kBlockWeight, c, e, q * w);
-                if (Layer) add(kBlockBias, c, e, q);
-                // (the weight is 0 behind the row's end)
-                q *= block_weight[c][e];
-                s2.x = fmaf(q, w, s2.x);
-                if (Layer) s2.y += q;
-              }
-              d[c][e] = q;
-            }
-          }
-        }
+      cols.store(static_cast<T*>(a.dresidual) + (live ? static_cast<int64_t>(row) * width : 0), o, live);
+      if (!kShort) {
+        cols.load(block_there ? row_of(a.block, row) : weights, now.b, live && block_there);
+        load_block_vectors();
+        if (gated) cols.load(gates, gate);
       }
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float q = d[c][e] * a.scale, u = now.b[c][e], w = 0.0f;
+          if (Post) {
+            w = (u - now.block_mean) * now.block_rstd;
+            if (gated) u = fmaf(w, block_weight[c][e], Layer ? block_bias[c][e] : 0.0f);
+          }
+          if (gated) {
+            gate_sum[c][e] += live ? q * u : 0.0f;
+            q *= gate[c][e];
+          }
+          if (Post) {
+            add(kBlockWeight, c, e, live ? q * w : 0.0f);
+            if (Layer) add(kBlockBias, c, e, live ? q : 0.0f);
+            // (the weight is 0 behind the row's end)
+            q *= block_weight[c][e];
+            s2.x = fmaf(q, w, s2.x);
+            if (Layer) s2.y += q;
+          }
+          d[c][e] = q;
+        }
       if (Post) s2 = team.sum(s2, Layer);
-      if (live && block_there) {
-        const float along = s2.x * inverse, level = Layer ? s2.y * inverse : 0.0f;
-        T* out = static_cast<T*>(a.dblock) + static_cast<int64_t>(row) * width;
+      const float block_along = s2.x * inverse, block_level = Layer ? s2.y * inverse : 0.0f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          Pack<T, V> o;
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            float q = d[c][e];
-            if (Post) {
-              const float w = (now.b[c][e] - now.block_mean) * now.block_rstd;
-              q = fmaf(-w, along, q);
-              if (Layer) q -= level;
-              q *= now.block_rstd;
-            }
-            o.v[e] = narrow<T>(q);
+        for (int e = 0; e < V; ++e) {
+          float q = d[c][e];
+          if (Post) {
+            const float w = (now.b[c][e] - now.block_mean) * now.block_rstd;
+            q = fmaf(-w, block_along, q);
+            if (Layer) q -= block_level;
+            q *= now.block_rstd;
           }
-          cols.store(out, c, o);
+          o[c].v[e] = narrow<T>(q);
         }
-      }
+      cols.store(static_cast<T*>(block_there ? a.dblock : a.dresidual) +
+                     (live ? static_cast<int64_t>(row) * width : 0),
+                 o, live && block_there);
     }
     if (gated && item < items) {
+      float* sums_out = a.gate_sums + static_cast<int64_t>(item) * width;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (a.gate_sums) {
-          float* out = a.gate_sums + static_cast<int64_t>(item) * width;
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (cols.in(c, e)) out[cols.column(c, e)] = gate_sum[c][e];
-        } else {
-          Pack<T, V> o;
-#pragma unroll
-          for (int e = 0; e < V; ++e) o.v[e] = narrow<T>(gate_sum[c][e]);
-          cols.store(static_cast<T*>(a.dgate) + static_cast<int64_t>(group) * width, c, o);
+        for (int e = 0; e < V; ++e) {
+          if (a.gate_sums && cols.in(c, e)) sums_out[cols.column(c, e)] = gate_sum[c][e];
+          o[c].v[e] = narrow<T>(gate_sum[c][e]);
+          gate_sum[c][e] = 0.0f;
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) gate_sum[c][e] = 0.0f;
-      }
+      cols.store(a.gate_sums ? static_cast<T*>(a.dresidual)
+                             : static_cast<T*>(a.dgate) + static_cast<int64_t>(group) * width,
+                 o, !a.gate_sums);
     }
     item = next_item;
     group = next_group;
