@@ -89,6 +89,29 @@ struct Words {
   }
 };
 
+// A thread's values narrowed in pairs, each rounded to nearest even (bf16 has an instruction for
+// two).
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> narrow_all(const float (&x)[V]) {
+  Pack<T, V> o;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) o.v[e] = x[e];
+  } else {
+    typedef float two __attribute__((ext_vector_type(2)));
+    typedef T halves __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      two pair = {x[e], x[e + 1]};
+      asm("" : "+v"(pair));      // (no product and narrowing in one instruction, as in narrow())
+      const halves h = __builtin_convertvector(pair, halves);
+      o.v[e] = h[0];
+      o.v[e + 1] = h[1];
+    }
+  }
+  return o;
+}
+
 // The columns of a thread: 16 bytes at each of C byte offsets in a row.  Rows are reached as
 // buffers that end with them, so that what lies behind the end is neither loaded (zeros) nor
 // stored, by words and without a branch: behind a branch a wave could no longer tell its
@@ -246,12 +269,11 @@ __global__ __launch_bounds__(W < 4 ? 256 : W * 64) void k_norm(forward_args a) {
         for (int e = 0; e < V; ++e) x[c][e] *= gate[c][e];
     }
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        x[c][e] = fmaf(x[c][e], a.scale, residual[c][e]);
-        o[c].v[e] = narrow<T>(x[c][e]);
-      }
+      for (int e = 0; e < V; ++e) x[c][e] = fmaf(x[c][e], a.scale, residual[c][e]);
+      o[c] = narrow_all<T>(x[c]);
+    }
     cols.store(static_cast<T*>(a.next) + row * width, o);
   } else {
 #pragma unroll
@@ -261,11 +283,12 @@ __global__ __launch_bounds__(W < 4 ? 256 : W * 64) void k_norm(forward_args a) {
   }
   const float2 pre = row_stats<Layer>(x, cols, a.eps, team);
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+  for (int c = 0; c < C; ++c) {
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      o[c].v[e] =
-          narrow<T>(fmaf((x[c][e] - pre.x) * pre.y, weight[c][e], Layer ? bias[c][e] : 0.0f));
+      x[c][e] = fmaf((x[c][e] - pre.x) * pre.y, weight[c][e], Layer ? bias[c][e] : 0.0f);
+    o[c] = narrow_all<T>(x[c]);
+  }
   cols.store(static_cast<T*>(a.out) + row * width, o);
   if (a.stats && lane == 0) {
     float* s = a.stats + row * (Post ? 4 : 2);
@@ -332,12 +355,14 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
   if (!kShort) {
     for (int k = tid; k < kInLds * W * 64 * C * V; k += W * 64) joined[k] = 0.0f;
   }
-  // (a thread's own places of it, so that no barrier is needed)
-  auto add = [&](int k, int c, int e, float x) {
-    if (k < kInLds)
-      joined[((k * C + c) * V + e) * W * 64 + lane] += x;
-    else
-      sums[k - kInLds][c][e] += x;
+  // x y to sum k.  (A thread's own places in LDS, so that no barrier is needed.)
+  auto add = [&](int k, int c, int e, float x, float y) {
+    if (k < kInLds) {
+      float* p = &joined[((k * C + c) * V + e) * W * 64 + lane];
+      *p = fmaf(x, y, *p);
+    } else {
+      sums[k - kInLds][c][e] = fmaf(x, y, sums[k - kInLds][c][e]);
+    }
   };
   const bool block_there = a.block.data != nullptr, gated = a.gate != nullptr;
   const bool dout_there = a.dout.data != nullptr, dnext_there = a.dnext.data != nullptr;
@@ -371,12 +396,13 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
       cols.load(dnext_there ? row_of(a.dnext, row) : weights, r.dx, live && dnext_there);
       cols.load(block_there ? row_of(a.block, row) : weights, r.b, live && block_there);
     }
+    // (zeros, with which the row that is none adds nothing to any sum)
     const float* s = a.stats + (live ? static_cast<int64_t>(row) * kFields : 0);
-    r.mean = s[0];
-    r.rstd = s[1];
+    r.mean = live ? s[0] : 0.0f;
+    r.rstd = live ? s[1] : 0.0f;
     if (Post) {
-      r.block_mean = s[2];
-      r.block_rstd = s[3];
+      r.block_mean = live ? s[2] : 0.0f;
+      r.block_rstd = live ? s[3] : 0.0f;
     }
   };
 
@@ -406,13 +432,16 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
         fetch(row, live, now);
         cols.load(weights, weight);
       }
+      // d: first the normalised row, then its gradient
       float2 s = make_float2(0.0f, 0.0f);
+      float d[C][V];
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float v = (now.x[c][e] - now.mean) * now.rstd, t = now.dy[c][e] * weight[c][e];
-          s.x = fmaf(t, v, s.x);
+          d[c][e] = (now.x[c][e] - now.mean) * now.rstd;
+          const float t = now.dy[c][e] * weight[c][e];
+          s.x = fmaf(t, d[c][e], s.x);
           if (Layer) s.y += t;
         }
       s = team.sum(s, Layer);
@@ -420,47 +449,46 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
         cols.load(weights, weight);
         cols.load(dnext_there ? row_of(a.dnext, row) : weights, now.dx, live && dnext_there);
       }
-      // (a row that is none has zeros for gradients, and adds them)
-      float d[C][V];
       float2 s2 = make_float2(0.0f, 0.0f);
       const float along = s.x * inverse, level = Layer ? s.y * inverse : 0.0f;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float v = (now.x[c][e] - now.mean) * now.rstd, g = now.dy[c][e];
-          add(kWeight, c, e, live ? g * v : 0.0f);
-          if (Layer) add(kBias, c, e, g);
+          const float v = d[c][e], g = now.dy[c][e];
+          add(kWeight, c, e, g, v);
+          if (Layer) add(kBias, c, e, g, 1.0f);
           float r = fmaf(-v, along, g * weight[c][e]);
           if (Layer) r -= level;
           d[c][e] = fmaf(r, now.rstd, now.dx[c][e]);
-          o[c].v[e] = narrow<T>(d[c][e]);
         }
+        o[c] = narrow_all<T>(d[c]);
+      }
       cols.store(static_cast<T*>(a.dresidual) + (live ? static_cast<int64_t>(row) * width : 0), o, live);
       if (!kShort) {
         cols.load(block_there ? row_of(a.block, row) : weights, now.b, live && block_there);
         load_block_vectors();
         if (gated) cols.load(gates, gate);
       }
+      float w[C][V];
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          float q = d[c][e] * a.scale, u = now.b[c][e], w = 0.0f;
-          if (Post) {
-            w = (u - now.block_mean) * now.block_rstd;
-            if (gated) u = fmaf(w, block_weight[c][e], Layer ? block_bias[c][e] : 0.0f);
-          }
+          float q = d[c][e] * a.scale;
+          w[c][e] = Post ? (now.b[c][e] - now.block_mean) * now.block_rstd : 0.0f;
           if (gated) {
-            gate_sum[c][e] += live ? q * u : 0.0f;
+            const float u = Post ? fmaf(w[c][e], block_weight[c][e], Layer ? block_bias[c][e] : 0.0f)
+                                 : now.b[c][e];
+            gate_sum[c][e] = fmaf(q, u, gate_sum[c][e]);
             q *= gate[c][e];
           }
           if (Post) {
-            add(kBlockWeight, c, e, live ? q * w : 0.0f);
-            if (Layer) add(kBlockBias, c, e, live ? q : 0.0f);
+            add(kBlockWeight, c, e, q, w[c][e]);
+            if (Layer) add(kBlockBias, c, e, q, 1.0f);
             // (the weight is 0 behind the row's end)
             q *= block_weight[c][e];
-            s2.x = fmaf(q, w, s2.x);
+            s2.x = fmaf(q, w[c][e], s2.x);
             if (Layer) s2.y += q;
           }
           d[c][e] = q;
@@ -468,18 +496,17 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
       if (Post) s2 = team.sum(s2, Layer);
       const float block_along = s2.x * inverse, block_level = Layer ? s2.y * inverse : 0.0f;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) {
+        if (Post) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float q = d[c][e];
-          if (Post) {
-            const float w = (now.b[c][e] - now.block_mean) * now.block_rstd;
-            q = fmaf(-w, block_along, q);
+          for (int e = 0; e < V; ++e) {
+            float q = fmaf(-w[c][e], block_along, d[c][e]);
             if (Layer) q -= block_level;
-            q *= now.block_rstd;
+            d[c][e] = q * now.block_rstd;
           }
-          o[c].v[e] = narrow<T>(q);
         }
+        o[c] = narrow_all<T>(d[c]);
+      }
       cols.store(static_cast<T*>(block_there ? a.dblock : a.dresidual) +
                      (live ? static_cast<int64_t>(row) * width : 0),
                  o, live && block_there);
