@@ -146,11 +146,12 @@ struct Columns {
     const int bytes = width * static_cast<int>(sizeof(T));
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row), 0, there ? bytes : 0, 0x00027000);
   }
+  template <bool NT = false>
   __device__ void load(const T* row, Words<T> (&x)[C], bool there = true) const {
     const __amdgpu_buffer_rsrc_t b = buffer(row, there);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const words4 r = __builtin_amdgcn_raw_buffer_load_b128(b, at[c], 0, 0);
+      const words4 r = __builtin_amdgcn_raw_buffer_load_b128(b, at[c], 0, NT ? 2 : 0);
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[c].w[k] = r[k];
     }
@@ -390,11 +391,11 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
   };
   // The loads of a row, of nothing where there is none
   auto fetch = [&](int row, bool live, Row& r) {
-    cols.load(row_of(a.next, row), r.x, live);
-    cols.load(dout_there ? row_of(a.dout, row) : weights, r.dy, live && dout_there);
+    cols.template load<true>(row_of(a.next, row), r.x, live);
+    cols.template load<true>(dout_there ? row_of(a.dout, row) : weights, r.dy, live && dout_there);
     if (kShort) {
-      cols.load(dnext_there ? row_of(a.dnext, row) : weights, r.dx, live && dnext_there);
-      cols.load(block_there ? row_of(a.block, row) : weights, r.b, live && block_there);
+      cols.template load<true>(dnext_there ? row_of(a.dnext, row) : weights, r.dx, live && dnext_there);
+      cols.template load<true>(block_there ? row_of(a.block, row) : weights, r.b, live && block_there);
     }
     // (zeros, with which the row that is none adds nothing to any sum)
     const float* s = a.stats + (live ? static_cast<int64_t>(row) * kFields : 0);
