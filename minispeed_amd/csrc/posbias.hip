@@ -114,86 +114,151 @@ struct bias_grad_args {
   const void* grad;
   int64_t batch_stride, head_stride, row_stride;
   int64_t batch, heads, queries, keys, first;
-  int64_t spans, bands;
-  int32_t rows, causal;
+  int64_t chunks, bands, units;    // of a row, of the rows, of a head
+  int32_t rows, causal;            // rows: of a band, a multiple of 8
   float* sums;                     // [head][block of the head][bucket]
 };
 
+// 16 bytes, taken apart where their values are used.
+template <typename T>
+struct Words {
+  uint32_t w[4];
+  __device__ float operator[](int e) const {
+    Pack<T, 16 / sizeof(T)> x;
+    __builtin_memcpy(&x, w, 16);
+    return widen(x.v[e]);
+  }
+};
+template <typename T>
+__device__ __forceinline__ Words<T> load_words(const T* p) {
+  const Pack<T, 16 / sizeof(T)> x = load_stream_any<16 / sizeof(T)>(p);
+  Words<T> r;
+  __builtin_memcpy(r.w, &x, 16);
+  return r;
+}
+
+// A wave goes down a band of rows in a chunk of 64 V columns, a lane with V of them.  Its V sums
+// are of diagonals: from row to row each moves one column on, the last one to the next
+// lane, and out of lane 63 to LDS.  (The sums move by the names of their registers, but for
+// the one that changes lanes.)
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_bias_grad(bias_grad_args a, edges_t edges) {
-  constexpr int V = 16 / sizeof(T), kSpan = kThreads * V;
-  __shared__ float strip[kSpan];
-  const int tid = threadIdx.x, n = edges.n;
-  const int64_t each = a.batch * a.bands * a.spans;
-  const int64_t h = blockIdx.x / each, of_head = blockIdx.x - h * each;
-  const int64_t span = of_head % a.spans, band = of_head / a.spans % a.bands,
-                batch = of_head / a.spans / a.bands;
-  const int64_t i0 = band * a.rows, i1 = min(i0 + a.rows, a.queries);
-  // this thread's diagonals: j - i from d to d + V - 1
-  const int64_t d0 = span * kSpan - (i1 - 1), d = d0 + tid * V;
-  const T* grad = static_cast<const T*>(a.grad) + batch * a.batch_stride + h * a.head_stride;
+  constexpr int V = 16 / sizeof(T), kWide = 64 * V, kWaves = kThreads / 64;
+  __shared__ float strips[kWaves][kWide + kMaxRows];
+  __shared__ int32_t edge[kMaxBuckets + 1];
+  __shared__ int64_t bases[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n = edges.n;
+  // (under way with the gradient's loads: arguments lie in memory too)
+  int32_t held[kMaxBuckets / kThreads + 1];
+#pragma unroll
+  for (int k = 0; k <= kMaxBuckets / kThreads; ++k)
+    held[k] = edges.edge[min(tid + k * kThreads, n)];
+  const int64_t blocks = (a.units + kWaves - 1) / kWaves;
+  const int64_t h = blockIdx.x / blocks, unit = (blockIdx.x - h * blocks) * kWaves + wave;
+  const int64_t chunk = unit % a.chunks, band = unit / a.chunks % a.bands,
+                batch = unit / a.chunks / a.bands;
+  const int64_t i0 = band * a.rows, c0 = chunk * kWide, c = c0 + lane * V;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(a.rows), a.queries - i0));
+  const int turns = (rows + 7) / 8 * 8;
+  float* strip = strips[wave];
   float sum[V] = {};
-  // rows where some of them lie within the keys, and where all do
-  const int64_t some0 = max(i0, -(d + V - 1)), some1 = min(i1, a.keys - d);
-  int64_t all0 = max(i0, -d), all1 = min(i1, a.keys - d - (V - 1));
-  if (all1 <= all0) all0 = all1 = some1;
-  if (!a.causal || d - a.first <= 0) {
-    // towards the diagonal's ends: value by value, from addresses within the row
-    auto part = [&](int64_t from, int64_t to) {
-      for (int64_t i = from; i < to; ++i) {
-        T x[V];
+  // (a unit behind the last, or one with keys behind all of its queries alone, has no sums)
+  const bool some = unit < a.units && !(a.causal && c0 - (i0 + rows - 1) - a.first > 0);
+  if (some) {
+    const T* row = static_cast<const T*>(a.grad) + batch * a.batch_stride + h * a.head_stride +
+                   i0 * a.row_stride;
+    // Beyond the last key a lane's 16 bytes run into the next row, and what lies there is
+    // masked.  The last row, and rows closer than 16 bytes, are loaded value by value.
+    const bool whole = c0 + kWide <= a.keys;
+    const T* column = row + min(c, a.keys - 1);
+    uint32_t mask[4];
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          x[e] = grad[i * a.row_stride + min(max(i + d + e, int64_t{0}), a.keys - 1)];
+    for (int k = 0; k < 4; ++k) {
+      mask[k] = 0;
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (i + d + e >= 0 && i + d + e < a.keys) sum[e] += widen(x[e]);
-      }
+      for (int e = 0; e < V / 4; ++e)
+        if (c + k * (V / 4) + e < a.keys) mask[k] |= (V == 4 ? ~0u : 0xffffu) << (e * 16);
+    }
+    auto masked = [&](Words<T> x) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x.w[q] &= mask[q];
+      return x;
     };
-    part(some0, min(all0, some1));
-    const T* p = grad + all0 * (a.row_stride + 1) + d;
-    const int64_t step = a.row_stride + 1;
-    int64_t i = all0;
-    for (; i + 8 <= all1; i += 8, p += 8 * step) {
-      Pack<T, V> x[8];
+    auto one_by_one = [&](int k) {
+      Pack<T, V> values;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = load_stream_any<V>(p + k * step);
+      for (int e = 0; e < V; ++e) values.v[e] = row[k * a.row_stride + min(c + e, a.keys - 1)];
+      Words<T> x;
+      __builtin_memcpy(x.w, &values, 16);
+      return masked(x);
+    };
+    // rows that are loaded as vectors
+    const int vectors =
+        whole ? rows : a.row_stride < V ? 0 : i0 + rows == a.queries ? rows - 1 : rows;
+    auto take = [&](const Words<T>& x, int k, int r) {     // r = k % V
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int e = 0; e < V; ++e) sum[(e - r) & (V - 1)] += x[e];
+      float& out = sum[(V - 1 - r) & (V - 1)];
+      if (lane == 63) strip[kWide - 1 + turns - k] = out;
+      out = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(out), 0x138, 0xf, 0xf, false));
+    };
+    int k = 0;
+    for (; k + 8 <= vectors; k += 8) {
+      Words<T> x[8];
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum[e] += widen(x[k].v[e]);
+      for (int q = 0; q < 8; ++q) x[q] = load_words(column + (k + q) * a.row_stride);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) take(whole ? x[q] : masked(x[q]), k + q, q & (V - 1));
     }
-    for (; i < all1; ++i, p += step) {
-      const Pack<T, V> x = load_stream_any<V>(p);
+    // the rows left, and rows of nothing up to a multiple of 8; all sums move
+#pragma unroll 1
+    for (; k < turns; ++k) {
+      Words<T> x = {{0, 0, 0, 0}};
+      if (k < vectors) x = masked(load_words(column + k * a.row_stride));
+      else if (k < rows) x = one_by_one(k);
+      take(x, k, 0);
+      const float first = sum[V - 1];
 #pragma unroll
-      for (int e = 0; e < V; ++e) sum[e] += widen(x.v[e]);
+      for (int e = V - 1; e > 0; --e) sum[e] = sum[e - 1];
+      sum[0] = first;
     }
-    part(max(all1, some0), some1);
+#pragma unroll
+    for (int e = 0; e < V; ++e) strip[lane * V + e] = sum[e];
   }
+  // strip[s] is the sum of j - i - first = s + bases[wave]
+  if (lane == 0) bases[wave] = c0 - i0 - turns - a.first;
+  const int length = some ? kWide + turns : 0;
+  __shared__ int lengths[kWaves];
+  if (lane == 0) lengths[wave] = length;
 #pragma unroll
-  for (int e = 0; e < V; ++e) strip[tid * V + e] = sum[e];
+  for (int k = 0; k <= kMaxBuckets / kThreads; ++k)
+    if (tid + k * kThreads <= n) edge[tid + k * kThreads] = held[k];
   __syncthreads();
-  // Buckets: each a run of strip[s], j - i - first = s + d0 - first
-  const int wave = uniform(tid >> 6), lane = tid & 63, buckets = n * (a.causal ? 1 : 2);
-  const int64_t base = d0 - a.first;
+  // Buckets: each a run of a strip; 16 lanes to one
+  const int buckets = n * (a.causal ? 1 : 2);
   float* out = a.sums + static_cast<int64_t>(blockIdx.x) * buckets;
-  for (int b = wave; b < buckets; b += kThreads / 64) {
+  for (int b = tid >> 4; b < buckets; b += kThreads / 16) {
     const int k = b < n ? b : b - n;
     int64_t from, to;                // distances, both ends within
     if (b < n) {
-      from = k + 1 < n ? -static_cast<int64_t>(edges.edge[k + 1] - 1) : INT64_MIN / 2;
-      to = -static_cast<int64_t>(edges.edge[k]);
+      from = k + 1 < n ? -static_cast<int64_t>(edge[k + 1] - 1) : INT64_MIN / 2;
+      to = -static_cast<int64_t>(edge[k]);
     } else {
-      from = max(edges.edge[k], 1);
-      to = k + 1 < n ? edges.edge[k + 1] - 1 : INT64_MAX / 2;
+      from = max(edge[k], 1);
+      to = k + 1 < n ? edge[k + 1] - 1 : INT64_MAX / 2;
     }
-    from = max(from - base, int64_t{0});
-    to = min(to - base, static_cast<int64_t>(kSpan) - 1);
     float x = 0.0f;
-    for (int64_t s = from + lane; s <= to; s += 64) x += strip[s];
 #pragma unroll
-    for (int m = 32; m; m /= 2) x += __shfl_xor(x, m);
-    if (lane == 0) out[b] = x;
+    for (int w = 0; w < kWaves; ++w) {
+      const int64_t base = bases[w], long_ = lengths[w];
+      const int first = static_cast<int>(min(max(from - base, int64_t{0}), long_));
+      const int end = static_cast<int>(min(max(to - base + 1, int64_t{0}), long_));
+#pragma unroll 4
+      for (int s = first + (tid & 15); s < end; s += 16) x += strips[w][s];
+    }
+#pragma unroll
+    for (int m = 8; m; m /= 2) x += __shfl_xor(x, m);
+    if ((tid & 15) == 0) out[b] = x;
   }
 }
 
@@ -253,22 +318,26 @@ bool good_plane(int64_t heads, int64_t queries, int64_t keys, int64_t first) {
          (heads == 0 || queries == 0 || (countable(heads, queries) && countable(heads * queries, keys)));
 }
 
+constexpr int64_t kGradUnits = 3072;      // waves, 12 to a CU
+
 int64_t span_of(int32_t dtype) { return kThreads * (16 / dtype_bytes(dtype)); }
 
 // Rows of a block: many, as its diagonals are worked out once, but so few that there are
 // blocks for all CUs.
-int32_t rows_of(int64_t queries, int64_t blocks_of_a_row, int64_t least) {
+int32_t rows_of(int64_t queries, int64_t blocks_of_a_row, int64_t least, int64_t blocks) {
   int32_t rows = kMaxRows;
-  while (rows > least && ceil_div(queries, rows) * blocks_of_a_row < 2048) rows /= 2;
+  while (rows > least && ceil_div(queries, rows) * blocks_of_a_row < blocks) rows /= 2;
   return static_cast<int32_t>(std::min<int64_t>(rows, std::max<int64_t>(queries, 1)));
 }
 
 void lay_out(bias_grad_args& a, int32_t dtype) {
-  const int64_t span = span_of(dtype);
-  a.rows = rows_of(a.queries, a.batch * a.heads * ceil_div(a.keys, span), 16);
+  a.chunks = ceil_div(a.keys, span_of(dtype) / (kThreads / 64));
+  a.rows = (rows_of(a.queries, a.batch * a.heads * a.chunks, 16, kGradUnits) + 7) / 8 * 8;
   a.bands = ceil_div(a.queries, a.rows);
-  a.spans = ceil_div(a.keys + a.rows - 1, span);
+  a.units = a.batch * a.bands * a.chunks;
 }
+
+int64_t blocks_of_a_head(const bias_grad_args& a) { return ceil_div(a.units, kThreads / 64); }
 
 }  // namespace
 }  // namespace ops
@@ -286,7 +355,7 @@ int ms_position_bias(const void* table, int32_t dtype, int64_t buckets, int64_t 
   if (!table || !out) return MS_OPS_EINVAL;
   bias_args a{table, bucket_stride, head_stride, queries, keys, first, 0, causal ? 1 : 0, out};
   const int64_t spans = ceil_div(keys, span_of(dtype));
-  a.rows = rows_of(queries, heads * spans, 4);
+  a.rows = rows_of(queries, heads * spans, 4, 2048);
   const int64_t blocks = heads * spans * ceil_div(queries, a.rows);
   if (!fits(blocks, kThreads)) return MS_OPS_EINVAL;
   const edges_t e = edges_of(buckets, max_distance, causal);
@@ -311,9 +380,9 @@ int64_t ms_position_bias_grad_workspace(int32_t dtype, int64_t buckets, int64_t 
   a.queries = queries;
   a.keys = keys;
   lay_out(a, dtype);
-  if (!countable(batch * heads, a.bands) || !countable(batch * heads * a.bands, a.spans * buckets))
+  if (!countable(heads, blocks_of_a_head(a)) || !countable(heads * blocks_of_a_head(a), buckets))
     return MS_OPS_EINVAL;
-  return batch * heads * a.bands * a.spans * buckets * 4;
+  return heads * blocks_of_a_head(a) * buckets * 4;
 }
 
 int ms_position_bias_grad(const void* grad, int32_t dtype, int64_t batch, int64_t batch_stride,
@@ -332,12 +401,12 @@ int ms_position_bias_grad(const void* grad, int32_t dtype, int64_t batch, int64_
   if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)))
     return MS_OPS_EWORKSPACE;
   bias_grad_args a{grad, batch_stride, head_stride, row_stride, batch, heads, queries, keys, first,
-                   0, 0, 0, causal ? 1 : 0, static_cast<float*>(workspace)};
+                   0, 0, 0, 0, causal ? 1 : 0, static_cast<float*>(workspace)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   int64_t count = 0;
   if (need) {
     lay_out(a, dtype);
-    count = batch * a.bands * a.spans;
+    count = blocks_of_a_head(a);
     const int64_t blocks = heads * count;
     if (!fits(blocks, kThreads)) return MS_OPS_EINVAL;
     const edges_t e = edges_of(buckets, max_distance, causal);
