@@ -412,39 +412,112 @@ __global__ __launch_bounds__(256) void k_zero(uint16_t* to, int64_t n) {
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t ceil_div(int64_t x, int64_t by) { return (x + by - 1) / by; }
 
-// How the products' tiles are cut: 256 x 256 by 8 waves, 128 x 128 or 128 x 32 by 4.
-struct Cut {
-  int m, n, wm;
-};
-constexpr Cut kLarge{256, 256, 2}, kMedium{128, 128, 2}, kFew{128, 32, 4};
+// How the products' tiles are cut.  Large ones, one block to a CU, have the highest rate (1230
+// TFLOP/s at 16384 x 2048 x 4096, medium ones 1130), but leave more of the chip idle at
+// the end and beside a small product.
+enum Cut { kLarge, kMedium, kFew };
+typedef Tiles<256, 256, 2, 4> Large;
+typedef Tiles<128, 128, 2, 2> Medium;
+typedef Tiles<128, 32, 4, 1> Few;
 
-// The tile for an M x N product: few columns waste what a wide tile computes beyond them;
-// below two large tiles to a CU the medium ones spread better.
-Cut cut_of(int64_t m, int64_t n) {
-  if (n <= 64) return kFew;
-  if (ceil_div(m, 256) * ceil_div(n, 256) < 256) return kMedium;
-  return kLarge;
+struct Shape {
+  int m, n, wm, threads, slots;    // slots: blocks that the chip runs at a time
+  double step, rest;               // us of a block for 64 k, and for what is around them
+};
+constexpr Shape kShapes[] = {{256, 256, 2, 512, 256, 1.75, 4.0},
+                             {128, 128, 2, 256, 512, 0.95, 3.0},
+                             {128, 32, 4, 256, 1024, 0.55, 2.0}};
+
+int64_t tiles_of(int64_t m, int64_t n, Cut c) {
+  return ceil_div(m, kShapes[c].m) * ceil_div(n, kShapes[c].n);
 }
 
-// Parts of k that give every CU a block, each of 8 steps or more.
-int splits_of(int64_t m, int64_t n, int64_t steps, Cut c) {
-  const int64_t tiles = ceil_div(m, c.m) * ceil_div(n, c.n);
-  const int64_t want = c.m == 256 ? 256 : 512;
-  if (tiles * 2 > want) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(want, tiles), steps / 8)));
+// The cut of one product without parts of k: the one whose blocks are done first.
+Cut cut_of(int64_t m, int64_t n, int64_t steps) {
+  Cut best = kLarge;
+  double least = 1e300;
+  for (Cut c : {kLarge, kMedium, kFew}) {
+    const Shape& s = kShapes[c];
+    const double us = static_cast<double>(ceil_div(tiles_of(m, n, c), s.slots)) * (steps * s.step + s.rest);
+    if (us < least) least = us, best = c;
+  }
+  return best;
+}
+
+// A product whose k can be cut into parts (m = 0: none): its size, 64 k at a time, and whether its
+// sums go through memory also if there is one part.
+struct Job {
+  int64_t m, n, steps;
+  bool summed;
+};
+
+struct Plan {
+  Cut cut;
+  int splits[2];
+};
+
+// The cut and parts with which two products in one launch are done first.  One by itself takes
+// whole rounds of blocks; behind another its blocks start as those end, and half a block's time
+// is left over.  Each part's sums are written and read at 4 TB/s, and joined by a launch of
+// 5 us (summed ones are joined anyhow).
+Plan plan_of(const Job& p, const Job& q) {
+  constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 16, 32, 64};
+  Plan best{kLarge, {1, 1}};
+  double least = 1e300;
+  const auto joining = [](const Job& j, int splits) {
+    double us = 0.0;
+    if (splits > 1 || j.summed) us += splits * 8e-6 / 4 * static_cast<double>(j.m * j.n);
+    return splits > 1 && !j.summed ? us + 5.0 : us;
+  };
+  for (Cut c : {kLarge, kMedium, kFew}) {
+    const Shape& s = kShapes[c];
+    const int64_t tp = tiles_of(p.m, p.n, c), tq = q.m ? tiles_of(q.m, q.n, c) : 0;
+    for (int i : kSplits) {
+      if (i > 1 && p.steps / i < 8) break;
+      const double us1 = ceil_div(p.steps, i) * s.step + s.rest, more1 = joining(p, i);
+      for (int j : kSplits) {
+        if (j > 1 && (!q.m || q.steps / j < 8)) break;
+        double us;
+        if (q.m) {
+          const double us2 = ceil_div(q.steps, j) * s.step + s.rest;
+          us = std::max(std::max(us1, us2),
+                        (tp * i * us1 + tq * j * us2) / s.slots + 0.5 * us2) + joining(q, j);
+        } else {
+          us = ceil_div(tp * i, s.slots) * us1;
+        }
+        us += more1;
+        if (us < least) least = us, best = {c, {i, j}};
+      }
+    }
+  }
+  return best;
+}
+
+int64_t set_tiles(product_args& p, Cut c) {
+  p.tiles_m = static_cast<int32_t>(ceil_div(p.a.rows, kShapes[c].m));
+  p.tiles_n = static_cast<int32_t>(ceil_div(p.b.rows, kShapes[c].n));
+  return int64_t{p.tiles_m} * p.tiles_n * p.splits;
 }
 
 template <typename T, Side SA, Side SB, typename E>
-int run_product(Cut c, const product_args& args, const E& epilogue, hipStream_t s) {
-  product_args p = args;
-  p.tiles_m = static_cast<int32_t>(ceil_div(p.a.rows, c.m));
-  p.tiles_n = static_cast<int32_t>(ceil_div(p.b.rows, c.n));
-  const int64_t blocks = int64_t{p.tiles_m} * p.tiles_n * p.splits;
-  const int threads = c.m == 256 ? 512 : 256;
-  if (!fits(blocks, threads)) return MS_OPS_EINVAL;
-  if (c.m == 256) return launch(k_product<T, 256, 256, 2, 4, SA, SB, E>, blocks, threads, s, p, epilogue);
-  if (c.n == 128) return launch(k_product<T, 128, 128, 2, 2, SA, SB, E>, blocks, threads, s, p, epilogue);
-  return launch(k_product<T, 128, 32, 4, 1, SA, SB, E>, blocks, threads, s, p, epilogue);
+int run_product(Cut c, product_args p, const E& epilogue, hipStream_t s) {
+  const int64_t blocks = set_tiles(p, c);
+  if (!fits(blocks, kShapes[c].threads)) return MS_OPS_EINVAL;
+  if (c == kLarge) return launch(k_product<T, Large, SA, SB, E>, blocks, Large::kThreads, s, p, epilogue);
+  if (c == kMedium) return launch(k_product<T, Medium, SA, SB, E>, blocks, Medium::kThreads, s, p, epilogue);
+  return launch(k_product<T, Few, SA, SB, E>, blocks, Few::kThreads, s, p, epilogue);
+}
+
+template <typename T, Side SB1, Side SB2, typename E>
+int run_products(Cut c, product_args p, const E& e, product_args q, const E& f, hipStream_t s) {
+  const int64_t first = set_tiles(p, c), blocks = first + set_tiles(q, c);
+  if (!fits(blocks, kShapes[c].threads)) return MS_OPS_EINVAL;
+  const uint32_t n = static_cast<uint32_t>(first);
+  if (c == kLarge)
+    return launch(k_products<T, Large, SB1, SB2, E>, blocks, Large::kThreads, s, p, e, q, f, n);
+  if (c == kMedium)
+    return launch(k_products<T, Medium, SB1, SB2, E>, blocks, Medium::kThreads, s, p, e, q, f, n);
+  return launch(k_products<T, Few, SB1, SB2, E>, blocks, Few::kThreads, s, p, e, q, f, n);
 }
 
 // Space cut from the workspace, or only counted while `at` is null.
@@ -515,8 +588,8 @@ int forward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t*
   p.k = static_cast<int32_t>(hidden.width);
   p.pairs = pairs_of(hidden);
   p.splits = 1;
-  const Cut c = cut_of(vocab, n);
-  const int64_t count = ceil_div(vocab, c.m) * c.wm;
+  const Cut c = cut_of(vocab, n, ceil_div(hidden.width, kStep) * p.pairs);
+  const int64_t count = ceil_div(vocab, kShapes[c].m) * kShapes[c].wm;
   sum_epilogue e{};
   e.parts = space.take<float2>(count * n);
   e.picked = space.take<float>(n);
@@ -575,15 +648,24 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
   const int64_t pieces = ceil_div(vocab, piece);
   const int64_t plane = round_up(n * piece, 128);
   T* d = space.take<T>(plane * Planes);
+  const int64_t wide = std::min(piece, vocab);
+  const Cut cut_d = cut_of(wide, n, ceil_div(width, kStep) * pairs);
   // dhidden sums over the pieces in fp32
-  const Cut cut_h = cut_of(width, n);
-  const int splits_h = dhidden ? splits_of(width, n, ceil_div(piece, kStep) * pairs, cut_h) : 1;
+  const Job job_h{width, n, ceil_div(wide, kStep) * pairs, pieces > 1};
+  const Job job_w{width, wide, ceil_div(n, kStep) * pairs, false}, none{};
+  // The two products in one launch, if one cut is best for both, the one of more k first
+  Plan plan_h = plan_of(job_h, none), plan_w = plan_of(job_w, none);
+  const bool both = dhidden && dweight && plan_h.cut != kFew && plan_w.cut != kFew;
+  const bool w_first = job_w.steps >= job_h.steps;
+  if (both) {
+    const Plan plan = w_first ? plan_of(job_w, job_h) : plan_of(job_h, job_w);
+    plan_h = {plan.cut, {plan.splits[w_first], 1}};
+    plan_w = {plan.cut, {plan.splits[!w_first], 1}};
+  }
+  const int splits_h = plan_h.splits[0], splits_w = plan_w.splits[0];
   float* parts_h = dhidden && (splits_h > 1 || pieces > 1) ? space.take<float>(splits_h * n * width)
                                                            : nullptr;
-  const Cut cut_w = cut_of(width, std::min(piece, vocab));
-  const int splits_w =
-      dweight ? splits_of(width, std::min(piece, vocab), ceil_div(n, kStep) * pairs, cut_w) : 1;
-  float* parts_w = splits_w > 1 ? space.take<float>(splits_w * std::min(piece, vocab) * width) : nullptr;
+  float* parts_w = dweight && splits_w > 1 ? space.take<float>(splits_w * wide * width) : nullptr;
   if (!run || rc) return rc;
 
   for (int64_t first = 0; first < vocab; first += piece) {
@@ -594,32 +676,33 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
 
     product_args p{w_here, h, static_cast<int32_t>(width), pairs, 0, 0, 1};
     soft_epilogue<T, Planes> soft{d, piece, plane, rows, *targets, scale, static_cast<int32_t>(first)};
-    rc = run_product<T, kAlong, kAlong>(cut_of(here, n), p, soft, s);
+    rc = run_product<T, kAlong, kAlong>(cut_d, p, soft, s);
     if (rc) return rc;
 
-    if (dhidden) {
-      operand a = w_here, b{reinterpret_cast<const uint16_t*>(d), piece, plane,
-                            static_cast<int32_t>(n)};
-      a.rows = static_cast<int32_t>(width);
-      product_args q{a, b, static_cast<int32_t>(here), pairs, 0, 0, splits_h};
-      out_epilogue<Out> out{static_cast<Out*>(dhidden), parts_h, rows, nullptr, scale, first > 0};
-      rc = run_product<T, kAcross, kAlong>(cut_h, q, out, s);
-      if (rc) return rc;
+    // dhidden: d, its tokens' rows along k, the vocabulary
+    const uint16_t* some = reinterpret_cast<const uint16_t*>(d);
+    product_args ph{w_here, {some, piece, plane, static_cast<int32_t>(n)}, static_cast<int32_t>(here),
+                    pairs, 0, 0, splits_h};
+    ph.a.rows = static_cast<int32_t>(width);
+    const out_epilogue<Out> out_h{static_cast<Out*>(dhidden), parts_h, rows, nullptr, scale, first > 0};
+    // dweight: d, its tokens' rows across k, the tokens
+    product_args pw{scaled, {some, piece, plane, static_cast<int32_t>(here)}, static_cast<int32_t>(n),
+                    pairs, 0, 0, splits_w};
+    pw.a.rows = static_cast<int32_t>(width);
+    Out* to = static_cast<Out*>(dweight) + first * width;
+    const float* by = lifted ? factor : nullptr;
+    const out_epilogue<Out> out_w{to, parts_w, nullptr, by, scale, 0};
+    if (both) {
+      rc = w_first ? run_products<T, kAcross, kAlong>(plan_h.cut, pw, out_w, ph, out_h, s)
+                   : run_products<T, kAlong, kAcross>(plan_h.cut, ph, out_h, pw, out_w, s);
+    } else {
+      if (dhidden) rc = run_product<T, kAcross, kAlong>(plan_h.cut, ph, out_h, s);
+      if (!rc && dweight) rc = run_product<T, kAcross, kAcross>(plan_w.cut, pw, out_w, s);
     }
-    if (dweight) {
-      operand a = scaled, b{reinterpret_cast<const uint16_t*>(d), piece, plane,
-                            static_cast<int32_t>(here)};
-      a.rows = static_cast<int32_t>(width);
-      product_args q{a, b, static_cast<int32_t>(n), pairs, 0, 0, splits_w};
-      Out* to = static_cast<Out*>(dweight) + first * width;
-      const float* by = lifted ? factor : nullptr;
-      out_epilogue<Out> out{to, parts_w, nullptr, by, scale, 0};
-      rc = run_product<T, kAcross, kAcross>(cut_w, q, out, s);
+    if (rc) return rc;
+    if (parts_w) {
+      rc = fold<Out>(parts_w, splits_w, here, width, nullptr, by, scale, to, s);
       if (rc) return rc;
-      if (parts_w) {
-        rc = fold<Out>(parts_w, splits_w, here, width, nullptr, by, scale, to, s);
-        if (rc) return rc;
-      }
     }
   }
   if (parts_h) return fold<Out>(parts_h, splits_h, n, width, rows, nullptr, scale, dhidden, s);

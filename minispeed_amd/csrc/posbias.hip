@@ -294,17 +294,18 @@ bool good_buckets(int64_t buckets, int64_t max_distance, int32_t causal) {
          max_distance <= INT32_MAX;
 }
 
-// Where buckets begin.  A border that is a whole number is one also after the rounding of
-// the power (2^-60 of it; the next whole numbers are 2^-31 away).
+// Where buckets begin.  A border that is a whole number is taken for one although up to 256
+// powers of a rounded root lie behind it (512 2^-64 of it, 3e-17; other borders are 1e-13 from one
+// by chance alone).
 edges_t edges_of(int64_t buckets, int64_t max_distance, int32_t causal) {
   edges_t e;
   e.n = static_cast<int32_t>(causal ? buckets : buckets / 2);
   e.one = e.n / 2;
   for (int k = 0; k < e.one; ++k) e.edge[k] = k;
   const int steps = e.n - e.one;
-  const long double ratio = static_cast<long double>(max_distance) / e.one;
-  for (int s = 0; s < steps; ++s) {
-    const long double at = e.one * std::pow(ratio, static_cast<long double>(s) / steps);
+  const long double root = std::pow(static_cast<long double>(max_distance) / e.one, 1.0L / steps);
+  long double at = e.one;
+  for (int s = 0; s < steps; ++s, at *= root) {
     const long double near = std::round(at);
     e.edge[e.one + s] = static_cast<int32_t>(std::fabs(at - near) < 1e-13L * at ? near : std::ceil(at));
   }

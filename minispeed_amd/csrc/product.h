@@ -199,20 +199,30 @@ __device__ __forceinline__ void place(uint32_t b, uint32_t total, int tiles_m, i
   tn = first + t % wide;
 }
 
+// A way to cut a product into tiles of BM x BN by WM x WN waves.
+template <int BM_, int BN_, int WM_, int WN_>
+struct Tiles {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = WM * WN * 64;
+  static constexpr int kBytes = 2 * (BM + BN) * kStep * 2;      // of LDS
+};
+
 namespace {
-template <typename T, int BM, int BN, int WM, int WN, Side SA, Side SB, typename Epilogue>
-__global__ __launch_bounds__(WM * WN * 64, 2) void k_product(product_args p, Epilogue epilogue) {
+
+// Block `block` of `blocks`: one tile, or one part of its k.
+template <typename T, typename Tile, Side SA, Side SB, typename Epilogue>
+__device__ __forceinline__ void multiply_tile(const product_args& p, const Epilogue& epilogue,
+                                              uint32_t block, uint32_t blocks, char* memory) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host has none of the built-in functions)
-  constexpr int NT = WM * WN * 64, MI = BM / WM / 32, NI = BN / WN / 32;
+  constexpr int BM = Tile::BM, BN = Tile::BN, WM = Tile::WM, WN = Tile::WN;
+  constexpr int NT = Tile::kThreads, MI = BM / WM / 32, NI = BN / WN / 32;
   constexpr int kTileA = BM * kStep * 2, kTile = kTileA + BN * kStep * 2;
   static_assert(BM % (WM * 32) == 0 && BN % (WN * 32) == 0, "");
-  __shared__ __attribute__((aligned(1024))) char memory[2 * kTile];
   char MS_LDS* const lds = (char MS_LDS*)memory;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
   int tm, tn, split;
-  place(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn, split);
+  place(block, blocks, p.tiles_m, p.tiles_n, tm, tn, split);
 
   const Fetch<BM, NT, SA> fetch_a(p.a, tm * BM, tid);
   const Fetch<BN, NT, SB> fetch_b(p.b, tn * BN, tid);
@@ -281,6 +291,25 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product(product_args p, Epi
   epilogue.template store<MI, NI>(acc, tm * BM + wm * MI * 32, tn * BN + wn * NI * 32,
                                   tm * WM + wm, split, lane, p.a.rows, p.b.rows);
 #endif
+}
+
+template <typename T, typename Tile, Side SA, Side SB, typename Epilogue>
+__global__ __launch_bounds__(Tile::kThreads, 2) void k_product(product_args p, Epilogue epilogue) {
+  __shared__ __attribute__((aligned(1024))) char memory[Tile::kBytes];
+  multiply_tile<T, Tile, SA, SB>(p, epilogue, blockIdx.x, gridDim.x, memory);
+}
+
+// Two products in one launch, the first `first` blocks and the others: so that the last
+// tiles of the one do not leave CUs idle before the other begins.
+template <typename T, typename Tile, Side SB1, Side SB2, typename Epilogue>
+__global__ __launch_bounds__(Tile::kThreads, 2) void k_products(product_args p, Epilogue e,
+                                                                product_args q, Epilogue f,
+                                                                uint32_t first) {
+  __shared__ __attribute__((aligned(1024))) char memory[Tile::kBytes];
+  if (blockIdx.x < first)
+    multiply_tile<T, Tile, kAcross, SB1>(p, e, blockIdx.x, first, memory);
+  else
+    multiply_tile<T, Tile, kAcross, SB2>(q, f, blockIdx.x - first, gridDim.x - first, memory);
 }
 
 }  // namespace
