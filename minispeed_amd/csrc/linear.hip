@@ -36,7 +36,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kMaxWidth = 1 << 20;
 constexpr int64_t kMaxRows = INT32_MAX - 1024;     // a tile behind the last row stays in 32 bits
-constexpr int64_t kPiece = int64_t{256} << 20;     // bytes of d at a time
+constexpr int64_t kPiece = int64_t{512} << 20;     // bytes of d at a time
 
 // What a token's row of d is made of, by k_rows.
 struct __attribute__((aligned(16))) row_t {
@@ -112,7 +112,15 @@ struct sum_epilogue {
   }
 };
 
-// A piece's columns of d: d[t, m], dense rows of ld elements; planes of bf16 for fp32.
+// Four values of a type as two words.
+template <typename T>
+struct Quad {
+  uint32_t w[2];
+  __device__ explicit Quad(const T (&v)[4]) { __builtin_memcpy(w, v, 8); }
+};
+
+// A piece's columns of d: d[t, m], dense rows of ld elements; planes of bf16 for fp32.  Two lanes
+// that have one token change places with half of their values, so that each stores 16 bytes.
 template <typename T, int Planes>
 struct soft_epilogue {
   T* d;
@@ -125,44 +133,72 @@ struct soft_epilogue {
   template <int MI, int NI>
   __device__ void store(const f32x16 (&acc)[MI][NI], int m0, int n0, int, int, int lane, int m,
                         int n) const {
-    const int half = 4 * (lane >> 5);
-    const float unit = scale * kLog2e;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int t = n0 + j * 32 + (lane & 31);
-      if (t >= n) continue;
-      const row_t row = rows[t];
-      const int64_t y = token(targets, t) - first - m0;
-      T* out = d + t * ld + m0 + half;
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          Pack<T, 4> o[Planes];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int at = i * 32 + q * 8 + e;
-            float v = __builtin_amdgcn_exp2f(fmaf(acc[i][j][q * 4 + e], unit, -row.lse2)) * row.soft;
-            if (at + half == y) v += row.given;
-            if (row.soft == 0.0f && row.given == 0.0f) v = 0.0f;
-            if (m0 + at + half >= m) v = 0.0f;
-#pragma unroll
-            for (int s = 0; s < Planes; ++s) {
-              o[s].v[e] = narrow<T>(v);
-              v -= widen(o[s].v[e]);
-            }
-          }
-#pragma unroll
-          for (int s = 0; s < Planes; ++s) store_words(out + s * plane + i * 32 + q * 8, o[s]);
-        }
+      const row_t row = rows[min(t, n - 1)];
+      const int64_t y = token(targets, min(t, n - 1)) - first - m0;
+      // The given token, and what is behind the vocabulary's end, are few tiles' concern.
+      if (__any(y >= 0 && y < MI * 32) || m - m0 < MI * 32)
+        put<MI, true>(&acc[0][j], NI, m0, t, lane, m, n, row, y);
+      else
+        put<MI, false>(&acc[0][j], NI, m0, t, lane, m, n, row, y);
     }
   }
 
-  __device__ static void store_words(T* p, const Pack<T, 4>& x) {
-    typedef uint32_t raw __attribute__((ext_vector_type(2)));
-    raw r;
-    __builtin_memcpy(&r, &x, 8);
-    *reinterpret_cast<raw*>(p) = r;
+  template <int MI, bool Special>
+  __device__ __forceinline__ void put(const f32x16* acc, int step, int m0, int t, int lane, int m, int n,
+                                      const row_t& row, int64_t y) const {
+    const int half = 4 * (lane >> 5);
+    const float unit = scale * kLog2e;
+    const int where = y >= 0 && y < MI * 32 ? static_cast<int>(y) : -1, left = m - m0;
+    // rows without a gradient are zeros, whatever their logits are
+    const uint32_t keep = row.soft == 0.0f && row.given == 0.0f ? 0u : ~0u;
+    T* out = d + t * ld + m0 + 8 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; q += 2) {
+        uint32_t words[2][Planes][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[4];
+          T o[Planes][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = i * 32 + (q + h) * 8 + e + half;
+            v[e] = __builtin_amdgcn_exp2f(fmaf(acc[i * step][(q + h) * 4 + e], unit, -row.lse2)) * row.soft;
+            if (Special) {
+              if (at == where) v[e] += row.given;
+              if (at >= left) v[e] = 0.0f;
+            }
+#pragma unroll
+            for (int s = 0; s < Planes; ++s) {
+              o[s][e] = narrow<T>(v[e]);
+              if (s + 1 < Planes) v[e] -= widen(o[s][e]);
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < Planes; ++s) {
+            const Quad<T> x(o[s]);
+            words[h][s][0] = x.w[0] & keep;
+            words[h][s][1] = x.w[1] & keep;
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < Planes; ++s) {
+          u32x4 r;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const auto swapped =
+                __builtin_amdgcn_permlane32_swap(words[0][s][k], words[1][s][k], false, false);
+            r[k] = swapped[0];
+            r[2 + k] = swapped[1];
+          }
+          if (t < n) *reinterpret_cast<u32x4*>(out + s * plane + i * 32 + q * 8) = r;
+        }
+        __builtin_amdgcn_sched_barrier(0);      // (all at once they would not fit in the registers)
+      }
   }
 };
 
@@ -422,11 +458,18 @@ typedef Tiles<128, 32, 4, 1> Few;
 
 struct Shape {
   int m, n, wm, threads, slots;    // slots: blocks that the chip runs at a time
-  double step, rest;               // us of a block for 64 k, and for what is around them
+  double step, alone, rest;        // us of a block for 64 k beside others and by itself, and
+                                   // for what is around them
 };
-constexpr Shape kShapes[] = {{256, 256, 2, 512, 256, 1.75, 4.0},
-                             {128, 128, 2, 256, 512, 0.95, 3.0},
-                             {128, 32, 4, 256, 1024, 0.55, 2.0}};
+constexpr Shape kShapes[] = {{256, 256, 2, 512, 256, 1.75, 1.75, 4.0},
+                             {128, 128, 2, 256, 512, 0.95, 0.65, 3.0},
+                             {128, 32, 4, 256, 1024, 1.2, 0.45, 2.0}};
+
+// us of a block among `blocks` for so many steps.
+double block_us(const Shape& s, int64_t blocks, int64_t steps) {
+  const double fill = std::min(1.0, static_cast<double>(blocks) / s.slots);
+  return steps * std::max(s.alone, s.step * fill) + s.rest;
+}
 
 int64_t tiles_of(int64_t m, int64_t n, Cut c) {
   return ceil_div(m, kShapes[c].m) * ceil_div(n, kShapes[c].n);
@@ -438,7 +481,8 @@ Cut cut_of(int64_t m, int64_t n, int64_t steps) {
   double least = 1e300;
   for (Cut c : {kLarge, kMedium, kFew}) {
     const Shape& s = kShapes[c];
-    const double us = static_cast<double>(ceil_div(tiles_of(m, n, c), s.slots)) * (steps * s.step + s.rest);
+    const int64_t tiles = tiles_of(m, n, c);
+    const double us = static_cast<double>(ceil_div(tiles, s.slots)) * block_us(s, tiles, steps);
     if (us < least) least = us, best = c;
   }
   return best;
@@ -458,7 +502,7 @@ struct Plan {
 
 // The cut and parts with which two products in one launch are done first.  One by itself takes
 // whole rounds of blocks; behind another its blocks start as those end, and half a block's time
-// is left over.  Each part's sums are written and read at 4 TB/s, and joined by a launch of
+// is left over.  Each part's sums are written and read at 2.5 TB/s, and joined by a launch of
 // 5 us (summed ones are joined anyhow).
 Plan plan_of(const Job& p, const Job& q) {
   constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 16, 32, 64};
@@ -466,7 +510,7 @@ Plan plan_of(const Job& p, const Job& q) {
   double least = 1e300;
   const auto joining = [](const Job& j, int splits) {
     double us = 0.0;
-    if (splits > 1 || j.summed) us += splits * 8e-6 / 4 * static_cast<double>(j.m * j.n);
+    if (splits > 1 || j.summed) us += splits * 8e-6 / 2.5 * static_cast<double>(j.m * j.n);
     return splits > 1 && !j.summed ? us + 5.0 : us;
   };
   for (Cut c : {kLarge, kMedium, kFew}) {
@@ -474,16 +518,17 @@ Plan plan_of(const Job& p, const Job& q) {
     const int64_t tp = tiles_of(p.m, p.n, c), tq = q.m ? tiles_of(q.m, q.n, c) : 0;
     for (int i : kSplits) {
       if (i > 1 && p.steps / i < 8) break;
-      const double us1 = ceil_div(p.steps, i) * s.step + s.rest, more1 = joining(p, i);
+      const double more1 = joining(p, i);
       for (int j : kSplits) {
         if (j > 1 && (!q.m || q.steps / j < 8)) break;
         double us;
         if (q.m) {
-          const double us2 = ceil_div(q.steps, j) * s.step + s.rest;
+          const double us1 = block_us(s, tp * i + tq * j, ceil_div(p.steps, i));
+          const double us2 = block_us(s, tp * i + tq * j, ceil_div(q.steps, j));
           us = std::max(std::max(us1, us2),
                         (tp * i * us1 + tq * j * us2) / s.slots + 0.5 * us2) + joining(q, j);
         } else {
-          us = ceil_div(tp * i, s.slots) * us1;
+          us = ceil_div(tp * i, s.slots) * block_us(s, tp * i, ceil_div(p.steps, i));
         }
         us += more1;
         if (us < least) least = us, best = {c, {i, j}};
@@ -641,11 +686,11 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
     if (run && !rc)
       rc = launch(k_layout<f16>, blocks, 256, s, hidden, scaled.ld, rows, factor, to);
   }
-  // A piece of the vocabulary: whole large tiles, as many as kPiece holds
-  int64_t piece = kPiece / (n * 2 * Planes) / 256 * 256;
-  piece = std::min(std::max<int64_t>(piece, 256), round_up(vocab, 256));
-  piece = std::min(piece, kMaxWidth);
-  const int64_t pieces = ceil_div(vocab, piece);
+  // Pieces of the vocabulary, all of one size: whole large tiles, and no more of them than
+  // kPiece holds
+  const int64_t most = std::min(std::max<int64_t>(kPiece / (n * 2 * Planes) / 256 * 256, 256), kMaxWidth);
+  const int64_t pieces = ceil_div(vocab, most);
+  const int64_t piece = round_up(ceil_div(vocab, pieces), 256);
   const int64_t plane = round_up(n * piece, 128);
   T* d = space.take<T>(plane * Planes);
   const int64_t wide = std::min(piece, vocab);

@@ -44,7 +44,7 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
     ``hidden`` is ``[..., width]``, ``weight`` ``[vocab, width]``, of one type (float32 /
     float16 / bfloat16), ``targets`` ``[...]`` (int64 or int32).  The logits are not stored,
     forward or backward: beside the operands and the gradients a call takes some
-    bytes for each token and 128 words of the vocabulary, and backward 256 MiB at most
+    bytes for each token and 128 words of the vocabulary, and backward 512 MiB at most
     (or 256 words' worth of the vocabulary, and copies of 2-byte operands whose rows
     are not on 16-byte boundaries; of float32 operands always).
 
