@@ -215,51 +215,84 @@ struct out_epilogue {
   template <int MI, int NI>
   __device__ void store(const f32x16 (&acc)[MI][NI], int m0, int n0, int, int split, int lane, int m,
                         int n) const {
-    const int half = 4 * (lane >> 5);
     const float all = factor ? *factor * scale : scale;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int t = n0 + j * 32 + (lane & 31);
-      if (t >= n) continue;
-      const float by = rows ? rows[t].down * all : all;
+      const float by = rows ? rows[min(t, n - 1)].down * all : all;
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int at = m0 + i * 32 + q * 8 + half;
-          if (at >= m) continue;
+        for (int q = 0; q < 4; q += 2) {
           if (parts) {
-            float* p = parts + (static_cast<int64_t>(split) * n + t) * m + at;
-            if (at + 4 <= m) {
-              Pack<float, 4> x;
-              if (add) x = load<4>(p);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x.v[e] = (add ? x.v[e] : 0.0f) + acc[i][j][q * 4 + e];
-              store_any(p, x);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (at + e < m) p[e] = (add ? p[e] : 0.0f) + acc[i][j][q * 4 + e];
-            }
+            put_sums(acc[i][j], q, m0 + i * 32, t, split, lane, m, n);
+            put_sums(acc[i][j], q + 1, m0 + i * 32, t, split, lane, m, n);
           } else {
-            T* p = out + static_cast<int64_t>(t) * m + at;
-            Pack<T, 4> x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x.v[e] = narrow<T>(acc[i][j][q * 4 + e] * by);
-            if (at + 4 <= m) {
-              store_any(p, x);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (at + e < m) p[e] = x.v[e];
-            }
+            put(acc[i][j], q, m0 + i * 32, t, lane, m, n, by);
           }
         }
     }
   }
-  template <typename U>
-  __device__ static void store_any(U* p, const Pack<U, 4>& x) { ops::store<4>(p, x); }
+
+  __device__ __forceinline__ void put_sums(const f32x16& acc, int q, int m0, int t, int split, int lane,
+                                           int m, int n) const {
+    const int at = m0 + q * 8 + 4 * (lane >> 5);
+    if (t >= n || at >= m) return;
+    float* p = parts + (static_cast<int64_t>(split) * n + t) * m + at;
+    if (at + 4 <= m) {
+      Pack<float, 4> x;
+      if (add) x = load<4>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x.v[e] = (add ? x.v[e] : 0.0f) + acc[q * 4 + e];
+      ops::store<4>(p, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (at + e < m) p[e] = (add ? p[e] : 0.0f) + acc[q * 4 + e];
+    }
+  }
+
+  // Rows 8 q to 8 q + 15 of a square.  2-byte values: two lanes of one n change places with half of
+  // them, so that each stores 16 bytes.
+  __device__ __forceinline__ void put(const f32x16& acc, int q, int m0, int t, int lane, int m, int n,
+                                      float by) const {
+    constexpr int V = 16 / sizeof(T);
+    T x[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[h][e] = narrow<T>(acc[(q + h) * 4 + e] * by);
+#pragma unroll
+    for (int h = 0; h < 8 / V; ++h) {
+      Pack<T, V> o;
+      int at;
+      if constexpr (V == 8) {
+        const Quad<T> a(x[0]), b(x[1]);
+        uint32_t r[4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const auto swapped = __builtin_amdgcn_permlane32_swap(a.w[k], b.w[k], false, false);
+          r[k] = swapped[0];
+          r[2 + k] = swapped[1];
+        }
+        __builtin_memcpy(&o, r, 16);
+        at = m0 + 8 * (q + (lane >> 5));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o.v[e] = x[h][e];
+        at = m0 + (q + h) * 8 + 4 * (lane >> 5);
+      }
+      if (t >= n) continue;
+      T* p = out + static_cast<int64_t>(t) * m + at;
+      if (at + V <= m) {
+        ops::store<V>(p, o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (at + e < m) p[e] = o.v[e];
+      }
+    }
+  }
 };
 
 // ---------------------------------------------------------------------------
