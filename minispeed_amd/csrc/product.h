@@ -240,13 +240,17 @@ __device__ __forceinline__ void multiply_tile(const product_args& p, const Epilo
 #pragma unroll
     for (int j = 0; j < NI; ++j) acc[i][j] = f32x16{};
 
-  int pair = begin / steps, k0 = (begin - pair * steps) * kStep;
+  // Where no two blocks share a tile's rows, each begins elsewhere in k: in step they would
+  // ask for the same columns of all rows at once, which lie in few of the memory's channels.
+  const int turn = p.tiles_n == 1 ? tm % steps : 0;
+  int pair = begin / steps, done = begin - pair * steps, k0 = (done + turn) % steps * kStep;
   auto issue = [&](int buffer) {
     const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + buffer * kTile;
     fetch_a.issue(plane_a(pair) * p.a.plane, k0, p.k - k0, to, wave);
     fetch_b.issue(plane_b(pair) * p.b.plane, k0, p.k - k0, to + kTileA, wave);
     k0 += kStep;
-    if (k0 >= p.k) k0 = 0, ++pair;
+    if (k0 >= p.k) k0 = 0;
+    if (++done == steps) done = 0, ++pair;
   };
   typedef typename frag_of<T>::type frag;
   frag a[2][MI], b[2][NI];
