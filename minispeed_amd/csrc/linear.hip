@@ -17,7 +17,7 @@
 // Numbers.  Products of 16-bit values are exact in the fp32 sums.  d is rounded once
 // to the operands' type, as the products take it: an error of half an ulp of each
 // term, which the sums average.  In fp16 a row of d is scaled by a power of two that
-// brings its bound to 2^14 (p reaches down to 2^-20 over large vocabularies, and g is
+// brings its bound below 2^15 (p reaches down to 2^-20 over large vocabularies, and g is
 // an inverse count of tokens); dhidden's rows are scaled back, and dweight takes its
 // scales from a copy of hidden multiplied by them, exactly but for underflow of
 // rows whose gradients are 2^14 times smaller than the largest.
@@ -342,22 +342,35 @@ __global__ __launch_bounds__(256) void k_join(const float2* parts, const float* 
   }
 }
 
-// The exponent of a row's bound on |d|, such that bound * 2^up < 2^15; 0 for zero rows.
+// The power of two that brings a row's d below 2^15, given the larger one of the two terms that
+// meet in it; 0 for zero rows.
 __device__ __forceinline__ int lift(float bound) {
   const int e = static_cast<int>(__float_as_uint(bound) >> 23 & 255);
   // (the smallest numbers, infinities and NaN are left as they are)
-  return e == 0 || e == 255 ? 0 : min(max(14 + 127 - e, -100), 100);
+  return e == 0 || e == 255 ? 0 : min(13 + 127 - e, 100);
 }
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((e + 127) << 23); }
 
-// Row numbers for the backward pass.  With `lifted` (fp16) one block does all rows and
-// leaves the least power of two of any row's scale in factor[0].
+constexpr int kRowBlocks = 256;
+
+// The least of a block's numbers, in thread 0.
+__device__ __forceinline__ int block_least(int low, int* held) {
+#pragma unroll
+  for (int s = 32; s; s /= 2) low = min(low, __shfl_xor(low, s));
+  if ((threadIdx.x & 63) == 0) held[threadIdx.x >> 6] = low;
+  __syncthreads();
+  for (unsigned w = 0; w < blockDim.x / 64; ++w) low = min(low, held[w]);
+  return low;
+}
+
+// Row numbers for the backward pass.  With `lifted` (fp16) the least power of two of any row's
+// scale goes to factor[0], or each block's to least[block] where there are several.
 __global__ __launch_bounds__(1024) void k_rows(const float* lse, const float* grad_logprob,
                                                const float* grad_lse, ms_tokens_t targets,
                                                int64_t vocab, int64_t ignore_index, int lifted,
-                                               row_t* rows, float* factor) {
-  __shared__ int least[16];
+                                               row_t* rows, float* factor, int* least) {
+  __shared__ int held[16];
   int low = 100;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; t < targets.n;
        t += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -370,21 +383,24 @@ __global__ __launch_bounds__(1024) void k_rows(const float* lse, const float* gr
     const float soft = l - g;
     int up = 0;
     if (lifted) {
-      const float bound = fabsf(soft) + fabsf(g);
+      const float bound = fmaxf(fabsf(soft), fabsf(g));
       up = lift(bound);
       if (bound > 0.0f) low = min(low, up);
     }
     rows[t] = {of == -__builtin_inff() ? 0.0f : of * kLog2e, soft * pow2(up), g * pow2(up), pow2(-up)};
   }
   if (!lifted) return;
-#pragma unroll
-  for (int s = 32; s; s /= 2) low = min(low, __shfl_xor(low, s));
-  if ((threadIdx.x & 63) == 0) least[threadIdx.x >> 6] = low;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (unsigned w = 0; w < blockDim.x / 64; ++w) low = min(low, least[w]);
-    factor[0] = pow2(-low);
-  }
+  low = block_least(low, held);
+  if (threadIdx.x) return;
+  if (gridDim.x == 1) factor[0] = pow2(-low);
+  else least[blockIdx.x] = low;
+}
+
+__global__ __launch_bounds__(kRowBlocks) void k_least(const int* least, int count, float* factor) {
+  __shared__ int held[16];
+  const int low =
+      block_least(static_cast<int>(threadIdx.x) < count ? least[threadIdx.x] : 100, held);
+  if (threadIdx.x == 0) factor[0] = pow2(-low);
 }
 
 // A matrix as the products take it: rows at `ld`, zeros behind `width`; times a row's
@@ -618,9 +634,10 @@ bool good_sizes(const ms_rows_t* hidden, const ms_rows_t* weight) {
 
 // Whether the products can take the matrix as it lies.
 bool lies_well(const ms_rows_t& m) {
-  return m.dtype != MS_OPS_F32 && m.inner >= m.n && m.inner_stride % 8 == 0 &&
-         m.inner_stride >= m.width && m.inner_stride <= kMaxWidth && m.width % 8 == 0 &&
-         reinterpret_cast<uintptr_t>(m.data) % 16 == 0;
+  // (one row has no stride)
+  return m.dtype != MS_OPS_F32 && m.width % 8 == 0 && reinterpret_cast<uintptr_t>(m.data) % 16 == 0 &&
+         (m.n == 1 || (m.inner >= m.n && m.inner_stride % 8 == 0 && m.inner_stride >= m.width &&
+                       m.inner_stride <= kMaxWidth));
 }
 
 int planes_of(const ms_rows_t& m) { return m.dtype == MS_OPS_F32 ? 3 : 1; }
@@ -632,7 +649,7 @@ operand prepare(const ms_rows_t& m, Space& space, int& rc, hipStream_t s, bool r
   o.rows = static_cast<int32_t>(m.n);
   if (lies_well(m)) {
     o.data = static_cast<const uint16_t*>(m.data);
-    o.ld = m.inner_stride;
+    o.ld = m.n == 1 ? m.width : m.inner_stride;
     o.plane = 0;
     return o;
   }
@@ -705,9 +722,15 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
   const bool lifted = hidden.dtype == MS_OPS_F16;
   row_t* rows = space.take<row_t>(n);
   float* factor = space.take<float>(1);
-  if (run)
-    rc = launch(k_rows, lifted ? 1 : std::min<int64_t>(ceil_div(n, 1024), 1024), 1024, s, lse,
-                grad_logprob, grad_lse, *targets, vocab, ignore_index, lifted ? 1 : 0, rows, factor);
+  int* least = space.take<int>(kRowBlocks);
+  if (run) {
+    // (fp16: one block up to 16384 tokens, as several take another launch)
+    const int64_t blocks = lifted && n <= 16384 ? 1 : std::min<int64_t>(ceil_div(n, 1024), kRowBlocks);
+    rc = launch(k_rows, blocks, 1024, s, lse, grad_logprob, grad_lse, *targets, vocab, ignore_index,
+                lifted ? 1 : 0, rows, factor, least);
+    if (!rc && lifted && blocks > 1)
+      rc = launch(k_least, 1, kRowBlocks, s, least, blocks, factor);
+  }
   const operand h = prepare(hidden, space, rc, s, run), w = prepare(weight, space, rc, s, run);
   operand scaled = h;
   if (lifted && dweight) {

@@ -9,7 +9,7 @@ exponential), the sum of V terms, up to 128 + V / 128 of them one after the othe
 many u more, and lse by that and 2^-22 |lse|.
 Gradients: each term d W is off by what its p is, by half an ulp of d (2^-24 of three
 planes), by (terms) u in the sums; the result is rounded once.  In fp16, rows of d are scaled so
-that half a subnormal step (2^-25) is 2^-39 of the row's bound; hidden, multiplied by a power of
+that half a subnormal step (2^-25) is 2^-38 of the larger of a row's two terms (scaled to 2^13 or more); hidden, multiplied by a power of
 two up to the ratio of the rows' bounds, is off by 2^-25 of the largest row's scale.
 """
 
@@ -86,7 +86,7 @@ def backward(h, w, t, gr, gl, scale=1.0, ignore=-100):
     bound = (l - g).abs() + g.abs()
     # The exponential instruction gives 0 in the place of numbers below 2^-126, the smallest
     # normal one, so p is off by that; d and its planes by as much where they are so small.
-    small = bound * 2.0 ** -39 if h.dtype == torch.float16 else (bound + 4) * 2.0 ** -126
+    small = bound * 2.0 ** -38 if h.dtype == torch.float16 else (bound + 4) * 2.0 ** -126
     err = size * rel + small[:, None]
     th = abs(scale) * (err + size * many * v) @ wd.abs() + ref.rounding(dh, h.dtype)
     tw = abs(scale) * (err + size * many * n).T @ hd.abs() + ref.rounding(dw, h.dtype)
@@ -213,6 +213,19 @@ def test_gradients_of_very_different_rows(dtype):
         eh = torch.where(eh.abs() >= 65520.0, torch.sign(eh) * INF, eh)
         dh, eh = dh.double().masked_fill(edge, 0.0), eh.masked_fill(edge, 0.0)
     ref.close(dh, eh, th)
+
+
+def test_many_rows_of_very_different_gradients():
+    """fp16 beyond the rows that one block numbers; gradients up to the largest."""
+    h, w, t, gr, gl = make(20000, 16, 70, "fp16", 30, ignored=0.0)
+    check(h, w, t, gr * 2.0 ** torch.arange(20000, device=DEV).remainder(9), gl)
+    h, w, t, gr, gl = make(40, 16, 70, "fp16", 31, ignored=0.0)
+    huge = torch.full_like(gr, 2.0 ** 127)
+    r = ms.ops.linear_logprobs(h, w, t, scale=2.0 ** -125)
+    dh, dw = ms.ops.linear_logprobs_grad(h, w, t, r.lse, huge, scale=2.0 ** -125)
+    eh, ew, th, tw = backward(h, w, t, huge, None, 2.0 ** -125)
+    ref.close(dh, eh, th)
+    ref.close(dw, ew, tw)
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
