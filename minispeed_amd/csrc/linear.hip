@@ -307,6 +307,7 @@ __global__ __launch_bounds__(256) void k_join(const float2* parts, const float* 
   const int64_t t = static_cast<int64_t>(blockIdx.x) * each + which;
   float most = -__builtin_inff(), sum = 0.0f;
   if (t < n) {
+#pragma unroll 8
     for (int64_t k = lane; k < count; k += lanes) {
       const float2 x = parts[k * n + t];
       const float top = fmaxf(most, x.x), base = top == -__builtin_inff() ? 0.0f : top;
@@ -696,7 +697,7 @@ int forward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t*
   if (rc) return rc;
   // few tokens: more threads to each, as one after the other they would wait for memory
   int lanes = 8;
-  while (lanes < 256 && n * lanes < 65536 && lanes * 2 <= count) lanes *= 2;
+  while (lanes < 256 && n * lanes < 262144 && lanes * 2 <= count) lanes *= 2;
   return launch(k_join, ceil_div(n, 256 / lanes), 256, s, e.parts, e.picked, count, n, lanes, *targets,
                 vocab, ignore_index, logprob, lse);
 }
