@@ -12,10 +12,15 @@
 //
 // A value depends on j - i alone.  Forward, which only writes, a block sets down the
 // values of its diagonals in LDS; a thread has 16 bytes of a row in registers and goes
-// down the rows, each time shifting one value in.  Backward, which only reads, a thread
-// follows its 16 bytes of neighbouring diagonals down the rows with one register for each
-// (loads take any alignment); a block then adds up its diagonals' sums by bucket, each a
-// run of neighbours, and a second kernel joins the blocks' sums in their order.
+// down the rows, each time shifting one value in.  Backward, which only reads, the sums of the
+// diagonals move through the registers of a wave as the rows go by; a block then adds up its
+// diagonals' sums by bucket, each a run of neighbours, and a second kernel joins the
+// blocks' sums in their order.
+//
+// Memory bounds both.  Forward 16 x 2048 x 2048 fp16 23.9 us, 5.6 TB/s (floor at 6.9 TB/s of writes 19.5);
+// backward 8 x 12 x 1024 x 1024 bf16 40 us (kernel 36 to 43, the join 4.6; floor at 7.3 TB/s of reads 27.6).
+// A thread that follows its diagonals down the rows by loads that move along instead took 59 to
+// 69 us: at every wave's edges they run out of the rows.
 #include "ops_common.h"
 
 #include <algorithm>

@@ -5,12 +5,19 @@
 * :func:`token_logprobs`, :func:`token_logprobs_grad` — the log probability of a
   given token per position, with entropy and the most likely alternatives, and
   the gradient of the logits;
+* :func:`linear_logprobs`, :func:`linear_logprobs_grad` — the same log probability straight
+  from the hidden states and the head's weight, without storing the logits, and both
+  gradients;
+* :func:`norm`, :func:`residual_norm`, :func:`residual_norm_grad` — the norms before and
+  after a block with its gate, residual scale and residual sum, and all their gradients;
+* :func:`position_bias`, :func:`position_bias_grad` — the learned relative position bias of
+  attention by buckets of distances, and its table's gradient;
 * :func:`pack8`, :func:`unpack8`, :func:`checkpoint8`, :func:`activation8`,
   :func:`activation8_grad`, :func:`activation8_linear` — activations held in 8
   bits between forward and backward.
 
-``embedding``, ``token_logprobs``, ``activation8``, ``checkpoint8`` and
-``activation8_linear`` take part in autograd; the ``_grad`` functions are the same backward
+``embedding``, ``token_logprobs``, ``linear_logprobs``, ``norm``, ``residual_norm``,
+``position_bias``, ``activation8``, ``checkpoint8`` and ``activation8_linear`` take part in autograd; the ``_grad`` functions are the same backward
 passes for a program that calls them itself, and are not differentiable again.  Forward-mode derivatives are refused.  All of them
 run on the current stream, allocate through torch's caching allocator and return before
 the kernels have finished.
