@@ -122,7 +122,7 @@ struct sum_epilogue {
 template <typename T>
 struct Quad {
   uint32_t w[2];
-  __device__ explicit Quad(const T (&v)[4]) { __builtin_memcpy(w, v, 8); }
+  __device__ explicit Quad(const T (&v)[4]) { __builtin_memcpy(w, v, sizeof(w)); }
 };
 
 // A piece's columns of d: d[t, m], dense rows of ld elements; planes of bf16 for fp32.  Two lanes
@@ -160,6 +160,24 @@ struct soft_epilogue {
     const int where = y >= 0 && y < MI * 32 ? static_cast<int>(y) : -1, left = m - m0;
     // rows without a gradient are zeros, whatever their logits are
     const uint32_t keep = row.soft == 0.0f && row.given == 0.0f ? 0u : ~0u;
+    if constexpr (sizeof(T) == 4) {
+      if (t >= n) return;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          Pack<T, 4> o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = i * 32 + q * 8 + e + half;
+            float v = __builtin_amdgcn_exp2f(fmaf(acc[i * step][q * 4 + e], unit, -row.lse2)) * row.soft;
+            if (Special && at == where) v += row.given;
+            o.v[e] = (Special && at >= left) || !keep ? 0.0f : v;
+          }
+          ops::store<4>(d + t * ld + m0 + i * 32 + q * 8 + half, o);
+        }
+      return;
+    }
     T* out = d + t * ld + m0 + 8 * (lane >> 5);
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -415,25 +433,26 @@ __global__ __launch_bounds__(kRowBlocks) void k_least(const int* least, int coun
 template <typename T>
 __global__ __launch_bounds__(256) void k_layout(ms_rows_t from, int64_t ld, const row_t* rows,
                                                 const float* factor, T* to) {
-  const int64_t chunks = ld / 8;
+  constexpr int V = 16 / sizeof(T);
+  const int64_t chunks = ld / V;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= from.n * chunks) return;
-  const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+  const int64_t r = i / chunks, c = (i - r * chunks) * V;
   const T* p = static_cast<const T*>(from.data) + row_start(from, r) + c;
-  Pack<T, 8> x;
-  if (c + 8 <= from.width) {
-    x = load<8>(p);
+  Pack<T, V> x;
+  if (c + V <= from.width) {
+    x = load<V>(p);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x.v[e] = c + e < from.width ? p[e] : static_cast<T>(0.0f);
+    for (int e = 0; e < V; ++e) x.v[e] = c + e < from.width ? p[e] : static_cast<T>(0.0f);
   }
   if (rows) {
     // a row without a gradient keeps the scale 1 that it was given: its d is zero
     const float by = rows[r].soft == 0.0f && rows[r].given == 0.0f ? 1.0f : rows[r].down / *factor;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x.v[e] = narrow<T>(widen(x.v[e]) * by);
+    for (int e = 0; e < V; ++e) x.v[e] = narrow<T>(widen(x.v[e]) * by);
   }
-  ops::store<8>(to + r * ld + c, x);
+  ops::store<V>(to + r * ld + c, x);
 }
 
 // Three planes of bf16: the leading 8 bits of each value, the next 8, the rest.  Cut off
@@ -531,11 +550,13 @@ int64_t tiles_of(int64_t m, int64_t n, Cut c) {
   return ceil_div(m, kShapes[c].m) * ceil_div(n, kShapes[c].n);
 }
 
-// The cut of one product without parts of k: the one whose blocks are done first.
-Cut cut_of(int64_t m, int64_t n, int64_t steps) {
-  Cut best = kLarge;
+// The cut of one product without parts of k: the one whose blocks are done first.  (32-bit
+// products have small tiles alone, for few tokens.)
+Cut cut_of(int64_t m, int64_t n, int64_t steps, bool wide) {
+  Cut best = kFew;
   double least = 1e300;
   for (Cut c : {kLarge, kMedium, kFew}) {
+    if (wide && c != kFew) continue;
     const Shape& s = kShapes[c];
     const int64_t tiles = tiles_of(m, n, c);
     const double us = static_cast<double>(ceil_div(tiles, s.slots)) * block_us(s, tiles, steps);
@@ -560,9 +581,9 @@ struct Plan {
 // whole rounds of blocks; behind another its blocks start as those end, and half a block's time
 // is left over.  Each part's sums are written and read at 2.5 TB/s, and joined by a launch of
 // 5 us (summed ones are joined anyhow).
-Plan plan_of(const Job& p, const Job& q) {
+Plan plan_of(const Job& p, const Job& q, bool wide = false) {
   constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 16, 32, 64};
-  Plan best{kLarge, {1, 1}};
+  Plan best{kFew, {1, 1}};
   double least = 1e300;
   const auto joining = [](const Job& j, int splits) {
     double us = 0.0;
@@ -570,6 +591,7 @@ Plan plan_of(const Job& p, const Job& q) {
     return splits > 1 && !j.summed ? us + 5.0 : us;
   };
   for (Cut c : {kLarge, kMedium, kFew}) {
+    if (wide && c != kFew) continue;
     const Shape& s = kShapes[c];
     const int64_t tp = tiles_of(p.m, p.n, c), tq = q.m ? tiles_of(q.m, q.n, c) : 0;
     for (int i : kSplits) {
@@ -604,9 +626,14 @@ template <typename T, Side SA, Side SB, typename E>
 int run_product(Cut c, product_args p, const E& epilogue, hipStream_t s) {
   const int64_t blocks = set_tiles(p, c);
   if (!fits(blocks, kShapes[c].threads)) return MS_OPS_EINVAL;
-  if (c == kLarge) return launch(k_product<T, Large, SA, SB, E>, blocks, Large::kThreads, s, p, epilogue);
-  if (c == kMedium) return launch(k_product<T, Medium, SA, SB, E>, blocks, Medium::kThreads, s, p, epilogue);
-  return launch(k_product<T, Few, SA, SB, E>, blocks, Few::kThreads, s, p, epilogue);
+  if constexpr (sizeof(T) == 4)
+    return launch(k_product<T, Few, SA, SB, E>, blocks, Few::kThreads, s, p, epilogue);
+  else if (c == kLarge)
+    return launch(k_product<T, Large, SA, SB, E>, blocks, Large::kThreads, s, p, epilogue);
+  else if (c == kMedium)
+    return launch(k_product<T, Medium, SA, SB, E>, blocks, Medium::kThreads, s, p, epilogue);
+  else
+    return launch(k_product<T, Few, SA, SB, E>, blocks, Few::kThreads, s, p, epilogue);
 }
 
 template <typename T, Side SB1, Side SB2, typename E>
@@ -639,45 +666,64 @@ bool good_sizes(const ms_rows_t* hidden, const ms_rows_t* weight) {
          weight->n >= 1 && hidden->n <= kMaxRows && weight->n <= kMaxRows && countable(hidden->n, weight->n);
 }
 
-// Whether the products can take the matrix as it lies.
+// Few tokens of 32 bits are multiplied as they are, at a sixteenth of the rate of 16 bits but
+// without the planes, which take several times as long to make as to read the weight: 1 x 1920 x
+// 45061 forward 396 us by planes.
+constexpr int64_t kAsTheyAre = 64;
+bool as_it_is(const ms_rows_t& hidden) {
+  return hidden.dtype != MS_OPS_F32 || hidden.n <= kAsTheyAre;
+}
+
+// Whether the products can take the matrix as it lies: rows on 16 bytes.
 bool lies_well(const ms_rows_t& m) {
+  const int64_t v = 16 / dtype_bytes(m.dtype);
   // (one row has no stride)
-  return m.dtype != MS_OPS_F32 && m.width % 8 == 0 && reinterpret_cast<uintptr_t>(m.data) % 16 == 0 &&
-         (m.n == 1 || (m.inner >= m.n && m.inner_stride % 8 == 0 && m.inner_stride >= m.width &&
+  return m.width % v == 0 && reinterpret_cast<uintptr_t>(m.data) % 16 == 0 &&
+         (m.n == 1 || (m.inner >= m.n && m.inner_stride % v == 0 && m.inner_stride >= m.width &&
                        m.inner_stride <= kMaxWidth));
 }
 
-int planes_of(const ms_rows_t& m) { return m.dtype == MS_OPS_F32 ? 3 : 1; }
-int pairs_of(const ms_rows_t& m) { return m.dtype == MS_OPS_F32 ? 6 : 1; }
+template <typename T>
+int lay_out(const ms_rows_t& m, int64_t ld, const row_t* rows, const float* factor, void* to,
+            hipStream_t s) {
+  const int64_t blocks = ceil_div(m.n * (ld * static_cast<int64_t>(sizeof(T)) / 16), 256);
+  if (!fits(blocks, 256)) return MS_OPS_EINVAL;
+  return launch(k_layout<T>, blocks, 256, s, m, ld, rows, factor, static_cast<T*>(to));
+}
 
-// The matrix as an operand, laid out in the workspace where it does not lie well.
-operand prepare(const ms_rows_t& m, Space& space, int& rc, hipStream_t s, bool run) {
+// The matrix as an operand, laid out in the workspace where it does not lie well, or by planes.
+operand prepare(const ms_rows_t& m, bool planes, Space& space, int& rc, hipStream_t s, bool run) {
   operand o;
   o.rows = static_cast<int32_t>(m.n);
-  if (lies_well(m)) {
-    o.data = static_cast<const uint16_t*>(m.data);
+  if (!planes && lies_well(m)) {
+    o.data = m.data;
     o.ld = m.n == 1 ? m.width : m.inner_stride;
     o.plane = 0;
     return o;
   }
   o.ld = round_up(m.width, 8);
   o.plane = round_up(m.n * o.ld, 128);
-  uint16_t* to = space.take<uint16_t>(o.plane * planes_of(m));
+  const int64_t bytes = o.plane * (planes ? 6 : dtype_bytes(m.dtype));
+  char* to = space.take<char>(bytes);
   o.data = to;
   if (!run || rc) return o;
-  const int64_t blocks = ceil_div(m.n * (o.ld / 8), 256);
-  if (!fits(blocks, 256)) {
-    rc = MS_OPS_EINVAL;
+  if (planes) {
+    const int64_t blocks = ceil_div(m.n * (o.ld / 8), 256);
+    rc = fits(blocks, 256) ? launch(k_planes, blocks, 256, s, m, o.ld, o.plane,
+                                    reinterpret_cast<uint16_t*>(to))
+                           : MS_OPS_EINVAL;
   } else if (m.dtype == MS_OPS_F32) {
-    rc = launch(k_planes, blocks, 256, s, m, o.ld, o.plane, to);
+    rc = lay_out<float>(m, o.ld, nullptr, nullptr, to, s);
   } else if (m.dtype == MS_OPS_F16) {
-    rc = launch(k_layout<f16>, blocks, 256, s, m, o.ld, nullptr, nullptr, reinterpret_cast<f16*>(to));
+    rc = lay_out<f16>(m, o.ld, nullptr, nullptr, to, s);
   } else {
-    rc = launch(k_layout<bf16>, blocks, 256, s, m, o.ld, nullptr, nullptr,
-                reinterpret_cast<bf16*>(to));
+    rc = lay_out<bf16>(m, o.ld, nullptr, nullptr, to, s);
   }
   return o;
 }
+
+// Of k in one tile: 64 values, or 32 of 4 bytes.
+int64_t steps_of(int64_t k, bool wide) { return ceil_div(k, wide ? 32 : 64); }
 
 // The forward pass, or with run = false what workspace it takes.
 int forward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t* targets, float scale,
@@ -685,12 +731,13 @@ int forward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t*
   int rc = 0;
   const int64_t n = hidden.n, vocab = weight.n;
   product_args p{};
-  p.b = prepare(hidden, space, rc, s, run);
-  p.a = prepare(weight, space, rc, s, run);
+  const bool planes = !as_it_is(hidden), wide = hidden.dtype == MS_OPS_F32 && !planes;
+  p.b = prepare(hidden, planes, space, rc, s, run);
+  p.a = prepare(weight, planes, space, rc, s, run);
   p.k = static_cast<int32_t>(hidden.width);
-  p.pairs = pairs_of(hidden);
+  p.pairs = planes ? 6 : 1;
   p.splits = 1;
-  const Cut c = cut_of(vocab, n, ceil_div(hidden.width, kStep) * p.pairs);
+  const Cut c = cut_of(vocab, n, steps_of(hidden.width, wide) * p.pairs, wide);
   const int64_t count = ceil_div(vocab, kShapes[c].m) * kShapes[c].wm;
   sum_epilogue e{};
   e.parts = space.take<float2>(count * n);
@@ -698,8 +745,9 @@ int forward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t*
   if (!run || rc) return rc;
   e.targets = *targets;
   e.scale = scale;
-  rc = hidden.dtype == MS_OPS_F16 ? run_product<f16, kAlong, kAlong>(c, p, e, s)
-                                  : run_product<bf16, kAlong, kAlong>(c, p, e, s);
+  rc = wide                        ? run_product<float, kAlong, kAlong>(c, p, e, s)
+       : hidden.dtype == MS_OPS_F16 ? run_product<f16, kAlong, kAlong>(c, p, e, s)
+                                    : run_product<bf16, kAlong, kAlong>(c, p, e, s);
   if (rc) return rc;
   // few tokens: more threads to each, as one after the other they would wait for memory
   int lanes = 8;
@@ -725,7 +773,8 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
              bool run) {
   int rc = 0;
   const int64_t n = hidden.n, vocab = weight.n, width = hidden.width;
-  const int pairs = pairs_of(hidden);
+  constexpr bool planes = Planes > 1, wide = sizeof(T) == 4;
+  constexpr int pairs = planes ? 6 : 1;
   const bool lifted = hidden.dtype == MS_OPS_F16;
   row_t* rows = space.take<row_t>(n);
   float* factor = space.take<float>(1);
@@ -738,31 +787,29 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
     if (!rc && lifted && blocks > 1)
       rc = launch(k_least, 1, kRowBlocks, s, least, blocks, factor);
   }
-  const operand h = prepare(hidden, space, rc, s, run), w = prepare(weight, space, rc, s, run);
+  const operand h = prepare(hidden, planes, space, rc, s, run);
+  const operand w = prepare(weight, planes, space, rc, s, run);
   operand scaled = h;
   if (lifted && dweight) {
     scaled.ld = round_up(width, 8);
     f16* to = space.take<f16>(n * scaled.ld);
-    scaled.data = reinterpret_cast<const uint16_t*>(to);
-    const int64_t blocks = ceil_div(n * (scaled.ld / 8), 256);
-    if (!fits(blocks, 256)) return MS_OPS_EINVAL;
-    if (run && !rc)
-      rc = launch(k_layout<f16>, blocks, 256, s, hidden, scaled.ld, rows, factor, to);
+    scaled.data = to;
+    if (run && !rc) rc = lay_out<f16>(hidden, scaled.ld, rows, factor, to, s);
   }
   // Pieces of the vocabulary, all of one size: whole large tiles, and no more of them than
   // kPiece holds
-  const int64_t most = std::min(std::max<int64_t>(kPiece / (n * 2 * Planes) / 256 * 256, 256), kMaxWidth);
+  const int64_t most = std::min(std::max<int64_t>(kPiece / (n * static_cast<int64_t>(sizeof(T)) * Planes) / 256 * 256, 256), kMaxWidth);
   const int64_t pieces = ceil_div(vocab, most);
   const int64_t piece = round_up(ceil_div(vocab, pieces), 256);
   const int64_t plane = round_up(n * piece, 128);
   T* d = space.take<T>(plane * Planes);
-  const int64_t wide = std::min(piece, vocab);
-  const Cut cut_d = cut_of(wide, n, ceil_div(width, kStep) * pairs);
+  const int64_t columns = std::min(piece, vocab);
+  const Cut cut_d = cut_of(columns, n, steps_of(width, wide) * pairs, wide);
   // dhidden sums over the pieces in fp32
-  const Job job_h{width, n, ceil_div(wide, kStep) * pairs, pieces > 1};
-  const Job job_w{width, wide, ceil_div(n, kStep) * pairs, false}, none{};
+  const Job job_h{width, n, steps_of(columns, wide) * pairs, pieces > 1};
+  const Job job_w{width, columns, steps_of(n, wide) * pairs, false}, none{};
   // The two products in one launch, if one cut is best for both, the one of more k first
-  Plan plan_h = plan_of(job_h, none), plan_w = plan_of(job_w, none);
+  Plan plan_h = plan_of(job_h, none, wide), plan_w = plan_of(job_w, none, wide);
   const bool both = dhidden && dweight && plan_h.cut != kFew && plan_w.cut != kFew;
   const bool w_first = job_w.steps >= job_h.steps;
   if (both) {
@@ -773,13 +820,13 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
   const int splits_h = plan_h.splits[0], splits_w = plan_w.splits[0];
   float* parts_h = dhidden && (splits_h > 1 || pieces > 1) ? space.take<float>(splits_h * n * width)
                                                            : nullptr;
-  float* parts_w = dweight && splits_w > 1 ? space.take<float>(splits_w * wide * width) : nullptr;
+  float* parts_w = dweight && splits_w > 1 ? space.take<float>(splits_w * columns * width) : nullptr;
   if (!run || rc) return rc;
 
   for (int64_t first = 0; first < vocab; first += piece) {
     const int64_t here = std::min(piece, vocab - first);
     operand w_here = w;
-    w_here.data += first * w.ld;
+    w_here.data = static_cast<const char*>(w.data) + first * w.ld * static_cast<int64_t>(sizeof(T));
     w_here.rows = static_cast<int32_t>(here);
 
     product_args p{w_here, h, static_cast<int32_t>(width), pairs, 0, 0, 1};
@@ -788,19 +835,21 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
     if (rc) return rc;
 
     // dhidden: d, its tokens' rows along k, the vocabulary
-    const uint16_t* some = reinterpret_cast<const uint16_t*>(d);
-    product_args ph{w_here, {some, piece, plane, static_cast<int32_t>(n)}, static_cast<int32_t>(here),
+    product_args ph{w_here, {d, piece, plane, static_cast<int32_t>(n)}, static_cast<int32_t>(here),
                     pairs, 0, 0, splits_h};
     ph.a.rows = static_cast<int32_t>(width);
     const out_epilogue<Out> out_h{static_cast<Out*>(dhidden), parts_h, rows, nullptr, scale, first > 0};
     // dweight: d, its tokens' rows across k, the tokens
-    product_args pw{scaled, {some, piece, plane, static_cast<int32_t>(here)}, static_cast<int32_t>(n),
+    product_args pw{scaled, {d, piece, plane, static_cast<int32_t>(here)}, static_cast<int32_t>(n),
                     pairs, 0, 0, splits_w};
     pw.a.rows = static_cast<int32_t>(width);
     Out* to = static_cast<Out*>(dweight) + first * width;
     const float* by = lifted ? factor : nullptr;
     const out_epilogue<Out> out_w{to, parts_w, nullptr, by, scale, 0};
-    if (both) {
+    if constexpr (wide) {
+      if (dhidden) rc = run_product<T, kAcross, kAlong>(plan_h.cut, ph, out_h, s);
+      if (!rc && dweight) rc = run_product<T, kAcross, kAcross>(plan_w.cut, pw, out_w, s);
+    } else if (both) {
       rc = w_first ? run_products<T, kAcross, kAlong>(plan_h.cut, pw, out_w, ph, out_h, s)
                    : run_products<T, kAlong, kAcross>(plan_h.cut, ph, out_h, pw, out_w, s);
     } else {
@@ -829,6 +878,9 @@ int backward_of(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_token
       return backward<bf16, bf16, 1>(hidden, weight, targets, scale, ignore_index, lse, grad_logprob,
                                      grad_lse, dhidden, dweight, space, s, run);
     default:
+      if (as_it_is(hidden))
+        return backward<float, float, 1>(hidden, weight, targets, scale, ignore_index, lse,
+                                         grad_logprob, grad_lse, dhidden, dweight, space, s, run);
       return backward<bf16, float, 3>(hidden, weight, targets, scale, ignore_index, lse, grad_logprob,
                                       grad_lse, dhidden, dweight, space, s, run);
   }

@@ -1,7 +1,7 @@
 // Matrix products with an epilogue of their own, for operators that use the
 // product's values where they arise instead of storing them (linear.hip).
 //
-//   C[m, n] = sum over k of A[m, k] B[n, k],   2-byte elements, fp32 sums
+//   C[m, n] = sum over k of A[m, k] B[n, k],   elements of 2 (or 4) bytes, fp32 sums
 //
 // A block computes a tile of C; its waves hold it as 32 x 32 squares of matrix
 // instructions (v_mfma_f32_32x32x16).  Of such a square a lane has one column
@@ -33,7 +33,7 @@
 
 namespace ops {
 
-constexpr int kStep = 64;                 // k of one tile
+constexpr int kStepBytes = 128;           // of k in one tile: 64 values of 2 bytes, 32 of 4
 constexpr uint32_t kBeyond = 0x7f000000;  // an offset outside of every buffer
 constexpr uint32_t kRange = 0x40000000;   // bytes that a tile's offsets stay within
 
@@ -43,17 +43,25 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 #define MS_LDS __attribute__((address_space(3)))
 
 template <typename T> struct frag_of;
 template <> struct frag_of<f16> { typedef f16x8 type; };
 template <> struct frag_of<bf16> { typedef bf16x8 type; };
+template <> struct frag_of<float> { typedef f32x4 type; };
 
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// The instruction takes two k, one from each half of the wave: here value e of both halves' four.
+__device__ __forceinline__ f32x16 mfma(f32x4 a, f32x4 b, f32x16 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
 }
 
 // One operand: `rows` of m or n against k.  Along k: row r starts at r * ld, and ld and
@@ -62,8 +70,8 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
 // the next); the product then runs over the six pairs of planes whose product is not
 // below the last bit, as if k were six times as long.
 struct operand {
-  const uint16_t* data;
-  int64_t ld;
+  const void* data;
+  int64_t ld;              // elements, as plane
   int64_t plane;
   int32_t rows;
 };
@@ -93,13 +101,14 @@ __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t offset, uint32_
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // One operand's tile of R rows, fetched by NT threads.
-template <int R, int NT, Side S>
+template <typename T, int R, int NT, Side S>
 struct Fetch {
-  static constexpr int kIssues = R * kStep * 2 / (NT * 16);
-  static constexpr int kChunks = R / 8;              // across: 16-byte chunks of a row
+  static constexpr int kIssues = R * kStepBytes / (NT * 16), kStep = kStepBytes / sizeof(T);
+  static constexpr int V = 16 / sizeof(T);
+  static constexpr int kChunks = R / V;              // across: 16-byte chunks of a row
   static constexpr int kRowsPer = S == kAlong ? NT / 8 : NT / kChunks;
-  static constexpr int kTurn = kChunks >= 16 ? 3 : 0;
-  static_assert(kIssues >= 1 && R * kStep * 2 % (NT * 16) == 0, "");
+  static constexpr int kTurn = sizeof(T) == 2 && kChunks >= 16 ? 3 : 0;
+  static_assert(kIssues >= 1 && R * kStepBytes % (NT * 16) == 0, "");
   static_assert(S == kAlong ? kRowsPer % 16 == 0 : kRowsPer % 4 == 0, "");
 
   const char* base;
@@ -108,11 +117,11 @@ struct Fetch {
   int first_k;        // k of this thread's first chunk, within the tile
 
   __device__ Fetch(const operand& o, int row0, int tid) {
-    ld_bytes = o.ld * 2;
+    ld_bytes = o.ld * static_cast<int64_t>(sizeof(T));
     if (S == kAlong) {
       base = reinterpret_cast<const char*>(o.data) + row0 * ld_bytes;
       const int r = tid >> 3, chunk = (tid & 7) ^ (r >> 1 & 7);
-      first_k = chunk * 8;
+      first_k = chunk * V;
 #pragma unroll
       for (int i = 0; i < kIssues; ++i) {
         const int row = r + i * kRowsPer;
@@ -121,12 +130,12 @@ struct Fetch {
                         : kBeyond;
       }
     } else {
-      base = reinterpret_cast<const char*>(o.data) + static_cast<int64_t>(row0) * 2;
+      base = reinterpret_cast<const char*>(o.data) + static_cast<int64_t>(row0) * sizeof(T);
       first_k = tid / kChunks;
       const int chunk = tid % kChunks ^ (first_k & kTurn) << 2;
 #pragma unroll
       for (int i = 0; i < kIssues; ++i)
-        offset[i] = row0 + chunk * 8 < o.rows
+        offset[i] = row0 + chunk * V < o.rows
                         ? static_cast<uint32_t>((first_k + i * kRowsPer) * static_cast<int>(ld_bytes)) +
                               chunk * 16
                         : kBeyond;
@@ -135,7 +144,8 @@ struct Fetch {
 
   // The tile at k0 of plane `shift` elements further, into LDS at `to`; `left` is k - k0.
   __device__ void issue(int64_t shift, int k0, int left, uint32_t to, int wave) const {
-    const char* p = base + shift * 2 + (S == kAlong ? static_cast<int64_t>(k0) * 2 : k0 * ld_bytes);
+    const char* p = base + shift * static_cast<int64_t>(sizeof(T)) +
+                    (S == kAlong ? k0 * static_cast<int64_t>(sizeof(T)) : k0 * ld_bytes);
     const u32x4 rsrc = {static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)),
                         static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) >> 32) & 0xffff, kRange,
                         0x00027000};
@@ -166,6 +176,10 @@ struct Frags {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
         at[ks] = (first + r) * 128 + (((ks * 2 + (lane >> 5)) ^ (r >> 1 & 7)) << 4);
+    } else if (sizeof(T) == 4) {
+      // (a value of m for each lane, four k one after the other)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) at[q] = (lane >> 5) * 4 * R * 4 + (first + q * 32 + (lane & 31)) * 4;
     } else {
       constexpr int kTurn = R / 8 >= 16 ? 3 : 0;
       const int k = (lane >> 5) * 8 + ((lane & 15) >> 2);
@@ -181,6 +195,13 @@ struct Frags {
   __device__ frag read(const char MS_LDS* tile, int q, int ks) const {
     if (S == kAlong)
       return *reinterpret_cast<const frag MS_LDS*>(tile + at[ks] + q * 32 * 128);
+    if constexpr (sizeof(T) == 4) {
+      frag x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] = *reinterpret_cast<const float MS_LDS*>(tile + at[q & 3] + (ks * 8 + e) * R * 4);
+      return x;
+    } else {
     union { s16x4 half[2]; frag whole; } u;
     const char MS_LDS* p = tile + at[q & 3] + (q >> 2) * 256 + ks * 16 * R * 2;
     u.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -188,6 +209,7 @@ struct Frags {
     u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         reinterpret_cast<s16x4 MS_LDS*>(const_cast<char MS_LDS*>(p + 4 * R * 2)));
     return u.whole;
+    }
   }
 };
 
@@ -212,7 +234,7 @@ __device__ __forceinline__ void place(uint32_t b, uint32_t total, int tiles_m, i
 template <int BM_, int BN_, int WM_, int WN_>
 struct Tiles {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kThreads = WM * WN * 64;
-  static constexpr int kBytes = 2 * (BM + BN) * kStep * 2;      // of LDS
+  static constexpr int kBytes = 2 * (BM + BN) * kStepBytes;     // of LDS
 };
 
 namespace {
@@ -224,7 +246,8 @@ __device__ __forceinline__ void multiply_tile(const product_args& p, const Epilo
 #ifdef __HIP_DEVICE_COMPILE__  // (the host has none of the built-in functions)
   constexpr int BM = Tile::BM, BN = Tile::BN, WM = Tile::WM, WN = Tile::WN;
   constexpr int NT = Tile::kThreads, MI = BM / WM / 32, NI = BN / WN / 32;
-  constexpr int kTileA = BM * kStep * 2, kTile = kTileA + BN * kStep * 2;
+  constexpr int kStep = kStepBytes / sizeof(T);
+  constexpr int kTileA = BM * kStepBytes, kTile = kTileA + BN * kStepBytes;
   static_assert(BM % (WM * 32) == 0 && BN % (WN * 32) == 0, "");
   char MS_LDS* const lds = (char MS_LDS*)memory;
 
@@ -233,8 +256,8 @@ __device__ __forceinline__ void multiply_tile(const product_args& p, const Epilo
   int tm, tn, split;
   place(block, blocks, p.tiles_m, p.tiles_n, tm, tn, split);
 
-  const Fetch<BM, NT, SA> fetch_a(p.a, tm * BM, tid);
-  const Fetch<BN, NT, SB> fetch_b(p.b, tn * BN, tid);
+  const Fetch<T, BM, NT, SA> fetch_a(p.a, tm * BM, tid);
+  const Fetch<T, BN, NT, SB> fetch_b(p.b, tn * BN, tid);
   const Frags<T, BM, SA> frags_a(wm * MI * 32, lane);
   const Frags<T, BN, SB> frags_b(wn * NI * 32, lane);
 
