@@ -181,7 +181,7 @@ int ms_act8_grad(const int8_t* codes, const uint8_t* exponents, const int8_t* up
  * both of at most 2^31 - 1025 rows.  Outputs as of ms_logprobs, fp32, dense:
  * lse, and logprob (0 where target == ignore_index, NaN where it is outside of [0, vocab)).
  * A token whose logits hold NaN or +inf has NaN in both, one whose logits are all -inf
- * has -inf in both.
+ * has -inf in both (fp32 operands that hold infinities: or NaN).
  */
 int64_t ms_linear_logprobs_workspace(const ms_rows_t* hidden, const ms_rows_t* weight);
 int ms_linear_logprobs(const ms_rows_t* hidden, const ms_rows_t* weight,
@@ -195,7 +195,7 @@ int ms_linear_logprobs(const ms_rows_t* hidden, const ms_rows_t* weight,
  *   dweight = scale d^T hidden
  * with g = grad_logprob (0 where target == ignore_index, and where NULL) and l = grad_lse
  * (0 where NULL); lse is the forward pass's.  dhidden or dweight may be NULL: not
- * computed.  d is rounded to the operands' type (three times, for fp32: 24 bits).
+ * computed.  d is rounded to the operands' type.
  * Tokens whose lse is -inf, and those with g = l = 0, have d = 0.
  */
 int64_t ms_linear_logprobs_grad_workspace(const ms_rows_t* hidden, const ms_rows_t* weight);

@@ -21,9 +21,10 @@
 // an inverse count of tokens); dhidden's rows are scaled back, and dweight takes its
 // scales from a copy of hidden multiplied by them, exactly but for underflow of
 // rows whose gradients are 2^14 times smaller than the largest.
-// 32-bit operands are split into three bf16 planes of 8 bits each (x = a + b + c,
+// 32-bit operands of many tokens are split into three bf16 planes of 8 bits each (x = a + b + c,
 // exactly), and six products of planes are summed; what is left out is below 2^-22 of
-// the terms.  The matrix units' own 32-bit products have a sixteenth of the bf16 rate.
+// the terms.  The matrix units' own 32-bit products have a sixteenth of the bf16 rate, and are
+// for few tokens and small products.
 //
 // exp and log are taken in units of log 2.
 //
@@ -666,12 +667,15 @@ bool good_sizes(const ms_rows_t* hidden, const ms_rows_t* weight) {
          weight->n >= 1 && hidden->n <= kMaxRows && weight->n <= kMaxRows && countable(hidden->n, weight->n);
 }
 
-// Few tokens of 32 bits are multiplied as they are, at a sixteenth of the rate of 16 bits but
-// without the planes, which take several times as long to make as to read the weight: 1 x 1920 x
-// 45061 forward 396 us by planes.
-constexpr int64_t kAsTheyAre = 64;
-bool as_it_is(const ms_rows_t& hidden) {
-  return hidden.dtype != MS_OPS_F32 || hidden.n <= kAsTheyAre;
+// Few tokens of 32 bits, and small products, are multiplied as they are, at 120 TFLOP/s where six
+// products of planes have 190, but without the planes: of 1920 x 45061, 1 token forward 81 us
+// (396 by planes), 256 tokens 363 (656), their gradients 1106 (1395); 256 x 256 x 2000 12.5
+// (27.4).  Between 384 and 512 tokens the planes' gradients are as fast.
+constexpr int64_t kAsTheyAre = 384;
+constexpr double kSmallProduct = 1 << 29;
+bool as_it_is(const ms_rows_t& hidden, const ms_rows_t& weight) {
+  return hidden.dtype != MS_OPS_F32 || hidden.n <= kAsTheyAre ||
+         static_cast<double>(hidden.n) * hidden.width * weight.n <= kSmallProduct;
 }
 
 // Whether the products can take the matrix as it lies: rows on 16 bytes.
@@ -731,7 +735,7 @@ int forward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t*
   int rc = 0;
   const int64_t n = hidden.n, vocab = weight.n;
   product_args p{};
-  const bool planes = !as_it_is(hidden), wide = hidden.dtype == MS_OPS_F32 && !planes;
+  const bool planes = !as_it_is(hidden, weight), wide = hidden.dtype == MS_OPS_F32 && !planes;
   p.b = prepare(hidden, planes, space, rc, s, run);
   p.a = prepare(weight, planes, space, rc, s, run);
   p.k = static_cast<int32_t>(hidden.width);
@@ -878,7 +882,7 @@ int backward_of(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_token
       return backward<bf16, bf16, 1>(hidden, weight, targets, scale, ignore_index, lse, grad_logprob,
                                      grad_lse, dhidden, dweight, space, s, run);
     default:
-      if (as_it_is(hidden))
+      if (as_it_is(hidden, weight))
         return backward<float, float, 1>(hidden, weight, targets, scale, ignore_index, lse,
                                          grad_logprob, grad_lse, dhidden, dweight, space, s, run);
       return backward<bf16, float, 3>(hidden, weight, targets, scale, ignore_index, lse, grad_logprob,

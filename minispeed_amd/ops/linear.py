@@ -46,7 +46,7 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
     forward or backward: beside the operands and the gradients a call takes some
     bytes for each token and 128 words of the vocabulary, and backward 512 MiB at most
     (or 256 words' worth of the vocabulary, and copies of 2-byte operands whose rows
-    are not on 16-byte boundaries; of float32 operands always).
+    are not on 16-byte boundaries; of float32 ones of many tokens always).
 
     Per row: ``logprob`` of the target (0 where it is ``ignore_index``, NaN where it is outside
     the vocabulary) and ``lse``, the log of the sum of exponentials.  Both are

@@ -125,6 +125,30 @@ def test_wide_tiles(dtype, n, d, v):
     check(*make(n, d, v, dtype, n + d))
 
 
+@pytest.mark.parametrize("n,d,v", [(700, 257, 3001), (390, 65, 22000), (500, 131, 9001), (385, 2056, 700)])
+def test_many_tokens_of_32_bits(n, d, v):
+    """Those are multiplied by planes of 16 bits."""
+    h, w, t, gr, gl = make(n, d, v, "fp32", n)
+    first = check(h, w, t, gr, gl)
+    base = torch.zeros(v, d + 3, device=DEV)
+    base[:, 1:d + 1] = w
+    again = check(h, base[:, 1:d + 1], t.int(), gr, gl, scale=1.0)
+    assert all(torch.equal(a, b) for a, b in zip((*first[0], *first[1:]), (*again[0], *again[1:])))
+    check(h * 1e-3, w * 1e3, t, gr, None, scale=-0.5)
+    bad = h.clone()
+    bad[3, 1], bad[4, 0] = NAN, INF
+    r = ms.ops.linear_logprobs(bad, w, t)
+    assert r.lse[3].isnan() and r.lse[4].isnan()
+    keep = torch.ones(n, dtype=torch.bool, device=DEV)
+    keep[3:5] = False
+    assert torch.equal(r.lse[keep], first[0].lse[keep])
+
+
+@pytest.mark.parametrize("n,d,v", [(384, 520, 3001), (383, 65, 22001), (300, 2050, 701)])
+def test_tokens_of_32_bits_as_they_are(n, d, v):
+    check(*make(n, d, v, "fp32", n))
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_several_pieces_of_the_vocabulary(dtype):
     check(*make(60000, 16, 3000, dtype, 5))
