@@ -29,7 +29,7 @@
 // exp and log are taken in units of log 2.
 //
 // Measured: 8192 x 2048 x 50257 fp16 forward 1.51-1.57 ms, 1080-1120 TFLOP/s (the product alone, by the
-// library, 1.56 ms); the exponentials are 12% of it.  4 x 4096 x 128256 bf16 187 us, 5.6 TB/s, reading the
+// library, 1.56 ms).  4 x 4096 x 128256 bf16 187 us, 5.6 TB/s, reading the
 // weight.  Backward 16384 x 768 x 50257 bf16 3.9-4.0 ms (four pieces: d 390 us, 820 TFLOP/s
 // as its 12 steps of k do not hide the exponentials and stores; both products 595 us, 1080
 // TFLOP/s), 2048 x 4096 x 128256 5.7 ms (1130 TFLOP/s over all).

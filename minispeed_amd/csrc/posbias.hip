@@ -324,7 +324,7 @@ bool good_plane(int64_t heads, int64_t queries, int64_t keys, int64_t first) {
          (heads == 0 || queries == 0 || (countable(heads, queries) && countable(heads * queries, keys)));
 }
 
-constexpr int64_t kGradUnits = 3072;      // waves, 12 to a CU
+constexpr int64_t kGradUnits = 12 * 256;   // waves, 12 to a CU
 
 int64_t span_of(int32_t dtype) { return kThreads * (16 / dtype_bytes(dtype)); }
 

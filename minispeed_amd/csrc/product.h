@@ -191,7 +191,7 @@ struct Frags {
     }
   }
 
-  // Square q (32 rows further each), 16 k from 16 ks.
+  // Square q (32 rows further each), 32 bytes of k from 32 ks.
   __device__ frag read(const char MS_LDS* tile, int q, int ks) const {
     if (S == kAlong)
       return *reinterpret_cast<const frag MS_LDS*>(tile + at[ks] + q * 32 * 128);
@@ -202,13 +202,13 @@ struct Frags {
         x[e] = *reinterpret_cast<const float MS_LDS*>(tile + at[q & 3] + (ks * 8 + e) * R * 4);
       return x;
     } else {
-    union { s16x4 half[2]; frag whole; } u;
-    const char MS_LDS* p = tile + at[q & 3] + (q >> 2) * 256 + ks * 16 * R * 2;
-    u.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        reinterpret_cast<s16x4 MS_LDS*>(const_cast<char MS_LDS*>(p)));
-    u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        reinterpret_cast<s16x4 MS_LDS*>(const_cast<char MS_LDS*>(p + 4 * R * 2)));
-    return u.whole;
+      union { s16x4 half[2]; frag whole; } u;
+      const char MS_LDS* p = tile + at[q & 3] + (q >> 2) * 256 + ks * 16 * R * 2;
+      u.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          reinterpret_cast<s16x4 MS_LDS*>(const_cast<char MS_LDS*>(p)));
+      u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          reinterpret_cast<s16x4 MS_LDS*>(const_cast<char MS_LDS*>(p + 4 * R * 2)));
+      return u.whole;
     }
   }
 };
