@@ -197,8 +197,12 @@ int ms_linear_logprobs(const ms_rows_t* hidden, const ms_rows_t* weight,
  * (0 where NULL); lse is the forward pass's.  dhidden or dweight may be NULL: not
  * computed.  d is rounded to the operands' type.
  * Tokens whose lse is -inf, and those with g = l = 0, have d = 0.
+ * Workspace: the first function gives what is enough whichever gradients are wanted; the second
+ * what a call takes that wants these (one alone may take more than both, and less).
  */
 int64_t ms_linear_logprobs_grad_workspace(const ms_rows_t* hidden, const ms_rows_t* weight);
+int64_t ms_linear_logprobs_grad_workspace_for(const ms_rows_t* hidden, const ms_rows_t* weight,
+                                              int32_t want_hidden, int32_t want_weight);
 int ms_linear_logprobs_grad(const ms_rows_t* hidden, const ms_rows_t* weight,
                             const ms_tokens_t* targets, float scale, int64_t ignore_index,
                             const float* lse, const float* grad_logprob, const float* grad_lse,

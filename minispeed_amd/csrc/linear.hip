@@ -926,16 +926,27 @@ int ms_linear_logprobs(const ms_rows_t* hidden, const ms_rows_t* weight, const m
                  static_cast<hipStream_t>(stream), true);
 }
 
-int64_t ms_linear_logprobs_grad_workspace(const ms_rows_t* hidden, const ms_rows_t* weight) {
+int64_t ms_linear_logprobs_grad_workspace_for(const ms_rows_t* hidden, const ms_rows_t* weight,
+                                              int32_t want_hidden, int32_t want_weight) {
   using namespace ops;
   if (!good_sizes(hidden, weight)) return MS_OPS_EINVAL;
-  if (hidden->n == 0) return 0;
+  if (hidden->n == 0 || (!want_hidden && !want_weight)) return 0;
   Space space{nullptr};
-  // (any address: both gradients)
+  // (any address: a gradient that is wanted)
   char some;
-  backward_of(*hidden, *weight, nullptr, 1.0f, 0, nullptr, nullptr, nullptr, &some, &some, space,
-              nullptr, false);
+  backward_of(*hidden, *weight, nullptr, 1.0f, 0, nullptr, nullptr, nullptr,
+              want_hidden ? &some : nullptr, want_weight ? &some : nullptr, space, nullptr, false);
   return space.used;
+}
+
+// One gradient alone has a plan of its own, which may cut k into more parts than that of both in
+// one launch and then takes more (4096 x 5120 x 32000 bf16: 430 MB for dhidden, 262 for both).
+int64_t ms_linear_logprobs_grad_workspace(const ms_rows_t* hidden, const ms_rows_t* weight) {
+  const auto of = [&](int32_t h, int32_t w) {
+    return ms_linear_logprobs_grad_workspace_for(hidden, weight, h, w);
+  };
+  const int64_t both = of(1, 1);
+  return both < 0 ? both : std::max(both, std::max(of(1, 0), of(0, 1)));
 }
 
 int ms_linear_logprobs_grad(const ms_rows_t* hidden, const ms_rows_t* weight,
@@ -956,8 +967,10 @@ int ms_linear_logprobs_grad(const ms_rows_t* hidden, const ms_rows_t* weight,
   }
   if (!lse) return MS_OPS_EINVAL;
   if (!dhidden && !dweight) return MS_OPS_OK;
-  if (workspace_bytes < ms_linear_logprobs_grad_workspace(hidden, weight) || !workspace ||
-      !aligned(workspace))
+  // what these gradients take, by the same steps as the run itself
+  const int64_t need =
+      ms_linear_logprobs_grad_workspace_for(hidden, weight, dhidden != nullptr, dweight != nullptr);
+  if (workspace_bytes < need || !workspace || !aligned(workspace))
     return MS_OPS_EWORKSPACE;
   Space space{static_cast<char*>(workspace)};
   return backward_of(*hidden, *weight, targets, scale, ignore_index, lse, grad_logprob, grad_lse,

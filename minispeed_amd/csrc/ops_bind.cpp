@@ -466,7 +466,7 @@ py::tuple linear_logprobs_grad(const Tensor& hidden, const Tensor& weight, const
   const float* gl = per_row(grad_lse, hidden, h.n, "grad_lse", hold[2]);
   const Tensor dh = want_hidden ? make(hidden, hidden.sizes(), hidden.scalar_type()) : Tensor();
   const Tensor dw = want_weight ? make(weight, weight.sizes(), weight.scalar_type()) : Tensor();
-  const int64_t bytes = ms_linear_logprobs_grad_workspace(&h, &w);
+  const int64_t bytes = ms_linear_logprobs_grad_workspace_for(&h, &w, want_hidden, want_weight);
   const Tensor work = scratch(hidden, bytes);
   check(ms_linear_logprobs_grad(&h, &w, &y, static_cast<float>(scale), ignore_index, l, g, gl,
                                 data_of(dh), data_of(dw), data_of(work), bytes, stream_of(hidden)),
