@@ -368,12 +368,15 @@ __global__ __launch_bounds__(256) void k_join(const float2* parts, const float* 
   }
 }
 
+// Whether a row's d is made of finite numbers that are not all zeros.
+__device__ __forceinline__ bool lifts(float bound) { return bound > 0.0f && bound < __builtin_inff(); }
+
 // The power of two that brings a row's d below 2^15, given the larger one of the two terms that
-// meet in it; 0 for zero rows.
+// meet in it; 0 for rows of zeros, infinities and NaN.  (Numbers below 2^-87, the subnormal ones
+// among them, stay as far below 2^14.)
 __device__ __forceinline__ int lift(float bound) {
   const int e = static_cast<int>(__float_as_uint(bound) >> 23 & 255);
-  // (the smallest numbers, infinities and NaN are left as they are)
-  return e == 0 || e == 255 ? 0 : min(13 + 127 - e, 100);
+  return lifts(bound) ? min(13 + 127 - e, 100) : 0;
 }
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((e + 127) << 23); }
@@ -411,7 +414,7 @@ __global__ __launch_bounds__(1024) void k_rows(const float* lse, const float* gr
     if (lifted) {
       const float bound = fmaxf(fabsf(soft), fabsf(g));
       up = lift(bound);
-      if (bound > 0.0f) low = min(low, up);
+      if (lifts(bound)) low = min(low, up);
     }
     rows[t] = {of == -__builtin_inff() ? 0.0f : of * kLog2e, soft * pow2(up), g * pow2(up), pow2(-up)};
   }
