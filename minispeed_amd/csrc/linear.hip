@@ -19,8 +19,9 @@
 // term, which the sums average.  In fp16 a row of d is scaled by a power of two that
 // brings its bound below 2^15 (p reaches down to 2^-20 over large vocabularies, and g is
 // an inverse count of tokens); dhidden's rows are scaled back, and dweight takes its
-// scales from a copy of hidden multiplied by them, exactly but for underflow of
-// rows whose gradients are 2^14 times smaller than the largest.
+// scales from a copy of hidden multiplied by them, lifted as far as fp16 goes: exactly but for
+// underflow below 2^-40 of the largest row's gradient times its largest value, which is
+// where the results themselves underflow if that row's do not overflow.
 // 32-bit operands of many tokens are split into three bf16 planes of 8 bits each (x = a + b + c,
 // exactly), and six products of planes are summed; what is left out is below 2^-22 of
 // the terms.  The matrix units' own 32-bit products have a sixteenth of the bf16 rate, and are
@@ -381,67 +382,61 @@ __device__ __forceinline__ int lift(float bound) {
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((e + 127) << 23); }
 
-constexpr int kRowBlocks = 256;
+// What the row numbers follow from.
+struct rows_args {
+  const float *lse, *grad_logprob, *grad_lse;
+  ms_tokens_t targets;
+  int64_t vocab, ignore_index;
+  int32_t lifted;          // fp16
+};
 
-// The least of a block's numbers, in thread 0.
-__device__ __forceinline__ int block_least(int low, int* held) {
+// A token's numbers; `up`, the power of two in them, is kNoLift where the row's scale does not matter.
+constexpr int kNoLift = INT32_MAX;
+__device__ __forceinline__ row_t row_numbers(const rows_args& a, int64_t t, int& up) {
+  // (all loads at once: none waits for the token)
+  const float given = a.grad_logprob ? a.grad_logprob[t] : 0.0f, of = a.lse[t];
+  float l = a.grad_lse ? a.grad_lse[t] : 0.0f;
+  const int64_t y = token(a.targets, t);
+  float g = y != a.ignore_index ? given : 0.0f;
+  if (y != a.ignore_index && (y < 0 || y >= a.vocab) && a.grad_logprob) g = quiet_nan();
+  if (of == -__builtin_inff()) g = l = 0.0f;
+  const float soft = l - g, bound = fmaxf(fabsf(soft), fabsf(g));
+  const int by = a.lifted ? lift(bound) : 0;
+  up = lifts(bound) ? by : kNoLift;
+  return {of == -__builtin_inff() ? 0.0f : of * kLog2e, soft * pow2(by), g * pow2(by), pow2(-by)};
+}
+
+// Row numbers for the backward pass.
+__global__ __launch_bounds__(256) void k_rows(rows_args a, row_t* rows) {
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  int up;
+  if (t < a.targets.n) rows[t] = row_numbers(a, t, up);
+}
+
+// The same for an fp16 dweight.  Its sums over the tokens have one scale, so what d's row is lifted
+// by, hidden's gives way for: hidden[t] 2^(low - up[t]).  `low` is the largest power of two for
+// which no such row passes fp16's largest number: the least of up[t] + 30 - e, e the exponent bits of
+// the row's largest value, so that all of fp16's 40 powers of two are there for rows whose
+// gradients are smaller than others'.  16 lanes to a token; each block's least goes to
+// least[block].  (3.7 us of 28.9 for 1024 x 256 x 512, where one block without a look at hidden took
+// 2.5; 16384 x 768 x 50257 is as fast as by that.)
+constexpr int kScaleBlocks = 512, kScaleThreads = 1024, kScaleRows = kScaleThreads / 16, kMostLow = 126;
+
+// The least of the numbers of a block of W waves, in every thread.
+template <int W>
+__device__ __forceinline__ int block_least(int low, int (&held)[W]) {
 #pragma unroll
   for (int s = 32; s; s /= 2) low = min(low, __shfl_xor(low, s));
   if ((threadIdx.x & 63) == 0) held[threadIdx.x >> 6] = low;
   __syncthreads();
-  for (unsigned w = 0; w < blockDim.x / 64; ++w) low = min(low, held[w]);
+#pragma unroll
+  for (int w = 0; w < W; ++w) low = min(low, held[w]);
   return low;
 }
 
-// Row numbers for the backward pass.  With `lifted` (fp16) the least power of two of any row's
-// scale goes to factor[0], or each block's to least[block] where there are several.
-__global__ __launch_bounds__(1024) void k_rows(const float* lse, const float* grad_logprob,
-                                               const float* grad_lse, ms_tokens_t targets,
-                                               int64_t vocab, int64_t ignore_index, int lifted,
-                                               row_t* rows, float* factor, int* least) {
-  __shared__ int held[16];
-  int low = 100;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; t < targets.n;
-       t += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t y = token(targets, t);
-    float g = grad_logprob && y != ignore_index ? grad_logprob[t] : 0.0f;
-    float l = grad_lse ? grad_lse[t] : 0.0f;
-    const float of = lse[t];
-    if (y != ignore_index && (y < 0 || y >= vocab) && grad_logprob) g = quiet_nan();
-    if (of == -__builtin_inff()) g = l = 0.0f;
-    const float soft = l - g;
-    int up = 0;
-    if (lifted) {
-      const float bound = fmaxf(fabsf(soft), fabsf(g));
-      up = lift(bound);
-      if (lifts(bound)) low = min(low, up);
-    }
-    rows[t] = {of == -__builtin_inff() ? 0.0f : of * kLog2e, soft * pow2(up), g * pow2(up), pow2(-up)};
-  }
-  if (!lifted) return;
-  low = block_least(low, held);
-  if (threadIdx.x) return;
-  if (gridDim.x == 1) factor[0] = pow2(-low);
-  else least[blockIdx.x] = low;
-}
-
-__global__ __launch_bounds__(kRowBlocks) void k_least(const int* least, int count, float* factor) {
-  __shared__ int held[16];
-  const int low =
-      block_least(static_cast<int>(threadIdx.x) < count ? least[threadIdx.x] : 100, held);
-  if (threadIdx.x == 0) factor[0] = pow2(-low);
-}
-
-// A matrix as the products take it: rows at `ld`, zeros behind `width`; times a row's
-// scale relative to the largest (fp16), or as three planes (fp32).
-template <typename T>
-__global__ __launch_bounds__(256) void k_layout(ms_rows_t from, int64_t ld, const row_t* rows,
-                                                const float* factor, T* to) {
-  constexpr int V = 16 / sizeof(T);
-  const int64_t chunks = ld / V;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= from.n * chunks) return;
-  const int64_t r = i / chunks, c = (i - r * chunks) * V;
+// Chunk c .. c + V - 1 of a row, zeros behind its end.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_chunk(const ms_rows_t& from, int64_t r, int64_t c) {
   const T* p = static_cast<const T*>(from.data) + row_start(from, r) + c;
   Pack<T, V> x;
   if (c + V <= from.width) {
@@ -450,13 +445,87 @@ __global__ __launch_bounds__(256) void k_layout(ms_rows_t from, int64_t ld, cons
 #pragma unroll
     for (int e = 0; e < V; ++e) x.v[e] = c + e < from.width ? p[e] : static_cast<T>(0.0f);
   }
-  if (rows) {
-    // a row without a gradient keeps the scale 1 that it was given: its d is zero
-    const float by = rows[r].soft == 0.0f && rows[r].given == 0.0f ? 1.0f : rows[r].down / *factor;
+  return x;
+}
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+__global__ __launch_bounds__(kScaleThreads) void k_scaled_rows(rows_args a, ms_rows_t hidden, row_t* rows,
+                                                               int* least) {
+  __shared__ int held[kScaleThreads / 64];
+  const int lane = threadIdx.x & 15;
+  const int64_t n = a.targets.n;
+  int low = kMostLow;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kScaleRows + threadIdx.x / 16; t < n;
+       t += static_cast<int64_t>(gridDim.x) * kScaleRows) {
+    const uint16_t* p = static_cast<const uint16_t*>(hidden.data) + row_start(hidden, t);
+    const int width = static_cast<int>(hidden.width);
+    // By pairs of 2-byte numbers: adding 2^10 to one and dropping its sign puts its size in order
+    // behind the infinities and NaN, which have no say.
+    u16x2 most = {0x400, 0x400};
+    auto take = [&](u16x2 x) {
+      most = __builtin_elementwise_max(most, (x + u16x2{0x400, 0x400}) & u16x2{0x7fff, 0x7fff});
+    };
+    if (width >= 8) {
+      // (what would pass the row's end is its last 8 values again)
+      for (int c = lane * 8; c < width; c += 4 * 128) {
+        Pack<u16x2, 4> x[4];
 #pragma unroll
-    for (int e = 0; e < V; ++e) x.v[e] = narrow<T>(widen(x.v[e]) * by);
+        for (int k = 0; k < 4; ++k)
+          x[k] = load<4>(reinterpret_cast<const u16x2*>(p + min(c + k * 128, width - 8)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) take(x[k].v[e]);
+      }
+    } else if (lane < width) {
+      take(u16x2{p[lane], p[lane]});
+    }
+    int up, size = max(most[0], most[1]) - 0x400;
+    const row_t row = row_numbers(a, t, up);
+    if (lane == 0) rows[t] = row;
+#pragma unroll
+    for (int s = 8; s; s /= 2) size = max(size, __shfl_xor(size, s));
+    if (size && up != kNoLift) low = min(low, up + 30 - (size >> 10));
   }
-  ops::store<V>(to + r * ld + c, x);
+  low = block_least(low, held);
+  if (threadIdx.x == 0) least[blockIdx.x] = low;
+}
+
+// A matrix as the products take it: rows at `ld`, zeros behind `width`.
+template <typename T>
+__global__ __launch_bounds__(256) void k_layout(ms_rows_t from, int64_t ld, T* to) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t chunks = ld / V;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= from.n * chunks) return;
+  const int64_t r = i / chunks, c = (i - r * chunks) * V;
+  ops::store<V>(to + r * ld + c, load_chunk<T, V>(from, r, c));
+}
+
+// hidden with its rows' scales, and the factor 2^-low that dweight takes back.
+__global__ __launch_bounds__(256) void k_scaled_layout(ms_rows_t from, int64_t ld, const row_t* rows,
+                                                       const int* least, int count, f16* to,
+                                                       float* factor) {
+  __shared__ int held[4];
+  const int64_t chunks = ld / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const bool there = i < from.n * chunks;
+  const int64_t r = there ? i / chunks : 0, c = there ? (i - r * chunks) * 8 : 0;
+  Pack<f16, 8> x = load_chunk<f16, 8>(from, r, c);
+  const row_t row = rows[r];
+  int low = kMostLow;
+#pragma unroll
+  for (int k = 0; k < kScaleBlocks / 256; ++k)
+    low = min(low, least[min(static_cast<int>(threadIdx.x) + k * 256, count - 1)]);
+  low = block_least(low, held);
+  if (i == 0) *factor = pow2(-low);
+  if (!there) return;
+  // (a row without a gradient or with one that is not finite was lifted by nothing)
+  const float by = lifts(fmaxf(fabsf(row.soft), fabsf(row.given))) ? row.down * pow2(low) : 1.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x.v[e] = narrow<f16>(widen(x.v[e]) * by);
+  ops::store<8>(to + r * ld + c, x);
 }
 
 // Three planes of bf16: the leading 8 bits of each value, the next 8, the rest.  Cut off
@@ -695,11 +764,10 @@ bool lies_well(const ms_rows_t& m) {
 }
 
 template <typename T>
-int lay_out(const ms_rows_t& m, int64_t ld, const row_t* rows, const float* factor, void* to,
-            hipStream_t s) {
+int lay_out(const ms_rows_t& m, int64_t ld, void* to, hipStream_t s) {
   const int64_t blocks = ceil_div(m.n * (ld * static_cast<int64_t>(sizeof(T)) / 16), 256);
   if (!fits(blocks, 256)) return MS_OPS_EINVAL;
-  return launch(k_layout<T>, blocks, 256, s, m, ld, rows, factor, static_cast<T*>(to));
+  return launch(k_layout<T>, blocks, 256, s, m, ld, static_cast<T*>(to));
 }
 
 // The matrix as an operand, laid out in the workspace where it does not lie well, or by planes.
@@ -724,11 +792,11 @@ operand prepare(const ms_rows_t& m, bool planes, Space& space, int& rc, hipStrea
                                     reinterpret_cast<uint16_t*>(to))
                            : MS_OPS_EINVAL;
   } else if (m.dtype == MS_OPS_F32) {
-    rc = lay_out<float>(m, o.ld, nullptr, nullptr, to, s);
+    rc = lay_out<float>(m, o.ld, to, s);
   } else if (m.dtype == MS_OPS_F16) {
-    rc = lay_out<f16>(m, o.ld, nullptr, nullptr, to, s);
+    rc = lay_out<f16>(m, o.ld, to, s);
   } else {
-    rc = lay_out<bf16>(m, o.ld, nullptr, nullptr, to, s);
+    rc = lay_out<bf16>(m, o.ld, to, s);
   }
   return o;
 }
@@ -787,25 +855,28 @@ int backward(const ms_rows_t& hidden, const ms_rows_t& weight, const ms_tokens_t
   constexpr bool planes = Planes > 1, wide = sizeof(T) == 4;
   constexpr int pairs = planes ? 6 : 1;
   const bool lifted = hidden.dtype == MS_OPS_F16;
+  const bool scaled_weight = lifted && dweight;
   row_t* rows = space.take<row_t>(n);
   float* factor = space.take<float>(1);
-  int* least = space.take<int>(kRowBlocks);
+  int* least = scaled_weight ? space.take<int>(kScaleBlocks) : nullptr;
+  const int64_t scale_blocks = std::min<int64_t>(ceil_div(n, kScaleRows), kScaleBlocks);
   if (run) {
-    // (fp16: one block up to 16384 tokens, as several take another launch)
-    const int64_t blocks = lifted && n <= 16384 ? 1 : std::min<int64_t>(ceil_div(n, 1024), kRowBlocks);
-    rc = launch(k_rows, blocks, 1024, s, lse, grad_logprob, grad_lse, *targets, vocab, ignore_index,
-                lifted ? 1 : 0, rows, factor, least);
-    if (!rc && lifted && blocks > 1)
-      rc = launch(k_least, 1, kRowBlocks, s, least, blocks, factor);
+    const rows_args a{lse, grad_logprob, grad_lse, *targets, vocab, ignore_index, lifted ? 1 : 0};
+    rc = scaled_weight ? launch(k_scaled_rows, scale_blocks, kScaleThreads, s, a, hidden, rows, least)
+                       : launch(k_rows, ceil_div(n, 256), 256, s, a, rows);
   }
   const operand h = prepare(hidden, planes, space, rc, s, run);
   const operand w = prepare(weight, planes, space, rc, s, run);
   operand scaled = h;
-  if (lifted && dweight) {
+  if (scaled_weight) {
     scaled.ld = round_up(width, 8);
     f16* to = space.take<f16>(n * scaled.ld);
     scaled.data = to;
-    if (run && !rc) rc = lay_out<f16>(hidden, scaled.ld, rows, factor, to, s);
+    const int64_t blocks = ceil_div(n * (scaled.ld / 8), 256);
+    if (run && !rc)
+      rc = fits(blocks, 256) ? launch(k_scaled_layout, blocks, 256, s, hidden, scaled.ld, rows, least,
+                                      scale_blocks, to, factor)
+                             : MS_OPS_EINVAL;
   }
   // Pieces of the vocabulary, all of one size: whole large tiles, and no more of them than
   // kPiece holds
