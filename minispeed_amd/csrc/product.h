@@ -316,9 +316,11 @@ __device__ __forceinline__ void multiply_tile(const product_args& p, const Epilo
       read(buffer, ks + 1, (ks + 1) & 1);
       multiply(ks & 1);
     }
-    // This tile's fragments are in registers and the next tile is in LDS, in all waves
+    // This tile's fragments are in registers and the next tile is in LDS, in all waves.  (The
+    // barrier says nothing of memory to the compiler: nothing may be moved across it either way.)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     if (s + 2 < end) issue(buffer);
     if (s + 1 < end) read(buffer ^ 1, 0, 0);
     multiply(1);
