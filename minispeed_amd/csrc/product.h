@@ -91,13 +91,17 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // 16 bytes from each lane's offset to `to` + 16 lane in LDS.  In assembly, as the compiler
 // would wait for it before the next read of LDS, of the other tile too; the wait is wait_loads().
-// (An instruction between setting m0 and its use is required.)
+// (An instruction between setting m0 and its use is required.  The compiler keeps nothing in m0
+// and warns that it would not; the clobber orders the uses that it may make of it by itself.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t offset, uint32_t to) {
   asm volatile(
       "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset),
       "s"(rsrc)
       : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // One operand's tile of R rows, fetched by NT threads.
