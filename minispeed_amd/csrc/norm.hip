@@ -377,20 +377,23 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
   const bool dout_there = a.dout.data != nullptr, dnext_there = a.dnext.data != nullptr;
   constexpr int kFields = Post ? 4 : 2;
 
-  const int teams = static_cast<int>(gridDim.x) * kTeams, items = static_cast<int>(a.items);
-  const int rounds = (items + teams - 1) / teams;
-  const int parts = static_cast<int>(a.parts), item_rows = static_cast<int>(a.item_rows);
-  // The rows [row, end) of the team's item of a round: none where it has no item.
-  auto place_of = [&](int round, int& item, int& group, int& row, int& end) {
-    item = uniform(round * teams + static_cast<int>(blockIdx.x) * kTeams + wave / W);
+  // (Unsigned: what lies up to a turn of all teams, or an item's rows, behind the last of 2^31 - 1
+  // is counted too.)
+  const uint32_t teams = gridDim.x * kTeams, items = static_cast<uint32_t>(a.items);
+  const uint32_t rounds = (items + teams - 1) / teams;
+  const uint32_t parts = static_cast<uint32_t>(a.parts), gate_rows = static_cast<uint32_t>(a.gate_rows);
+  const int item_rows = static_cast<int>(a.item_rows);
+  // The team's item of a round, `count` rows from `row` on: none where it has no item.
+  auto place_of = [&](uint32_t round, uint32_t& item, uint32_t& group, uint32_t& row, int& count) {
+    item = static_cast<uint32_t>(uniform(static_cast<int>(round * teams + blockIdx.x * kTeams + wave / W)));
     const bool live = round < rounds && item < items;
     group = live ? item / parts : 0;
-    const int begin = group * static_cast<int>(a.gate_rows);
-    row = begin + (live ? item - group * parts : 0) * item_rows;
-    end = live ? min(row + item_rows, begin + static_cast<int>(a.gate_rows)) : row;
+    const uint32_t begin = (live ? item - group * parts : 0) * static_cast<uint32_t>(item_rows);
+    row = group * gate_rows + begin;
+    count = live ? static_cast<int>(min(static_cast<uint32_t>(item_rows), gate_rows - begin)) : 0;
   };
 
-  auto row_of = [](const ms_rows_t& m, int row) {
+  auto row_of = [](const ms_rows_t& m, uint32_t row) {
     return static_cast<const T*>(m.data) + row_start(m, row);
   };
   struct Row {
@@ -398,7 +401,7 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
     float mean, rstd, block_mean, block_rstd;
   };
   // The loads of a row, of nothing where there is none
-  auto fetch = [&](int row, bool live, Row& r) {
+  auto fetch = [&](uint32_t row, bool live, Row& r) {
     cols.template load<true>(row_of(a.next, row), r.x, live);
     cols.template load<true>(dout_there ? row_of(a.dout, row) : weights, r.dy, live && dout_there);
     if (kShort) {
@@ -416,27 +419,29 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
   };
 
   Row now, then;
-  int item, group, row, end;
-  place_of(0, item, group, row, end);
+  uint32_t item, group, row;
+  int count;
+  place_of(0, item, group, row, count);
   Pack<T, V> o[C];
   if (kShort) {
-    fetch(row, row < end, then);
+    fetch(row, count > 0, then);
     // Two stores of nothing: as many follow the loads of every later row, so that the wait
     // for loads is known not to be one for those stores.
     cols.store(static_cast<T*>(a.dresidual), o, false);
     cols.store(static_cast<T*>(a.dresidual), o, false);
   }
-  for (int round = 0; round < rounds; ++round) {
-    int next_item, next_group, next_row, next_end;
-    place_of(round + 1, next_item, next_group, next_row, next_end);
+  for (uint32_t round = 0; round < rounds; ++round) {
+    uint32_t next_item, next_group, next_row;
+    int next_count;
+    place_of(round + 1, next_item, next_group, next_row, next_count);
     const T* gates = static_cast<const T*>(a.gate) + static_cast<int64_t>(group) * width;
     if (gated && kShort) cols.load(gates, gate);
     for (int k = 0; k < item_rows; ++k, ++row) {
-      const bool live = row < end;
+      const bool live = k < count;
       if (kShort) {
         now = then;
         const bool last = k + 1 == item_rows;
-        fetch(last ? next_row : row + 1, last ? next_row < next_end : row + 1 < end, then);
+        fetch(last ? next_row : row + 1, last ? next_count > 0 : k + 1 < count, then);
       } else {
         fetch(row, live, now);
         cols.load(weights, weight);
@@ -537,7 +542,7 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
     item = next_item;
     group = next_group;
     row = next_row;
-    end = next_end;
+    count = next_count;
   }
 
   // The block's sums: one team after the other adds in LDS.
