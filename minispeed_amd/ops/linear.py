@@ -7,6 +7,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _native
+from ._types import of_one_type
 
 
 class LinearLogprobs(NamedTuple):
@@ -54,7 +55,11 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
     penalty on the normaliser.  Gradients are rounded once to the operands' type, from sums in
     32 bits over terms of that type.  Rows without a gradient add nothing to ``weight``'s
     unless they hold infinities or NaN themselves.
+
+    Under ``torch.autocast``, operands of two types are cast to autocast's, as a product's are.
     """
+    if torch.is_autocast_enabled():
+        hidden, weight = of_one_type((hidden, weight))
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return LinearLogprobs(*_LinearLogprobs.apply(hidden, weight, targets, scale, ignore_index))
     return LinearLogprobs(*_native.linear_logprobs(hidden, weight, targets, scale, ignore_index))

@@ -7,6 +7,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native
+from ._types import of_one_type
 
 KINDS = {"rms": 0, "layer": 1}
 
@@ -67,6 +68,8 @@ class _ResidualNorm(torch.autograd.Function):
 
 def _norm(residual, block, weight, bias, block_weight, block_bias, gate, scale, eps, kind):
     args = (residual, block, weight, bias, block_weight, block_bias, gate)
+    if torch.is_autocast_enabled():
+        args = of_one_type(args, torch.float32)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
         return _ResidualNorm.apply(*args, scale, eps, _kind(kind))
     return _native.norm(*args, scale, eps, _kind(kind))
@@ -78,7 +81,8 @@ def norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = N
 
     ``kind`` is ``"rms"`` (``x / sqrt(mean(x ** 2) + eps)``) or ``"layer"`` (the same of ``x``
     without its mean, with an optional ``bias``).  Rows have 1 to 16384 values of float32 / float16 /
-    bfloat16, at any stride; weights are ``[width]``, of the same type.  For the norms at a
+    bfloat16, at any stride; weights are ``[width]``, of the same type (under ``torch.autocast``
+    operands of several types are cast to float32, in which torch's norms run there).  For the norms at a
     model's beginning; :func:`residual_norm` is the norm behind a residual sum.
     """
     return _norm(x, None, weight, bias, None, None, None, 1.0, eps, kind)[1]
