@@ -44,10 +44,18 @@ def linear_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.T
 
     ``hidden`` is ``[..., width]``, ``weight`` ``[vocab, width]``, of one type (float32 /
     float16 / bfloat16), ``targets`` ``[...]`` (int64 or int32).  The logits are not stored,
-    forward or backward: beside the operands and the gradients a call takes some
-    bytes for each token and 128 words of the vocabulary, and backward 512 MiB at most
-    (or 256 words' worth of the vocabulary, and copies of 2-byte operands whose rows
-    are not on 16-byte boundaries; of float32 ones of many tokens always).
+    forward or backward.  Beside the operands and the gradients a call takes some
+    bytes for each token and 128 words of the vocabulary.  Backward takes
+
+    * the gradients of a piece of the logits, in the operands' type: 512 MiB at most, or 256 words'
+      worth of the vocabulary;
+    * sums in 32 bits: of ``hidden``'s gradient where the vocabulary is gone through in several
+      pieces (4 bytes for each value), and of products that are cut into parts: 128 MiB of these at
+      most, but up to 1.25 GiB for float32 operands and where one gradient is wanted alone;
+    * a copy of ``hidden`` in float16, if the weight's gradient is wanted.
+
+    Both take copies of 2-byte operands whose rows are not on 16-byte boundaries, and of
+    float32 ones of many tokens always (6 bytes for each value).
 
     Per row: ``logprob`` of the target (0 where it is ``ignore_index``, NaN where it is outside
     the vocabulary) and ``lse``, the log of the sum of exponentials.  Both are

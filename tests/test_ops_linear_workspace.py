@@ -84,3 +84,51 @@ def test_refused_sizes(lib):
     assert lib.ms_linear_logprobs_grad_workspace_for(None, REF(w), I32(1), I32(1)) == -1
     assert _query(lib, _rows(4, 17, 1), w) == -1
     assert _takes(lib, _rows(0, 16, 1), w, BOTH) == 0 and _takes(lib, _rows(4, 16, 1), w, (0, 0)) == 0
+
+
+def _up(x, to):
+    return -(-x // to) * to
+
+
+def _terms(n, d, v, dtype):
+    """What the operator holds whatever the parts of its sums: (bytes, columns of a piece, pieces, bytes of a
+    copy of hidden).  Operands on 16 bytes."""
+    size, planes = (2, 1) if dtype else (4, 1)
+    if dtype == 0 and n > 384 and n * d * v > 1 << 29:
+        size, planes = 2, 3
+    most = min(max((512 << 20) // (n * size * planes) // 256 * 256, 256), 1 << 20)
+    pieces = -(-v // most)
+    piece = _up(-(-v // pieces), 256)
+    held = _up(16 * n, 256) + 256 + _up(_up(n * piece, 128) * planes * size, 256)
+    if planes == 3:
+        held += sum(_up(_up(rows * d, 128) * 6, 256) for rows in (n, v))
+    return held, min(piece, v), pieces, _up(n * d * 2, 256) + 2048 if dtype == 1 else 0
+
+
+PARTS = (1, 2, 3, 4, 6, 8, 16, 32, 64)
+
+
+def test_the_workspace_by_its_terms(lib):
+    """Row numbers, a piece of d, the copies, and whole sets of sums in 32 bits, within what the
+    documentation states."""
+    rng = random.Random(12)
+    log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))  # noqa: E731
+    cases = [(8192, 2048, 50257, 1), (16384, 768, 50257, 2), (2 ** 20, 64, 128256, 2), (4, 4096, 128256, 2)]
+    cases += [(log(1, 200000), _up(log(8, 16384), 8), log(64, 300000), rng.randrange(3)) for _ in range(3000)]
+    for n, d, v, dtype in cases:
+        h, w = _rows(n, d, dtype), _rows(v, d, dtype)
+        held, columns, pieces, copy = _terms(n, d, v, dtype)
+        of_h = {0} if pieces == 1 else set()
+        of_h |= {_up(s * n * d * 4, 256) for s in PARTS if s > 1 or pieces > 1}
+        of_w = {0} | {_up(s * columns * d * 4, 256) for s in PARTS if s > 1}
+        one = n * d * 4 if pieces > 1 else 0
+        for wanted in (BOTH, HIDDEN, WEIGHT):
+            sums = _takes(lib, h, w, wanted) - held - (copy if wanted[1] else 0)
+            if wanted == HIDDEN:
+                assert sums in of_h
+            elif wanted == WEIGHT:
+                assert sums in of_w
+            else:
+                assert any(sums - x in of_w for x in of_h)
+            more = sums - (one if wanted[0] else 0)
+            assert more <= (128 << 20 if dtype and wanted == BOTH else 1280 << 20)
