@@ -70,3 +70,37 @@ def test_frozen_operands(n, d, v, dtype, need):
         ref.close(a.grad, eh, th, "dhidden")
     else:
         ref.close(b.grad, ew, tw, "dweight")
+
+
+@pytest.mark.parametrize("n,d,v,dtype", [(1090, 576, 8059, "bf16"), (2986, 131, 3493, "fp16"),
+                                         (587, 64, 14418, "fp32")])
+@pytest.mark.parametrize("wanted", [(True, False), (False, True)])
+def test_in_a_graph_and_beside_another_stream(n, d, v, dtype, wanted):
+    h, w, t, gr, gl = make(n, d, v, dtype, n)
+    native = ms.ops._native
+
+    def step():
+        r = ms.ops.linear_logprobs(h, w, t)
+        return [x for x in native.linear_logprobs_grad(h, w, t, r.lse, gr, gl, 1.0, -100, *wanted)
+                if x is not None]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        new = make(n, d, v, dtype, 100 + seed)
+        h.copy_(new[0])
+        gr.copy_(new[3] * 10.0 ** -seed)
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = step()
+        want = step()
+        torch.cuda.synchronize()
+        assert len(out) == 1 and torch.isfinite(want[0]).all()
+        assert torch.equal(out[0], want[0]) and torch.equal(beside[0], want[0])
