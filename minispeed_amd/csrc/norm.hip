@@ -133,9 +133,9 @@ struct Columns {
   static constexpr int V = 16 / sizeof(T);
   uint32_t at[C], last_at, last_word;
   int width;
-  bool odd;
+  bool odd, ragged;       // ragged: the row ends inside a thread's 16 bytes
 
-  __device__ Columns(int lane, int width_of) : width(width_of) {
+  __device__ Columns(int lane, int width_of) : width(width_of), ragged(width_of % V != 0) {
     odd = sizeof(T) == 2 && width % 2 != 0;
     const uint32_t end = (width - 1) * sizeof(T);
     last_at = kNowhere;
@@ -149,6 +149,17 @@ struct Columns {
   }
   __device__ int column(int c, int e) const { return static_cast<int>(at[c] / sizeof(T)) + e; }
   __device__ bool in(int c, int e = 0) const { return column(c, e) < width; }
+  // Behind the row's end the zeros that were loaded stay zeros: a mean stands alone there, and times its
+  // deviation's reciprocal it can pass fp32's range where no value of the row does.  A mean for group c,
+  // and what is left to do where a thread has the end among its values.
+  __device__ float level(int c, float mean) const { return in(c) ? mean : 0.0f; }
+  __device__ void clear(float (&y)[C][V]) const {
+    if (!ragged) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 1; e < V; ++e) y[c][e] = in(c, e) ? y[c][e] : 0.0f;
+  }
   // A row's buffer, or with there = false one of nothing.
   __device__ __amdgpu_buffer_rsrc_t buffer(const T* row, bool there = true) const {
     const int bytes = width * static_cast<int>(sizeof(T));
@@ -197,8 +208,12 @@ struct forward_args {
   float* stats;                        // [rows][2 or 4], or NULL
 };
 
-// Mean and reciprocal deviation of the team's row, held as C groups of V.
-template <bool Layer, int C, int V, typename Cols, typename Of>
+// Mean and reciprocal deviation of the team's row, held as C groups of V.  (The sum is taken 2^-14
+// times, a row's longest, so that it stays within fp32's range as each value does; the same bits.
+// What lies behind the row's end are zeros, or with `Behind` numbers of no meaning.)
+constexpr float kDown = 0x1p-14f;
+static_assert(kMaxWidth <= 1 << 14, "");
+template <bool Layer, bool Behind, int C, int V, typename Cols, typename Of>
 __device__ __forceinline__ float2 row_stats(const float (&x)[C][V], const Cols& cols, float eps,
                                             Of& team) {
   const float width = static_cast<float>(cols.width);
@@ -208,8 +223,9 @@ __device__ __forceinline__ float2 row_stats(const float (&x)[C][V], const Cols& 
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += x[c][e];
-    mean = team.sum(s) / width;
+      for (int e = 0; e < V; ++e)
+        if (!Behind || cols.in(c, e)) s = fmaf(x[c][e], kDown, s);
+    mean = team.sum(s) / width * (1.0f / kDown);
   }
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -264,7 +280,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : W * 64) void k_norm(forward_args a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) x[c][e] = more[c][e];
     if (Post) {
-      post = row_stats<Layer>(x, cols, a.eps, team);
+      post = row_stats<Layer, false>(x, cols, a.eps, team);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -290,7 +306,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : W * 64) void k_norm(forward_args a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) x[c][e] = residual[c][e];
   }
-  const float2 pre = row_stats<Layer>(x, cols, a.eps, team);
+  const float2 pre = row_stats<Layer, Post>(x, cols, a.eps, team);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -450,10 +466,16 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
       float2 s = make_float2(0.0f, 0.0f);
       float d[C][V];
 #pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float level = Layer ? cols.level(c, now.mean) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[c][e] = (now.x[c][e] - level) * now.rstd;
+      }
+      if (Layer) cols.clear(d);
+#pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          d[c][e] = (now.x[c][e] - now.mean) * now.rstd;
           const float t = now.dy[c][e] * weight[c][e];
           s.x = fmaf(t, d[c][e], s.x);
           if (Layer) s.y += t;
@@ -484,13 +506,21 @@ __global__ __launch_bounds__(block_waves(W) * 64, Layer && Post && W < 16 ? 2 : 
         load_block_vectors();
         if (gated) cols.load(gates, gate);
       }
-      float w[C][V];
+      float w[C][V] = {};
+      if (Post) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const float level = Layer ? cols.level(c, now.block_mean) : 0.0f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) w[c][e] = (now.b[c][e] - level) * now.block_rstd;
+        }
+        if (Layer) cols.clear(w);
+      }
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float q = d[c][e] * a.scale;
-          w[c][e] = Post ? (now.b[c][e] - now.block_mean) * now.block_rstd : 0.0f;
           if (gated) {
             const float u = Post ? fmaf(w[c][e], block_weight[c][e], Layer ? block_bias[c][e] : 0.0f)
                                  : now.b[c][e];
