@@ -82,9 +82,10 @@ def norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = N
     ``kind`` is ``"rms"`` (``x / sqrt(mean(x ** 2) + eps)``) or ``"layer"`` (the same of ``x``
     without its mean, with an optional ``bias``).  Rows have 1 to 16384 values of float32 / float16 /
     bfloat16, at any stride; weights are ``[width]``, of the same type (under ``torch.autocast``
-    operands of several types are cast to float32, in which torch's norms run there).  Squares are
-    taken in 32 bits: a row whose mean square passes their range is normalised to zeros.  For the
-    norms at a model's beginning; :func:`residual_norm` is the norm behind a residual sum.
+    operands of several types are cast to float32, in which torch's norms run there).  Differences from
+    the mean and their squares are taken in 32 bits; a row where they pass these comes out as
+    zeros or NaN.  For the norms at a model's beginning; :func:`residual_norm` is the norm behind a
+    residual sum.
     """
     return _norm(x, None, weight, bias, None, None, None, 1.0, eps, kind)[1]
 
